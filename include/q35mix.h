@@ -227,6 +227,91 @@ int q35m_attn_decode_noalloc(q35m_ctx* ctx, int layer, int n, const int* seqs, c
 int q35m_attn_prefill(q35m_ctx* ctx, int layer, int seq, int T, const float* q_gate,
                       const float* k, const float* v, float* out);
 
+/* ---- paged K/V cache and the attention over it ------------------------- */
+
+/* Full-attention K/V rows in pages, for hosts that serve many sequences from
+ * one pool: a page holds page_rows rows of every kv head of one layer, and a
+ * sequence's row r lies in its page r / page_rows, which the caller chooses
+ * (q35m_paged_map).  Sequences may share pages (a common prefix), come and go
+ * without moving rows, and take memory by page.  The cache has sequences and
+ * lengths of its own, apart from the context's; the context gives the layers,
+ * the heads, the q / k norm weights (q35m_set_attn_weights) and the stream.
+ * No counterpart in the reference, whose cache is one growing array per layer
+ * (Qwen35Model.cs:293-353); the operators are its DecodeAttention /
+ * PrefillAttention after the projections (Qwen35Model.Decode.cs:294-323,
+ * Qwen35Model.Prefill.cs:113-149), as q35m_attn_decode / q35m_attn_prefill
+ * above. */
+typedef struct q35m_paged q35m_paged;
+
+/* How a cache holds K and V: fp32, or fp16 (half the memory and the traffic:
+ * the values of an fp32 cache, rounded to nearest even when their row is
+ * written, beyond the range of fp16 to infinities; activations and outputs are
+ * fp32, and the attention adds no rounding beyond fp32's). */
+#define Q35M_KV_F32 0
+#define Q35M_KV_F16 1
+
+/* A cache of n_pages pages for every full-attention layer of ctx and n_seqs
+ * sequences of up to max_rows rows each (max_rows up to 2^24); page_rows is a
+ * power of two from 16 to 1024.  Allocates here, and nothing afterwards.  At
+ * first no page is mapped and every length is 0.  Destroy it before ctx. */
+int q35m_paged_create(q35m_ctx* ctx, int n_seqs, int max_rows, int n_pages, int page_rows, int kv_type,
+                      q35m_paged** out);
+int q35m_paged_destroy(q35m_paged* p);
+/* Pages first .. first + n - 1 of sequence seq (its rows first * page_rows and
+ * on) become pages[0 .. n) of the pool (HOST array; NULL: not mapped).  An id
+ * outside [0, n_pages) is Q35M_ERR_INVALID, entries past max_rows
+ * Q35M_ERR_RANGE; then nothing changes.  A page that more than one entry maps
+ * is read-only: calls that would write a row into it are refused
+ * (Q35M_ERR_INVALID).  Contents and lengths stay as they are. */
+int q35m_paged_map(q35m_paged* p, int seq, int first, int n, const int* pages);
+/* Lengths, as q35m_advance / q35m_truncate / q35m_kv_len: the operators below
+ * write and read from the current length on and leave it; once every layer has
+ * run, advance moves n sequences (HOST arrays; distinct, up to 64 a call) by
+ * their tokens (>= 0; past max_rows Q35M_ERR_CAPACITY, and then none is moved);
+ * truncate shortens one (extending is Q35M_ERR_RANGE).
+ * q35m_paged_map, _advance and _truncate enqueue a small kernel each, and are
+ * refused (Q35M_ERR_INVALID) while the context's stream is being captured,
+ * since a replay would repeat them. */
+int q35m_paged_advance(q35m_paged* p, int n, const int* seqs, const int* tokens);
+int q35m_paged_truncate(q35m_paged* p, int seq, int length);
+int q35m_paged_len(const q35m_paged* p, int seq, int* length);
+/* Device address and size of one layer's pages, for zero-copy callers: kind
+ * Q35M_STATE_KEYS or Q35M_STATE_VALUES, [n_pages][kv_heads][page_rows]
+ * [head_dim] values of the cache's type. */
+int q35m_paged_device_ptr(q35m_paged* p, int layer, int kind, void** dptr, size_t* bytes);
+
+/* The rows of new tokens of n sequences put into their pages: for each
+ * sequence seqs[i] its next tokens[i] rows (HOST arrays; seqs distinct, up to
+ * 64; tokens >= 0) of k and v [sum of tokens][kv_heads*head_dim], in the
+ * sequences' order, go to rows length(seqs[i]) and on: K rotated to its
+ * position, then (1+w)-normed, V as it is, both rounded to the cache's type.
+ * What the two attention calls below do for their rows; by itself for tokens
+ * whose attention nobody reads (all of a prompt but its last token, in the
+ * model's last layer).  Rows past the last sequence's are not read.  Pages
+ * must be mapped up to the last new row (Q35M_ERR_CAPACITY otherwise, as past
+ * max_rows). */
+int q35m_paged_append(q35m_paged* p, int layer, int n, const int* seqs, const int* tokens, const float* k,
+                      const float* v);
+/* q35m_attn_decode over paged rows: one new token of each of n sequences.
+ * q_gate [n][heads*2*head_dim], k, v [n][kv_heads*head_dim], out
+ * [n][heads*head_dim].  The lengths and page tables are read on the device:
+ * captured into a HIP graph on the context's stream, a replay decodes at the
+ * lengths and pages of its time (the checks above are made when a call is
+ * enqueued or captured: keep the pages of every row that a replay writes
+ * mapped, and shared by nobody). */
+int q35m_paged_attn_decode(q35m_paged* p, int layer, int n, const int* seqs, const float* q_gate, const float* k,
+                           const float* v, float* out);
+/* q35m_attn_prefill over paged rows, for chunks of new tokens of n sequences
+ * at once: tokens[i] >= 0 rows of sequence seqs[i], in the sequences' order,
+ * row j of a sequence at position length + j attending over the rows up to its
+ * own.  q_gate [sum][heads*2*head_dim], k, v [sum][kv_heads*head_dim], out
+ * [sum][heads*head_dim]; rows past the sum are neither read nor written.
+ * Captured and replayed as q35m_paged_attn_decode.
+ * The attention calls on one cache share its workspace: graphs that hold them
+ * are replayed in order, on one stream. */
+int q35m_paged_attn_prefill(q35m_paged* p, int layer, int n, const int* seqs, const int* tokens,
+                            const float* q_gate, const float* k, const float* v, float* out);
+
 /* ---- one decode step of every layer, captured once, replayed per token ---- */
 
 /* Per-layer activations of a decode step, device pointers fixed for the life

@@ -1,0 +1,557 @@
+// Paged K/V cache: attention of one new token per sequence.
+//
+// Per sequence at length p, q head h of kv head g: q = norm(rope(q, p)) (1 + w),
+// s_j = q . K_j / 16 over rows j = 0 .. p (the p cached rows and the new one),
+// out = sigmoid(gate) sum_j e^{s_j - m} V_j / sum_j e^{s_j - m}: DecodeAttention
+// after the projections (src/Qwen35Sharp.Model/Qwen35Model.Decode.cs:294-323).
+// Every cached row is read once, so the bound is the cache's bytes over HBM's
+// rate; the products are a few operations a byte.
+//
+// Work is cut into units of kUnit rows of one (sequence, head group) and dealt
+// out evenly: workgroup w takes units [w per, (w + 1) per) of the units of all
+// sequences in order, per = ceil(units / workgroups), both found on the device
+// from the lengths there, so batches of unequal lengths fill the card and a
+// captured launch fits any lengths.  A stretch of units of one (sequence, head
+// group) is a segment: whole ones are finished where they are, of the others
+// the maximum, the sum and the unnormalised output go to the workspace (two
+// segments of a workgroup at most are not whole, its first and its last), and
+// paged_decode_merge joins them.
+//
+// A unit's rows go to the four waves, which keep an online softmax each and
+// meet at the segment's end.  All products are matrix instructions with the
+// (up to 16) q heads of the kv head as columns:
+//   S^T = K Q^T  (rows of K: the 16 lanes l % 16; dims: lane group l / 16)
+//   O^T = V^T P^T, whose P^T operand is S^T's own register layout (a lane
+//   holds, of its q column, rows 4 (l / 16) + i), with V rows read in that
+//   order; so neither P nor V crosses lanes.
+// fp32 caches use the fp32 instruction (16 x 16 x 4).  fp16 caches use
+// 16 x 16 x 32 on fp16 with the fp32 operands q and P as two fp16 values each
+// (hi + lo, 22 bits; q's row and P scaled by powers of two into the range),
+// and a register transpose of V (8 rows x 8 dims a lane).
+#include "paged_device.h"
+
+namespace q35 {
+namespace {
+
+constexpr int NT = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+// P is formed as e^{s - m} 2^kPShift, so that its low fp16 half loses nothing
+// that fp32 holds (the normalisation divides the factor out).
+constexpr float kPShift = 7.0f;
+
+template <typename T>
+struct Tile;
+
+// 16 rows of an fp32 cache a wave.
+template <>
+struct Tile<float> {
+    static constexpr int kRows = 16;
+    float q[64];            // dims 16 t + 4 g + c at [4 t + c]
+    float4 k[16], v[4][4];  // K row l % 16, dims 16 t + 4 g; V row 4 g + i, dims 64 t + 4 m
+    f32x4 o[16];            // dims 64 t + 4 row + c at [4 t + c]
+
+    __device__ __forceinline__ float set_q(float (&x)[64]) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) q[i] = x[i];
+        return 1.0f;
+    }
+    // First dim of the 4 that x[4 t ..] of set_q holds.
+    static __device__ __forceinline__ int q_dim(int t, int g) { return 16 * t + 4 * g; }
+    static constexpr int kRopePair = 8;     // x index of dim d + 32 less that of dim d
+
+    __device__ __forceinline__ void load_k(const float* p, int, int lane) {
+        const float* a = p + (lane & 15) * kHd + 4 * (lane >> 4);
+#pragma unroll
+        for (int t = 0; t < 16; ++t) k[t] = load_nt(a + 16 * t);
+    }
+    __device__ __forceinline__ void load_v(const float* p, int, int lane) {
+        const float* a = p + (lane >> 4) * 4 * kHd + 4 * (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) v[i][t] = load_nt(a + i * kHd + 64 * t);
+    }
+    // Row `at` of the tile (none if negative) comes from kn / vn, rows from
+    // `rows` on are masked: their V must not meet the products (0 x NaN).
+    __device__ __forceinline__ void fix(const float* kn, const float* vn, int at, int rows, int lane) {
+        const int g = lane >> 4, m = lane & 15;
+#pragma unroll
+        for (int t = 0; t < 16; ++t)
+            if (m == at) k[t] = *reinterpret_cast<const float4*>(kn + 16 * t + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (4 * g + i == at) v[i][t] = *reinterpret_cast<const float4*>(vn + 64 * t + 4 * m);
+                if (4 * g + i >= rows) v[i][t] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+    }
+    __device__ __forceinline__ void scores(float (&s)[4]) const {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].x, q[4 * t], a, 0, 0, 0);
+            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].y, q[4 * t + 1], b, 0, 0, 0);
+            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].z, q[4 * t + 2], a, 0, 0, 0);
+            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].w, q[4 * t + 3], b, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = a[i] + b[i];
+    }
+    static __device__ __forceinline__ int row_of(int i, int g) { return 4 * g + i; }
+    static constexpr int kScores = 4;
+    __device__ __forceinline__ void pv(const float (&p)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                o[4 * t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][t].x, p[i], o[4 * t], 0, 0, 0);
+                o[4 * t + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][t].y, p[i], o[4 * t + 1], 0, 0, 0);
+                o[4 * t + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][t].z, p[i], o[4 * t + 2], 0, 0, 0);
+                o[4 * t + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][t].w, p[i], o[4 * t + 3], 0, 0, 0);
+            }
+    }
+    // The lane's output values, 4 consecutive dims at a time.
+    template <typename F>
+    __device__ __forceinline__ void each4(int g, F f) const {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                f(64 * t + 4 * (4 * g + i), make_float4(o[4 * t][i], o[4 * t + 1][i], o[4 * t + 2][i], o[4 * t + 3][i]));
+    }
+};
+
+// 32 rows of an fp16 cache a wave, as two groups of 16.
+template <>
+struct Tile<_Float16> {
+    static constexpr int kRows = 32;
+    f16x8 qh[8], ql[8];        // dims 32 t + 8 g ..
+    u32x4 k[2][8], v[2][8];    // K row l % 16 of group kb, dims 32 t + 8 g; V row 16 (j / 4) + 4 g + j % 4, dims 128 u + 8 m
+    f32x4 o[16];               // dims 128 u + 8 row + b at [8 u + b]
+
+    // Scales the row into fp16's range by a power of two, splits it, and
+    // returns the factor that undoes the scale.
+    __device__ __forceinline__ float set_q(float (&x)[64]) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 64; ++i) mx = fmaxf(mx, fabsf(x[i]));
+        mx = xor16_max(xor32_max(mx));
+        const int e = 10 - max(__builtin_amdgcn_frexp_expf(mx), -100);
+        const float up = ldexpf(1.0f, e);
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float y = x[8 * t + j] * up;
+                qh[t][j] = (_Float16)y;
+                ql[t][j] = (_Float16)(y - (float)qh[t][j]);
+            }
+        return ldexpf(1.0f, -e);
+    }
+    static __device__ __forceinline__ int q_dim(int t, int g) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1); }
+    static constexpr int kRopePair = 8;
+
+    __device__ __forceinline__ void load_k(const _Float16* p, int kb, int lane) {
+        const _Float16* a = p + (lane & 15) * kHd + 8 * (lane >> 4);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) k[kb][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a + 32 * t));
+    }
+    __device__ __forceinline__ void load_v(const _Float16* p, int kb, int lane) {
+        const _Float16* a = p + (lane >> 4) * 4 * kHd + 8 * (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                v[u][4 * kb + i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a + i * kHd + 128 * u));
+    }
+    __device__ __forceinline__ void fix(const _Float16* kn, const _Float16* vn, int at, int rows, int lane) {
+        const int g = lane >> 4, m = lane & 15;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                if (16 * kb + m == at) k[kb][t] = *reinterpret_cast<const u32x4*>(kn + 32 * t + 8 * g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = row_of(j, g);
+                if (r == at) v[u][j] = *reinterpret_cast<const u32x4*>(vn + 128 * u + 8 * m);
+                if (r >= rows) v[u][j] = u32x4{0, 0, 0, 0};
+            }
+    }
+    __device__ __forceinline__ void scores(float (&s)[8]) const {
+        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[0][t]), ql[t], a, 0, 0, 0);
+            b = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[1][t]), ql[t], b, 0, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[0][t]), qh[t], a, 0, 0, 0);
+            b = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[1][t]), qh[t], b, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[i] = a[i];
+            s[4 + i] = b[i];
+        }
+    }
+    static __device__ __forceinline__ int row_of(int j, int g) { return 16 * (j >> 2) + 4 * g + (j & 3); }
+    static constexpr int kScores = 8;
+    __device__ __forceinline__ void pv(const float (&p)[8]) {
+        f16x8 ph, pl;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            ph[j] = (_Float16)p[j];
+            pl[j] = (_Float16)(p[j] - (float)ph[j]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                // dim 128 u + 8 m + b of the lane's 8 rows
+                const uint32_t sel = (b & 1) ? 0x07060302u : 0x05040100u;
+                u32x4 a;
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    a[w] = __builtin_amdgcn_perm(v[u][2 * w + 1][b >> 1], v[u][2 * w][b >> 1], sel);
+                const f16x8 av = __builtin_bit_cast(f16x8, a);
+                o[8 * u + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pl, o[8 * u + b], 0, 0, 0);
+                o[8 * u + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, ph, o[8 * u + b], 0, 0, 0);
+            }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each4(int g, F f) const {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int b = 0; b < 8; b += 4)
+                    f(128 * u + 8 * (4 * g + i) + b,
+                      make_float4(o[8 * u + b][i], o[8 * u + b + 1][i], o[8 * u + b + 2][i], o[8 * u + b + 3][i]));
+    }
+};
+
+// The units of a call's sequences, one sequence a lane: `end` is the number of
+// units up to and with the lane's.
+struct Units {
+    int rows, tiles, end, total;
+};
+template <typename T>
+__device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch& b, int groups, int lane) {
+    constexpr int kUnit = 4 * Tile<T>::kRows;
+    Units u;
+    // (the row past max_rows of a replayed call that its caller let run over)
+    u.rows = lane < b.n ? min(pv.lens[b.seq[lane]] + 1, pv.max_rows) : 0;
+    u.tiles = (u.rows + kUnit - 1) / kUnit;
+    u.end = u.tiles * groups;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int x = __shfl_up(u.end, o, kWave);
+        if (lane >= o) u.end += x;
+    }
+    u.total = __builtin_amdgcn_readlane(u.end, kWave - 1);
+    return u;
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
+                                                      const float* __restrict__ knew, const float* __restrict__ vnew,
+                                                      const float* __restrict__ q_norm,
+                                                      const float* __restrict__ k_norm, float* __restrict__ out,
+                                                      float* __restrict__ part_o, float* __restrict__ part_ml, int hg,
+                                                      int ng, float eps) {
+    using Tl = Tile<T>;
+    constexpr int R = Tl::kRows;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int groups = pv.nkv * ng, nh = groups * hg;
+
+    __shared__ float obuf[4][kPagedDecodeHeads][kHd];
+    __shared__ float ml[4][kPagedDecodeHeads][2];
+    __shared__ __align__(16) T newrow[4][2][kHd];
+
+    const Units un = units_of<T>(pv, b, groups, lane);
+    const int per = (un.total + (int)gridDim.x - 1) / (int)gridDim.x;
+    int u = blockIdx.x * per;
+    const int u_end = min(u + per, un.total);
+
+    while (u < u_end) {
+        const int i = __popcll(__ballot(un.end <= u));            // the unit's sequence in the batch
+        const int tiles = __builtin_amdgcn_readlane(un.tiles, i);
+        const int rows = __builtin_amdgcn_readlane(un.rows, i);
+        const int local = u - (__builtin_amdgcn_readlane(un.end, i) - tiles * groups);
+        const int y = local / tiles, t0 = local - y * tiles;      // head group, first unit of the segment
+        const int t1 = min(tiles, t0 + (u_end - u));
+        u += t1 - t0;
+        const int kvh = y / ng, seq = b.seq[i], pos = rows - 1;
+        const int* table = pv.table + (size_t)seq * pv.max_pages;
+        const int first = t0 * 4 * R + wave * R, stop = min(rows, t1 * 4 * R);
+        const int last16 = pos & ~15;
+
+        Tl tl;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) tl.o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        auto page16 = [&](int r) {     // page of the 16-row group at r (the last one past the end)
+            return page_of(table, min(r, last16) >> pv.page_shift, pv.max_pages, pv.n_pages);
+        };
+        int pg[R / 16];
+        auto pages = [&](int base) {
+#pragma unroll
+            for (int kb = 0; kb < R / 16; ++kb) pg[kb] = page16(base + 16 * kb);
+        };
+        auto load_k = [&](int base, const int (&p)[R / 16]) {
+#pragma unroll
+            for (int kb = 0; kb < R / 16; ++kb)
+                tl.load_k((const T*)pv.k + row_offset<T>(pv, p[kb], kvh, min(base + 16 * kb, last16)), kb, lane);
+        };
+        auto load_v = [&](int base, const int (&p)[R / 16]) {
+#pragma unroll
+            for (int kb = 0; kb < R / 16; ++kb)
+                tl.load_v((const T*)pv.v + row_offset<T>(pv, p[kb], kvh, min(base + 16 * kb, last16)), kb, lane);
+        };
+        if (first < stop) {
+            pages(first);
+            load_k(first, pg);
+            load_v(first, pg);
+        }
+
+        // q: the rotation, the norm, the scale 1/16 (and log2 e, for exp2).
+        float down = 1.0f;
+        {
+            const int h = y * hg + min(n, hg - 1);
+            const float* qp = q_gate + ((size_t)i * nh + h) * 2 * kHd;
+            const double* rope = pv.rope + (size_t)pos * kRopeDim;
+            float x[64], ss = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                const float4 a = *reinterpret_cast<const float4*>(qp + Tl::q_dim(t, g));
+                x[4 * t] = a.x; x[4 * t + 1] = a.y; x[4 * t + 2] = a.z; x[4 * t + 3] = a.w;
+            }
+#pragma unroll
+            for (int t = 0; t < Tl::kRopePair / 4; ++t)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int d = Tl::q_dim(t, g) + c;
+                    const float cs = (float)rope[d], sn = (float)rope[kRopeHalf + d];
+                    const float lo = x[4 * t + c], hi = x[4 * t + c + Tl::kRopePair];
+                    x[4 * t + c] = lo * cs - hi * sn;
+                    x[4 * t + c + Tl::kRopePair] = lo * sn + hi * cs;
+                }
+#pragma unroll
+            for (int t = 0; t < 64; ++t) ss += x[t] * x[t];
+            ss = xor16_sum(xor32_sum(ss));
+            const float scale = n < hg ? kLog2e / 16.0f / sqrtf(ss / (float)kHd + eps) : 0.0f;
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                const float4 w = *reinterpret_cast<const float4*>(q_norm + Tl::q_dim(t, g));
+                x[4 * t] *= scale * (1.0f + w.x);
+                x[4 * t + 1] *= scale * (1.0f + w.y);
+                x[4 * t + 2] *= scale * (1.0f + w.z);
+                x[4 * t + 3] *= scale * (1.0f + w.w);
+            }
+            down = tl.set_q(x);
+        }
+
+        // The wave that holds the new row makes it (every head group needs it;
+        // one writes it to the page, and none reads it from there).
+        const int new_tile = pos / R * R;
+        if (first <= new_tile && new_tile < stop && (new_tile - first) % (4 * R) == 0) {
+            const size_t at = ((size_t)i * pv.nkv + kvh) * kHd + 4 * lane;
+            const float4 xk = *reinterpret_cast<const float4*>(knew + at);
+            const float4 xv = *reinterpret_cast<const float4*>(vnew + at);
+            const float4 yk = paged_key_row(xk, pv.rope + (size_t)pos * kRopeDim, k_norm, lane, (double)eps);
+            store_row4(&newrow[wave][0][4 * lane], yk);
+            store_row4(&newrow[wave][1][4 * lane], xv);
+            const int pnew = page_of(table, pos >> pv.page_shift, pv.max_pages, pv.n_pages);
+            if (y % ng == 0 && pnew >= 0 && pv.lens[seq] < pv.max_rows) {
+                const size_t to = row_offset<T>(pv, pnew, kvh, pos) + 4 * lane;
+                store_row4((T*)pv.k + to, yk);
+                store_row4((T*)pv.v + to, xv);
+            }
+        }
+
+        float m_run = -INFINITY, l_run = 0.0f;
+        for (int base = first; base < stop; base += 4 * R) {
+            const int next = base + 4 * R;
+            const bool more = next < stop;
+            if (more) pages(next);
+            if (base + R > pos) tl.fix(newrow[wave][0], newrow[wave][1], pos - base, rows - base, lane);
+            float s[Tl::kScores];
+            tl.scores(s);
+            if (more) load_k(next, pg);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < Tl::kScores; ++j) {
+                s[j] = base + Tl::row_of(j, g) < rows ? s[j] * down : -INFINITY;
+                mx = fmaxf(mx, s[j]);
+            }
+            mx = fmaxf(m_run, xor16_max(xor32_max(mx)));
+            const float mu = mx == -INFINITY ? 0.0f : mx;
+            const float alpha = __builtin_amdgcn_exp2f(m_run - mu);
+            m_run = mx;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < Tl::kScores; ++j) {
+                s[j] = __builtin_amdgcn_exp2f(s[j] - mu + kPShift);
+                sum += s[j];
+            }
+            l_run = l_run * alpha + sum;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) tl.o[x] *= alpha;
+            tl.pv(s);
+            if (more) load_v(next, pg);
+        }
+
+        // The four waves of the segment join.
+        l_run = xor16_sum(xor32_sum(l_run));
+        if (n < hg) {
+            tl.each4(g, [&](int d, float4 x) { *reinterpret_cast<float4*>(&obuf[wave][n][d]) = x; });
+            if (g == 0) {
+                ml[wave][n][0] = m_run;
+                ml[wave][n][1] = l_run;
+            }
+        }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == tiles;
+        const int slot = 2 * blockIdx.x + (t0 == 0);
+        for (int h = 0; h < hg; ++h) {
+            float M = -INFINITY, l = 0.0f, o = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][h][0]);
+            const float mu = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float e = __builtin_amdgcn_exp2f(ml[w][h][0] - mu);
+                l += e * ml[w][h][1];
+                o += e * obuf[w][h][tid];
+            }
+            if (whole) {
+                const size_t row = (size_t)i * nh + y * hg + h;
+                const float gate = q_gate[row * 2 * kHd + kHd + tid];
+                out[row * kHd + tid] = o / l * (1.0f / (1.0f + expf(-gate)));
+            } else {
+                const size_t at = (size_t)slot * kPagedDecodeHeads + h;
+                part_o[at * kHd + tid] = o;
+                if (tid == 0) {
+                    part_ml[2 * at] = M;
+                    part_ml[2 * at + 1] = l;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// The parts of one (sequence, q head), where its units went to several
+// workgroups: waves take parts in turn, a lane four dims.
+constexpr int MW = 8;      // waves
+template <typename T>
+__global__ __launch_bounds__(MW * kWave) void paged_decode_merge(PagedView pv, PagedBatch b,
+                                                                 const float* __restrict__ part_o,
+                                                                 const float* __restrict__ part_ml,
+                                                                 const float* __restrict__ q_gate,
+                                                                 float* __restrict__ out, int hg, int ng, int nwg) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int groups = pv.nkv * ng, nh = groups * hg;
+    const int i = blockIdx.y, head = blockIdx.x, y = head / hg, h = head - y * hg;
+    const Units un = units_of<T>(pv, b, groups, lane);
+    const int per = (un.total + nwg - 1) / nwg;
+    const int tiles = __builtin_amdgcn_readlane(un.tiles, i);
+    const int s = __builtin_amdgcn_readlane(un.end, i) - tiles * groups + y * tiles;
+    const int w0 = s / per, w1 = (s + tiles - 1) / per;      // its first and last workgroup
+    if (w0 == w1) return;
+    const size_t row = (size_t)i * nh + head;
+    const float4 gate = *reinterpret_cast<const float4*>(q_gate + row * 2 * kHd + kHd + 4 * lane);
+    __shared__ float4 obuf[MW][kWave];
+    __shared__ float lbuf[MW];
+    // Part of workgroup w: its last segment for the first one, else its first.
+    auto part = [&](int w) { return (size_t)(2 * w + (w == w0)) * kPagedDecodeHeads + h; };
+    float M = -INFINITY;
+    for (int w = w0 + lane; w <= w1; w += kWave) M = fmaxf(M, part_ml[2 * part(w)]);
+    M = wave_max(M);
+    const float mu = M == -INFINITY ? 0.0f : M;
+    float l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int U = 4;       // parts whose loads are in flight together
+    for (int w = w0 + wave; w <= w1; w += U * MW) {
+        float4 x[U];
+        float e[U], ls[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const size_t at = part(min(w + k * MW, w1));
+            x[k] = reinterpret_cast<const float4*>(part_o + at * kHd)[lane];
+            e[k] = part_ml[2 * at];
+            ls[k] = part_ml[2 * at + 1];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if (w + k * MW > w1) break;
+            const float f = __builtin_amdgcn_exp2f(e[k] - mu);
+            l += f * ls[k];
+            o.x += f * x[k].x; o.y += f * x[k].y; o.z += f * x[k].z; o.w += f * x[k].w;
+        }
+    }
+    obuf[wave][lane] = o;
+    if (lane == 0) lbuf[wave] = l;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+        for (int w = 1; w < MW; ++w) {
+            const float4 x = obuf[w][lane];
+            o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+            l += lbuf[w];
+        }
+        const float inv = 1.0f / l;
+        float4 r;
+        r.x = o.x * inv * (1.0f / (1.0f + expf(-gate.x)));
+        r.y = o.y * inv * (1.0f / (1.0f + expf(-gate.y)));
+        r.z = o.z * inv * (1.0f / (1.0f + expf(-gate.z)));
+        r.w = o.w * inv * (1.0f / (1.0f + expf(-gate.w)));
+        *reinterpret_cast<float4*>(out + row * kHd + 4 * lane) = r;
+    }
+}
+
+// One workgroup a CU (300 registers a lane).
+int decode_workgroups(const q35m_ctx* c) { return c->n_cu; }
+
+}  // namespace
+
+size_t paged_decode_work_bytes(const q35m_ctx* c) {
+    return (size_t)2 * decode_workgroups(c) * kPagedDecodeHeads * (kHd + 2) * sizeof(float);
+}
+
+hipError_t launch_paged_decode(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, const float* k,
+                               const float* v, float* out) {
+    q35m_ctx* c = p->ctx;
+    const int per_kv = c->d.nh / c->d.nkv;
+    // q heads a workgroup: all of a kv head's up to 16, else 16 or 8 of them.
+    const int hg = per_kv <= 16 ? per_kv : per_kv % 16 == 0 ? 16 : 8;
+    const int ng = per_kv / hg, nwg = decode_workgroups(c);
+    float* part_o = p->work;
+    float* part_ml = part_o + (size_t)2 * nwg * kPagedDecodeHeads * kHd;
+    const PagedView pv = p->view(layer);
+    const AttnLayer& L = c->full[layer];
+    auto go = [&](auto part, auto merge) {
+        {
+            ProfScope ps(c, K_PAGED_DECODE);
+            hipExtLaunchKernelGGL(part, dim3(nwg), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b, q_gate, k, v, L.q_norm,
+                                  L.k_norm, out, part_o, part_ml, hg, ng, c->d.eps);
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        ProfScope ps(c, K_PAGED_DECODE_MERGE);
+        hipExtLaunchKernelGGL(merge, dim3(c->d.nh, b.n), dim3(MW * kWave), 0, c->stream, ps.a, ps.b, 0, pv, b, part_o,
+                              part_ml, q_gate, out, hg, ng, nwg);
+        return hipGetLastError();
+    };
+    if (p->type == Q35M_KV_F16) return go(paged_decode<_Float16>, paged_decode_merge<_Float16>);
+    return go(paged_decode<float>, paged_decode_merge<float>);
+}
+
+}  // namespace q35

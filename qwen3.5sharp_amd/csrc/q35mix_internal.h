@@ -100,6 +100,11 @@ enum KernelId {
     K_ATTN_SPLIT_MERGE,
     K_Q4K_SMALL,                 // linear_gemm and linear_gemm_split of Q4_K, Q6_K
     K_Q6K_SMALL,
+    K_PAGED_APPEND,
+    K_PAGED_DECODE,
+    K_PAGED_DECODE_MERGE,
+    K_PAGED_PREFILL,
+    K_PAGED_PREFILL_MERGE,
     K_COUNT
 };
 const char* kernel_name(int id);

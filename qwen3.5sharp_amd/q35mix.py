@@ -22,6 +22,7 @@ ERR_INVALID, ERR_UNSUPPORTED, ERR_CAPACITY, ERR_NO_DEVICE, ERR_HIP, ERR_OOM, ERR
     -1, -2, -3, -4, -5, -6, -7
 STATE_RECURRENT, STATE_CONV, STATE_KEYS, STATE_VALUES = 0, 1, 2, 3
 PROJ_REFERENCE, PROJ_BLOCK = 0, 1
+KV_F32, KV_F16 = 0, 1
 
 _lib = None
 _hip = None
@@ -99,6 +100,17 @@ def lib() -> ctypes.CDLL:
                                                   ctypes.POINTER(ctypes.c_void_p)]
         _lib.q35m_decode_graph_run.argtypes = [ctypes.c_void_p, ctypes.c_int]
         _lib.q35m_decode_graph_destroy.argtypes = [ctypes.c_void_p]
+        vp, ci, ip = ctypes.c_void_p, ctypes.c_int, ctypes.POINTER(ctypes.c_int)
+        _lib.q35m_paged_create.argtypes = [vp, ci, ci, ci, ci, ci, ctypes.POINTER(vp)]
+        _lib.q35m_paged_destroy.argtypes = [vp]
+        _lib.q35m_paged_map.argtypes = [vp, ci, ci, ci, vp]
+        _lib.q35m_paged_advance.argtypes = [vp, ci, ip, ip]
+        _lib.q35m_paged_truncate.argtypes = [vp, ci, ci]
+        _lib.q35m_paged_len.argtypes = [vp, ci, ip]
+        _lib.q35m_paged_device_ptr.argtypes = [vp, ci, ci, ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_size_t)]
+        _lib.q35m_paged_append.argtypes = [vp, ci, ci, ip, ip, vp, vp]
+        _lib.q35m_paged_attn_decode.argtypes = [vp, ci, ci, ip, vp, vp, vp, vp]
+        _lib.q35m_paged_attn_prefill.argtypes = [vp, ci, ci, ip, ip, vp, vp, vp, vp]
     return _lib
 
 
@@ -504,6 +516,76 @@ class Context:
         check(lib().q35m_state_device_ptr(self.handle, layer, seq, kind, ctypes.byref(p),
                                           ctypes.byref(n)))
         return p.value, n.value
+
+
+class PagedCache:
+    """q35m_paged: K/V rows of a context's full-attention layers in pages of
+    page_rows rows, for n_seqs sequences of their own (lengths and page tables
+    apart from the context's)."""
+
+    def __init__(self, ctx: Context, n_seqs: int, max_rows: int, n_pages: int, page_rows: int = 64,
+                 kv_type: int = KV_F16):
+        self.ctx = ctx
+        h = ctypes.c_void_p()
+        check(lib().q35m_paged_create(ctypes.c_void_p(ctx.handle), n_seqs, max_rows, n_pages, page_rows, kv_type,
+                                      ctypes.byref(h)))
+        self.handle = h.value
+        self.n_seqs, self.max_rows, self.n_pages = n_seqs, max_rows, n_pages
+        self.page_rows, self.kv_type = page_rows, kv_type
+
+    def close(self) -> None:
+        """Before the context's close()."""
+        if self.handle:
+            check(lib().q35m_paged_destroy(self.handle))
+            self.handle = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.close()
+
+    def map(self, seq: int, first: int, pages) -> None:
+        """Page entries first, first + 1, ... of seq become `pages`."""
+        a = np.ascontiguousarray(np.asarray(pages, dtype=np.int32).ravel())
+        check(lib().q35m_paged_map(self.handle, seq, first, a.size, ctypes.c_void_p(a.ctypes.data)))
+
+    def unmap(self, seq: int, first: int, n: int) -> None:
+        check(lib().q35m_paged_map(self.handle, seq, first, n, None))
+
+    def advance(self, seqs, tokens) -> None:
+        assert len(seqs) == len(tokens)
+        check(lib().q35m_paged_advance(self.handle, len(seqs), _seqs(seqs), _seqs(tokens)))
+
+    def truncate(self, seq: int, length: int) -> None:
+        check(lib().q35m_paged_truncate(self.handle, seq, length))
+
+    def length(self, seq: int) -> int:
+        n = ctypes.c_int()
+        check(lib().q35m_paged_len(self.handle, seq, ctypes.byref(n)))
+        return n.value
+
+    def device_ptr(self, layer: int, kind: int):
+        """(address, bytes) of one layer's key or value pages,
+        [n_pages][kv_heads][page_rows][256]."""
+        p = ctypes.c_void_p()
+        n = ctypes.c_size_t()
+        check(lib().q35m_paged_device_ptr(self.handle, layer, kind, ctypes.byref(p), ctypes.byref(n)))
+        return p.value, n.value
+
+    def append(self, layer, seqs, tokens, k, v) -> None:
+        """tokens[i] new rows of sequence seqs[i] from k, v [sum(tokens)][kv_heads*256]."""
+        assert len(seqs) == len(tokens)
+        check(lib().q35m_paged_append(self.handle, layer, len(seqs), _seqs(seqs), _seqs(tokens), k.ptr, v.ptr))
+
+    def attn_decode(self, layer, seqs, q_gate, k, v, out) -> None:
+        check(lib().q35m_paged_attn_decode(self.handle, layer, len(seqs), _seqs(seqs), q_gate.ptr, k.ptr, v.ptr,
+                                           out.ptr))
+
+    def attn_prefill(self, layer, seqs, tokens, q_gate, k, v, out) -> None:
+        assert len(seqs) == len(tokens)
+        check(lib().q35m_paged_attn_prefill(self.handle, layer, len(seqs), _seqs(seqs), _seqs(tokens), q_gate.ptr,
+                                            k.ptr, v.ptr, out.ptr))
 
 
 # ---- HIP event timing on the context stream ------------------------------
