@@ -13,6 +13,18 @@ __device__ __forceinline__ float silu(float x) {
     return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x));
 }
 
+// 1 / (1 + e^-x) to fp32 precision in a dozen instructions: the exponential
+// with the rounding error of its base-2 argument made good, the reciprocal
+// with one Newton step (expf and a division are 45).
+__device__ __forceinline__ float sigmoid_full(float x) {
+    const float n = __builtin_amdgcn_fmed3f(-x, -88.0f, 88.0f);    // (past it 0 and 1 in any case)
+    const float l2 = 1.44269502e+0f, l2lo = 1.92596303e-8f, ln2 = 0.693147182f;   // log2(e) as a sum, ln 2
+    const float t = n * l2, d = fmaf(n, l2lo, fmaf(n, l2, -t));
+    const float p = __builtin_amdgcn_exp2f(t), s = 1.0f + fmaf(p * ln2, d, p);
+    const float r = __builtin_amdgcn_rcpf(s);
+    return x != x ? x : fmaf(fmaf(-s, r, 1.0f), r, r);
+}
+
 // Qwen35Ops.SoftplusScalar / Log1pSafe (src/Qwen35Sharp.Model/Qwen35Ops.cs:
 // 121-142): identity above 20, exp below -10, otherwise log(1 + e^x) with a
 // 4-term Taylor series whenever e^x < 0.5.  The series is part of the

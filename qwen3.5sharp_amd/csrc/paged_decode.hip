@@ -50,10 +50,9 @@ struct Tile<float> {
     float4 k[16], v[4][4];  // K row l % 16, dims 16 t + 4 g; V row 4 g + i, dims 64 t + 4 m
     f32x4 o[16];            // dims 64 t + 4 row + c at [4 t + c]
 
-    __device__ __forceinline__ float set_q(float (&x)[64]) {
+    __device__ __forceinline__ void set_q(float (&x)[64]) {
 #pragma unroll
         for (int i = 0; i < 64; ++i) q[i] = x[i];
-        return 1.0f;
     }
     // First dim of the 4 that x[4 t ..] of set_q holds.
     static __device__ __forceinline__ int q_dim(int t, int g) { return 16 * t + 4 * g; }
@@ -130,24 +129,10 @@ struct Tile<_Float16> {
     u32x4 k[2][8], v[2][8];    // K row l % 16 of group kb, dims 32 t + 8 g; V row 16 (j / 4) + 4 g + j % 4, dims 128 u + 8 m
     f32x4 o[16];               // dims 128 u + 8 row + b at [8 u + b]
 
-    // Scales the row into fp16's range by a power of two, splits it, and
-    // returns the factor that undoes the scale.
-    __device__ __forceinline__ float set_q(float (&x)[64]) {
-        float mx = 0.0f;
+    // The row, already scaled into fp16's range, as hi + lo.
+    __device__ __forceinline__ void set_q(float (&x)[64]) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) mx = fmaxf(mx, fabsf(x[i]));
-        mx = xor16_max(xor32_max(mx));
-        const int e = 10 - max(__builtin_amdgcn_frexp_expf(mx), -100);
-        const float up = ldexpf(1.0f, e);
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float y = x[8 * t + j] * up;
-                qh[t][j] = (_Float16)y;
-                ql[t][j] = (_Float16)(y - (float)qh[t][j]);
-            }
-        return ldexpf(1.0f, -e);
+        for (int t = 0; t < 8; ++t) split16(x + 8 * t, qh[t], ql[t]);
     }
     static __device__ __forceinline__ int q_dim(int t, int g) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1); }
     static constexpr int kRopePair = 8;
@@ -203,11 +188,7 @@ struct Tile<_Float16> {
     static constexpr int kScores = 8;
     __device__ __forceinline__ void pv(const float (&p)[8]) {
         f16x8 ph, pl;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            ph[j] = (_Float16)p[j];
-            pl[j] = (_Float16)(p[j] - (float)ph[j]);
-        }
+        split16(p, ph, pl);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -276,6 +257,8 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
     __shared__ float ml[4][kPagedDecodeHeads][2];
     __shared__ __align__(16) T newrow[4][2][kHd];
 
+    const int qe = std::is_same_v<T, float> ? 0 : q_exponent(q_norm, lane);
+    const float up = ldexpf(1.0f, qe), down = ldexpf(1.0f, -qe);
     const Units un = units_of<T>(pv, b, groups, lane);
     const int per = (un.total + (int)gridDim.x - 1) / (int)gridDim.x;
     int u = blockIdx.x * per;
@@ -321,8 +304,8 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
             load_v(first, pg);
         }
 
-        // q: the rotation, the norm, the scale 1/16 (and log2 e, for exp2).
-        float down = 1.0f;
+        // q: the rotation, the norm, the scale 1/16 (and log2 e, for exp2; and a
+        // power of two for fp16).
         {
             const int h = y * hg + min(n, hg - 1);
             const float* qp = q_gate + ((size_t)i * nh + h) * 2 * kHd;
@@ -346,7 +329,7 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
 #pragma unroll
             for (int t = 0; t < 64; ++t) ss += x[t] * x[t];
             ss = xor16_sum(xor32_sum(ss));
-            const float scale = n < hg ? kLog2e / 16.0f / sqrtf(ss / (float)kHd + eps) : 0.0f;
+            const float scale = n < hg ? up * (kLog2e / 16.0f) / sqrtf(ss / (float)kHd + eps) : 0.0f;
 #pragma unroll
             for (int t = 0; t < 16; ++t) {
                 const float4 w = *reinterpret_cast<const float4*>(q_norm + Tl::q_dim(t, g));
@@ -355,7 +338,7 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
                 x[4 * t + 2] *= scale * (1.0f + w.z);
                 x[4 * t + 3] *= scale * (1.0f + w.w);
             }
-            down = tl.set_q(x);
+            tl.set_q(x);
         }
 
         // The wave that holds the new row makes it (every head group needs it;
@@ -434,7 +417,7 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
             if (whole) {
                 const size_t row = (size_t)i * nh + y * hg + h;
                 const float gate = q_gate[row * 2 * kHd + kHd + tid];
-                out[row * kHd + tid] = o / l * (1.0f / (1.0f + expf(-gate)));
+                out[row * kHd + tid] = o / l * sigmoid_full(gate);
             } else {
                 const size_t at = (size_t)slot * kPagedDecodeHeads + h;
                 part_o[at * kHd + tid] = o;
@@ -508,12 +491,7 @@ __global__ __launch_bounds__(MW * kWave) void paged_decode_merge(PagedView pv, P
             l += lbuf[w];
         }
         const float inv = 1.0f / l;
-        float4 r;
-        r.x = o.x * inv * (1.0f / (1.0f + expf(-gate.x)));
-        r.y = o.y * inv * (1.0f / (1.0f + expf(-gate.y)));
-        r.z = o.z * inv * (1.0f / (1.0f + expf(-gate.z)));
-        r.w = o.w * inv * (1.0f / (1.0f + expf(-gate.w)));
-        *reinterpret_cast<float4*>(out + row * kHd + 4 * lane) = r;
+        *reinterpret_cast<float4*>(out + row * kHd + 4 * lane) = gated(make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), gate);
     }
 }
 

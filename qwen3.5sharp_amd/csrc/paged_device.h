@@ -73,6 +73,48 @@ __device__ __forceinline__ float4 paged_key_row(float4 x, const double* __restri
     return r;
 }
 
+// Exponent e such that every value of a normed q row, times log2(e) / 16 and
+// 2^e, is below 2^15: its fp16 halves are in range whatever the norm weights,
+// and values 2^-10 of the largest keep all 22 bits.  |q_d| <= 16 |1 + w_d|.
+__device__ __forceinline__ int q_exponent(const float* __restrict__ w, int lane) {
+    const float4 a = *reinterpret_cast<const float4*>(w + 4 * lane);
+    const float m = fmaxf(fmaxf(fabsf(1.0f + a.x), fabsf(1.0f + a.y)), fmaxf(fabsf(1.0f + a.z), fabsf(1.0f + a.w)));
+    const int e = __builtin_amdgcn_frexp_expf(1.4426951f * wave_max(m));
+    return 15 - __builtin_amdgcn_readfirstlane(max(min(e, 100), -100));
+}
+
+// (a, b) = hi + lo to 22 bits each: one conversion of the pair and a fused
+// multiply-add for each remainder (a - hi, exact, rounded to fp16).  hi is made a
+// value of its own before it is used: where a is a product, the compiler would
+// otherwise round it to fp16 in one step for one use and in two for another,
+// which differ by an fp16 step now and then.
+__device__ __forceinline__ void split16(float a, float b, f16x2& hi, f16x2& lo) {
+    uint32_t x = __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b}), y;
+    asm("" : "+v"(x));
+    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\t"
+        "v_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=&v"(y)
+        : "v"(x), "v"(a), "v"(b));
+    hi = __builtin_bit_cast(f16x2, x);
+    lo = __builtin_bit_cast(f16x2, y);
+}
+// Eight values, as one operand each.
+__device__ __forceinline__ void split16(const float* y, f16x8& hi, f16x8& lo) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        f16x2 h, l;
+        split16(y[j], y[j + 1], h, l);
+        hi[j] = h.x; hi[j + 1] = h.y;
+        lo[j] = l.x; lo[j + 1] = l.y;
+    }
+}
+
+// x times the output gate's sigmoid.
+__device__ __forceinline__ float4 gated(float4 x, float4 gate) {
+    return make_float4(x.x * sigmoid_full(gate.x), x.y * sigmoid_full(gate.y), x.z * sigmoid_full(gate.z),
+                       x.w * sigmoid_full(gate.w));
+}
+
 // Four values rounded to the cache's type, stored as one vector.
 __device__ __forceinline__ void store_row4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ void store_row4(_Float16* p, float4 v) {

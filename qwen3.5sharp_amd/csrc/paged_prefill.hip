@@ -71,6 +71,12 @@ __device__ __forceinline__ long readlane_long(long v, int i) {
     return ((long)hi << 32) | (unsigned)lo;
 }
 
+// A value that is the same in every lane, as one the compiler knows to be.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long uniform(long v) {
+    return ((long)uniform((int)(v >> 32)) << 32) | (unsigned)uniform((int)(unsigned)v);
+}
+
 // Lane i: the units of the call's sequences up to and with the i-th.
 struct Units {
     int start;
@@ -102,7 +108,7 @@ struct Walk {
     int o, n;
 
     __device__ __forceinline__ void begin(const Units& un, int wg, int nwg) {
-        const long per = (un.total + nwg - 1) / nwg;
+        const long per = uniform((un.total + nwg - 1) / nwg);
         u = wg * per;
         u_end = min(u + per, un.total);
         i = -1;
@@ -115,7 +121,7 @@ struct Walk {
             ++o;
             within = 0;
         } else {
-            i = __popcll(__ballot(un.end <= u));
+            i = uniform((int)__popcll(__ballot(un.end <= u)));
             start = __builtin_amdgcn_readlane(un.start, i);
             tokens = b.off[i + 1] - b.off[i];
             const Tiles ts(start, tokens, hg_shift);
@@ -134,22 +140,30 @@ struct Walk {
             within = rest - ts.ordered(o);
         }
         const Tiles ts(start, tokens, hg_shift);
+        y = uniform(y);
+        o = uniform(o);
+        n = uniform(n);
         j = ts.tile(o);
-        tiles = (int)ts.cnt(j);
-        t0 = (int)within;
-        t1 = (int)min((long)tiles, within + (u_end - u));
-        u += t1 - t0;
+        tiles = uniform((int)ts.cnt(j));
+        t0 = uniform((int)within);
+        t1 = uniform((int)min((long)tiles, within + (u_end - u)));
+        u = uniform(u + t1 - t0);
         return true;
     }
 };
 
 // ---- fp16 cache -----------------------------------------------------------
 
-// 16 bytes a lane from global memory straight to LDS at lds + 16 lane.
-__device__ __forceinline__ void dma16(const void* p, void* lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
-                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+// 16 bytes a lane from global memory straight to LDS at address at + 16 lane (at
+// the same in every lane).  Complete once vmcnt says so: dma_wait() before the
+// barrier that publishes the rows.  The instruction is written out because the
+// compiler, told of it, waits for all such loads before the next LDS read, also
+// one of the other buffer.
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const lds_void*)p; }
+__device__ __forceinline__ void dma16(const void* p, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
 }
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // V rows of a unit that not every query row of the tile sees.  Rows past the
 // tile's last row hold anything and become zeros; a value that is not finite
@@ -194,256 +208,265 @@ __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, 
     }
 }
 
-// Four waves, one a SIMD: wave (rg, kh) takes query rows 32 rg .. and, of each
-// unit, cache rows 32 kh ..; the two halves of a row meet at the segment's end.
-// 32 x 32 x 16 instructions on fp16 with the fp32 operands q (in registers for
-// the whole segment, its row scaled by a power of two) and P as two fp16 values
-// each: hi + lo, 22 bits, two products an operand pair.  K and V units are
-// double-buffered in LDS by loads that bypass the registers; K's 16-byte chunks
-// are permuted by row (chunk ^ row % 16) so that the 32 rows a read touches
-// fall into different banks, V rows are read whole and transposed in registers
-// (8 rows x 8 dims a lane).
-__global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
+// Four waves, two workgroups a CU: one computes while the other's rows arrive or
+// its exponentials run.  Wave (rg, half) has query rows 32 rg .. and half of the
+// 256 dims: it forms the scores' sums over its dims, exchanges them with its
+// partner through LDS, takes the exponentials of all 32 cache rows of a step
+// (both partners the same ones) and adds to its dims of the output.  So a wave
+// holds half of a row's q (64 registers) and half of its output (64), two waves
+// fit a SIMD, and each K and V value is read from LDS by two waves.
+// 32 x 32 x 16 instructions on fp16 with the fp32 operands q and P as two fp16
+// values each: hi + lo, 22 bits, two products an operand pair.  K and V steps of
+// 32 rows come to LDS by loads that bypass the registers, K once the step's
+// scores are formed, V into a second buffer.  K's 16-byte chunks are permuted by
+// row (chunk ^ row % 16) so that the 32 rows a read touches fall into different
+// banks; V rows are read as they are and transposed in registers (8 rows x 4
+// dims a lane).  q rows come, and output rows go, through LDS too, a row a wave
+// at a time (32 rows an instruction took 10 us a tile).
+constexpr int kStep = 32;                 // cache rows of a step
+
+__global__ __launch_bounds__(NT, 2) void paged_prefill_f16(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
                                                            const float* __restrict__ q_norm, float* __restrict__ out,
                                                            float* __restrict__ part_o, float* __restrict__ part_ml,
                                                            int hg_shift, int ng, float eps) {
-    __shared__ __align__(16) _Float16 ks[2][kUnit][kHd], vs[2][kUnit][kHd];
-    __shared__ float mls[4][32][2];
+    // One block of 64 KiB: K and V of the steps and the exchanged scores, or the
+    // tile's 64 rows of q or of the output.
+    struct Steps {
+        _Float16 k[kStep][kHd], v[2][kStep][kHd];
+        float4 x[4][4][kWave];
+    };
+    __shared__ __align__(16) char smem[sizeof(Steps)];
+    static_assert(sizeof(Steps) == kPagedTileRows * kHd * sizeof(float), "the rows take the block's place");
     __shared__ uint32_t poison[kPagedTileRows][kHd / 32];
+    Steps& st = *reinterpret_cast<Steps*>(smem);
+    float4* const tile = reinterpret_cast<float4*>(smem);         // [64][64] 16-byte chunks, chunk ^ row % 32
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rg = wave & 1, kh = wave >> 1;
+    const int rg = wave & 1, half = wave >> 1;
     const int nn = lane & 31, h = lane >> 5;
     const int hg = 1 << hg_shift, tm = kPagedTileRows >> hg_shift;
     const int groups = pv.nkv * ng, nh = groups << hg_shift;
+    const int wg = xcd_remap(blockIdx.x, gridDim.x);      // neighbours, which share K and V, on one XCD's L2
+    const uint32_t kaddr = lds_address(&st.k[8 * wave][0]), vaddr = lds_address(&st.v[0][8 * wave][0]);
 
+    const int qe = q_exponent(q_norm, lane);
+    const float up = ldexpf(1.0f, qe), down = ldexpf(1.0f, -qe);
     const Units un = units_of(pv, b, groups, hg_shift, lane);
     Walk wk;
-    wk.begin(un, blockIdx.x, gridDim.x);
+    wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
         const int seq = b.seq[wk.i], kvh = wk.y / ng;
         const int* table = pv.table + (size_t)seq * pv.max_pages;
         // Rows the tile's tokens see: [0, rows); the lane's query row sees [0, mine].
         const int rows = min(wk.start + min((wk.j + 1) * tm, wk.tokens), pv.max_rows);
-        const int tok = min(wk.j * tm + ((rg * 32 + nn) >> hg_shift), wk.tokens - 1);
-        const int mine = min(wk.start + tok, pv.max_rows - 1);
-        const int head = (wk.y << hg_shift) + ((rg * 32 + nn) & (hg - 1));
-        const bool real = wk.j * tm + ((rg * 32 + nn) >> hg_shift) < wk.tokens;
-        const size_t qrow = (size_t)(b.off[wk.i] + tok) * nh + head;
-        const int last16 = (rows - 1) & ~15;
-
-        // A wave brings its 16 rows of a unit's K and V.
-        auto issue = [&](int t, int buf) {
-            const int r = min(t * kUnit + 16 * wave, last16);
-            const int page = page_of(table, r >> pv.page_shift, pv.max_pages, pv.n_pages);
-            const size_t at = row_offset<_Float16>(pv, page, kvh, r);
-            const _Float16* kp = (const _Float16*)pv.k + at + (lane >> 5) * kHd;
-            const _Float16* vp = (const _Float16*)pv.v + at + 8 * lane;
-            const int c0 = (lane & 31) ^ (lane >> 5);
-#pragma unroll
-            for (int r2 = 0; r2 < 8; ++r2) dma16(kp + 2 * r2 * kHd + 8 * (c0 ^ (2 * r2)), &ks[buf][16 * wave + 2 * r2][0]);
-#pragma unroll
-            for (int r2 = 0; r2 < 8; ++r2) dma16(vp + 2 * r2 * kHd, &vs[buf][16 * wave + 2 * r2][0]);
+        const int stop = min(rows, wk.t1 * kUnit), last16 = (rows - 1) & ~15;
+        const int first = wk.start + wk.j * tm;            // position of the tile's first token
+        // Query row r of the tile: token, and the row of q and out.
+        auto token = [&](int r) { return wk.j * tm + (r >> hg_shift); };
+        auto row_at = [&](int r) {
+            return (size_t)(b.off[wk.i] + min(token(r), wk.tokens - 1)) * nh + (wk.y << hg_shift) + (r & (hg - 1));
         };
-        issue(wk.t0, 0);
+        const int mine = min(wk.start + min(token(32 * rg + nn), wk.tokens - 1), pv.max_rows - 1);
+
+        // q rows to LDS.
+#pragma unroll 4
+        for (int r = 16 * wave; r < 16 * wave + 16; ++r)
+            dma16(q_gate + row_at(r) * 2 * kHd + 4 * (lane ^ (r & 31)), lds_address(tile + r * (kHd / 4)));
         for (int x = tid; x < kPagedTileRows * (kHd / 32); x += NT) (&poison[0][0])[x] = 0;
 
-        // q: lane (row nn, h) holds dims 16 s + 8 h + j of its row.
-        f16x8 qh[16], ql[16];
-        float down;
+        // A wave brings 8 rows of a step's K and V.  It holds 64 entries of the page
+        // table, one a lane, from entry `held` on.
+        int held = 0, ids = 0;
+        auto hold = [&](int entry) {
+            held = entry;
+            ids = page_of(table, entry + lane, pv.max_pages, pv.n_pages);
+        };
+        auto row8 = [&](int base) { return min(base + 8 * wave, last16 + (8 * wave & 8)); };
+        hold(row8(wk.t0 * kUnit) >> pv.page_shift);
+        auto issue = [&](int base, int par) {
+            const int r = row8(base), entry = r >> pv.page_shift;
+            if (__builtin_expect(entry - held >= kWave, 0)) hold(entry);
+            const size_t at = row_offset<_Float16>(pv, __builtin_amdgcn_readlane(ids, entry - held), kvh, r);
+            const _Float16* kp = (const _Float16*)pv.k + at + h * kHd;
+            const _Float16* vp = (const _Float16*)pv.v + at + 8 * lane;
+            const int c0 = (lane & 31) ^ h ^ (8 * (wave & 1));
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) dma16(kp + k * kHd + 8 * (c0 ^ k), kaddr + (uint32_t)(k * kHd * 2));
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) dma16(vp + k * kHd, vaddr + (uint32_t)((par * kStep + k) * kHd * 2));
+        };
+
+        // q: lane (row nn, h) holds dims 128 half + 16 s + 8 h + j of its row: norm
+        // (which the rotation leaves), then rotation, scale and the two halves.
+        f16x8 qh[8], ql[8];
         {
-            const float* qp = q_gate + qrow * 2 * kHd + 8 * h;
+            auto dims8 = [&](int c, float (&x)[8]) {       // chunks c, c + 1 of the lane's row
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float4 a = tile[(32 * rg + nn) * (kHd / 4) + ((c + k) ^ nn)];
+                    x[4 * k] = a.x; x[4 * k + 1] = a.y; x[4 * k + 2] = a.z; x[4 * k + 3] = a.w;
+                }
+            };
+            dma_wait();
+            __syncthreads();
+            float ss = 0.0f;
+#pragma unroll 4
+            for (int s = 0; s < 16; ++s) {
+                float x[8];
+                dims8(4 * s + 2 * h, x);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) ss += x[c] * x[c];
+            }
+            const float scale = up * (kLog2e / 16.0f) / sqrtf(xor32_sum(ss) / (float)kHd + eps);
             const double* rope = pv.rope + (size_t)mine * kRopeDim + 8 * h;
-            float x[128], ss = 0.0f;
 #pragma unroll
-            for (int s = 0; s < 16; ++s)
+            for (int s = 0; s < 8; ++s) {
+                float x[8], y[8];
+                dims8(32 * half + 4 * s + 2 * h, x);
+                if (half == 0 && s < 4) {                  // dims 16 (s % 2) + 8 h .. and 32 further
+                    dims8(4 * (s ^ 2) + 2 * h, y);
 #pragma unroll
-                for (int c = 0; c < 8; c += 4) {
-                    const float4 a = *reinterpret_cast<const float4*>(qp + 16 * s + c);
-                    x[8 * s + c] = a.x; x[8 * s + c + 1] = a.y; x[8 * s + c + 2] = a.z; x[8 * s + c + 3] = a.w;
+                    for (int c = 0; c < 8; ++c) {
+                        const float cs = (float)rope[16 * (s & 1) + c], sn = (float)rope[kRopeHalf + 16 * (s & 1) + c];
+                        x[c] = s < 2 ? x[c] * cs - y[c] * sn : y[c] * sn + x[c] * cs;
+                    }
                 }
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float cs = (float)rope[16 * s + c], sn = (float)rope[kRopeHalf + 16 * s + c];
-                    const float lo = x[8 * s + c], hi = x[8 * s + 16 + c];
-                    x[8 * s + c] = lo * cs - hi * sn;
-                    x[8 * s + 16 + c] = lo * sn + hi * cs;
-                }
-#pragma unroll
-            for (int k = 0; k < 128; ++k) ss += x[k] * x[k];
-            const float scale = kLog2e / 16.0f / sqrtf(xor32_sum(ss) / (float)kHd + eps);
-            float mx = 0.0f;
-#pragma unroll
-            for (int s = 0; s < 16; ++s)
-#pragma unroll
-                for (int c = 0; c < 8; c += 4) {
-                    const float4 w = *reinterpret_cast<const float4*>(q_norm + 16 * s + 8 * h + c);
-                    x[8 * s + c] *= scale * (1.0f + w.x);
-                    x[8 * s + c + 1] *= scale * (1.0f + w.y);
-                    x[8 * s + c + 2] *= scale * (1.0f + w.z);
-                    x[8 * s + c + 3] *= scale * (1.0f + w.w);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mx = fmaxf(mx, fabsf(x[8 * s + c + k]));
-                }
-            const int e = 10 - max(__builtin_amdgcn_frexp_expf(xor32_max(mx)), -100);
-            const float up = ldexpf(1.0f, e);
-            down = ldexpf(1.0f, -e);
-#pragma unroll
-            for (int s = 0; s < 16; ++s)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const float y = x[8 * s + c] * up;
-                    qh[s][c] = (_Float16)y;
-                    ql[s][c] = (_Float16)(y - (float)qh[s][c]);
-                }
+                for (int c = 0; c < 8; ++c) y[c] = x[c] * (scale * (1.0f + q_norm[128 * half + 16 * s + 8 * h + c]));
+                split16(y, qh[s], ql[s]);
+            }
         }
 
-        f32x16 o[8];
+        f32x16 o[4];                                       // dims 128 half + 4 row + d at [d]
 #pragma unroll
-        for (int d = 0; d < 8; ++d)
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int k = 0; k < 16; ++k) o[d][k] = 0.0f;
         float m_run = -INFINITY, l_run = 0.0f;
 
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        for (int t = wk.t0; t < wk.t1; ++t) {
-            const int buf = (t - wk.t0) & 1;
-            if (t + 1 < wk.t1) issue(t + 1, buf ^ 1);
-            const int base = t * kUnit + 32 * kh;          // the wave's 32 rows
-            // Some row of the tile does not see some row of the unit.
-            const bool masked = t * kUnit + kUnit - 1 > wk.start + wk.j * tm;
-            if (masked) {
-                guard_rows(&vs[buf][16 * wave][0], 16, t * kUnit + 16 * wave, rows, poison, wk.start + wk.j * tm,
-                           wk.tokens - wk.j * tm, hg_shift, lane);
-                lds_barrier();
-            }
-            const _Float16* kt = &ks[buf][32 * kh + nn][0];
-            const int sw = (h ^ (nn & 15)) * 8;
+        __syncthreads();                                   // q is read
+        int par = 0;
+        if (wk.t0 * kUnit < stop) issue(wk.t0 * kUnit, 0);
+        for (int base = wk.t0 * kUnit; base < stop; base += kStep) {
+            dma_wait();
+            __syncthreads();                               // the step's rows are there, the last one's V and scores read
+            // Some row of the tile does not see some row of the step.
+            const bool masked = base + kStep - 1 > first;
+            if (masked)
+                guard_rows(&st.v[par][8 * wave][0], 8, base + 8 * wave, rows, poison, first, wk.tokens - wk.j * tm,
+                           hg_shift, lane);
             f32x16 sc;
 #pragma unroll
             for (int k = 0; k < 16; ++k) sc[k] = 0.0f;
 #pragma unroll
-            for (int s = 0; s < 16; ++s) {
-                const f16x8 a = *reinterpret_cast<const f16x8*>(kt + (sw ^ (16 * s)));
+            for (int s = 0; s < 8; ++s) {                  // K operand: lane (row nn, h), dims 128 half + 16 s + 8 h ..
+                const f16x8 a = *reinterpret_cast<const f16x8*>(&st.k[nn][8 * ((16 * half + 2 * s + h) ^ (nn & 15))]);
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[s], sc, 0, 0, 0);
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[s], sc, 0, 0, 0);
             }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) st.x[wave][k][lane] = make_float4(sc[4 * k], sc[4 * k + 1], sc[4 * k + 2], sc[4 * k + 3]);
+            lds_barrier();                                 // the scores are there, K is read
+            if (base + kStep < stop) issue(base + kStep, par ^ 1);
             float mx = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) sc[k] *= down;
+            for (int k = 0; k < 4; ++k) {
+                const float4 y = st.x[wave ^ 2][k][lane];
+                sc[4 * k] += y.x; sc[4 * k + 1] += y.y; sc[4 * k + 2] += y.z; sc[4 * k + 3] += y.w;
+            }
             if (masked) {
+                asm volatile("");                          // a branch: selects on every step cost more
                 const int lim = mine - base - 4 * h;
 #pragma unroll
                 for (int k = 0; k < 16; ++k) sc[k] = 8 * (k >> 2) + (k & 3) <= lim ? sc[k] : -INFINITY;
             }
 #pragma unroll
             for (int k = 0; k < 16; ++k) mx = fmaxf(mx, sc[k]);
-            mx = xor32_max(mx);
+            mx = xor32_max(mx * down);
             if (__any(mx > m_run + kLazy)) {               // (m_run is -inf at first)
                 const float m_new = fmaxf(m_run, mx);
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
                 m_run = m_new;
                 l_run *= alpha;
 #pragma unroll
-                for (int d = 0; d < 8; ++d) o[d] *= alpha;
+                for (int d = 0; d < 4; ++d) o[d] *= alpha;
             }
-            const float sub = (m_run == -INFINITY ? 0.0f : m_run) - kPShift;
+            const float sub = kPShift - (m_run == -INFINITY ? 0.0f : m_run);
             f16x8 ph[2], pl[2];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float p = __builtin_amdgcn_exp2f(sc[k] - sub);
-                l_run += p;
-                ph[k >> 3][k & 7] = (_Float16)p;
-                pl[k >> 3][k & 7] = (_Float16)(p - (float)ph[k >> 3][k & 7]);
+            for (int c = 0; c < 2; ++c) {
+                float p[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    p[k] = __builtin_amdgcn_exp2f(fmaf(sc[8 * c + k], down, sub));
+                    l_run += p[k];
+                }
+                split16(p, ph[c], pl[c]);
             }
-            // V rows 16 c + 4 h + {0..3, 8..11}: P's rows of the lane's half.
-            const _Float16* vt = &vs[buf][32 * kh + 4 * h][8 * nn];
-            u32x4 vr[2][8];
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c) {
+                // V rows 16 c + 4 h + {0..3, 8..11}: the weights' rows of the lane's half.
+                const _Float16* vt = &st.v[par][16 * c + 4 * h][128 * half + 4 * nn];
+                uint2 v8[8];
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    vr[c][r] = *reinterpret_cast<const u32x4*>(vt + (16 * c + (r & 3) + 8 * (r >> 2)) * kHd);
-            auto v_operand = [](const u32x4 (&v8)[8], int d) {      // dims 8 m + d of the lane's 8 rows
-                const uint32_t sel = (d & 1) ? 0x07060302u : 0x05040100u;
-                u32x4 a;
+                for (int r = 0; r < 8; ++r) v8[r] = *reinterpret_cast<const uint2*>(vt + ((r & 3) + 8 * (r >> 2)) * kHd);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) a[w] = __builtin_amdgcn_perm(v8[2 * w + 1][d >> 1], v8[2 * w][d >> 1], sel);
-                return __builtin_bit_cast(f16x8, a);
-            };
+                for (int d = 0; d < 4; ++d) {              // dims 4 m + d of the lane's 8 rows
+                    const uint32_t sel = (d & 1) ? 0x07060302u : 0x05040100u;
+                    u32x4 a;
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    const f16x8 av = v_operand(vr[c], d);
+                    for (int w = 0; w < 4; ++w)
+                        a[w] = d < 2 ? __builtin_amdgcn_perm(v8[2 * w + 1].x, v8[2 * w].x, sel)
+                                     : __builtin_amdgcn_perm(v8[2 * w + 1].y, v8[2 * w].y, sel);
+                    const f16x8 av = __builtin_bit_cast(f16x8, a);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pl[c], o[d], 0, 0, 0);
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ph[c], o[d], 0, 0, 0);
                 }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
+            }
+            par ^= 1;
         }
 
-        // The two halves of the cache rows join: each wave finishes half of its
-        // rows' dims and hands over the other half (in the K and V buffers).
+        // The tile's rows to LDS, then a row a wave at a time: finished, or as a part
+        // to the workspace.  Both partners have the rows' sums.
+        const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
+        const int slot = 2 * wg + (wk.t0 == 0);
         l_run = xor32_sum(l_run);
-        float4* ex = reinterpret_cast<float4*>(&ks[0][0][0]);
-        if (h == 0) {
-            mls[wave][nn][0] = m_run;
-            mls[wave][nn][1] = l_run;
+        const float inv = whole ? 1.0f / l_run : 1.0f;
+        __syncthreads();                                   // V and the scores are read
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const int chunk = 32 * half + 8 * (k >> 2) + 4 * h + (k & 3);
+            tile[(32 * rg + nn) * (kHd / 4) + (chunk ^ nn)] =
+                make_float4(o[0][k] * inv, o[1][k] * inv, o[2][k] * inv, o[3][k] * inv);
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            float x[8];
-#pragma unroll
-            for (int d = 0; d < 8; ++d) x[d] = kh == 0 ? o[d][8 + k] : o[d][k];
-            ex[(wave * 16 + 2 * k) * 64 + lane] = make_float4(x[0], x[1], x[2], x[3]);
-            ex[(wave * 16 + 2 * k + 1) * 64 + lane] = make_float4(x[4], x[5], x[6], x[7]);
+        if (!whole && half == 0 && h == 0) {
+            const size_t r = (size_t)slot * kPagedTileRows + 32 * rg + nn;
+            part_ml[2 * r] = m_run;
+            part_ml[2 * r + 1] = l_run;
         }
         __syncthreads();
-        const int other = wave ^ 2;
-        const float m2 = mls[other][nn][0], l2 = mls[other][nn][1];
-        const float M = fmaxf(m_run, m2), mu = M == -INFINITY ? 0.0f : M;
-        const float e1 = __builtin_amdgcn_exp2f(m_run - mu), e2 = __builtin_amdgcn_exp2f(m2 - mu);
-        const float l = l_run * e1 + l2 * e2;
-        const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
-        const int slot = 2 * blockIdx.x + (wk.t0 == 0);
-        const float inv = 1.0f / l;
-        float* po = part_o + ((size_t)slot * kPagedTileRows + 32 * rg + nn) * kHd;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float4 a = ex[(other * 16 + 2 * k) * 64 + lane], c = ex[(other * 16 + 2 * k + 1) * 64 + lane];
-            const float y[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
-            float x[8];
-#pragma unroll
-            for (int d = 0; d < 8; ++d) x[d] = (kh == 0 ? o[d][k] : o[d][8 + k]) * e1 + y[d] * e2;
-            const int at = 8 * (16 * kh + 8 * (k >> 2) + 4 * h + (k & 3));
-            const uint32_t nan = poison[32 * rg + nn][at >> 5] >> (at & 31);
-#pragma unroll
-            for (int d = 0; d < 8; ++d) x[d] = (nan >> d) & 1 ? NAN : x[d];
+        for (int k0 = 0; k0 < 16; k0 += 8) {
+            float4 gate[8];
             if (whole) {
-                if (real) {
-                    const float* gp = q_gate + qrow * 2 * kHd + kHd + at;
-                    float* dst = out + qrow * kHd + at;
 #pragma unroll
-                    for (int d = 0; d < 8; d += 4) {
-                        const float4 gt = *reinterpret_cast<const float4*>(gp + d);
-                        *reinterpret_cast<float4*>(dst + d) =
-                            make_float4(x[d] * inv * (1.0f / (1.0f + expf(-gt.x))), x[d + 1] * inv * (1.0f / (1.0f + expf(-gt.y))),
-                                        x[d + 2] * inv * (1.0f / (1.0f + expf(-gt.z))), x[d + 3] * inv * (1.0f / (1.0f + expf(-gt.w))));
-                    }
-                }
-            } else {
-                *reinterpret_cast<float4*>(po + at) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4*>(po + at + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                for (int k = 0; k < 8; ++k)
+                    gate[k] = *reinterpret_cast<const float4*>(q_gate + row_at(16 * wave + k0 + k) * 2 * kHd + kHd + 4 * lane);
             }
-        }
-        if (!whole && kh == 0 && h == 0) {
-            const size_t r = (size_t)slot * kPagedTileRows + 32 * rg + nn;
-            part_ml[2 * r] = M;
-            part_ml[2 * r + 1] = l;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int r = 16 * wave + k0 + k;
+                float4 x = tile[r * (kHd / 4) + (lane ^ (r & 31))];
+                const uint32_t nan = poison[r][lane >> 3] >> (4 * (lane & 7));
+                x.x = nan & 1 ? NAN : x.x;
+                x.y = nan & 2 ? NAN : x.y;
+                x.z = nan & 4 ? NAN : x.z;
+                x.w = nan & 8 ? NAN : x.w;
+                if (!whole)
+                    *reinterpret_cast<float4*>(part_o + ((size_t)slot * kPagedTileRows + r) * kHd + 4 * lane) = x;
+                else if (token(r) < wk.tokens)
+                    *reinterpret_cast<float4*>(out + row_at(r) * kHd + 4 * lane) = gated(x, gate[k]);
+            }
         }
         __syncthreads();
     }
@@ -467,10 +490,13 @@ __global__ __launch_bounds__(NT, 2) void paged_prefill_f32(PagedView pv, PagedBa
     const int n = lane & 15, g = lane >> 4;
     const int hg = 1 << hg_shift, tm = kPagedTileRows >> hg_shift;
     const int groups = pv.nkv * ng, nh = groups << hg_shift;
+    const int wg = xcd_remap(blockIdx.x, gridDim.x);
+
+    const uint32_t kaddr = lds_address(&ks[8 * wave][0]), vaddr = lds_address(&vs[8 * wave][0]);
 
     const Units un = units_of(pv, b, groups, hg_shift, lane);
     Walk wk;
-    wk.begin(un, blockIdx.x, gridDim.x);
+    wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
         const int seq = b.seq[wk.i], kvh = wk.y / ng;
         const int* table = pv.table + (size_t)seq * pv.max_pages;
@@ -533,11 +559,11 @@ __global__ __launch_bounds__(NT, 2) void paged_prefill_f32(PagedView pv, PagedBa
                 const size_t at = row_offset<float>(pv, page, kvh, r);
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    dma16((const float*)pv.k + at + k * kHd + 4 * (lane ^ ((8 * wave + k) & 15)), &ks[8 * wave + k][0]);
+                    dma16((const float*)pv.k + at + k * kHd + 4 * (lane ^ ((8 * wave + k) & 15)), kaddr + k * kHd * 4);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) dma16((const float*)pv.v + at + k * kHd + 4 * lane, &vs[8 * wave + k][0]);
+                for (int k = 0; k < 8; ++k) dma16((const float*)pv.v + at + k * kHd + 4 * lane, vaddr + k * kHd * 4);
             }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            dma_wait();
             __syncthreads();
             const bool masked = base + kF32Rows - 1 > wk.start + wk.j * tm;
             if (masked) {
@@ -594,7 +620,7 @@ __global__ __launch_bounds__(NT, 2) void paged_prefill_f32(PagedView pv, PagedBa
 
         l_run = xor16_sum(xor32_sum(l_run));
         const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
-        const int slot = 2 * blockIdx.x + (wk.t0 == 0);
+        const int slot = 2 * wg + (wk.t0 == 0);
         const size_t prow = (size_t)slot * kPagedTileRows + 16 * wave + n;
         const float inv = 1.0f / l_run;
 #pragma unroll
@@ -612,11 +638,8 @@ __global__ __launch_bounds__(NT, 2) void paged_prefill_f32(PagedView pv, PagedBa
                     *reinterpret_cast<float4*>(part_o + prow * kHd + at) = x;
                 } else if (real) {
                     const float4 gt = *reinterpret_cast<const float4*>(q_gate + qrow * 2 * kHd + kHd + at);
-                    x.x *= inv * (1.0f / (1.0f + expf(-gt.x)));
-                    x.y *= inv * (1.0f / (1.0f + expf(-gt.y)));
-                    x.z *= inv * (1.0f / (1.0f + expf(-gt.z)));
-                    x.w *= inv * (1.0f / (1.0f + expf(-gt.w)));
-                    *reinterpret_cast<float4*>(out + qrow * kHd + at) = x;
+                    *reinterpret_cast<float4*>(out + qrow * kHd + at) =
+                        gated(make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), gt);
                 }
             }
         if (!whole && g == 0) {
@@ -690,27 +713,25 @@ __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBat
             }
         }
         const float inv = 1.0f / l;
-        x.x *= inv * (1.0f / (1.0f + expf(-gt.x)));
-        x.y *= inv * (1.0f / (1.0f + expf(-gt.y)));
-        x.z *= inv * (1.0f / (1.0f + expf(-gt.z)));
-        x.w *= inv * (1.0f / (1.0f + expf(-gt.w)));
-        *reinterpret_cast<float4*>(out + qrow * kHd + 4 * lane) = x;
+        *reinterpret_cast<float4*>(out + qrow * kHd + 4 * lane) =
+            gated(make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), gt);
     }
 }
 
-int prefill_workgroups(const q35m_ctx* c, int type) { return type == Q35M_KV_F16 ? c->n_cu : 2 * c->n_cu; }
+// Two workgroups a CU.
+int prefill_workgroups(const q35m_ctx* c) { return 2 * c->n_cu; }
 
 }  // namespace
 
 size_t paged_prefill_work_bytes(const q35m_ctx* c) {
-    return (size_t)2 * prefill_workgroups(c, Q35M_KV_F32) * kPagedTileRows * (kHd + 2) * sizeof(float);
+    return (size_t)2 * prefill_workgroups(c) * kPagedTileRows * (kHd + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, float* out) {
     q35m_ctx* c = p->ctx;
     const int per_kv = c->d.nh / c->d.nkv;
     const int hg = per_kv <= 16 ? per_kv : per_kv % 16 == 0 ? 16 : 8;
-    const int ng = per_kv / hg, nwg = prefill_workgroups(c, p->type), tm = kPagedTileRows / hg;
+    const int ng = per_kv / hg, nwg = prefill_workgroups(c), tm = kPagedTileRows / hg;
     int hg_shift = 0;
     while ((1 << hg_shift) < hg) ++hg_shift;
     float* part_o = p->work;
