@@ -30,7 +30,6 @@ namespace {
 constexpr int NT = 256;
 constexpr int kUnit = 64;               // cache rows of a unit
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kPShift = 7.0f;         // P = e^{s - m} 2^7: see paged_decode.hip
 constexpr float kLazy = 8.0f;           // log2 of how far a score may pass the running maximum before it moves
 
 // ---- the units of a call ------------------------------------------------
@@ -175,7 +174,8 @@ __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINI
 __device__ __forceinline__ bool not_finite(_Float16 x) {
     return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
 }
-template <typename T>
+// 16-byte chunks are permuted by row: chunk ^ S (row % 4).
+template <int S, typename T>
 __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, uint32_t (*poison)[kHd / 32], int first,
                                            int tokens_left, int hg_shift, int lane) {
     constexpr int E = 16 / sizeof(T);          // values of 16 bytes
@@ -193,7 +193,7 @@ __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, 
             for (int k = 0; k < E; ++k) {
                 const T one = v[x * E + k];
                 if (!not_finite(one)) continue;
-                const int d = (x % (kHd / E)) * E + k;
+                const int d = (x % (kHd / E) ^ (S * (r & 3))) * E + k;
                 // query row q: token min(q >> hg_shift, tokens_left - 1) of the tile, at first + that
 #pragma nounroll
                 for (int q = 0; q < kPagedTileRows; ++q)
@@ -208,264 +208,483 @@ __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, 
     }
 }
 
-// Four waves, two workgroups a CU: one computes while the other's rows arrive or
-// its exponentials run.  Wave (rg, half) has query rows 32 rg .. and half of the
-// 256 dims: it forms the scores' sums over its dims, exchanges them with its
-// partner through LDS, takes the exponentials of all 32 cache rows of a step
-// (both partners the same ones) and adds to its dims of the output.  So a wave
-// holds half of a row's q (64 registers) and half of its output (64), two waves
-// fit a SIMD, and each K and V value is read from LDS by two waves.
+// Four waves, one a SIMD.  Wave (rg, half) has query rows 32 rg ..: it forms the
+// scores and weights of the unit's cache rows 32 half .., hands its weights to
+// its partner through LDS, and adds all 64 rows' values to output dims 128 half
+// ..; so a row's q is in both waves' registers (128 of them) but its output in
+// one's (64), and the two never have to be joined.
 // 32 x 32 x 16 instructions on fp16 with the fp32 operands q and P as two fp16
-// values each: hi + lo, 22 bits, two products an operand pair.  K and V steps of
-// 32 rows come to LDS by loads that bypass the registers, K once the step's
-// scores are formed, V into a second buffer.  K's 16-byte chunks are permuted by
-// row (chunk ^ row % 16) so that the 32 rows a read touches fall into different
-// banks; V rows are read as they are and transposed in registers (8 rows x 4
-// dims a lane).  q rows come, and output rows go, through LDS too, a row a wave
-// at a time (32 rows an instruction took 10 us a tile).
-constexpr int kStep = 32;                 // cache rows of a step
+// values each: hi + lo, 22 bits, two products an operand pair.  K and V units
+// are double-buffered in LDS by loads that bypass the registers, 16-byte chunks
+// permuted by row so that the rows that one read touches fall into different
+// banks (K: chunk ^ row % 16, V: chunk ^ 4 (row % 4)); V is transposed as it is
+// read.  q rows come, and output rows go, through LDS too, a row a wave at a time
+// (32 rows an instruction took 10 us a tile).
+// The units are software-pipelined: a unit's exponentials run among the score
+// products of the next one, whose K is there a unit ahead of its V, and its last
+// eight products among the first K reads of the next.  Both partners keep one
+// maximum a row that the weights refer to; the maxima of a unit's two halves meet
+// with the weights of the unit before, and it moves only when a score passes it by
+// kMove.
+// What bounds it: the matrix instructions' power.  64 a unit and SIMD are 2048
+// cycles, at which random operands pull the clock to 1.55 GHz (20 ns each where
+// zeros take 15): 1.3 us a unit.  It takes 3400 cycles at 1.8 GHz: a single wave a
+// SIMD issues everything in order, about four vector instructions in a matrix
+// instruction's shadow (16.4 ns a product with up to 4, 22.9 with 6, 34 with 12),
+// so what is the same every unit is a kept address, a scalar or an offset in the
+// instruction, the loads of the next unit are spread over the score products
+// (in one run of 16 they held the wave for 800 cycles), and every LDS read is a
+// step ahead.  2048 rows over as many: 99 us; 512 over 16384: 280 us.  Two
+// workgroups a CU with half the registers each, partners splitting the dims and
+// exchanging scores (twice the exponentials): 133 and 318 us.
+struct F16Tile {
+    _Float16 k[2][kUnit][kHd], v[2][kUnit][kHd];
+    f16x8 p[4][4][kWave];                 // a wave's weights: operands (hi, lo) of its two 16-row steps
+    float mx[2][4][32];                   // maxima of a unit's halves; at the end sums and maxima
+    uint32_t poison[kPagedTileRows][kHd / 32];
+};
+typedef const __attribute__((address_space(3))) f16x8 lds_f16x8;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-__global__ __launch_bounds__(NT, 2) void paged_prefill_f16(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
+// The i-th of eight loads of dma16 for 16 rows of 512 bytes, two rows each: global
+// rows from `from` on, LDS rows from `at` on; off: the lane's place in two rows.
+// (The offset in the instruction counts on both sides.)
+__device__ __forceinline__ void dma_pair(int i, const void* from, uint32_t off, uint32_t at) {
+#define Q35_DMA_PAIR(imm)                                                                                     \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:" imm ::"s"(at), "v"(off), \
+                 "s"(from)                                                                                    \
+                 : "memory")
+    if (i & 4) at += 4096, from = (const char*)from + 4096;
+    if ((i & 3) == 0) Q35_DMA_PAIR("0");
+    if ((i & 3) == 1) Q35_DMA_PAIR("1024");
+    if ((i & 3) == 2) Q35_DMA_PAIR("2048");
+    if ((i & 3) == 3) Q35_DMA_PAIR("3072");
+#undef Q35_DMA_PAIR
+}
+// A pointer that all lanes have the same, as the compiler cannot see.
+__device__ __forceinline__ const void* uniform(const void* p) {
+    const uint64_t x = (uint64_t)p;
+    return (const void*)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
+}
+
+__global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
                                                            const float* __restrict__ q_norm, float* __restrict__ out,
                                                            float* __restrict__ part_o, float* __restrict__ part_ml,
                                                            int hg_shift, int ng, float eps) {
-    // One block of 64 KiB: K and V of the steps and the exchanged scores, or the
-    // tile's 64 rows of q or of the output.
-    struct Steps {
-        _Float16 k[kStep][kHd], v[2][kStep][kHd];
-        float4 x[4][4][kWave];
-    };
-    __shared__ __align__(16) char smem[sizeof(Steps)];
-    static_assert(sizeof(Steps) == kPagedTileRows * kHd * sizeof(float), "the rows take the block's place");
-    __shared__ uint32_t poison[kPagedTileRows][kHd / 32];
-    Steps& st = *reinterpret_cast<Steps*>(smem);
-    float4* const tile = reinterpret_cast<float4*>(smem);         // [64][64] 16-byte chunks, chunk ^ row % 32
-    const int tid = threadIdx.x, lane = tid & 63;
+    constexpr float kShift = 1.0f;                        // weights are e^{s - m} 2^kShift,
+    constexpr float kMove = 14.0f;                        // so below 2^15: in fp16's range
+    __shared__ __align__(16) F16Tile st;
+    const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rg = wave & 1, half = wave >> 1;
-    const int nn = lane & 31, h = lane >> 5;
     const int hg = 1 << hg_shift, tm = kPagedTileRows >> hg_shift;
     const int groups = pv.nkv * ng, nh = groups << hg_shift;
     const int wg = xcd_remap(blockIdx.x, gridDim.x);      // neighbours, which share K and V, on one XCD's L2
-    const uint32_t kaddr = lds_address(&st.k[8 * wave][0]), vaddr = lds_address(&st.v[0][8 * wave][0]);
+    constexpr int kBuf = kUnit * kHd * 2;                 // bytes of a buffer
+    const uint32_t kaddr = lds_address(&st.k[0][16 * wave][0]), vaddr = lds_address(&st.v[0][16 * wave][0]);
 
-    const int qe = q_exponent(q_norm, lane);
+    const int qe = q_exponent(q_norm, tid & 63);
     const float up = ldexpf(1.0f, qe), down = ldexpf(1.0f, -qe);
-    const Units un = units_of(pv, b, groups, hg_shift, lane);
+    const Units un = units_of(pv, b, groups, hg_shift, tid & 63);
     Walk wk;
     wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
+        const int start = uniform(wk.start), tokens = uniform(wk.tokens);
         const int seq = b.seq[wk.i], kvh = wk.y / ng;
         const int* table = pv.table + (size_t)seq * pv.max_pages;
+        // (the lane's own places as values of this segment: addresses made of them
+        // would else be kept over all segments)
+        int lane = tid & 63, nn = lane & 31;
+        asm volatile("" : "+v"(lane), "+v"(nn));
+        const int h = lane >> 5;
         // Rows the tile's tokens see: [0, rows); the lane's query row sees [0, mine].
-        const int rows = min(wk.start + min((wk.j + 1) * tm, wk.tokens), pv.max_rows);
-        const int stop = min(rows, wk.t1 * kUnit), last16 = (rows - 1) & ~15;
-        const int first = wk.start + wk.j * tm;            // position of the tile's first token
+        const int rows = uniform(min(start + min((wk.j + 1) * tm, tokens), pv.max_rows));
+        const int last16 = (rows - 1) & ~15;
+        const int first = uniform(start + wk.j * tm);          // position of the tile's first token
+        const int mine = min(start + min(wk.j * tm + ((32 * rg + nn) >> hg_shift), tokens - 1), pv.max_rows - 1);
         // Query row r of the tile: token, and the row of q and out.
-        auto token = [&](int r) { return wk.j * tm + (r >> hg_shift); };
-        auto row_at = [&](int r) {
-            return (size_t)(b.off[wk.i] + min(token(r), wk.tokens - 1)) * nh + (wk.y << hg_shift) + (r & (hg - 1));
+        auto token = [&](int j, int r) { return j * tm + (r >> hg_shift); };
+        auto row_at = [&](int j, int r) {
+            return (size_t)(b.off[wk.i] + min(token(j, r), tokens - 1)) * nh + (wk.y << hg_shift) + (r & (hg - 1));
         };
-        const int mine = min(wk.start + min(token(32 * rg + nn), wk.tokens - 1), pv.max_rows - 1);
 
-        // q rows to LDS.
-#pragma unroll 4
-        for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-            dma16(q_gate + row_at(r) * 2 * kHd + 4 * (lane ^ (r & 31)), lds_address(tile + r * (kHd / 4)));
-        for (int x = tid; x < kPagedTileRows * (kHd / 32); x += NT) (&poison[0][0])[x] = 0;
-
-        // A wave brings 8 rows of a step's K and V.  It holds 64 entries of the page
-        // table, one a lane, from entry `held` on.
+        // A wave brings its 16 rows of a unit's K or V.  It holds 64 entries of the
+        // page table, one a lane, from entry `held` on.
         int held = 0, ids = 0;
         auto hold = [&](int entry) {
             held = entry;
             ids = page_of(table, entry + lane, pv.max_pages, pv.n_pages);
         };
-        auto row8 = [&](int base) { return min(base + 8 * wave, last16 + (8 * wave & 8)); };
-        hold(row8(wk.t0 * kUnit) >> pv.page_shift);
-        auto issue = [&](int base, int par) {
-            const int r = row8(base), entry = r >> pv.page_shift;
-            if (__builtin_expect(entry - held >= kWave, 0)) hold(entry);
-            const size_t at = row_offset<_Float16>(pv, __builtin_amdgcn_readlane(ids, entry - held), kvh, r);
-            const _Float16* kp = (const _Float16*)pv.k + at + h * kHd;
-            const _Float16* vp = (const _Float16*)pv.v + at + 8 * lane;
-            const int c0 = (lane & 31) ^ h ^ (8 * (wave & 1));
-#pragma unroll
-            for (int k = 0; k < 8; k += 2) dma16(kp + k * kHd + 8 * (c0 ^ k), kaddr + (uint32_t)(k * kHd * 2));
-#pragma unroll
-            for (int k = 0; k < 8; k += 2) dma16(vp + k * kHd, vaddr + (uint32_t)((par * kStep + k) * kHd * 2));
+        hold(min(wk.t0 * kUnit + 16 * wave, last16) >> pv.page_shift);
+        auto group_at = [&](int t) {
+            const int r = uniform(min(t * kUnit + 16 * wave, last16)), entry = r >> pv.page_shift;
+            if (__builtin_expect(uniform(entry - held) >= kWave, 0)) hold(entry);
+            return row_offset<_Float16>(pv, __builtin_amdgcn_readlane(ids, uniform(entry - held)), kvh, r);
         };
-
-        // q: lane (row nn, h) holds dims 128 half + 16 s + 8 h + j of its row: norm
-        // (which the rotation leaves), then rotation, scale and the two halves.
-        f16x8 qh[8], ql[8];
-        {
-            auto dims8 = [&](int c, float (&x)[8]) {       // chunks c, c + 1 of the lane's row
+        uint32_t ko[8], vo[2];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float4 a = tile[(32 * rg + nn) * (kHd / 4) + ((c + k) ^ nn)];
-                    x[4 * k] = a.x; x[4 * k + 1] = a.y; x[4 * k + 2] = a.z; x[4 * k + 3] = a.w;
-                }
-            };
+        for (int r = 0; r < 16; r += 2) ko[r / 2] = 512u * h + 16u * (nn ^ h ^ r);
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) vo[r / 2] = 512u * h + 16u * (nn ^ (4 * (h + r)));
+        auto issue_k = [&](int i, const void* from, int buf) { dma_pair(i, from, ko[i], kaddr + buf * kBuf); };
+        auto issue_v = [&](int i, const void* from, int buf) { dma_pair(i, from, vo[i & 1], vaddr + buf * kBuf); };
+        auto k_from = [&](size_t at) { return uniform((const _Float16*)pv.k + at); };
+        auto v_from = [&](size_t at) { return uniform((const _Float16*)pv.v + at); };
+
+        // q rows to where V will be, 16-byte chunks permuted by row (chunk ^ row % 32).
+        const float4* const qs = reinterpret_cast<const float4*>(&st.v[0][0][0]);
+#pragma unroll 4
+        for (int r = 16 * wave; r < 16 * wave + 16; ++r)
+            dma16(q_gate + row_at(wk.j, r) * 2 * kHd + 4 * (lane ^ (r & 31)), lds_address(&st.v[0][0][0]) + r * kHd * 4);
+        // Where the wave's rows of the next units lie: found a unit before they are asked for.
+        const size_t at0 = group_at(wk.t0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) issue_k(i, k_from(at0), 0);
+        size_t at1 = group_at(wk.t0 + 1), at2 = group_at(wk.t0 + 2);
+        for (int x = tid; x < kPagedTileRows * (kHd / 32); x += NT) (&st.poison[0][0])[x] = 0;
+
+        // q: lane (row nn, h) holds dims 16 s + 8 h + j of its row: norm (which the
+        // rotation leaves), then rotation, scale and the two halves.
+        f16x8 qh[16], ql[16];
+        {
+            const double* rope = pv.rope + (size_t)mine * kRopeDim + 8 * h;
+            double cs[16], sn[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                cs[k] = rope[(k & 8) * 2 + (k & 7)];
+                sn[k] = rope[kRopeHalf + (k & 8) * 2 + (k & 7)];
+            }
             dma_wait();
             __syncthreads();
+            auto row8 = [&](int s, float (&x)[8]) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float4 a = qs[(32 * rg + nn) * (kHd / 4) + ((4 * s + 2 * h + c) ^ nn)];
+                    x[4 * c] = a.x; x[4 * c + 1] = a.y; x[4 * c + 2] = a.z; x[4 * c + 3] = a.w;
+                }
+            };
             float ss = 0.0f;
-#pragma unroll 4
+#pragma unroll
             for (int s = 0; s < 16; ++s) {
                 float x[8];
-                dims8(4 * s + 2 * h, x);
+                row8(s, x);
 #pragma unroll
                 for (int c = 0; c < 8; ++c) ss += x[c] * x[c];
             }
             const float scale = up * (kLog2e / 16.0f) / sqrtf(xor32_sum(ss) / (float)kHd + eps);
-            const double* rope = pv.rope + (size_t)mine * kRopeDim + 8 * h;
+            auto put = [&](int s, const float (&x)[8]) {
+                float y[8];
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                float x[8], y[8];
-                dims8(32 * half + 4 * s + 2 * h, x);
-                if (half == 0 && s < 4) {                  // dims 16 (s % 2) + 8 h .. and 32 further
-                    dims8(4 * (s ^ 2) + 2 * h, y);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const float cs = (float)rope[16 * (s & 1) + c], sn = (float)rope[kRopeHalf + 16 * (s & 1) + c];
-                        x[c] = s < 2 ? x[c] * cs - y[c] * sn : y[c] * sn + x[c] * cs;
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < 8; ++c) y[c] = x[c] * (scale * (1.0f + q_norm[128 * half + 16 * s + 8 * h + c]));
+                for (int c = 0; c < 8; ++c) y[c] = x[c] * (scale * (1.0f + q_norm[16 * s + 8 * h + c]));
                 split16(y, qh[s], ql[s]);
+            };
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                float a[8], c[8], x[8];
+                row8(s, a);
+                row8(s + 2, c);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = a[k] * (float)cs[8 * s + k] - c[k] * (float)sn[8 * s + k];
+                put(s, x);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = a[k] * (float)sn[8 * s + k] + c[k] * (float)cs[8 * s + k];
+                put(s + 2, x);
+            }
+#pragma unroll
+            for (int s = 4; s < 16; ++s) {
+                float x[8];
+                row8(s, x);
+                put(s, x);
             }
         }
 
-        f32x16 o[4];                                       // dims 128 half + 4 row + d at [d]
+        // The output stays in accumulation registers all along: pin() is a use there,
+        // without which the compiler moves all of it to vector registers and back on
+        // every unit, for the rare branch that scales it.
+        f32x16 o[4];                                       // dims 128 half + 32 d + row at [d]
+        auto pin = [&]() { asm volatile("" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3])); };
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int k = 0; k < 16; ++k) o[d][k] = 0.0f;
-        float m_run = -INFINITY, l_run = 0.0f;
+        pin();
+        float m_run = -INFINITY, l_run = 0.0f, mx = -INFINITY;
+        float sc[16];                                      // the wave's scores of a unit, before `down`
 
-        __syncthreads();                                   // q is read
-        int par = 0;
-        if (wk.t0 * kUnit < stop) issue(wk.t0 * kUnit, 0);
-        for (int base = wk.t0 * kUnit; base < stop; base += kStep) {
-            dma_wait();
-            __syncthreads();                               // the step's rows are there, the last one's V and scores read
-            // Some row of the tile does not see some row of the step.
-            const bool masked = base + kStep - 1 > first;
-            if (masked)
-                guard_rows(&st.v[par][8 * wave][0], 8, base + 8 * wave, rows, poison, first, wk.tokens - wk.j * tm,
-                           hg_shift, lane);
-            f32x16 sc;
+        // K operands of the wave's 32 rows: lane (row nn, h), dims 16 s + 8 h ..; V
+        // operands of 16 rows and 32 dims: lane (dim nn, h), rows 4 h + {0..3, 8..11},
+        // which the transposing read gathers from lanes of 4 rows x 16 dims.
+        uint32_t ka[8], va[2][4];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) sc[k] = 0.0f;
+        for (int s = 0; s < 8; ++s) ka[s] = lds_address(&st.k[0][32 * half + nn][0]) + 16 * ((2 * s + h) ^ (nn & 15));
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {                  // K operand: lane (row nn, h), dims 128 half + 16 s + 8 h ..
-                const f16x8 a = *reinterpret_cast<const f16x8*>(&st.k[nn][8 * ((16 * half + 2 * s + h) ^ (nn & 15))]);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[s], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[s], sc, 0, 0, 0);
+        for (int d = 0; d < 4; ++d) {
+            va[0][d] = lds_address(&st.v[0][32 * half + 4 * h + ((lane >> 2) & 3)][0]) + 32 * (8 * half + ((2 * d + ((lane >> 4) & 1)) ^ (2 * ((lane >> 2) & 3)))) +
+                    8 * (lane & 3);
+            va[1][d] = va[0][d] + (half ? -32 * 512 : 32 * 512);   // the partner's rows
+        }
+        auto k_at = [&](int s) { return *(lds_f16x8*)(ka[s & 7] + 256 * (s >> 3)); };
+        // Score products, K read four steps ahead (the first four by begin()), with
+        // beside(s) among the products of step s.
+        f16x8 kk[4];
+        f32x16 x;
+        auto begin = [&]() {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) kk[s] = k_at(s);
+        };
+        auto scores = [&](auto beside) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[k] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 16; ++s) {
+                const f16x8 k = kk[s & 3];
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[s], x, 0, 0, 0);
+                beside(s);
+                if (s + 4 < 16) kk[s & 3] = k_at(s + 4);
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[s], x, 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        auto take = [&]() {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) st.x[wave][k][lane] = make_float4(sc[4 * k], sc[4 * k + 1], sc[4 * k + 2], sc[4 * k + 3]);
-            lds_barrier();                                 // the scores are there, K is read
-            if (base + kStep < stop) issue(base + kStep, par ^ 1);
-            float mx = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float4 y = st.x[wave ^ 2][k][lane];
-                sc[4 * k] += y.x; sc[4 * k + 1] += y.y; sc[4 * k + 2] += y.z; sc[4 * k + 3] += y.w;
+            for (int k = 0; k < 16; ++k) {
+                sc[k] = x[k];
+                asm volatile("" : "+v"(sc[k]));            // moved once, to vector registers
             }
-            if (masked) {
-                asm volatile("");                          // a branch: selects on every step cost more
-                const int lim = mine - base - 4 * h;
+        };
+        // Whether some row of the tile does not see some row of unit t.
+        auto masked = [&](int t) { return t * kUnit + kUnit - 1 > first; };
+        auto mask = [&](int t) {
+            const int lim = mine - (t * kUnit + 32 * half) - 4 * h;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) sc[k] = 8 * (k >> 2) + (k & 3) <= lim ? sc[k] : -INFINITY;
-            }
+            for (int k = 0; k < 16; ++k) sc[k] = 8 * (k >> 2) + (k & 3) <= lim ? sc[k] : -INFINITY;
+        };
+        // Posts the maximum of the unit's scores.
+        auto post = [&]() {
+            mx = fmaxf(sc[0], sc[1]);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) mx = fmaxf(mx, sc[k]);
+            for (int k = 2; k < 16; ++k) mx = fmaxf(mx, sc[k]);
             mx = xor32_max(mx * down);
-            if (__any(mx > m_run + kLazy)) {               // (m_run is -inf at first)
+            if (h == 0) st.mx[0][wave][nn] = mx;
+        };
+        // The row's maximum over both halves of the unit, which may move the one the
+        // weights refer to (known a while before it is done).
+        bool moves;
+        float sub;                                         // what the weights' exponents have added
+        auto meet = [&](float other) {
+            mx = fmaxf(mx, other);
+            moves = __any(mx > m_run + kMove);             // (m_run is -inf at first)
+        };
+        auto move = [&]() {
+            if (__builtin_expect_with_probability(moves, 0, 0.99)) {
                 const float m_new = fmaxf(m_run, mx);
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
                 m_run = m_new;
                 l_run *= alpha;
+                pin();
 #pragma unroll
                 for (int d = 0; d < 4; ++d) o[d] *= alpha;
+                pin();
             }
-            const float sub = kPShift - (m_run == -INFINITY ? 0.0f : m_run);
-            f16x8 ph[2], pl[2];
+            sub = kShift - (m_run == -INFINITY ? 0.0f : m_run);
+        };
+        f16x8 ph[2], pl[2];
+        float p_even = 0.0f;
+        auto weight = [&](int k) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[k], down, sub));
+            l_run += p;
+            asm volatile("" : "+v"(l_run));                 // here, among the products
+            if (k & 1) {
+                f16x2 hi, lo;
+                split16(p_even, p, hi, lo);
+                ph[k >> 3][(k & 7) - 1] = hi.x; ph[k >> 3][k & 7] = hi.y;
+                pl[k >> 3][(k & 7) - 1] = lo.x; pl[k >> 3][k & 7] = lo.y;
+            } else {
+                p_even = p;
+            }
+        };
+        auto hand_over = [&]() {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float p[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    p[k] = __builtin_amdgcn_exp2f(fmaf(sc[8 * c + k], down, sub));
-                    l_run += p[k];
-                }
-                split16(p, ph[c], pl[c]);
+                st.p[wave][2 * c][lane] = ph[c];
+                st.p[wave][2 * c + 1][lane] = pl[c];
             }
+        };
+        auto v_read = [&](int whose, int step, f16x8 (&v)[4]) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                // V rows 16 c + 4 h + {0..3, 8..11}: the weights' rows of the lane's half.
-                const _Float16* vt = &st.v[par][16 * c + 4 * h][128 * half + 4 * nn];
-                uint2 v8[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) v8[r] = *reinterpret_cast<const uint2*>(vt + ((r & 3) + 8 * (r >> 2)) * kHd);
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {              // dims 4 m + d of the lane's 8 rows
-                    const uint32_t sel = (d & 1) ? 0x07060302u : 0x05040100u;
-                    u32x4 a;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w)
-                        a[w] = d < 2 ? __builtin_amdgcn_perm(v8[2 * w + 1].x, v8[2 * w].x, sel)
-                                     : __builtin_amdgcn_perm(v8[2 * w + 1].y, v8[2 * w].y, sel);
-                    const f16x8 av = __builtin_bit_cast(f16x8, a);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pl[c], o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, ph[c], o[d], 0, 0, 0);
-                }
+            for (int d = 0; d < 4; ++d) {
+                const uint32_t at = va[whose][d] + step * 16 * 512;
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * 512));
+                typedef short s16x8 __attribute__((ext_vector_type(8)));
+                v[d] = __builtin_bit_cast(f16x8, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
             }
-            par ^= 1;
-        }
+        };
+        auto add = [&](const f16x8 (&v)[4], f16x8 hi, f16x8 lo) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], lo, o[d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], hi, o[d], 0, 0, 0);
+        };
 
-        // The tile's rows to LDS, then a row a wave at a time: finished, or as a part
-        // to the workspace.  Both partners have the rows' sums.
+        __syncthreads();                                   // q is read
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            issue_v(i, v_from(at0), 0);
+            issue_k(i, k_from(at1), 1);
+        }
+        begin();
+        scores([](int) {});
+        take();
+        if (masked(wk.t0)) mask(wk.t0);
+        post();
+        int t = wk.t0, buf = 0;
+        lds_barrier();
+        meet(st.mx[0][wave ^ 2][nn]);
+        // Output products of unit t: the wave's own 32 rows, whose first 16 rows of V
+        // are read by now, then its partner's.  The last 16 rows' wait, read, for the
+        // next unit's beginning.  behind() runs among the first products, ahead() with
+        // the partner's maxima.
+        f16x8 v0[4], v1[4], h1, l1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            h1[k] = l1[k] = (_Float16)0.0f;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) v1[d][k] = (_Float16)0.0f;
+        }
+        auto output = [&](auto behind, auto ahead) {
+            hand_over();
+            v_read(0, 1, v1);
+            __builtin_amdgcn_sched_barrier(0);
+            behind();
+            __builtin_amdgcn_sched_barrier(0);
+            lds_barrier();                                 // the partner's weights and maxima
+            const float other = st.mx[0][wave ^ 2][nn];
+            const f16x8 h0 = st.p[wave ^ 2][0][lane], l0 = st.p[wave ^ 2][1][lane];
+            h1 = st.p[wave ^ 2][2][lane];
+            l1 = st.p[wave ^ 2][3][lane];
+            v_read(1, 0, v0);
+            __builtin_amdgcn_sched_barrier(0);
+            add(v1, ph[1], pl[1]);
+            ahead(other);
+            __builtin_amdgcn_sched_barrier(0);
+            v_read(1, 1, v1);
+            add(v0, h0, l0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // What every unit begins with: its rows and maxima are there (and K of the next
+        // unit), every wave is past the buffers that the next rows go to.
+        auto guard = [&]() {
+            if (masked(t)) {
+                guard_rows<4>(&st.v[buf][16 * wave][0], 16, t * kUnit + 16 * wave, rows, st.poison, first,
+                              tokens - wk.j * tm, hg_shift, lane);
+                lds_barrier();
+            }
+        };
+#pragma nounroll
+        for (; t + 1 < wk.t1; ++t) {
+            dma_wait();
+            __syncthreads();
+            const int flip = buf ? -kBuf : kBuf;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) ka[s] += flip;
+            begin();
+            __builtin_amdgcn_sched_barrier(0);
+            const void* const next_k = k_from(at2);
+            const void* const next_v = v_from(at1);
+            at1 = at2;
+            at2 = group_at(t + 3);
+            guard();
+            add(v1, h1, l1);
+            move();
+            scores([&](int s) {
+                weight(s);
+                if (s < 8)
+                    issue_k(s, next_k, buf);
+                else
+                    issue_v(s - 8, next_v, buf ^ 1);
+                if (s == 12) v_read(0, 0, v0);
+            });
+            output(
+                [&]() {
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0[d], pl[0], o[d], 0, 0, 0);
+                    take();
+                    if (masked(t + 1)) {
+                        asm volatile("");                  // a branch, not selects
+                        mask(t + 1);
+                    }
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0[d], ph[0], o[d], 0, 0, 0);
+                    post();
+                },
+                meet);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) va[0][d] += flip, va[1][d] += flip;
+            buf ^= 1;
+        }
+        dma_wait();
+        __syncthreads();
+        guard();
+        add(v1, h1, l1);
+        move();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) weight(k);
+        v_read(0, 0, v0);
+        output([&]() { add(v0, ph[0], pl[0]); }, [](float) {});
+        add(v1, h1, l1);
+        pin();
+
+        // The tile's rows to LDS (chunk ^ row % 32, as q's), then a row a wave at a
+        // time: finished, or as a part to the workspace.  (Places again as values of
+        // this part: kept from the segment's beginning they would be in registers all
+        // the while.)
+        int j2 = uniform(wk.j);
+        asm volatile("" : "+s"(j2), "+v"(lane), "+v"(nn));
+        const int h2 = lane >> 5;
         const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
         const int slot = 2 * wg + (wk.t0 == 0);
-        l_run = xor32_sum(l_run);
-        const float inv = whole ? 1.0f / l_run : 1.0f;
-        __syncthreads();                                   // V and the scores are read
+        float4 gate[16];
+        if (whole) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const int chunk = 32 * half + 8 * (k >> 2) + 4 * h + (k & 3);
-            tile[(32 * rg + nn) * (kHd / 4) + (chunk ^ nn)] =
-                make_float4(o[0][k] * inv, o[1][k] * inv, o[2][k] * inv, o[3][k] * inv);
+            for (int r = 0; r < 16; ++r)
+                gate[r] = *reinterpret_cast<const float4*>(q_gate + row_at(j2, 16 * wave + r) * 2 * kHd + kHd + 4 * lane);
         }
-        if (!whole && half == 0 && h == 0) {
-            const size_t r = (size_t)slot * kPagedTileRows + 32 * rg + nn;
-            part_ml[2 * r] = m_run;
-            part_ml[2 * r + 1] = l_run;
-        }
+        l_run = xor32_sum(l_run);
+        if (h2 == 0) st.mx[1][wave][nn] = l_run;
+        if (half == 0 && h2 == 0) st.mx[0][rg][nn] = m_run;
+        __syncthreads();                                   // K and V are read, the last maxima too
+        float4* const os = reinterpret_cast<float4*>(&st.k[0][0][0]);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int k = 0; k < 16; k += 4)
+                os[(32 * rg + nn) * (kHd / 4) + ((32 * half + 8 * d + 2 * (k >> 2) + h2) ^ nn)] =
+                    make_float4(o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]);
         __syncthreads();
 #pragma unroll
-        for (int k0 = 0; k0 < 16; k0 += 8) {
-            float4 gate[8];
+        for (int k = 0; k < 16; ++k) {
+            const int r = 16 * wave + k;
+            const float l = st.mx[1][r >> 5][r & 31] + st.mx[1][2 + (r >> 5)][r & 31];
+            float4 x = os[r * (kHd / 4) + (lane ^ (r & 31))];
+            const uint32_t nan = st.poison[r][lane >> 3] >> (4 * (lane & 7));
+            x.x = nan & 1 ? NAN : x.x;
+            x.y = nan & 2 ? NAN : x.y;
+            x.z = nan & 4 ? NAN : x.z;
+            x.w = nan & 8 ? NAN : x.w;
+            const size_t prow = (size_t)slot * kPagedTileRows + r;
             if (whole) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    gate[k] = *reinterpret_cast<const float4*>(q_gate + row_at(16 * wave + k0 + k) * 2 * kHd + kHd + 4 * lane);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int r = 16 * wave + k0 + k;
-                float4 x = tile[r * (kHd / 4) + (lane ^ (r & 31))];
-                const uint32_t nan = poison[r][lane >> 3] >> (4 * (lane & 7));
-                x.x = nan & 1 ? NAN : x.x;
-                x.y = nan & 2 ? NAN : x.y;
-                x.z = nan & 4 ? NAN : x.z;
-                x.w = nan & 8 ? NAN : x.w;
-                if (!whole)
-                    *reinterpret_cast<float4*>(part_o + ((size_t)slot * kPagedTileRows + r) * kHd + 4 * lane) = x;
-                else if (token(r) < wk.tokens)
-                    *reinterpret_cast<float4*>(out + row_at(r) * kHd + 4 * lane) = gated(x, gate[k]);
+                const float inv = 1.0f / l;
+                x = gated(make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), gate[k]);
+                if (token(j2, r) < tokens) *reinterpret_cast<float4*>(out + row_at(j2, r) * kHd + 4 * lane) = x;
+            } else {
+                *reinterpret_cast<float4*>(part_o + prow * kHd + 4 * lane) = x;
+                if (lane == 0) {
+                    part_ml[2 * prow] = st.mx[0][r >> 5][r & 31];
+                    part_ml[2 * prow + 1] = l;
+                }
             }
         }
         __syncthreads();
@@ -567,7 +786,7 @@ __global__ __launch_bounds__(NT, 2) void paged_prefill_f32(PagedView pv, PagedBa
             __syncthreads();
             const bool masked = base + kF32Rows - 1 > wk.start + wk.j * tm;
             if (masked) {
-                guard_rows(&vs[8 * wave][0], 8, base + 8 * wave, rows, poison, wk.start + wk.j * tm,
+                guard_rows<0>(&vs[8 * wave][0], 8, base + 8 * wave, rows, poison, wk.start + wk.j * tm,
                            wk.tokens - wk.j * tm, hg_shift, lane);
                 lds_barrier();
             }
@@ -718,20 +937,19 @@ __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBat
     }
 }
 
-// Two workgroups a CU.
-int prefill_workgroups(const q35m_ctx* c) { return 2 * c->n_cu; }
+int prefill_workgroups(const q35m_ctx* c, int type) { return type == Q35M_KV_F16 ? c->n_cu : 2 * c->n_cu; }
 
 }  // namespace
 
 size_t paged_prefill_work_bytes(const q35m_ctx* c) {
-    return (size_t)2 * prefill_workgroups(c) * kPagedTileRows * (kHd + 2) * sizeof(float);
+    return (size_t)2 * prefill_workgroups(c, Q35M_KV_F32) * kPagedTileRows * (kHd + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, float* out) {
     q35m_ctx* c = p->ctx;
     const int per_kv = c->d.nh / c->d.nkv;
     const int hg = per_kv <= 16 ? per_kv : per_kv % 16 == 0 ? 16 : 8;
-    const int ng = per_kv / hg, nwg = prefill_workgroups(c), tm = kPagedTileRows / hg;
+    const int ng = per_kv / hg, nwg = prefill_workgroups(c, p->type), tm = kPagedTileRows / hg;
     int hg_shift = 0;
     while ((1 << hg_shift) < hg) ++hg_shift;
     float* part_o = p->work;
