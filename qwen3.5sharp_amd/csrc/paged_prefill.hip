@@ -90,11 +90,11 @@ __device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch&
         const Tiles t(u.start, b.off[lane + 1] - b.off[lane], hg_shift);
         u.end = t.before(t.n) * groups;
     }
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
+    for (int o = 1; o < b.n; o <<= 1) {
         const long x = shfl_up_long(u.end, o);
         if (lane >= o) u.end += x;
     }
+    u.end = lane < b.n ? u.end : readlane_long(u.end, b.n - 1);
     u.total = readlane_long(u.end, kWave - 1);
     return u;
 }
@@ -129,13 +129,15 @@ struct Walk {
             long rest = u - (readlane_long(un.end, i) - each * groups);
             y = (int)(rest / each);
             rest -= (long)y * each;
-            int lo = 0, hi = n - 1;                      // last place whose units begin at or before rest
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (ts.ordered(mid) <= rest) lo = mid;
-                else hi = mid - 1;
+            // The last place whose units begin at or before rest: 64 places a step.
+            const int lane = threadIdx.x & (kWave - 1);
+            o = 0;
+            for (int left = n; left > 1;) {              // among places [o, o + left)
+                const int step = (left + kWave - 1) / kWave, c = lane * step;
+                const int hits = __popcll(__ballot(c < left && ts.ordered(o + c) <= rest));
+                o = uniform(o + (hits - 1) * step);
+                left = uniform(min(step, left - (hits - 1) * step));
             }
-            o = lo;
             within = rest - ts.ordered(o);
         }
         const Tiles ts(start, tokens, hg_shift);
@@ -170,9 +172,17 @@ __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" :
 // see it), and the outputs of the query rows that do are marked in `poison`, a
 // bit a (query row, dim), which turns them to NaN at the segment's end.  A wave
 // takes `count` rows of kHd values from v on; base: their first row's position.
+// (Rows up to `first` are seen by all of the tile.)
 __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 __device__ __forceinline__ bool not_finite(_Float16 x) {
     return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
+}
+// NaN in place of the values marked in `nan`, a bit a value.
+__device__ __forceinline__ float4 marked(float4 x, uint32_t nan) {
+    auto one = [&](float v, int k) {
+        return __builtin_bit_cast(float, __builtin_bit_cast(int, v) | ((int)(nan << (31 - k)) >> 31));
+    };
+    return make_float4(one(x.x, 0), one(x.y, 1), one(x.z, 2), one(x.w, 3));
 }
 // 16-byte chunks are permuted by row: chunk ^ S (row % 4).
 template <int S, typename T>
@@ -180,15 +190,27 @@ __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, 
                                            int tokens_left, int hg_shift, int lane) {
     constexpr int E = 16 / sizeof(T);          // values of 16 bytes
     typedef T vec __attribute__((ext_vector_type(E)));
+    constexpr int U = 4;                       // chunks a lane looks at together
 #pragma nounroll
-    for (int x = lane; x < count * (kHd / E); x += kWave) {
-        const int r = base + x / (kHd / E);
-        vec y = *reinterpret_cast<vec*>(v + x * E);
-        bool bad = false;
+    for (int x0 = max(0, first + 1 - base) * (kHd / E) + lane; x0 < count * (kHd / E); x0 += U * kWave) {
+        vec y[U];
+        bool look = false;
 #pragma unroll
-        for (int k = 0; k < E; ++k) bad |= not_finite(y[k]);
-        if (r < rows && !bad) continue;
-        if (r < rows) {
+        for (int u = 0; u < U; ++u) {
+            const int x = min(x0 + u * kWave, count * (kHd / E) - 1);
+            y[u] = *reinterpret_cast<vec*>(v + x * E);
+            look |= base + x / (kHd / E) >= rows;
+#pragma unroll
+            for (int k = 0; k < E; ++k) look |= not_finite(y[u][k]);
+        }
+        if (!look) continue;
+#pragma nounroll
+        for (int x = x0; x < min(x0 + U * kWave, count * (kHd / E)); x += kWave) {
+            const int r = base + x / (kHd / E);
+            if (r >= rows) {
+                *reinterpret_cast<vec*>(v + x * E) = vec{};
+                continue;
+            }
 #pragma nounroll
             for (int k = 0; k < E; ++k) {
                 const T one = v[x * E + k];
@@ -200,10 +222,6 @@ __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, 
                     if (r <= first + min(q >> hg_shift, tokens_left - 1)) atomicOr(&poison[q][d >> 5], 1u << (d & 31));
                 v[x * E + k] = (T)0.0f;
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < E; ++k) y[k] = (T)0.0f;
-            *reinterpret_cast<vec*>(v + x * E) = y;
         }
     }
 }
@@ -234,14 +252,19 @@ __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, 
 // so what is the same every unit is a kept address, a scalar or an offset in the
 // instruction, the loads of the next unit are spread over the score products
 // (in one run of 16 they held the wave for 800 cycles), and every LDS read is a
-// step ahead.  2048 rows over as many: 99 us; 512 over 16384: 280 us.  Two
+// step ahead.  2048 rows over as many: 98 us; 512 over 16384: 268 us.  Two
 // workgroups a CU with half the registers each, partners splitting the dims and
 // exchanging scores (twice the exponentials): 133 and 318 us.
+// A segment's beginning and end are 30000 cycles of it: partners form half of q
+// each (9000 -> 5800 cycles), and the last rows' LDS reads and the gates come
+// before the first store, whose end a later load's wait would wait for (16000 ->
+// 7000).
 struct F16Tile {
     _Float16 k[2][kUnit][kHd], v[2][kUnit][kHd];
     f16x8 p[4][4][kWave];                 // a wave's weights: operands (hi, lo) of its two 16-row steps
     float mx[2][4][32];                   // maxima of a unit's halves; at the end sums and maxima
     uint32_t poison[kPagedTileRows][kHd / 32];
+    float w[kHd];                         // 1 + the norm's weights
 };
 typedef const __attribute__((address_space(3))) f16x8 lds_f16x8;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -284,13 +307,14 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
     constexpr int kBuf = kUnit * kHd * 2;                 // bytes of a buffer
     const uint32_t kaddr = lds_address(&st.k[0][16 * wave][0]), vaddr = lds_address(&st.v[0][16 * wave][0]);
 
+    st.w[tid] = 1.0f + q_norm[tid];                       // (read behind the first segment's first barrier)
     const int qe = q_exponent(q_norm, tid & 63);
     const float up = ldexpf(1.0f, qe), down = ldexpf(1.0f, -qe);
     const Units un = units_of(pv, b, groups, hg_shift, tid & 63);
     Walk wk;
     wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
-        const int start = uniform(wk.start), tokens = uniform(wk.tokens);
+        const int start = uniform(wk.start), tokens = uniform(wk.tokens), first_row = uniform(b.off[wk.i]);
         const int seq = b.seq[wk.i], kvh = wk.y / ng;
         const int* table = pv.table + (size_t)seq * pv.max_pages;
         // (the lane's own places as values of this segment: addresses made of them
@@ -306,7 +330,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         // Query row r of the tile: token, and the row of q and out.
         auto token = [&](int j, int r) { return j * tm + (r >> hg_shift); };
         auto row_at = [&](int j, int r) {
-            return (size_t)(b.off[wk.i] + min(token(j, r), tokens - 1)) * nh + (wk.y << hg_shift) + (r & (hg - 1));
+            return (size_t)(first_row + min(token(j, r), tokens - 1)) * nh + (wk.y << hg_shift) + (r & (hg - 1));
         };
 
         // A wave brings its 16 rows of a unit's K or V.  It holds 64 entries of the
@@ -336,7 +360,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         const float4* const qs = reinterpret_cast<const float4*>(&st.v[0][0][0]);
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-            dma16(q_gate + row_at(wk.j, r) * 2 * kHd + 4 * (lane ^ (r & 31)), lds_address(&st.v[0][0][0]) + r * kHd * 4);
+            dma_pair(0, uniform(q_gate + row_at(wk.j, r) * 2 * kHd), 16 * (lane ^ (r & 31)),
+                     lds_address(&st.v[0][0][0]) + r * kHd * 4);
         // Where the wave's rows of the next units lie: found a unit before they are asked for.
         const size_t at0 = group_at(wk.t0);
 #pragma unroll
@@ -344,60 +369,70 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         size_t at1 = group_at(wk.t0 + 1), at2 = group_at(wk.t0 + 2);
         for (int x = tid; x < kPagedTileRows * (kHd / 32); x += NT) (&st.poison[0][0])[x] = 0;
 
-        // q: lane (row nn, h) holds dims 16 s + 8 h + j of its row: norm (which the
-        // rotation leaves), then rotation, scale and the two halves.
-        f16x8 qh[16], ql[16];
+        // q: lane (row nn, h) forms dims 128 half + 16 s + 8 h + j of its row, s < 8:
+        // norm (which the rotation leaves), rotation, scale and the two halves, which
+        // take the raw values' place.
         {
-            const double* rope = pv.rope + (size_t)mine * kRopeDim + 8 * h;
+            float4* const at = const_cast<float4*>(qs) + (32 * rg + nn) * (kHd / 4);
+            float x[8][8];
             double cs[16], sn[16];
+            if (half == 0) {
+                const double* rope = pv.rope + (size_t)mine * kRopeDim + 8 * h;
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                cs[k] = rope[(k & 8) * 2 + (k & 7)];
-                sn[k] = rope[kRopeHalf + (k & 8) * 2 + (k & 7)];
+                for (int k = 0; k < 16; ++k) {
+                    cs[k] = rope[(k & 8) * 2 + (k & 7)];
+                    sn[k] = rope[kRopeHalf + (k & 8) * 2 + (k & 7)];
+                }
             }
             dma_wait();
             __syncthreads();
-            auto row8 = [&](int s, float (&x)[8]) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float4 a = qs[(32 * rg + nn) * (kHd / 4) + ((4 * s + 2 * h + c) ^ nn)];
-                    x[4 * c] = a.x; x[4 * c + 1] = a.y; x[4 * c + 2] = a.z; x[4 * c + 3] = a.w;
-                }
-            };
             float ss = 0.0f;
 #pragma unroll
-            for (int s = 0; s < 16; ++s) {
-                float x[8];
-                row8(s, x);
+            for (int s = 0; s < 8; ++s)
 #pragma unroll
-                for (int c = 0; c < 8; ++c) ss += x[c] * x[c];
+                for (int c = 0; c < 2; ++c) {
+                    const float4 a = at[(32 * half + 4 * s + 2 * h + c) ^ nn];
+                    x[s][4 * c] = a.x; x[s][4 * c + 1] = a.y; x[s][4 * c + 2] = a.z; x[s][4 * c + 3] = a.w;
+                    ss += a.x * a.x; ss += a.y * a.y; ss += a.z * a.z; ss += a.w * a.w;
+                }
+            ss = xor32_sum(ss);
+            if (h == 0) st.mx[0][wave][nn] = ss;
+            if (half == 0) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const float lo = x[k >> 3][k & 7], hi = x[2 + (k >> 3)][k & 7];
+                    x[k >> 3][k & 7] = lo * (float)cs[k] - hi * (float)sn[k];
+                    x[2 + (k >> 3)][k & 7] = lo * (float)sn[k] + hi * (float)cs[k];
+                }
             }
-            const float scale = up * (kLog2e / 16.0f) / sqrtf(xor32_sum(ss) / (float)kHd + eps);
-            auto put = [&](int s, const float (&x)[8]) {
+            lds_barrier();
+            const float scale =
+                up * (kLog2e / 16.0f) / sqrtf((st.mx[0][rg][nn] + st.mx[0][rg + 2][nn]) / (float)kHd + eps);
+            const float* const w = &st.w[128 * half + 8 * h];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
                 float y[8];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) y[c] = x[c] * (scale * (1.0f + q_norm[16 * s + 8 * h + c]));
-                split16(y, qh[s], ql[s]);
-            };
-            asm volatile("" ::: "memory");
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                float a[8], c[8], x[8];
-                row8(s, a);
-                row8(s + 2, c);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = a[k] * (float)cs[8 * s + k] - c[k] * (float)sn[8 * s + k];
-                put(s, x);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = a[k] * (float)sn[8 * s + k] + c[k] * (float)cs[8 * s + k];
-                put(s + 2, x);
+                for (int c = 0; c < 8; c += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(&w[16 * s + c]);
+                    y[c] = x[s][c] * (scale * v.x);
+                    y[c + 1] = x[s][c + 1] * (scale * v.y);
+                    y[c + 2] = x[s][c + 2] * (scale * v.z);
+                    y[c + 3] = x[s][c + 3] * (scale * v.w);
+                }
+                f16x8 hi, lo;
+                split16(y, hi, lo);
+                at[(32 * half + 4 * s + 2 * h) ^ nn] = __builtin_bit_cast(float4, hi);
+                at[(32 * half + 4 * s + 2 * h + 1) ^ nn] = __builtin_bit_cast(float4, lo);
             }
+            lds_barrier();
+        }
+        // Then lane (row nn, h) holds dims 16 s + 8 h + j, s < 16.
+        f16x8 qh[16], ql[16];
 #pragma unroll
-            for (int s = 4; s < 16; ++s) {
-                float x[8];
-                row8(s, x);
-                put(s, x);
-            }
+        for (int s = 0; s < 16; ++s) {
+            qh[s] = __builtin_bit_cast(f16x8, qs[(32 * rg + nn) * (kHd / 4) + ((4 * s + 2 * h) ^ nn)]);
+            ql[s] = __builtin_bit_cast(f16x8, qs[(32 * rg + nn) * (kHd / 4) + ((4 * s + 2 * h + 1) ^ nn)]);
         }
 
         // The output stays in accumulation registers all along: pin() is a use there,
@@ -529,7 +564,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
             for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], hi, o[d], 0, 0, 0);
         };
 
-        __syncthreads();                                   // q is read
+        lds_barrier();                                     // q is read
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             issue_v(i, v_from(at0), 0);
@@ -627,6 +662,13 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         }
         dma_wait();
         __syncthreads();
+        const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
+        float4 gate[16];                                   // of the wave's rows 16 wave ..
+        if (whole) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                gate[r] = reinterpret_cast<const float4*>(uniform(q_gate + row_at(wk.j, 16 * wave + r) * 2 * kHd + kHd))[lane];
+        }
         guard();
         add(v1, h1, l1);
         move();
@@ -644,18 +686,11 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         int j2 = uniform(wk.j);
         asm volatile("" : "+s"(j2), "+v"(lane), "+v"(nn));
         const int h2 = lane >> 5;
-        const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
         const int slot = 2 * wg + (wk.t0 == 0);
-        float4 gate[16];
-        if (whole) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                gate[r] = *reinterpret_cast<const float4*>(q_gate + row_at(j2, 16 * wave + r) * 2 * kHd + kHd + 4 * lane);
-        }
         l_run = xor32_sum(l_run);
         if (h2 == 0) st.mx[1][wave][nn] = l_run;
         if (half == 0 && h2 == 0) st.mx[0][rg][nn] = m_run;
-        __syncthreads();                                   // K and V are read, the last maxima too
+        lds_barrier();                                     // K and V are read, the last maxima too
         float4* const os = reinterpret_cast<float4*>(&st.k[0][0][0]);
 #pragma unroll
         for (int d = 0; d < 4; ++d)
@@ -663,31 +698,47 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
             for (int k = 0; k < 16; k += 4)
                 os[(32 * rg + nn) * (kHd / 4) + ((32 * half + 8 * d + 2 * (k >> 2) + h2) ^ nn)] =
                     make_float4(o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]);
-        __syncthreads();
+        lds_barrier();
+        const int row = 16 * wave + (lane & 15);           // a row's sum and maximum in lane row % 16
+        const float l = st.mx[1][row >> 5][row & 31] + st.mx[1][2 + (row >> 5)][row & 31];
+        const float m = st.mx[0][row >> 5][row & 31];
+        auto rows8 = [&](int k0, auto&& put) {
+            float4 x[8];
+            uint32_t nan[8];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const int r = 16 * wave + k;
-            const float l = st.mx[1][r >> 5][r & 31] + st.mx[1][2 + (r >> 5)][r & 31];
-            float4 x = os[r * (kHd / 4) + (lane ^ (r & 31))];
-            const uint32_t nan = st.poison[r][lane >> 3] >> (4 * (lane & 7));
-            x.x = nan & 1 ? NAN : x.x;
-            x.y = nan & 2 ? NAN : x.y;
-            x.z = nan & 4 ? NAN : x.z;
-            x.w = nan & 8 ? NAN : x.w;
-            const size_t prow = (size_t)slot * kPagedTileRows + r;
-            if (whole) {
-                const float inv = 1.0f / l;
-                x = gated(make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), gate[k]);
-                if (token(j2, r) < tokens) *reinterpret_cast<float4*>(out + row_at(j2, r) * kHd + 4 * lane) = x;
-            } else {
-                *reinterpret_cast<float4*>(part_o + prow * kHd + 4 * lane) = x;
-                if (lane == 0) {
-                    part_ml[2 * prow] = st.mx[0][r >> 5][r & 31];
-                    part_ml[2 * prow + 1] = l;
-                }
+            for (int k = 0; k < 8; ++k) {
+                const int r = 16 * wave + k0 + k;
+                x[k] = os[r * (kHd / 4) + (lane ^ (r & 31))];
+                nan[k] = st.poison[r][lane >> 3] >> (4 * (lane & 7));
             }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) put(k0 + k, marked(x[k], nan[k]));
+        };
+        if (whole) {
+            const float inv_l = 1.0f / l;
+            // (all gates before the first store: a wait for a load waits for the stores before it)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                gate[k] = make_float4(sigmoid(gate[k].x), sigmoid(gate[k].y), sigmoid(gate[k].z), sigmoid(gate[k].w));
+                asm volatile("" : "+v"(gate[k].x), "+v"(gate[k].y), "+v"(gate[k].z), "+v"(gate[k].w));
+            }
+            auto put = [&](int k, float4 x) {
+                const float inv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv_l), k));
+                const int r = 16 * wave + k;
+                const float4 g = gate[k];
+                x = make_float4(x.x * inv * g.x, x.y * inv * g.y, x.z * inv * g.z, x.w * inv * g.w);
+                if (token(j2, r) < tokens) *reinterpret_cast<float4*>(out + row_at(j2, r) * kHd + 4 * lane) = x;
+            };
+            rows8(0, put);
+            rows8(8, put);
+        } else {
+            float* const po = part_o + (size_t)(slot * kPagedTileRows + 16 * wave) * kHd;
+            auto put = [&](int k, float4 x) { *reinterpret_cast<float4*>(po + k * kHd + 4 * lane) = x; };
+            rows8(0, put);
+            rows8(8, put);
+            if (lane < 16) *reinterpret_cast<float2*>(part_ml + 2 * ((size_t)slot * kPagedTileRows + row)) = make_float2(m, l);
         }
-        __syncthreads();
+        lds_barrier();                                     // (the stores need no wait)
     }
 }
 
@@ -847,12 +898,8 @@ __global__ __launch_bounds__(NT, 2) void paged_prefill_f32(PagedView pv, PagedBa
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int at = 64 * t + 4 * (4 * g + i);
-                float4 x = make_float4(o[4 * t][i], o[4 * t + 1][i], o[4 * t + 2][i], o[4 * t + 3][i]);
-                const uint32_t nan = poison[16 * wave + n][at >> 5] >> (at & 31);
-                if (nan & 1) x.x = NAN;
-                if (nan & 2) x.y = NAN;
-                if (nan & 4) x.z = NAN;
-                if (nan & 8) x.w = NAN;
+                const float4 x = marked(make_float4(o[4 * t][i], o[4 * t + 1][i], o[4 * t + 2][i], o[4 * t + 3][i]),
+                                        poison[16 * wave + n][at >> 5] >> (at & 31));
                 if (!whole) {
                     *reinterpret_cast<float4*>(part_o + prow * kHd + at) = x;
                 } else if (real) {
