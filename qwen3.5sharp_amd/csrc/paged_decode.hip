@@ -28,6 +28,8 @@
 // 16 x 16 x 32 on fp16 with the fp32 operands q and P as two fp16 values each
 // (hi + lo, 22 bits; q's row and P scaled by powers of two into the range),
 // and a register transpose of V (8 rows x 8 dims a lane).
+// The waves share the forming of q rows through LDS: formed in every wave, behind
+// K and V in the queue of loads, they cost a call over 8192 rows 2 of its 13 us.
 #include "paged_device.h"
 
 namespace q35 {
@@ -50,13 +52,15 @@ struct Tile<float> {
     float4 k[16], v[4][4];  // K row l % 16, dims 16 t + 4 g; V row 4 g + i, dims 64 t + 4 m
     f32x4 o[16];            // dims 64 t + 4 row + c at [4 t + c]
 
-    __device__ __forceinline__ void set_q(float (&x)[64]) {
+    // q row n in LDS, 16-byte chunks permuted: chunk ^ n.
+    static __device__ __forceinline__ void put_q(float4* row, int r, float4 x, int lane) { row[lane ^ r] = x; }
+    __device__ __forceinline__ void load_q(const float4* row, int n, int g) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) q[i] = x[i];
+        for (int t = 0; t < 16; ++t) {
+            const float4 a = row[(4 * t + g) ^ n];
+            q[4 * t] = a.x; q[4 * t + 1] = a.y; q[4 * t + 2] = a.z; q[4 * t + 3] = a.w;
+        }
     }
-    // First dim of the 4 that x[4 t ..] of set_q holds.
-    static __device__ __forceinline__ int q_dim(int t, int g) { return 16 * t + 4 * g; }
-    static constexpr int kRopePair = 8;     // x index of dim d + 32 less that of dim d
 
     __device__ __forceinline__ void load_k(const float* p, int, int lane) {
         const float* a = p + (lane & 15) * kHd + 4 * (lane >> 4);
@@ -129,13 +133,23 @@ struct Tile<_Float16> {
     u32x4 k[2][8], v[2][8];    // K row l % 16 of group kb, dims 32 t + 8 g; V row 16 (j / 4) + 4 g + j % 4, dims 128 u + 8 m
     f32x4 o[16];               // dims 128 u + 8 row + b at [8 u + b]
 
-    // The row, already scaled into fp16's range, as hi + lo.
-    __device__ __forceinline__ void set_q(float (&x)[64]) {
-#pragma unroll
-        for (int t = 0; t < 8; ++t) split16(x + 8 * t, qh[t], ql[t]);
+    // The row, already scaled into fp16's range, as hi (chunks 0 .. 31) and lo.
+    static __device__ __forceinline__ void put_q(float4* row, int r, float4 x, int lane) {
+        f16x2 h[2], l[2];
+        split16(x.x, x.y, h[0], l[0]);
+        split16(x.z, x.w, h[1], l[1]);
+        f16x2* const at = reinterpret_cast<f16x2*>(row + ((lane >> 1) ^ r)) + 2 * (lane & 1);
+        at[0] = h[0]; at[1] = h[1];
+        f16x2* const to = reinterpret_cast<f16x2*>(row + (32 + (lane >> 1) ^ r)) + 2 * (lane & 1);
+        to[0] = l[0]; to[1] = l[1];
     }
-    static __device__ __forceinline__ int q_dim(int t, int g) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1); }
-    static constexpr int kRopePair = 8;
+    __device__ __forceinline__ void load_q(const float4* row, int n, int g) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            qh[t] = __builtin_bit_cast(f16x8, row[(4 * t + g) ^ n]);
+            ql[t] = __builtin_bit_cast(f16x8, row[(32 + 4 * t + g) ^ n]);
+        }
+    }
 
     __device__ __forceinline__ void load_k(const _Float16* p, int kb, int lane) {
         const _Float16* a = p + (lane & 15) * kHd + 8 * (lane >> 4);
@@ -253,10 +267,14 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
     const int n = lane & 15, g = lane >> 4;
     const int groups = pv.nkv * ng, nh = groups * hg;
 
-    __shared__ float obuf[4][kPagedDecodeHeads][kHd];
+    __shared__ __align__(16) float obuf[4][kPagedDecodeHeads][kHd];
     __shared__ float ml[4][kPagedDecodeHeads][2];
     __shared__ __align__(16) T newrow[4][2][kHd];
+    __shared__ float4 qbuf[kPagedDecodeHeads][kHd / 4];
 
+    float4 qw = *reinterpret_cast<const float4*>(q_norm + 4 * lane);
+    const float4 kw = *reinterpret_cast<const float4*>(k_norm + 4 * lane);
+    qw = make_float4(1.0f + qw.x, 1.0f + qw.y, 1.0f + qw.z, 1.0f + qw.w);
     const int qe = std::is_same_v<T, float> ? 0 : q_exponent(q_norm, lane);
     const float up = ldexpf(1.0f, qe), down = ldexpf(1.0f, -qe);
     const Units un = units_of<T>(pv, b, groups, lane);
@@ -298,57 +316,56 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
             for (int kb = 0; kb < R / 16; ++kb)
                 tl.load_v((const T*)pv.v + row_offset<T>(pv, p[kb], kvh, min(base + 16 * kb, last16)), kb, lane);
         };
+        // What q's rows and the new row are made of is asked for before K and V, so
+        // that they are formed while those are on their way; a wave forms every
+        // fourth q row, for all.
+        const bool has_new = first <= pos / R * R && pos / R * R < stop && (pos / R * R - first) % (4 * R) == 0;
+        if (first < stop) pages(first);
+        float4 xq[kPagedDecodeHeads / 4], xk{}, xv{};
+        const float* const q_rows = q_gate + ((size_t)i * nh + y * hg) * 2 * kHd + 4 * lane;
+#pragma unroll
+        for (int k = 0; k < kPagedDecodeHeads / 4; ++k)
+            if (wave + 4 * k < hg) xq[k] = *reinterpret_cast<const float4*>(q_rows + (size_t)(wave + 4 * k) * 2 * kHd);
+        if (has_new) {
+            const size_t at = ((size_t)i * pv.nkv + kvh) * kHd + 4 * lane;
+            xk = *reinterpret_cast<const float4*>(knew + at);
+            xv = *reinterpret_cast<const float4*>(vnew + at);
+        }
+        double cs[4], sn[4];                     // the rotation of dims 4 (lane % 8) ..
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            cs[k] = pv.rope[(size_t)pos * kRopeDim + 4 * (lane & 7) + k];
+            sn[k] = pv.rope[(size_t)pos * kRopeDim + kRopeHalf + 4 * (lane & 7) + k];
+        }
+        __builtin_amdgcn_sched_barrier(0);
         if (first < stop) {
-            pages(first);
             load_k(first, pg);
             load_v(first, pg);
         }
+        __builtin_amdgcn_sched_barrier(0);
 
         // q: the rotation, the norm, the scale 1/16 (and log2 e, for exp2; and a
         // power of two for fp16).
-        {
-            const int h = y * hg + min(n, hg - 1);
-            const float* qp = q_gate + ((size_t)i * nh + h) * 2 * kHd;
-            const double* rope = pv.rope + (size_t)pos * kRopeDim;
-            float x[64], ss = 0.0f;
 #pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                const float4 a = *reinterpret_cast<const float4*>(qp + Tl::q_dim(t, g));
-                x[4 * t] = a.x; x[4 * t + 1] = a.y; x[4 * t + 2] = a.z; x[4 * t + 3] = a.w;
+        for (int k = 0; k < kPagedDecodeHeads / 4; ++k) {
+            const int r = wave + 4 * k;
+            if (r >= hg) break;
+            float x[4] = {xq[k].x, xq[k].y, xq[k].z, xq[k].w}, ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float a = x[c], z = row_xor<8>(a), co = (float)cs[c], si = (float)sn[c];
+                x[c] = lane < 8 ? a * co - z * si : lane < 16 ? z * si + a * co : a;
+                ss += x[c] * x[c];
             }
-#pragma unroll
-            for (int t = 0; t < Tl::kRopePair / 4; ++t)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int d = Tl::q_dim(t, g) + c;
-                    const float cs = (float)rope[d], sn = (float)rope[kRopeHalf + d];
-                    const float lo = x[4 * t + c], hi = x[4 * t + c + Tl::kRopePair];
-                    x[4 * t + c] = lo * cs - hi * sn;
-                    x[4 * t + c + Tl::kRopePair] = lo * sn + hi * cs;
-                }
-#pragma unroll
-            for (int t = 0; t < 64; ++t) ss += x[t] * x[t];
-            ss = xor16_sum(xor32_sum(ss));
-            const float scale = n < hg ? up * (kLog2e / 16.0f) / sqrtf(ss / (float)kHd + eps) : 0.0f;
-#pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                const float4 w = *reinterpret_cast<const float4*>(q_norm + Tl::q_dim(t, g));
-                x[4 * t] *= scale * (1.0f + w.x);
-                x[4 * t + 1] *= scale * (1.0f + w.y);
-                x[4 * t + 2] *= scale * (1.0f + w.z);
-                x[4 * t + 3] *= scale * (1.0f + w.w);
-            }
-            tl.set_q(x);
+            const float scale = up * (kLog2e / 16.0f) / sqrtf(wave_sum(ss) / (float)kHd + eps);
+            Tl::put_q(qbuf[r], r,
+                      make_float4(x[0] * (scale * qw.x), x[1] * (scale * qw.y), x[2] * (scale * qw.z), x[3] * (scale * qw.w)),
+                      lane);
         }
-
         // The wave that holds the new row makes it (every head group needs it;
         // one writes it to the page, and none reads it from there).
-        const int new_tile = pos / R * R;
-        if (first <= new_tile && new_tile < stop && (new_tile - first) % (4 * R) == 0) {
-            const size_t at = ((size_t)i * pv.nkv + kvh) * kHd + 4 * lane;
-            const float4 xk = *reinterpret_cast<const float4*>(knew + at);
-            const float4 xv = *reinterpret_cast<const float4*>(vnew + at);
-            const float4 yk = paged_key_row(xk, pv.rope + (size_t)pos * kRopeDim, k_norm, lane, (double)eps);
+        if (has_new) {
+            const float4 yk = paged_key_row(xk, cs, sn, kw, lane, (double)eps);
             store_row4(&newrow[wave][0][4 * lane], yk);
             store_row4(&newrow[wave][1][4 * lane], xv);
             const int pnew = page_of(table, pos >> pv.page_shift, pv.max_pages, pv.n_pages);
@@ -357,6 +374,11 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
                 store_row4((T*)pv.k + to, yk);
                 store_row4((T*)pv.v + to, xv);
             }
+        }
+        lds_barrier();
+        {
+            const int r = min(n, hg - 1);        // columns from hg on are never read
+            tl.load_q(qbuf[r], r, g);
         }
 
         float m_run = -INFINITY, l_run = 0.0f;
@@ -400,34 +422,41 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
                 ml[wave][n][1] = l_run;
             }
         }
-        __syncthreads();
         const bool whole = t0 == 0 && t1 == tiles;
         const int slot = 2 * blockIdx.x + (t0 == 0);
-        for (int h = 0; h < hg; ++h) {
-            float M = -INFINITY, l = 0.0f, o = 0.0f;
+        float4 gate[kPagedDecodeHeads / 4];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][h][0]);
+        for (int k = 0; k < kPagedDecodeHeads / 4; ++k)
+            if (whole && wave + 4 * k < hg)
+                gate[k] = *reinterpret_cast<const float4*>(q_rows + (size_t)(wave + 4 * k) * 2 * kHd + kHd);
+        lds_barrier();
+#pragma unroll
+        for (int k = 0; k < kPagedDecodeHeads / 4; ++k) {
+            const int r = wave + 4 * k;
+            if (r >= hg) break;
+            float M = -INFINITY, l = 0.0f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][r][0]);
             const float mu = M == -INFINITY ? 0.0f : M;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float e = __builtin_amdgcn_exp2f(ml[w][h][0] - mu);
-                l += e * ml[w][h][1];
-                o += e * obuf[w][h][tid];
+                const float e = __builtin_amdgcn_exp2f(ml[w][r][0] - mu);
+                const float4 x = *reinterpret_cast<const float4*>(&obuf[w][r][4 * lane]);
+                l += e * ml[w][r][1];
+                o.x += e * x.x; o.y += e * x.y; o.z += e * x.z; o.w += e * x.w;
             }
             if (whole) {
-                const size_t row = (size_t)i * nh + y * hg + h;
-                const float gate = q_gate[row * 2 * kHd + kHd + tid];
-                out[row * kHd + tid] = o / l * sigmoid_full(gate);
+                const float inv = 1.0f / l;
+                *reinterpret_cast<float4*>(out + ((size_t)i * nh + y * hg + r) * kHd + 4 * lane) =
+                    gated(make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), gate[k]);
             } else {
-                const size_t at = (size_t)slot * kPagedDecodeHeads + h;
-                part_o[at * kHd + tid] = o;
-                if (tid == 0) {
-                    part_ml[2 * at] = M;
-                    part_ml[2 * at + 1] = l;
-                }
+                const size_t at = (size_t)slot * kPagedDecodeHeads + r;
+                *reinterpret_cast<float4*>(part_o + at * kHd + 4 * lane) = o;
+                if (lane == 0) *reinterpret_cast<float2*>(part_ml + 2 * at) = make_float2(M, l);
             }
         }
-        __syncthreads();
+        lds_barrier();
     }
 }
 

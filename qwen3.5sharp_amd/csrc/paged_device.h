@@ -42,17 +42,10 @@ __device__ __forceinline__ double wave_sum(double v) {
 // an fp16 cache rounds the row a second time: a value whose fp32 arithmetic is
 // an ulp off falls on the other side of an fp16 rounding border once in about
 // 2^13 values, and such a value is 2^-11 off.  A row is 256 values once per
-// token, so the cost is not seen.
-__device__ __forceinline__ float4 paged_key_row(float4 x, const double* __restrict__ rope, const float* __restrict__ w,
-                                                int lane, double eps) {
-    const float4 ww = *reinterpret_cast<const float4*>(w + 4 * lane);
-    const int d0 = 4 * (lane & 7);
-    double c[4], s[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        c[k] = rope[d0 + k];
-        s[k] = rope[kRopeHalf + d0 + k];
-    }
+// token, so the cost is not seen.  c, s: the rotation of dims 4 (lane % 8) ..,
+// ww: the norm's weights.
+__device__ __forceinline__ float4 paged_key_row(float4 x, const double (&c)[4], const double (&s)[4], float4 ww, int lane,
+                                                double eps) {
     const float xs[4] = {x.x, x.y, x.z, x.w};
     const float ws[4] = {ww.x, ww.y, ww.z, ww.w};
     double y[4], ss = 0.0;
@@ -71,6 +64,19 @@ __device__ __forceinline__ float4 paged_key_row(float4 x, const double* __restri
     // one from 64 bits, which differs where the fp32 value is a tie).
     asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w));
     return r;
+}
+
+// With the rotation and the norm weights as they lie in memory.
+__device__ __forceinline__ float4 paged_key_row(float4 x, const double* __restrict__ rope, const float* __restrict__ w,
+                                                int lane, double eps) {
+    const int d0 = 4 * (lane & 7);
+    double c[4], s[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        c[k] = rope[d0 + k];
+        s[k] = rope[kRopeHalf + d0 + k];
+    }
+    return paged_key_row(x, c, s, *reinterpret_cast<const float4*>(w + 4 * lane), lane, eps);
 }
 
 // Exponent e such that every value of a normed q row, times log2(e) / 16 and

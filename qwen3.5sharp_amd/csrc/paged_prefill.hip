@@ -30,7 +30,6 @@ namespace {
 constexpr int NT = 256;
 constexpr int kUnit = 64;               // cache rows of a unit
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 8.0f;           // log2 of how far a score may pass the running maximum before it moves
 
 // ---- the units of a call ------------------------------------------------
 
@@ -153,7 +152,7 @@ struct Walk {
     }
 };
 
-// ---- fp16 cache -----------------------------------------------------------
+// ---- loads, and rows that not every query sees ----------------------------
 
 // 16 bytes a lane from global memory straight to LDS at address at + 16 lane (at
 // the same in every lane).  Complete once vmcnt says so: dma_wait() before the
@@ -184,8 +183,8 @@ __device__ __forceinline__ float4 marked(float4 x, uint32_t nan) {
     };
     return make_float4(one(x.x, 0), one(x.y, 1), one(x.z, 2), one(x.w, 3));
 }
-// 16-byte chunks are permuted by row: chunk ^ S (row % 4).
-template <int S, typename T>
+// 16-byte chunks are permuted by row: chunk ^ S ((row >> H) & M).
+template <int S, int H, int M, typename T>
 __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, uint32_t (*poison)[kHd / 32], int first,
                                            int tokens_left, int hg_shift, int lane) {
     constexpr int E = 16 / sizeof(T);          // values of 16 bytes
@@ -215,7 +214,7 @@ __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, 
             for (int k = 0; k < E; ++k) {
                 const T one = v[x * E + k];
                 if (!not_finite(one)) continue;
-                const int d = (x % (kHd / E) ^ (S * (r & 3))) * E + k;
+                const int d = (x % (kHd / E) ^ (S * ((r >> H) & M))) * E + k;
                 // query row q: token min(q >> hg_shift, tokens_left - 1) of the tile, at first + that
 #pragma nounroll
                 for (int q = 0; q < kPagedTileRows; ++q)
@@ -225,6 +224,104 @@ __device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, 
         }
     }
 }
+
+// ---- a segment's beginning and end, one row of four waves' tile a lane -------
+
+// Half of a q row, of which LDS has the fp32 values at `at` (16-byte chunks ^ row %
+// 32) once every wave's loads are there: x[s] is dims 128 half + 16 s + 8 h .. of
+// row 32 rg + lane % 32, rotated; returned is what makes it the norm's row over 16
+// in powers of two.  ss: room for four waves' sums.
+__device__ __forceinline__ float q_row(float (&x)[8][8], const float4* at, const double* rope, float (*ss_of)[32], int rg,
+                                       int half, int lane, float eps) {
+    const int nn = lane & 31, h = lane >> 5;
+    double cs[16], sn[16];
+    if (half == 0) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            cs[k] = rope[8 * h + (k & 8) * 2 + (k & 7)];
+            sn[k] = rope[kRopeHalf + 8 * h + (k & 8) * 2 + (k & 7)];
+        }
+    }
+    dma_wait();
+    __syncthreads();
+    float ss = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const float4 a = at[(32 * half + 4 * s + 2 * h + c) ^ nn];
+            x[s][4 * c] = a.x; x[s][4 * c + 1] = a.y; x[s][4 * c + 2] = a.z; x[s][4 * c + 3] = a.w;
+            ss += a.x * a.x; ss += a.y * a.y; ss += a.z * a.z; ss += a.w * a.w;
+        }
+    ss = xor32_sum(ss);
+    if (h == 0) ss_of[2 * half + rg][nn] = ss;
+    if (half == 0) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const float lo = x[k >> 3][k & 7], hi = x[2 + (k >> 3)][k & 7];
+            x[k >> 3][k & 7] = lo * (float)cs[k] - hi * (float)sn[k];
+            x[2 + (k >> 3)][k & 7] = lo * (float)sn[k] + hi * (float)cs[k];
+        }
+    }
+    lds_barrier();                                         // (the raw values are read, too)
+    return kLog2e / 16.0f / sqrtf((ss_of[rg][nn] + ss_of[rg + 2][nn]) / (float)kHd + eps);
+}
+
+// Wave (rg, half)'s output, dims 128 half + 32 d + (its register's row) of query row
+// 32 rg + lane % 32 at [d], to LDS, 16-byte chunks ^ row % 32.
+__device__ __forceinline__ void put_rows(float4* os, const f32x16 (&o)[4], int rg, int half, int lane) {
+    const int nn = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int k = 0; k < 16; k += 4)
+            os[(32 * rg + nn) * (kHd / 4) + ((32 * half + 8 * d + 2 * (k >> 2) + h) ^ nn)] =
+                make_float4(o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]);
+}
+
+// From there a wave's 16 rows leave, one at a time: finished to out_row(row) (none
+// if null), or as parts.  l, m: sum and maximum of row 16 wave + lane % 16.
+template <typename F>
+__device__ __forceinline__ void leave_rows(const float4* os, const uint32_t (*poison)[kHd / 32], float l, float m, bool whole,
+                                           float4 (&gate)[16], float* part_o, float* part_ml, int wave, int lane, F out_row) {
+    auto rows8 = [&](int k0, auto&& put) {
+        float4 x[8];
+        uint32_t nan[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int r = 16 * wave + k0 + k;
+            x[k] = os[r * (kHd / 4) + (lane ^ (r & 31))];
+            nan[k] = poison[r][lane >> 3] >> (4 * (lane & 7));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) put(k0 + k, marked(x[k], nan[k]));
+    };
+    if (whole) {
+        const float inv_l = 1.0f / l;
+        // (all gates before the first store: a wait for a load waits for the stores before it)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            gate[k] = make_float4(sigmoid(gate[k].x), sigmoid(gate[k].y), sigmoid(gate[k].z), sigmoid(gate[k].w));
+            asm volatile("" : "+v"(gate[k].x), "+v"(gate[k].y), "+v"(gate[k].z), "+v"(gate[k].w));
+        }
+        auto put = [&](int k, float4 x) {
+            const float inv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv_l), k));
+            const float4 g = gate[k];
+            x = make_float4(x.x * inv * g.x, x.y * inv * g.y, x.z * inv * g.z, x.w * inv * g.w);
+            if (float* to = out_row(16 * wave + k)) reinterpret_cast<float4*>(to)[lane] = x;
+        };
+        rows8(0, put);
+        rows8(8, put);
+    } else {
+        float4* const po = reinterpret_cast<float4*>(part_o + 16 * wave * kHd);
+        auto put = [&](int k, float4 x) { po[k * (kHd / 4) + lane] = x; };
+        rows8(0, put);
+        rows8(8, put);
+        if (lane < 16) reinterpret_cast<float2*>(part_ml)[16 * wave + lane] = make_float2(m, l);
+    }
+}
+
+// ---- fp16 cache -----------------------------------------------------------
 
 // Four waves, one a SIMD.  Wave (rg, half) has query rows 32 rg ..: it forms the
 // scores and weights of the unit's cache rows 32 half .., hands its weights to
@@ -375,39 +472,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         {
             float4* const at = const_cast<float4*>(qs) + (32 * rg + nn) * (kHd / 4);
             float x[8][8];
-            double cs[16], sn[16];
-            if (half == 0) {
-                const double* rope = pv.rope + (size_t)mine * kRopeDim + 8 * h;
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    cs[k] = rope[(k & 8) * 2 + (k & 7)];
-                    sn[k] = rope[kRopeHalf + (k & 8) * 2 + (k & 7)];
-                }
-            }
-            dma_wait();
-            __syncthreads();
-            float ss = 0.0f;
-#pragma unroll
-            for (int s = 0; s < 8; ++s)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float4 a = at[(32 * half + 4 * s + 2 * h + c) ^ nn];
-                    x[s][4 * c] = a.x; x[s][4 * c + 1] = a.y; x[s][4 * c + 2] = a.z; x[s][4 * c + 3] = a.w;
-                    ss += a.x * a.x; ss += a.y * a.y; ss += a.z * a.z; ss += a.w * a.w;
-                }
-            ss = xor32_sum(ss);
-            if (h == 0) st.mx[0][wave][nn] = ss;
-            if (half == 0) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const float lo = x[k >> 3][k & 7], hi = x[2 + (k >> 3)][k & 7];
-                    x[k >> 3][k & 7] = lo * (float)cs[k] - hi * (float)sn[k];
-                    x[2 + (k >> 3)][k & 7] = lo * (float)sn[k] + hi * (float)cs[k];
-                }
-            }
-            lds_barrier();
-            const float scale =
-                up * (kLog2e / 16.0f) / sqrtf((st.mx[0][rg][nn] + st.mx[0][rg + 2][nn]) / (float)kHd + eps);
+            const float scale = up * q_row(x, at, pv.rope + (size_t)mine * kRopeDim, st.mx[0], rg, half, lane, eps);
             const float* const w = &st.w[128 * half + 8 * h];
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
@@ -613,7 +678,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         // unit), every wave is past the buffers that the next rows go to.
         auto guard = [&]() {
             if (masked(t)) {
-                guard_rows<4>(&st.v[buf][16 * wave][0], 16, t * kUnit + 16 * wave, rows, st.poison, first,
+                guard_rows<4, 0, 3>(&st.v[buf][16 * wave][0], 16, t * kUnit + 16 * wave, rows, st.poison, first,
                               tokens - wk.j * tm, hg_shift, lane);
                 lds_barrier();
             }
@@ -679,239 +744,352 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         add(v1, h1, l1);
         pin();
 
-        // The tile's rows to LDS (chunk ^ row % 32, as q's), then a row a wave at a
-        // time: finished, or as a part to the workspace.  (Places again as values of
-        // this part: kept from the segment's beginning they would be in registers all
-        // the while.)
+        // The tile's rows to LDS, then a row a wave at a time: finished, or as a part
+        // to the workspace.  (Places again as values of this part: kept from the
+        // segment's beginning they would be in registers all the while.)
         int j2 = uniform(wk.j);
         asm volatile("" : "+s"(j2), "+v"(lane), "+v"(nn));
-        const int h2 = lane >> 5;
         const int slot = 2 * wg + (wk.t0 == 0);
         l_run = xor32_sum(l_run);
-        if (h2 == 0) st.mx[1][wave][nn] = l_run;
-        if (half == 0 && h2 == 0) st.mx[0][rg][nn] = m_run;
+        if (lane < 32) st.mx[1][wave][nn] = l_run;
+        if (half == 0 && lane < 32) st.mx[0][rg][nn] = m_run;
         lds_barrier();                                     // K and V are read, the last maxima too
         float4* const os = reinterpret_cast<float4*>(&st.k[0][0][0]);
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int k = 0; k < 16; k += 4)
-                os[(32 * rg + nn) * (kHd / 4) + ((32 * half + 8 * d + 2 * (k >> 2) + h2) ^ nn)] =
-                    make_float4(o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]);
+        put_rows(os, o, rg, half, lane);
         lds_barrier();
         const int row = 16 * wave + (lane & 15);           // a row's sum and maximum in lane row % 16
-        const float l = st.mx[1][row >> 5][row & 31] + st.mx[1][2 + (row >> 5)][row & 31];
-        const float m = st.mx[0][row >> 5][row & 31];
-        auto rows8 = [&](int k0, auto&& put) {
-            float4 x[8];
-            uint32_t nan[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int r = 16 * wave + k0 + k;
-                x[k] = os[r * (kHd / 4) + (lane ^ (r & 31))];
-                nan[k] = st.poison[r][lane >> 3] >> (4 * (lane & 7));
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) put(k0 + k, marked(x[k], nan[k]));
-        };
-        if (whole) {
-            const float inv_l = 1.0f / l;
-            // (all gates before the first store: a wait for a load waits for the stores before it)
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                gate[k] = make_float4(sigmoid(gate[k].x), sigmoid(gate[k].y), sigmoid(gate[k].z), sigmoid(gate[k].w));
-                asm volatile("" : "+v"(gate[k].x), "+v"(gate[k].y), "+v"(gate[k].z), "+v"(gate[k].w));
-            }
-            auto put = [&](int k, float4 x) {
-                const float inv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv_l), k));
-                const int r = 16 * wave + k;
-                const float4 g = gate[k];
-                x = make_float4(x.x * inv * g.x, x.y * inv * g.y, x.z * inv * g.z, x.w * inv * g.w);
-                if (token(j2, r) < tokens) *reinterpret_cast<float4*>(out + row_at(j2, r) * kHd + 4 * lane) = x;
-            };
-            rows8(0, put);
-            rows8(8, put);
-        } else {
-            float* const po = part_o + (size_t)(slot * kPagedTileRows + 16 * wave) * kHd;
-            auto put = [&](int k, float4 x) { *reinterpret_cast<float4*>(po + k * kHd + 4 * lane) = x; };
-            rows8(0, put);
-            rows8(8, put);
-            if (lane < 16) *reinterpret_cast<float2*>(part_ml + 2 * ((size_t)slot * kPagedTileRows + row)) = make_float2(m, l);
-        }
+        leave_rows(
+            os, st.poison, st.mx[1][row >> 5][row & 31] + st.mx[1][2 + (row >> 5)][row & 31], st.mx[0][row >> 5][row & 31],
+            whole, gate, part_o + (size_t)slot * kPagedTileRows * kHd, part_ml + (size_t)2 * slot * kPagedTileRows, wave,
+            lane, [&](int r) { return token(j2, r) < tokens ? out + row_at(j2, r) * kHd : nullptr; });
         lds_barrier();                                     // (the stores need no wait)
     }
 }
 
 // ---- fp32 cache -----------------------------------------------------------
 
-constexpr int kF32Rows = 32;            // cache rows of an LDS tile (two tiles a unit)
+// The shape of the fp16 kernel, on steps of 32 cache rows, with every fp32 operand
+// as three bf16 values, the top 8, next 8 and last 8 bits of its mantissa (exact),
+// and the six products of an operand pair that reach 2^-16 of it: 24 bits and
+// fp32's range at six bf16 instructions, 192 cycles where the fp32 instruction
+// takes 512 for the same 32 x 32 x 16.
+// Wave (rg, half) has query rows 32 rg ..; partners split the dims: each forms the
+// scores' products of dims 128 half .. and hands them to the other, both form the
+// weights, and each adds the output dims 128 half ...
+// K and V come as fp32, K with 16-byte chunks ^ row % 16 and V with chunk ^ 8
+// (row / 4 % 2), and are cut up where they are read: six instructions a value.
+constexpr int kStep = 32;
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef const __attribute__((address_space(3))) f32x4 lds_f32x4;
+typedef const __attribute__((address_space(3))) float lds_float;
+struct F32Tile {
+    float k[2][kStep][kHd], v[2][kStep][kHd];
+    float4 x[4][4][kWave];                // a wave's half of the scores
+    float ss[4][32];                      // q's sums of squares; at the end sums and maxima
+    uint32_t poison[kPagedTileRows][kHd / 32];
+    float w[kHd];
+};
 
-// Four waves of 16 query rows each; fp32 instructions (16 x 16 x 4).  One LDS
-// tile of K and V at a time, two workgroups a CU: one computes while the
-// other's rows arrive.
-__global__ __launch_bounds__(NT, 2) void paged_prefill_f32(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
+struct Cut3 {
+    b16x8 hi, mid, lo;
+};
+__device__ __forceinline__ Cut3 cut3(const float (&y)[8]) {
+    u32x4 a, b, c;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        uint32_t u[2], r[2], q[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            u[i] = __builtin_bit_cast(uint32_t, y[j + i]);
+            const float x = y[j + i] - __builtin_bit_cast(float, u[i] & 0xffff0000u);
+            r[i] = __builtin_bit_cast(uint32_t, x);
+            q[i] = __builtin_bit_cast(uint32_t, x - __builtin_bit_cast(float, r[i] & 0xffff0000u));
+        }
+        a[j / 2] = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u);     // the upper halves of two
+        b[j / 2] = __builtin_amdgcn_perm(r[1], r[0], 0x07060302u);
+        c[j / 2] = __builtin_amdgcn_perm(q[1], q[0], 0x07060302u);
+    }
+    return {__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), __builtin_bit_cast(b16x8, c)};
+}
+// c += a b, the small products first.
+__device__ __forceinline__ f32x16 mul6(const Cut3& a, const Cut3& b, f32x16 c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.lo, b.hi, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.lo, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.mid, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.hi, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.mid, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.hi, c, 0, 0, 0);
+}
+
+__global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
                                                            const float* __restrict__ q_norm, float* __restrict__ out,
                                                            float* __restrict__ part_o, float* __restrict__ part_ml,
                                                            int hg_shift, int ng, float eps) {
-    __shared__ __align__(16) float ks[kF32Rows][kHd], vs[kF32Rows][kHd];
-    __shared__ uint32_t poison[kPagedTileRows][kHd / 32];
-    const int tid = threadIdx.x, lane = tid & 63;
+    constexpr float kMove = 14.0f;
+    __shared__ __align__(16) F32Tile st;
+    const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 15, g = lane >> 4;
+    const int rg = wave & 1, half = wave >> 1;
     const int hg = 1 << hg_shift, tm = kPagedTileRows >> hg_shift;
     const int groups = pv.nkv * ng, nh = groups << hg_shift;
     const int wg = xcd_remap(blockIdx.x, gridDim.x);
+    constexpr int kBuf = kStep * kHd * 4;                 // bytes of a buffer
+    const uint32_t kaddr = lds_address(&st.k[0][8 * wave][0]), vaddr = lds_address(&st.v[0][8 * wave][0]);
 
-    const uint32_t kaddr = lds_address(&ks[8 * wave][0]), vaddr = lds_address(&vs[8 * wave][0]);
-
-    const Units un = units_of(pv, b, groups, hg_shift, lane);
+    st.w[tid] = 1.0f + q_norm[tid];                       // (read behind the first segment's first barrier)
+    const Units un = units_of(pv, b, groups, hg_shift, tid & 63);
     Walk wk;
     wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
+        const int start = uniform(wk.start), tokens = uniform(wk.tokens), first_row = uniform(b.off[wk.i]);
         const int seq = b.seq[wk.i], kvh = wk.y / ng;
         const int* table = pv.table + (size_t)seq * pv.max_pages;
-        const int rows = min(wk.start + min((wk.j + 1) * tm, wk.tokens), pv.max_rows);
-        const int at_tok = wk.j * tm + ((wave * 16 + n) >> hg_shift);
-        const int tok = min(at_tok, wk.tokens - 1);
-        const int mine = min(wk.start + tok, pv.max_rows - 1);
-        const int head = (wk.y << hg_shift) + ((wave * 16 + n) & (hg - 1));
-        const bool real = at_tok < wk.tokens;
-        const size_t qrow = (size_t)(b.off[wk.i] + tok) * nh + head;
+        int lane = tid & 63, nn = lane & 31;
+        asm volatile("" : "+v"(lane), "+v"(nn));
+        const int h = lane >> 5;
+        const int rows = uniform(min(start + min((wk.j + 1) * tm, tokens), pv.max_rows));
         const int last16 = (rows - 1) & ~15;
+        const int first = uniform(start + wk.j * tm);     // position of the tile's first token
+        const int mine = min(start + min(wk.j * tm + ((32 * rg + nn) >> hg_shift), tokens - 1), pv.max_rows - 1);
+        auto token = [&](int j, int r) { return j * tm + (r >> hg_shift); };
+        auto row_at = [&](int j, int r) {
+            return (size_t)(first_row + min(token(j, r), tokens - 1)) * nh + (wk.y << hg_shift) + (r & (hg - 1));
+        };
 
-        __syncthreads();                           // the segment before has read its marks
-        for (int x = tid; x < kPagedTileRows * (kHd / 32); x += NT) (&poison[0][0])[x] = 0;
+        // A wave brings 8 rows of a step's K and V; it holds 64 entries of the page
+        // table, one a lane, from entry `held` on.
+        int held = 0, ids = 0;
+        auto hold = [&](int entry) {
+            held = entry;
+            ids = page_of(table, entry + lane, pv.max_pages, pv.n_pages);
+        };
+        auto row8 = [&](int s) { return uniform(min(s * kStep + 8 * wave, last16 + (8 * wave & 8))); };
+        const int s0 = 2 * wk.t0;
+        const int steps = max(1, (min(rows, wk.t1 * kUnit) - wk.t0 * kUnit + kStep - 1) / kStep);
+        hold(row8(s0) >> pv.page_shift);
+        auto group_at = [&](int s) {
+            const int r = row8(s), entry = r >> pv.page_shift;
+            if (__builtin_expect(uniform(entry - held) >= kWave, 0)) hold(entry);
+            return row_offset<float>(pv, __builtin_amdgcn_readlane(ids, uniform(entry - held)), kvh, r);
+        };
+        uint32_t ko[8], vo[2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ko[i] = 16u * (lane ^ ((8 * wave + i) & 15));
+        vo[0] = 16u * lane;
+        vo[1] = 16u * (lane ^ 8);
+        auto issue_k = [&](int i, const void* from, int buf) { dma_pair(i, from, ko[i], kaddr + buf * kBuf); };
+        auto issue_v = [&](int i, const void* from, int buf) { dma_pair(i, from, vo[i >> 2], vaddr + buf * kBuf); };
+        auto k_from = [&](size_t at) { return uniform((const float*)pv.k + at); };
+        auto v_from = [&](size_t at) { return uniform((const float*)pv.v + at); };
 
-        // q: lane (row n, g) holds dims 16 t + 4 g + c of its row.
-        float q[64];
+        // q rows to where V will be, 16-byte chunks permuted by row (chunk ^ row % 32).
+        const float4* const qs = reinterpret_cast<const float4*>(&st.v[0][0][0]);
+#pragma unroll 4
+        for (int r = 16 * wave; r < 16 * wave + 16; ++r)
+            dma_pair(0, uniform(q_gate + row_at(wk.j, r) * 2 * kHd), 16 * (lane ^ (r & 31)),
+                     lds_address(&st.v[0][0][0]) + r * kHd * 4);
+        const size_t at0 = group_at(s0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) issue_k(i, k_from(at0), 0);
+        size_t at1 = group_at(s0 + 1), at2 = group_at(s0 + 2);
+        for (int x = tid; x < kPagedTileRows * (kHd / 32); x += NT) (&st.poison[0][0])[x] = 0;
+
+        // q: lane (row nn, h) has dims 128 half + 16 s + 8 h + j of its row, s < 8.
+        Cut3 q[8];
         {
-            const float* qp = q_gate + qrow * 2 * kHd + 4 * g;
-            const double* rope = pv.rope + (size_t)mine * kRopeDim + 4 * g;
-            float ss = 0.0f;
+            float x[8][8];
+            const float scale = q_row(x, qs + (32 * rg + nn) * (kHd / 4), pv.rope + (size_t)mine * kRopeDim, st.ss, rg, half,
+                                      lane, eps);
+            const float* const w = &st.w[128 * half + 8 * h];
 #pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                const float4 a = *reinterpret_cast<const float4*>(qp + 16 * t);
-                q[4 * t] = a.x; q[4 * t + 1] = a.y; q[4 * t + 2] = a.z; q[4 * t + 3] = a.w;
-            }
+            for (int s = 0; s < 8; ++s) {
+                float y[8];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float cs = (float)rope[16 * t + c], sn = (float)rope[kRopeHalf + 16 * t + c];
-                    const float lo = q[4 * t + c], hi = q[4 * t + 8 + c];
-                    q[4 * t + c] = lo * cs - hi * sn;
-                    q[4 * t + 8 + c] = lo * sn + hi * cs;
+                for (int c = 0; c < 8; c += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(&w[16 * s + c]);
+                    y[c] = x[s][c] * (scale * v.x);
+                    y[c + 1] = x[s][c + 1] * (scale * v.y);
+                    y[c + 2] = x[s][c + 2] * (scale * v.z);
+                    y[c + 3] = x[s][c + 3] * (scale * v.w);
                 }
-#pragma unroll
-            for (int k = 0; k < 64; ++k) ss += q[k] * q[k];
-            const float scale = kLog2e / 16.0f / sqrtf(xor16_sum(xor32_sum(ss)) / (float)kHd + eps);
-#pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                const float4 w = *reinterpret_cast<const float4*>(q_norm + 16 * t + 4 * g);
-                q[4 * t] *= scale * (1.0f + w.x);
-                q[4 * t + 1] *= scale * (1.0f + w.y);
-                q[4 * t + 2] *= scale * (1.0f + w.z);
-                q[4 * t + 3] *= scale * (1.0f + w.w);
+                q[s] = cut3(y);
             }
         }
 
-        f32x4 o[16];            // dims 64 t + 4 (4 g + i) + c at [4 t + c][i]
+        f32x16 o[4];                                       // dims 128 half + 32 d + row at [d]
+        auto pin = [&]() { asm volatile("" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3])); };
 #pragma unroll
-        for (int x = 0; x < 16; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[d][k] = 0.0f;
+        pin();
         float m_run = -INFINITY, l_run = 0.0f;
 
-        const int stop = min(rows, wk.t1 * kUnit);
-        for (int base = wk.t0 * kUnit; base < stop; base += kF32Rows) {
-            __syncthreads();                       // the tile before is read
-            {
-                const int r = min(base + 8 * wave, last16 + (8 * wave & 8));   // 8 rows a wave, in one 16-row group
-                const int page = page_of(table, r >> pv.page_shift, pv.max_pages, pv.n_pages);
-                const size_t at = row_offset<float>(pv, page, kvh, r);
+        // K: lane (row nn, h), dims 128 half + 16 s + 8 h ..; V of 16 rows and 32 dims:
+        // lane (dim nn, h), rows 4 h + {0 .. 3, 8 .. 11}.
+        uint32_t ka[8], va[4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    dma16((const float*)pv.k + at + k * kHd + 4 * (lane ^ ((8 * wave + k) & 15)), kaddr + k * kHd * 4);
+        for (int s = 0; s < 8; ++s)
+            ka[s] = lds_address(&st.k[0][nn][128 * half]) + 16 * ((4 * (s >> 1) + 2 * h + (s & 1)) ^ (nn & 15));
 #pragma unroll
-                for (int k = 0; k < 8; ++k) dma16((const float*)pv.v + at + k * kHd + 4 * lane, vaddr + k * kHd * 4);
+        for (int d = 0; d < 4; ++d) va[d] = lds_address(&st.v[0][4 * h][128 * half]) + 4 * (32 * (d ^ h) + nn);
+        auto k_read = [&](int s, float (&y)[8]) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const f32x4 a = *(lds_f32x4*)(ka[2 * (s & 3) + c] + 256 * (s >> 2));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[4 * c + k] = a[k];
             }
-            dma_wait();
-            __syncthreads();
-            const bool masked = base + kF32Rows - 1 > wk.start + wk.j * tm;
-            if (masked) {
-                guard_rows<0>(&vs[8 * wave][0], 8, base + 8 * wave, rows, poison, wk.start + wk.j * tm,
-                           wk.tokens - wk.j * tm, hg_shift, lane);
-                lds_barrier();
+        };
+        auto v_read = [&](int row16, int d, float (&y)[8]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = *(lds_float*)(va[d] + (row16 + (j & 3) + 8 * (j >> 2)) * kHd * 4);
+        };
+        // The wave's half of a step's scores, to its partner; beside(s) among the products.
+        f32x16 x;
+        auto scores = [&](auto beside) {
+            float y[2][8];
+            k_read(0, y[0]);
+            k_read(1, y[1]);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[k] = 0.0f;
+            Cut3 a = cut3(y[0]);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                if (s + 2 < 8) k_read(s + 2, y[s & 1]);
+                x = mul6(a, q[s], x);
+                if (s + 1 < 8) a = cut3(y[(s + 1) & 1]);
+                beside(s);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            f32x4 sa[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-            for (int t = 0; t < 16; ++t) {
-                f32x4 kf[2];
+            for (int c = 0; c < 4; ++c)
+                st.x[wave][c][lane] = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+        };
+
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-                    kf[kb] = *reinterpret_cast<const f32x4*>(&ks[16 * kb + n][4 * ((4 * t + g) ^ n)]);
+        for (int i = 0; i < 8; ++i) {
+            issue_v(i, v_from(at0), 0);
+            issue_k(i, k_from(at1), 1);
+        }
+        scores([](int) {});
+        int buf = 0;
+        // What the scores say of a step: its weights, in three parts.
+        Cut3 p[2];
+        auto weigh = [&](int s) {
+            const int base = s * kStep;
+            float sc[16];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-                        sa[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[kb][c], q[4 * t + c], sa[kb], 0, 0, 0);
+            for (int c = 0; c < 4; ++c) {
+                const float4 y = st.x[wave ^ 2][c][lane];
+                sc[4 * c] = x[4 * c] + y.x; sc[4 * c + 1] = x[4 * c + 1] + y.y;
+                sc[4 * c + 2] = x[4 * c + 2] + y.z; sc[4 * c + 3] = x[4 * c + 3] + y.w;
             }
-            float s[8], mx = -INFINITY;
+            if (base + kStep - 1 > first) {
+                asm volatile("");                          // a branch, not selects
+                const int lim = mine - base - 4 * h;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                s[k] = sa[k >> 2][k & 3];
-                if (masked) s[k] = base + 16 * (k >> 2) + 4 * g + (k & 3) <= mine ? s[k] : -INFINITY;
-                mx = fmaxf(mx, s[k]);
+                for (int k = 0; k < 16; ++k) sc[k] = 8 * (k >> 2) + (k & 3) <= lim ? sc[k] : -INFINITY;
             }
-            mx = xor16_max(xor32_max(mx));
-            if (__any(mx > m_run + kLazy)) {
+            float mx = fmaxf(sc[0], sc[1]);
+#pragma unroll
+            for (int k = 2; k < 16; ++k) mx = fmaxf(mx, sc[k]);
+            mx = xor32_max(mx);
+            if (__builtin_expect_with_probability(__any(mx > m_run + kMove), 0, 0.99)) {   // (m_run is -inf at first)
                 const float m_new = fmaxf(m_run, mx);
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
                 m_run = m_new;
                 l_run *= alpha;
+                pin();
 #pragma unroll
-                for (int x = 0; x < 16; ++x) o[x] *= alpha;
+                for (int d = 0; d < 4; ++d) o[d] *= alpha;
+                pin();
             }
             const float sub = m_run == -INFINITY ? 0.0f : m_run;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                s[k] = __builtin_amdgcn_exp2f(s[k] - sub);
-                l_run += s[k];
+            for (int k = 0; k < 16; ++k) {
+                sc[k] = __builtin_amdgcn_exp2f(sc[k] - sub);
+                l_run += sc[k];
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int c = 0; c < 2; ++c) {
+                float y[8];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(&vs[16 * (k >> 2) + 4 * g + (k & 3)][64 * t + 4 * n]);
+                for (int k = 0; k < 8; ++k) y[k] = sc[8 * c + k];
+                p[c] = cut3(y);
+            }
+        };
+        auto output = [&]() {
+            float y[2][8];
+            v_read(0, 0, y[0]);
+            v_read(0, 1, y[1]);
+            Cut3 a = cut3(y[0]);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        o[4 * t + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[c], s[k], o[4 * t + c], 0, 0, 0);
-                }
+            for (int i = 0; i < 8; ++i) {
+                if (i + 2 < 8) v_read(16 * ((i + 2) >> 2), (i + 2) & 3, y[i & 1]);
+                o[i & 3] = mul6(a, p[i >> 2], o[i & 3]);
+                if (i + 1 < 8) a = cut3(y[(i + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        auto guard = [&](int s) {
+            if (s * kStep + kStep - 1 > first)
+                guard_rows<8, 2, 1>(&st.v[buf][8 * wave][0], 8, s * kStep + 8 * wave, rows, st.poison, first,
+                                    tokens - wk.j * tm, hg_shift, lane);
+        };
+#pragma nounroll
+        for (int s = s0; s + 1 < s0 + steps; ++s) {
+            dma_wait();
+            lds_barrier();                                 // rows, and the partner's scores
+            guard(s);
+            weigh(s);
+            lds_barrier();                                 // the scores are read
+            const int flip = buf ? -kBuf : kBuf;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ka[i] += flip;
+            const void* const next_k = k_from(at2);
+            const void* const next_v = v_from(at1);
+            at1 = at2;
+            at2 = group_at(s + 3);
+            scores([&](int i) {
+                issue_k(i, next_k, buf);
+                issue_v(i, next_v, buf ^ 1);
+            });
+            output();
+#pragma unroll
+            for (int d = 0; d < 4; ++d) va[d] += flip;
+            buf ^= 1;
         }
-        __syncthreads();
-
-        l_run = xor16_sum(xor32_sum(l_run));
+        dma_wait();
+        lds_barrier();
         const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
-        const int slot = 2 * wg + (wk.t0 == 0);
-        const size_t prow = (size_t)slot * kPagedTileRows + 16 * wave + n;
-        const float inv = 1.0f / l_run;
+        float4 gate[16];                                   // of the wave's rows 16 wave ..
+        if (whole) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int at = 64 * t + 4 * (4 * g + i);
-                const float4 x = marked(make_float4(o[4 * t][i], o[4 * t + 1][i], o[4 * t + 2][i], o[4 * t + 3][i]),
-                                        poison[16 * wave + n][at >> 5] >> (at & 31));
-                if (!whole) {
-                    *reinterpret_cast<float4*>(part_o + prow * kHd + at) = x;
-                } else if (real) {
-                    const float4 gt = *reinterpret_cast<const float4*>(q_gate + qrow * 2 * kHd + kHd + at);
-                    *reinterpret_cast<float4*>(out + qrow * kHd + at) =
-                        gated(make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), gt);
-                }
-            }
-        if (!whole && g == 0) {
-            part_ml[2 * prow] = m_run;
-            part_ml[2 * prow + 1] = l_run;
+            for (int r = 0; r < 16; ++r)
+                gate[r] = reinterpret_cast<const float4*>(uniform(q_gate + row_at(wk.j, 16 * wave + r) * 2 * kHd + kHd))[lane];
         }
+        guard(s0 + steps - 1);
+        weigh(s0 + steps - 1);
+        lds_barrier();                                     // the guarded rows
+        output();
+        pin();
+
+        int j2 = uniform(wk.j);
+        asm volatile("" : "+s"(j2), "+v"(lane), "+v"(nn));
+        const int slot = 2 * wg + (wk.t0 == 0);
+        l_run = xor32_sum(l_run);
+        if (lane < 32) st.ss[wave][nn] = half ? m_run : l_run;
+        lds_barrier();                                     // K and V are read
+        float4* const os = reinterpret_cast<float4*>(&st.k[0][0][0]);
+        put_rows(os, o, rg, half, lane);
+        lds_barrier();
+        const int row = 16 * wave + (lane & 15);
+        leave_rows(
+            os, st.poison, st.ss[row >> 5][row & 31], st.ss[2 + (row >> 5)][row & 31], whole, gate,
+            part_o + (size_t)slot * kPagedTileRows * kHd, part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane,
+            [&](int r) { return token(j2, r) < tokens ? out + row_at(j2, r) * kHd : nullptr; });
+        lds_barrier();                                     // (the stores need no wait)
     }
 }
 
@@ -984,19 +1162,19 @@ __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBat
     }
 }
 
-int prefill_workgroups(const q35m_ctx* c, int type) { return type == Q35M_KV_F16 ? c->n_cu : 2 * c->n_cu; }
+int prefill_workgroups(const q35m_ctx* c) { return c->n_cu; }
 
 }  // namespace
 
 size_t paged_prefill_work_bytes(const q35m_ctx* c) {
-    return (size_t)2 * prefill_workgroups(c, Q35M_KV_F32) * kPagedTileRows * (kHd + 2) * sizeof(float);
+    return (size_t)2 * prefill_workgroups(c) * kPagedTileRows * (kHd + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, float* out) {
     q35m_ctx* c = p->ctx;
     const int per_kv = c->d.nh / c->d.nkv;
     const int hg = per_kv <= 16 ? per_kv : per_kv % 16 == 0 ? 16 : 8;
-    const int ng = per_kv / hg, nwg = prefill_workgroups(c, p->type), tm = kPagedTileRows / hg;
+    const int ng = per_kv / hg, nwg = prefill_workgroups(c), tm = kPagedTileRows / hg;
     int hg_shift = 0;
     while ((1 << hg_shift) < hg) ++hg_shift;
     float* part_o = p->work;
