@@ -769,15 +769,20 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
 // ---- fp32 cache -----------------------------------------------------------
 
 // The shape of the fp16 kernel, on steps of 32 cache rows, with every fp32 operand
-// as three bf16 values, the top 8, next 8 and last 8 bits of its mantissa (exact),
-// and the six products of an operand pair that reach 2^-16 of it: 24 bits and
-// fp32's range at six bf16 instructions, 192 cycles where the fp32 instruction
-// takes 512 for the same 32 x 32 x 16.
+// as three bf16 values, 8 bits of its mantissa each (exact), and the six products
+// of an operand pair that reach 2^-16 of it: 24 bits, with fp32's range, at six
+// bf16 instructions, 192 cycles where the fp32 instruction takes 512 for the same
+// 32 x 32 x 16.  (A cache value's last parts are lost where they fall below 2^-126.)
 // Wave (rg, half) has query rows 32 rg ..; partners split the dims: each forms the
 // scores' products of dims 128 half .. and hands them to the other, both form the
 // weights, and each adds the output dims 128 half ...
 // K and V come as fp32, K with 16-byte chunks ^ row % 16 and V with chunk ^ 8
-// (row / 4 % 2), and are cut up where they are read: six instructions a value.
+// (row / 4 % 2), and are cut up where they are read, 5.5 instructions a value, in
+// each wave for its 32 query rows: 7.3 a product, in the shadow of which they are
+// placed one stage a product (left to itself the compiler puts 40 in a row: 3050
+// cycles for 48 products instead of 2390).  133 rows over 8000: 133 us, 1000 over
+// as many: 82 us; the kernel of fp32 instructions took 165 and 112, its products
+// alone 131 and 61 at their rate.
 constexpr int kStep = 32;
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef const __attribute__((address_space(3))) f32x4 lds_f32x4;
@@ -793,32 +798,64 @@ struct F32Tile {
 struct Cut3 {
     b16x8 hi, mid, lo;
 };
-__device__ __forceinline__ Cut3 cut3(const float (&y)[8]) {
-    u32x4 a, b, c;
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-        uint32_t u[2], r[2], q[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            u[i] = __builtin_bit_cast(uint32_t, y[j + i]);
-            const float x = y[j + i] - __builtin_bit_cast(float, u[i] & 0xffff0000u);
-            r[i] = __builtin_bit_cast(uint32_t, x);
-            q[i] = __builtin_bit_cast(uint32_t, x - __builtin_bit_cast(float, r[i] & 0xffff0000u));
-        }
-        a[j / 2] = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u);     // the upper halves of two
-        b[j / 2] = __builtin_amdgcn_perm(r[1], r[0], 0x07060302u);
-        c[j / 2] = __builtin_amdgcn_perm(q[1], q[0], 0x07060302u);
-    }
-    return {__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), __builtin_bit_cast(b16x8, c)};
+__device__ __forceinline__ uint32_t bits(float x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ __forceinline__ uint32_t tops(float a, float b) {   // the upper halves of two
+    return __builtin_amdgcn_perm(bits(b), bits(a), 0x07060302u);
 }
-// c += a b, the small products first.
-__device__ __forceinline__ f32x16 mul6(const Cut3& a, const Cut3& b, f32x16 c) {
+// The three parts of eight values, in six stages of about as many instructions (the
+// remainders by masks and subtractions: the dot product with (-1, 0) that would
+// take half the instructions shares the matrix pipe, and doubles a product's time).
+struct Cutter {
+    float mid[2], lo[2];
+    u32x4 p[3];
+    __device__ __forceinline__ void value(const float (&y)[8], int j) {
+        const float hi2 = __builtin_bit_cast(float, bits(y[j]) & 0xffffff00u);      // 16 bits of the mantissa
+        lo[j & 1] = y[j] - hi2;
+        mid[j & 1] = hi2 - __builtin_bit_cast(float, bits(y[j]) & 0xffff0000u);
+    }
+    __device__ __forceinline__ void pair(const float (&y)[8], int j) {
+        p[0][j] = tops(y[2 * j], y[2 * j + 1]);
+        p[1][j] = tops(mid[0], mid[1]);
+        p[2][j] = tops(lo[0], lo[1]);
+    }
+    __device__ __forceinline__ void stage(const float (&y)[8], int i) {
+        const int j = 4 * (i / 3);
+        if (i % 3 == 0) value(y, j), value(y, j + 1);
+        if (i % 3 == 1) pair(y, j / 2), value(y, j + 2);
+        if (i % 3 == 2) value(y, j + 3), pair(y, j / 2 + 1);
+    }
+    __device__ __forceinline__ Cut3 done() const {
+        return {__builtin_bit_cast(b16x8, p[0]), __builtin_bit_cast(b16x8, p[1]), __builtin_bit_cast(b16x8, p[2])};
+    }
+};
+__device__ __forceinline__ Cut3 cut3(const float (&y)[8]) {
+    Cutter c;
+#pragma unroll
+    for (int i = 0; i < 6; ++i) c.stage(y, i);
+    return c.done();
+}
+// c += a b, the small products first, with beside(i) behind the i-th.
+template <typename F>
+__device__ __forceinline__ f32x16 mul6(const Cut3& a, const Cut3& b, f32x16 c, F beside) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.lo, b.hi, c, 0, 0, 0);
+    beside(0);
+    __builtin_amdgcn_sched_barrier(0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.lo, c, 0, 0, 0);
+    beside(1);
+    __builtin_amdgcn_sched_barrier(0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.mid, c, 0, 0, 0);
+    beside(2);
+    __builtin_amdgcn_sched_barrier(0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.mid, b.hi, c, 0, 0, 0);
+    beside(3);
+    __builtin_amdgcn_sched_barrier(0);
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.mid, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.hi, c, 0, 0, 0);
+    beside(4);
+    __builtin_amdgcn_sched_barrier(0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.hi, b.hi, c, 0, 0, 0);
+    beside(5);
+    __builtin_amdgcn_sched_barrier(0);
+    return c;
 }
 
 __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
@@ -945,7 +982,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = *(lds_float*)(va[d] + (row16 + (j & 3) + 8 * (j >> 2)) * kHd * 4);
         };
-        // The wave's half of a step's scores, to its partner; beside(s) among the products.
+        // The wave's half of a step's scores, to its partner; beside(s, i) behind the i-th
+        // product of operand s.
         f32x16 x;
         auto scores = [&](auto beside) {
             float y[2][8];
@@ -957,10 +995,12 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
                 if (s + 2 < 8) k_read(s + 2, y[s & 1]);
-                x = mul6(a, q[s], x);
-                if (s + 1 < 8) a = cut3(y[(s + 1) & 1]);
-                beside(s);
-                __builtin_amdgcn_sched_barrier(0);
+                Cutter c;
+                x = mul6(a, q[s], x, [&](int i) {
+                    if (s + 1 < 8) c.stage(y[(s + 1) & 1], i);
+                    beside(s, i);
+                });
+                if (s + 1 < 8) a = c.done();
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -972,7 +1012,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
             issue_v(i, v_from(at0), 0);
             issue_k(i, k_from(at1), 1);
         }
-        scores([](int) {});
+        scores([](int, int) {});
         int buf = 0;
         // What the scores say of a step: its weights, in three parts.
         Cut3 p[2];
@@ -1027,9 +1067,11 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (i + 2 < 8) v_read(16 * ((i + 2) >> 2), (i + 2) & 3, y[i & 1]);
-                o[i & 3] = mul6(a, p[i >> 2], o[i & 3]);
-                if (i + 1 < 8) a = cut3(y[(i + 1) & 1]);
-                __builtin_amdgcn_sched_barrier(0);
+                Cutter c;
+                o[i & 3] = mul6(a, p[i >> 2], o[i & 3], [&](int k) {
+                    if (i + 1 < 8) c.stage(y[(i + 1) & 1], k);
+                });
+                if (i + 1 < 8) a = c.done();
             }
         };
         auto guard = [&](int s) {
@@ -1051,9 +1093,9 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
             const void* const next_v = v_from(at1);
             at1 = at2;
             at2 = group_at(s + 3);
-            scores([&](int i) {
-                issue_k(i, next_k, buf);
-                issue_v(i, next_v, buf ^ 1);
+            scores([&](int i, int k) {
+                if (k == 2) issue_k(i, next_k, buf);
+                if (k == 5) issue_v(i, next_v, buf ^ 1);
             });
             output();
 #pragma unroll
@@ -1096,7 +1138,10 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
 // ---- joining cut tiles ------------------------------------------------------
 
 // 16 query rows of one tile a workgroup, where the tile's units went to several
-// workgroups: a wave four rows, a lane four dims.
+// workgroups: four rows a wave together, a lane four dims.  Bound by latency: four
+// rows' parts are asked for four at a time, their maxima and sums 16 at a time, a
+// lane each (row lane / 16).  13 parts of 36 tiles: 7 us (one row after the other,
+// 15).
 __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBatch b, const float* __restrict__ part_o,
                                                           const float* __restrict__ part_ml,
                                                           const float* __restrict__ q_gate, float* __restrict__ out,
@@ -1107,13 +1152,12 @@ __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBat
     const long per = (un.total + nwg - 1) / nwg;
     // The workgroup's tile: the sequences' tiles in order.
     int tile_end = lane < b.n ? ((b.off[lane + 1] - b.off[lane] + tm - 1) / tm) * groups : 0;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
+    for (int o = 1; o < b.n; o <<= 1) {
         const int x = __shfl_up(tile_end, o, kWave);
         if (lane >= o) tile_end += x;
     }
     const int q = blockIdx.x >> 2;
-    const int i = __popcll(__ballot(tile_end <= q));
+    const int i = __popcll(__ballot(lane < b.n && tile_end <= q));
     const int tokens = b.off[i + 1] - b.off[i];
     const Tiles ts(__builtin_amdgcn_readlane(un.start, i), tokens, hg_shift);
     const int local = q - (__builtin_amdgcn_readlane(tile_end, i) - ts.n * groups);
@@ -1122,43 +1166,56 @@ __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBat
     const long s = readlane_long(un.end, i) - each * groups + y * each + ts.ordered(o);
     const int w0 = (int)(s / per), w1 = (int)((s + ts.cnt(j) - 1) / per);
     if (w0 == w1) return;
+    const int row0 = (blockIdx.x & 3) * 16 + 4 * wave;
+    auto token = [&](int r) { return j * tm + ((row0 + r) >> hg_shift); };
+    auto row_of = [&](int r) {
+        return (size_t)(b.off[i] + min(token(r), tokens - 1)) * nh + (y << hg_shift) + ((row0 + r) & ((1 << hg_shift) - 1));
+    };
+    // Part of workgroup w: its last segment for the first one, else its first.
+    auto part = [&](int w, int r) { return (size_t)(2 * w + (w == w0)) * kPagedTileRows + row0 + r; };
+    const int mine = lane >> 4, at = lane & 15;
+    float4 gate[4], x[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        const int row = (blockIdx.x & 3) * 16 + wave * 4 + r;
-        const int tok = j * tm + (row >> hg_shift);
-        if (tok >= tokens) continue;
-        const size_t qrow = (size_t)(b.off[i] + tok) * nh + (y << hg_shift) + (row & ((1 << hg_shift) - 1));
-        const float4 gt = *reinterpret_cast<const float4*>(q_gate + qrow * 2 * kHd + kHd + 4 * lane);
-        auto part = [&](int w) { return (size_t)(2 * w + (w == w0)) * kPagedTileRows + row; };
-        float M = -INFINITY;
-        for (int w = w0 + lane; w <= w1; w += kWave) M = fmaxf(M, part_ml[2 * part(w)]);
-        M = wave_max(M);
-        const float mu = M == -INFINITY ? 0.0f : M;
-        float l = 0.0f;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        gate[r] = *reinterpret_cast<const float4*>(q_gate + row_of(r) * 2 * kHd + kHd + 4 * lane);
+        x[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float M = -INFINITY, l = 0.0f;
+    for (int w = w0 + at; w <= w1; w += 16) M = fmaxf(M, part_ml[2 * part(w, mine)]);
+    M = row_max(M);
+    const float mu = M == -INFINITY ? 0.0f : M;
+    for (int c = w0; c <= w1; c += 16) {
+        float f = 0.0f;                                    // of part c + at
+        if (c + at <= w1) {
+            // a part none of whose rows this row sees has maximum -inf
+            const float2 ml = *reinterpret_cast<const float2*>(part_ml + 2 * part(c + at, mine));
+            f = __builtin_amdgcn_exp2f(ml.x - mu);
+            l += f * ml.y;
+        }
         constexpr int U = 4;
-        for (int w = w0; w <= w1; w += U) {
-            float4 p[U];
-            float e[U], ls[U];
+        for (int w = c; w <= min(w1, c + 15); w += U) {
+            float4 p[4][U];
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                const size_t at = part(min(w + k, w1));
-                p[k] = reinterpret_cast<const float4*>(part_o + at * kHd)[lane];
-                e[k] = part_ml[2 * at];
-                ls[k] = part_ml[2 * at + 1];
-            }
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int k = 0; k < U; ++k) p[r][k] = reinterpret_cast<const float4*>(part_o + part(min(w + k, w1), r) * kHd)[lane];
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 if (w + k > w1) break;
-                // a part none of whose rows this row sees has maximum -inf
-                const float f = __builtin_amdgcn_exp2f(e[k] - mu);
-                l += f * ls[k];
-                x.x += f * p[k].x; x.y += f * p[k].y; x.z += f * p[k].z; x.w += f * p[k].w;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float g = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), 16 * r + w + k - c));
+                    x[r].x += g * p[r][k].x; x[r].y += g * p[r][k].y; x[r].z += g * p[r][k].z; x[r].w += g * p[r][k].w;
+                }
             }
         }
-        const float inv = 1.0f / l;
-        *reinterpret_cast<float4*>(out + qrow * kHd + 4 * lane) =
-            gated(make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), gt);
+    }
+    const float inv_l = 1.0f / row_sum(l);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float inv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv_l), 16 * r));
+        x[r] = gated(make_float4(x[r].x * inv, x[r].y * inv, x[r].z * inv, x[r].w * inv), gate[r]);
+        if (token(r) < tokens) *reinterpret_cast<float4*>(out + row_of(r) * kHd + 4 * lane) = x[r];
     }
 }
 
