@@ -34,14 +34,20 @@ public:
     int page(int seq, int i) const { return table_[(size_t)seq * max_pages_ + i]; }
     bool has(int seq) const { return seq >= 0 && seq < n_seqs_; }
 
-    // Entries [first, first + n) of seq become pages[0 .. n) (null: unmapped).
-    // Nothing changes unless every argument is good.
-    Result map(int seq, int first, int n, const int* pages) {
+    // Whether map() would take these arguments.
+    Result can_map(int seq, int first, int n, const int* pages) const {
         if (!has(seq)) return kBadSeq;
         if (first < 0 || n < 0 || first > max_pages_ - n) return kBadRange;
         if (pages)
             for (int i = 0; i < n; ++i)
                 if (pages[i] < 0 || pages[i] >= n_pages_) return kBadPage;
+        return kOk;
+    }
+    // Entries [first, first + n) of seq become pages[0 .. n) (null: unmapped).
+    // Nothing changes unless every argument is good.
+    Result map(int seq, int first, int n, const int* pages) {
+        const Result r = can_map(seq, first, n, pages);
+        if (r != kOk) return r;
         int* t = &table_[(size_t)seq * max_pages_];
         for (int i = 0; i < n; ++i) {
             if (t[first + i] >= 0) --refs_[t[first + i]];

@@ -229,10 +229,11 @@ int q35m_paged_map(q35m_paged* p, int seq, int first, int n, const int* pages) {
     DeviceScope dev(p->ctx->device);
     int r = not_capturing(p, "paged_map");
     if (r) return r;
-    const q35::PageMap::Result m = p->map.map(seq, first, n, pages);
+    const q35::PageMap::Result m = p->map.can_map(seq, first, n, pages);
     if (m != q35::PageMap::kOk) return map_fail(p, m, seq);
     PHIP_TRY(q35::launch_paged_table(p->ctx, p->dev_table, (size_t)seq * p->map.max_pages() + first, pages, n),
              "paged_map");
+    (void)p->map.map(seq, first, n, pages);
     return Q35M_OK;
 }
 

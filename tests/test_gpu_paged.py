@@ -396,6 +396,65 @@ def test_prefill_longer(kv_type, start, T):
 
 
 @pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
+def test_prefill_full_batch(kv_type):
+    """64 sequences of 0 to 150 rows with chunks of 0 to 4 tokens each."""
+    lens, tokens = [(29 * i * i) % 151 for i in range(64)], [(7 * i) % 5 for i in range(64)]
+    T = sum(tokens)
+    with Paged(kv_type, nh=4, nkv=2, n_seqs=64, max_rows=155, page_rows=16, salt=11) as p:
+        p.seed_rows(lens, salt=3)
+        x = p.inputs(T, salt=67)
+        out = p.ctx.array((T, p.nh * HD))
+        p.c.attn_prefill(0, list(range(64)), tokens, *p.dev(x, "q_gate", "k", "v"), out)
+        p.put(range(64), tokens, x)
+        say(f"prefill of 64: {close_to(out.download(), p.attend(range(64), tokens, x)):.1e}")
+        p.check_pages()
+
+
+@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
+@pytest.mark.parametrize("max_rows", [117, 128])
+def test_a_sequence_filled_to_its_last_row(kv_type, max_rows):
+    """A chunk and then single tokens up to row max_rows - 1; the next is refused."""
+    with Paged(kv_type, n_seqs=1, max_rows=max_rows, page_rows=16, spare=0) as p:
+        T = max_rows - 2
+        x = p.inputs(max_rows, salt=68)
+        parts = [{k: v[a:b] for k, v in x.items()} for a, b in ((0, T), (T, T + 1), (T + 1, T + 2))]
+        some = [0, 15, 16, 63, 64, T - 1]
+        for part, n in zip(parts, (T, 1, 1)):
+            out = p.ctx.array((n, p.nh * HD))
+            d = p.dev(part, "q_gate", "k", "v")
+            p.c.attn_prefill(0, [0], [n], *d, out) if n > 1 else p.c.attn_decode(0, [0], *d, out)
+            p.put([0], [n], part)
+            close_to(out.download(), p.attend([0], [n], part, some if n > 1 else None))
+            p.step([n])
+        p.check_pages()
+        for call in (lambda: p.c.attn_decode(0, [0], *d, out), lambda: p.c.attn_prefill(0, [0], [1], *d, out)):
+            refused(q35mix.ERR_CAPACITY, call)
+
+
+def test_fp32_values_far_beyond_fp16():
+    """V of 2^100 in one head and of 2^-90 in another (2^-14 of it is still a normal number): fp32 all the way."""
+    T, n = 37, 300
+    with Paged(KV_F32, nh=4, nkv=2, n_seqs=1, max_rows=n + T, page_rows=64) as p:
+        p.seed_rows([n], salt=9)
+        scale = np.array([2.0 ** 100, 2.0 ** -90], np.float32)
+        t = np.arange(n)
+        p.pages[1][p.table[0][t // p.R], :, t % p.R] = p.rows_of(0, n, 1) * scale[:, None]
+        p.push()
+        x = {k: v.copy() for k, v in p.inputs(T, salt=69).items()}
+        x["v"] = (x["v"].reshape(T, 2, HD) * scale[:, None]).reshape(T, 2 * HD)
+        out, one = p.ctx.array((T, p.nh * HD)), p.ctx.array((1, p.nh * HD))
+        d = p.dev(x, "q_gate", "k", "v")
+        p.c.attn_decode(0, [0], *d, one)
+        p.c.attn_prefill(0, [0], [T], *d, out)
+        p.put([0], [T], x)
+        want, got, first = p.attend([0], [T], x), out.download(), one.download()
+        for heads in (slice(0, 2 * HD), slice(2 * HD, 4 * HD)):
+            close_to(got[:, heads], want[:, heads])
+            close_to(first[:, heads], want[:1, heads])
+        p.check_pages()
+
+
+@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
 def test_prefill_values_not_finite_stay_where_they_are_seen(kv_type, value):
     """A V value that is not finite reaches the tokens that see its row, in its dim and heads, and no other output."""
