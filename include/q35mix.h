@@ -246,7 +246,8 @@ typedef struct q35m_paged q35m_paged;
 /* How a cache holds K and V: fp32, or fp16 (half the memory and the traffic:
  * the values of an fp32 cache, rounded to nearest even when their row is
  * written, beyond the range of fp16 to infinities; activations and outputs are
- * fp32, and the attention adds no rounding beyond fp32's). */
+ * fp32, and the attention adds no rounding beyond fp32's, but that
+ * q35m_paged_attn_prefill takes the bits of an fp32 value below 2^-126 as 0). */
 #define Q35M_KV_F32 0
 #define Q35M_KV_F16 1
 

@@ -170,7 +170,7 @@ __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" :
 // becomes zero too (0 x inf is NaN in the products of the query rows that do not
 // see it), and the outputs of the query rows that do are marked in `poison`, a
 // bit a (query row, dim), which turns them to NaN at the segment's end.  A wave
-// takes `count` rows of kHd values from v on; base: their first row's position.
+// takes COUNT rows of kHd values from v on; base: their first row's position.
 // (Rows up to `first` are seen by all of the tile.)
 __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 __device__ __forceinline__ bool not_finite(_Float16 x) {
@@ -184,12 +184,17 @@ __device__ __forceinline__ float4 marked(float4 x, uint32_t nan) {
     return make_float4(one(x.x, 0), one(x.y, 1), one(x.z, 2), one(x.w, 3));
 }
 // 16-byte chunks are permuted by row: chunk ^ S ((row >> H) & M).
-template <int S, int H, int M, typename T>
-__device__ __forceinline__ void guard_rows(T* v, int count, int base, int rows, uint32_t (*poison)[kHd / 32], int first,
+template <int COUNT, int S, int H, int M, typename T>
+__device__ __forceinline__ void guard_rows(T* v, int base, int rows, uint32_t (*poison)[kHd / 32], int first,
                                            int tokens_left, int hg_shift, int lane) {
     constexpr int E = 16 / sizeof(T);          // values of 16 bytes
     typedef T vec __attribute__((ext_vector_type(E)));
-    constexpr int U = 4;                       // chunks a lane looks at together
+    if (base >= rows) {
+#pragma unroll
+        for (int x = 0; x < COUNT * (kHd / E); x += kWave) *reinterpret_cast<vec*>(v + (x + lane) * E) = vec{};
+        return;
+    }
+    constexpr int count = COUNT, U = 4;        // U chunks a lane looks at together
 #pragma nounroll
     for (int x0 = max(0, first + 1 - base) * (kHd / E) + lane; x0 < count * (kHd / E); x0 += U * kWave) {
         vec y[U];
@@ -411,7 +416,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
     Walk wk;
     wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
-        const int start = uniform(wk.start), tokens = uniform(wk.tokens), first_row = uniform(b.off[wk.i]);
+        const int start = uniform(wk.start), tokens = uniform(wk.tokens);
         const int seq = b.seq[wk.i], kvh = wk.y / ng;
         const int* table = pv.table + (size_t)seq * pv.max_pages;
         // (the lane's own places as values of this segment: addresses made of them
@@ -424,11 +429,11 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         const int last16 = (rows - 1) & ~15;
         const int first = uniform(start + wk.j * tm);          // position of the tile's first token
         const int mine = min(start + min(wk.j * tm + ((32 * rg + nn) >> hg_shift), tokens - 1), pv.max_rows - 1);
-        // Query row r of the tile: token, and the row of q and out.
-        auto token = [&](int j, int r) { return j * tm + (r >> hg_shift); };
-        auto row_at = [&](int j, int r) {
-            return (size_t)(first_row + min(token(j, r), tokens - 1)) * nh + (wk.y << hg_shift) + (r & (hg - 1));
-        };
+        // Query row r of the tile is row row0 + from_row0(r) of q and out (the last
+        // token's for rows past the `left` tokens).
+        const int left = uniform(tokens - wk.j * tm);
+        const long row0 = uniform((long)(uniform(b.off[wk.i]) + wk.j * tm) * nh + (wk.y << hg_shift));
+        auto from_row0 = [&](int r) { return min(r >> hg_shift, left - 1) * nh + (r & (hg - 1)); };
 
         // A wave brings its 16 rows of a unit's K or V.  It holds 64 entries of the
         // page table, one a lane, from entry `held` on.
@@ -457,7 +462,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         const float4* const qs = reinterpret_cast<const float4*>(&st.v[0][0][0]);
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-            dma_pair(0, uniform(q_gate + row_at(wk.j, r) * 2 * kHd), 16 * (lane ^ (r & 31)),
+            dma_pair(0, uniform(q_gate + row0 * 2 * kHd + from_row0(r) * 2 * kHd), 16 * (lane ^ (r & 31)),
                      lds_address(&st.v[0][0][0]) + r * kHd * 4);
         // Where the wave's rows of the next units lie: found a unit before they are asked for.
         const size_t at0 = group_at(wk.t0);
@@ -678,8 +683,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         // unit), every wave is past the buffers that the next rows go to.
         auto guard = [&]() {
             if (masked(t)) {
-                guard_rows<4, 0, 3>(&st.v[buf][16 * wave][0], 16, t * kUnit + 16 * wave, rows, st.poison, first,
-                              tokens - wk.j * tm, hg_shift, lane);
+                guard_rows<16, 4, 0, 3>(&st.v[buf][16 * wave][0], t * kUnit + 16 * wave, rows, st.poison, first,
+                              left, hg_shift, lane);
                 lds_barrier();
             }
         };
@@ -732,7 +737,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         if (whole) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                gate[r] = reinterpret_cast<const float4*>(uniform(q_gate + row_at(wk.j, 16 * wave + r) * 2 * kHd + kHd))[lane];
+                gate[r] = reinterpret_cast<const float4*>(
+                    uniform(q_gate + row0 * 2 * kHd + from_row0(16 * wave + r) * 2 * kHd + kHd))[lane];
         }
         guard();
         add(v1, h1, l1);
@@ -747,8 +753,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         // The tile's rows to LDS, then a row a wave at a time: finished, or as a part
         // to the workspace.  (Places again as values of this part: kept from the
         // segment's beginning they would be in registers all the while.)
-        int j2 = uniform(wk.j);
-        asm volatile("" : "+s"(j2), "+v"(lane), "+v"(nn));
+        asm volatile("" : "+v"(lane), "+v"(nn));
         const int slot = 2 * wg + (wk.t0 == 0);
         l_run = xor32_sum(l_run);
         if (lane < 32) st.mx[1][wave][nn] = l_run;
@@ -761,7 +766,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         leave_rows(
             os, st.poison, st.mx[1][row >> 5][row & 31] + st.mx[1][2 + (row >> 5)][row & 31], st.mx[0][row >> 5][row & 31],
             whole, gate, part_o + (size_t)slot * kPagedTileRows * kHd, part_ml + (size_t)2 * slot * kPagedTileRows, wave,
-            lane, [&](int r) { return token(j2, r) < tokens ? out + row_at(j2, r) * kHd : nullptr; });
+            lane, [&](int r) { return r >> hg_shift < left ? out + row0 * kHd + from_row0(r) * kHd : nullptr; });
         lds_barrier();                                     // (the stores need no wait)
     }
 }
@@ -772,7 +777,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
 // as three bf16 values, 8 bits of its mantissa each (exact), and the six products
 // of an operand pair that reach 2^-16 of it: 24 bits, with fp32's range, at six
 // bf16 instructions, 192 cycles where the fp32 instruction takes 512 for the same
-// 32 x 32 x 16.  (A cache value's last parts are lost where they fall below 2^-126.)
+// 32 x 32 x 16.  Those instructions take parts below 2^-126 as 0, so a value below
+// 2^-110 loses its last bits (2^-16 of it at 2^-118).
 // Wave (rg, half) has query rows 32 rg ..; partners split the dims: each forms the
 // scores' products of dims 128 half .. and hands them to the other, both form the
 // weights, and each adds the output dims 128 half ...
@@ -878,7 +884,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
     Walk wk;
     wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
-        const int start = uniform(wk.start), tokens = uniform(wk.tokens), first_row = uniform(b.off[wk.i]);
+        const int start = uniform(wk.start), tokens = uniform(wk.tokens);
         const int seq = b.seq[wk.i], kvh = wk.y / ng;
         const int* table = pv.table + (size_t)seq * pv.max_pages;
         int lane = tid & 63, nn = lane & 31;
@@ -888,10 +894,11 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         const int last16 = (rows - 1) & ~15;
         const int first = uniform(start + wk.j * tm);     // position of the tile's first token
         const int mine = min(start + min(wk.j * tm + ((32 * rg + nn) >> hg_shift), tokens - 1), pv.max_rows - 1);
-        auto token = [&](int j, int r) { return j * tm + (r >> hg_shift); };
-        auto row_at = [&](int j, int r) {
-            return (size_t)(first_row + min(token(j, r), tokens - 1)) * nh + (wk.y << hg_shift) + (r & (hg - 1));
-        };
+        // Query row r of the tile is row row0 + from_row0(r) of q and out (the last
+        // token's for rows past the `left` tokens).
+        const int left = uniform(tokens - wk.j * tm);
+        const long row0 = uniform((long)(uniform(b.off[wk.i]) + wk.j * tm) * nh + (wk.y << hg_shift));
+        auto from_row0 = [&](int r) { return min(r >> hg_shift, left - 1) * nh + (r & (hg - 1)); };
 
         // A wave brings 8 rows of a step's K and V; it holds 64 entries of the page
         // table, one a lane, from entry `held` on.
@@ -923,7 +930,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         const float4* const qs = reinterpret_cast<const float4*>(&st.v[0][0][0]);
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-            dma_pair(0, uniform(q_gate + row_at(wk.j, r) * 2 * kHd), 16 * (lane ^ (r & 31)),
+            dma_pair(0, uniform(q_gate + row0 * 2 * kHd + from_row0(r) * 2 * kHd), 16 * (lane ^ (r & 31)),
                      lds_address(&st.v[0][0][0]) + r * kHd * 4);
         const size_t at0 = group_at(s0);
 #pragma unroll
@@ -1076,8 +1083,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         };
         auto guard = [&](int s) {
             if (s * kStep + kStep - 1 > first)
-                guard_rows<8, 2, 1>(&st.v[buf][8 * wave][0], 8, s * kStep + 8 * wave, rows, st.poison, first,
-                                    tokens - wk.j * tm, hg_shift, lane);
+                guard_rows<8, 8, 2, 1>(&st.v[buf][8 * wave][0], s * kStep + 8 * wave, rows, st.poison, first,
+                                    left, hg_shift, lane);
         };
 #pragma nounroll
         for (int s = s0; s + 1 < s0 + steps; ++s) {
@@ -1109,7 +1116,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         if (whole) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                gate[r] = reinterpret_cast<const float4*>(uniform(q_gate + row_at(wk.j, 16 * wave + r) * 2 * kHd + kHd))[lane];
+                gate[r] = reinterpret_cast<const float4*>(
+                    uniform(q_gate + row0 * 2 * kHd + from_row0(16 * wave + r) * 2 * kHd + kHd))[lane];
         }
         guard(s0 + steps - 1);
         weigh(s0 + steps - 1);
@@ -1117,8 +1125,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         output();
         pin();
 
-        int j2 = uniform(wk.j);
-        asm volatile("" : "+s"(j2), "+v"(lane), "+v"(nn));
+        asm volatile("" : "+v"(lane), "+v"(nn));
         const int slot = 2 * wg + (wk.t0 == 0);
         l_run = xor32_sum(l_run);
         if (lane < 32) st.ss[wave][nn] = half ? m_run : l_run;
@@ -1130,7 +1137,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         leave_rows(
             os, st.poison, st.ss[row >> 5][row & 31], st.ss[2 + (row >> 5)][row & 31], whole, gate,
             part_o + (size_t)slot * kPagedTileRows * kHd, part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane,
-            [&](int r) { return token(j2, r) < tokens ? out + row_at(j2, r) * kHd : nullptr; });
+            [&](int r) { return r >> hg_shift < left ? out + row0 * kHd + from_row0(r) * kHd : nullptr; });
         lds_barrier();                                     // (the stores need no wait)
     }
 }
