@@ -29,7 +29,9 @@
 // (hi + lo, 22 bits; q's row and P scaled by powers of two into the range),
 // and a register transpose of V (8 rows x 8 dims a lane).
 // The waves share the forming of q rows through LDS: formed in every wave, behind
-// K and V in the queue of loads, they cost a call over 8192 rows 2 of its 13 us.
+// K and V in the queue of loads, they cost a call over 8192 rows 2 of its 13 us
+// (now 9.4, of which the 33.5 MB take 4.9 and two launches the most of the rest).
+// Two tiles a wave in flight instead of one spill, and K's alone are no faster.
 #include "paged_device.h"
 
 namespace q35 {
@@ -41,31 +43,49 @@ constexpr float kLog2e = 1.4426950408889634f;
 // that fp32 holds (the normalisation divides the factor out).
 constexpr float kPShift = 7.0f;
 
-template <typename T>
+// How a wave reads K.  The operand's own shape, 16 rows x 64 bytes an instruction,
+// takes half a cache line of a row at a time, which reads slower than whole lines:
+// 120 us against 112 for 64 sequences of up to 4000 fp16 rows (709 MB, 6.3 TB/s),
+// 247 against 220 for 8 of up to 32768 fp32 rows (1.52 GB, 6.9 TB/s).  (Whole lines
+// and an exchange between lanes l and l ^ 8 in front of the products: 128 and 261.)
+// So up to 8 q heads (S) it is 8 rows x 128 bytes: a lane has row l % 8 and 16-byte chunk 2 g +
+// l / 8 % 2 of the line, g = l / 16.  As an operand these are 16 rows of which the
+// upper 8 are the lower ones' odd chunks; q's columns are as well: column n < 8 is
+// head n's even chunks, column n + 8 its odd ones.  The product's quarter (lower
+// rows, lower columns) is the even chunks' part of a score and the quarter (upper,
+// upper) the odd ones'; the rest is not used.  joined() adds the two, of a product
+// of rows 0 .. 7 and one of rows 8 .. 15: to lane (n, g) rows 4 g + i.
+__device__ __forceinline__ float joined(float a, float b) {
+    const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
+    return __builtin_bit_cast(float, (uint32_t)x[0]) + row_xor<8>(__builtin_bit_cast(float, (uint32_t)x[1]));
+}
+
+template <typename T, bool S>
 struct Tile;
 
 // 16 rows of an fp32 cache a wave.
-template <>
-struct Tile<float> {
+template <bool S>
+struct Tile<float, S> {
     static constexpr int kRows = 16;
-    float q[64];            // dims 16 t + 4 g + c at [4 t + c]
-    float4 k[16], v[4][4];  // K row l % 16, dims 16 t + 4 g; V row 4 g + i, dims 64 t + 4 m
+    float q[S ? 32 : 64];   // dims 16 t + 4 g + c at [4 t + c]; S: 32 t + 8 g + 4 (l / 8 % 2) + c
+    float4 k[16], v[4][4];  // K row l % 16, dims 16 t + 4 g (S: see above, rows 0 .. 7 at [2 t]); V row 4 g + i, dims 64 t + 4 m
     f32x4 o[16];            // dims 64 t + 4 row + c at [4 t + c]
 
     // q row n in LDS, 16-byte chunks permuted: chunk ^ n.
     static __device__ __forceinline__ void put_q(float4* row, int r, float4 x, int lane) { row[lane ^ r] = x; }
-    __device__ __forceinline__ void load_q(const float4* row, int n, int g) {
+    __device__ __forceinline__ void load_q(const float4* row, int n, int lane) {
+        const int g = lane >> 4, odd = (lane >> 3) & 1;
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            const float4 a = row[(4 * t + g) ^ n];
+        for (int t = 0; t < (S ? 8 : 16); ++t) {
+            const float4 a = row[(S ? 8 * t + 2 * g + odd : 4 * t + g) ^ n];
             q[4 * t] = a.x; q[4 * t + 1] = a.y; q[4 * t + 2] = a.z; q[4 * t + 3] = a.w;
         }
     }
 
     __device__ __forceinline__ void load_k(const float* p, int, int lane) {
-        const float* a = p + (lane & 15) * kHd + 4 * (lane >> 4);
+        const float* a = p + (lane & (S ? 7 : 15)) * kHd + 4 * (lane >> (S ? 3 : 4));
 #pragma unroll
-        for (int t = 0; t < 16; ++t) k[t] = load_nt(a + 16 * t);
+        for (int t = 0; t < 16; ++t) k[t] = load_nt(a + (S ? 32 * (t >> 1) + 8 * (t & 1) * kHd : 16 * t));
     }
     __device__ __forceinline__ void load_v(const float* p, int, int lane) {
         const float* a = p + (lane >> 4) * 4 * kHd + 4 * (lane & 15);
@@ -80,7 +100,11 @@ struct Tile<float> {
         const int g = lane >> 4, m = lane & 15;
 #pragma unroll
         for (int t = 0; t < 16; ++t)
-            if (m == at) k[t] = *reinterpret_cast<const float4*>(kn + 16 * t + 4 * g);
+            if (S) {
+                if ((m & 7) + 8 * (t & 1) == at) k[t] = *reinterpret_cast<const float4*>(kn + 32 * (t >> 1) + 4 * (lane >> 3));
+            } else if (m == at) {
+                k[t] = *reinterpret_cast<const float4*>(kn + 16 * t + 4 * g);
+            }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -91,15 +115,29 @@ struct Tile<float> {
     }
     __device__ __forceinline__ void scores(float (&s)[4]) const {
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+        if constexpr (S) {
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].x, q[4 * t], a, 0, 0, 0);
-            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].y, q[4 * t + 1], b, 0, 0, 0);
-            a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].z, q[4 * t + 2], a, 0, 0, 0);
-            b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].w, q[4 * t + 3], b, 0, 0, 0);
+            for (int t = 0; t < 8; ++t) {
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[2 * t].x, q[4 * t], a, 0, 0, 0);
+                b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[2 * t + 1].x, q[4 * t], b, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[2 * t].y, q[4 * t + 1], a, 0, 0, 0);
+                b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[2 * t + 1].y, q[4 * t + 1], b, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[2 * t].z, q[4 * t + 2], a, 0, 0, 0);
+                b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[2 * t + 1].z, q[4 * t + 2], b, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[2 * t].w, q[4 * t + 3], a, 0, 0, 0);
+                b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[2 * t + 1].w, q[4 * t + 3], b, 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].x, q[4 * t], a, 0, 0, 0);
+                b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].y, q[4 * t + 1], b, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].z, q[4 * t + 2], a, 0, 0, 0);
+                b = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t].w, q[4 * t + 3], b, 0, 0, 0);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = a[i] + b[i];
+        for (int i = 0; i < 4; ++i) s[i] = S ? joined(a[i], b[i]) : a[i] + b[i];
     }
     static __device__ __forceinline__ int row_of(int i, int g) { return 4 * g + i; }
     static constexpr int kScores = 4;
@@ -126,11 +164,11 @@ struct Tile<float> {
 };
 
 // 32 rows of an fp16 cache a wave, as two groups of 16.
-template <>
-struct Tile<_Float16> {
+template <bool S>
+struct Tile<_Float16, S> {
     static constexpr int kRows = 32;
-    f16x8 qh[8], ql[8];        // dims 32 t + 8 g ..
-    u32x4 k[2][8], v[2][8];    // K row l % 16 of group kb, dims 32 t + 8 g; V row 16 (j / 4) + 4 g + j % 4, dims 128 u + 8 m
+    f16x8 qh[S ? 4 : 8], ql[S ? 4 : 8];        // dims 32 t + 8 g ..; S: 64 t + 16 g + 8 (l / 8 % 2) ..
+    u32x4 k[2][8], v[2][8];    // K row l % 16 of group kb, dims 32 t + 8 g (S: as above); V row 16 (j / 4) + 4 g + j % 4, dims 128 u + 8 m
     f32x4 o[16];               // dims 128 u + 8 row + b at [8 u + b]
 
     // The row, already scaled into fp16's range, as hi (chunks 0 .. 31) and lo.
@@ -143,18 +181,22 @@ struct Tile<_Float16> {
         f16x2* const to = reinterpret_cast<f16x2*>(row + (32 + (lane >> 1) ^ r)) + 2 * (lane & 1);
         to[0] = l[0]; to[1] = l[1];
     }
-    __device__ __forceinline__ void load_q(const float4* row, int n, int g) {
+    __device__ __forceinline__ void load_q(const float4* row, int n, int lane) {
+        const int g = lane >> 4, odd = (lane >> 3) & 1;
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            qh[t] = __builtin_bit_cast(f16x8, row[(4 * t + g) ^ n]);
-            ql[t] = __builtin_bit_cast(f16x8, row[(32 + 4 * t + g) ^ n]);
+        for (int t = 0; t < (S ? 4 : 8); ++t) {
+            const int at = S ? 8 * t + 2 * g + odd : 4 * t + g;
+            qh[t] = __builtin_bit_cast(f16x8, row[at ^ n]);
+            ql[t] = __builtin_bit_cast(f16x8, row[(32 + at) ^ n]);
         }
     }
 
     __device__ __forceinline__ void load_k(const _Float16* p, int kb, int lane) {
-        const _Float16* a = p + (lane & 15) * kHd + 8 * (lane >> 4);
+        const _Float16* a = p + (lane & (S ? 7 : 15)) * kHd + 8 * (lane >> (S ? 3 : 4));
 #pragma unroll
-        for (int t = 0; t < 8; ++t) k[kb][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a + 32 * t));
+        for (int t = 0; t < 8; ++t)
+            k[kb][t] = __builtin_nontemporal_load(
+                reinterpret_cast<const u32x4*>(a + (S ? 64 * (t >> 1) + 8 * (t & 1) * kHd : 32 * t)));
     }
     __device__ __forceinline__ void load_v(const _Float16* p, int kb, int lane) {
         const _Float16* a = p + (lane >> 4) * 4 * kHd + 8 * (lane & 15);
@@ -170,7 +212,12 @@ struct Tile<_Float16> {
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int t = 0; t < 8; ++t)
-                if (16 * kb + m == at) k[kb][t] = *reinterpret_cast<const u32x4*>(kn + 32 * t + 8 * g);
+                if (S) {
+                    if (16 * kb + (m & 7) + 8 * (t & 1) == at)
+                        k[kb][t] = *reinterpret_cast<const u32x4*>(kn + 64 * (t >> 1) + 8 * (lane >> 3));
+                } else if (16 * kb + m == at) {
+                    k[kb][t] = *reinterpret_cast<const u32x4*>(kn + 32 * t + 8 * g);
+                }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -181,21 +228,39 @@ struct Tile<_Float16> {
             }
     }
     __device__ __forceinline__ void scores(float (&s)[8]) const {
-        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+        if constexpr (S) {
+            f32x4 a[4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            // 8 rows each; the low halves' products first
+            auto all = [&](const f16x8 (&q)[4]) {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[0][t]), ql[t], a, 0, 0, 0);
-            b = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[1][t]), ql[t], b, 0, 0, 0);
-        }
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[0][t]), qh[t], a, 0, 0, 0);
-            b = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[1][t]), qh[t], b, 0, 0, 0);
-        }
+                    for (int r = 0; r < 4; ++r)
+                        a[r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[r >> 1][2 * t + (r & 1)]), q[t], a[r], 0, 0, 0);
+            };
+            all(ql);
+            all(qh);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[i] = a[i];
-            s[4 + i] = b[i];
+            for (int i = 0; i < 4; ++i) {
+                s[i] = joined(a[0][i], a[1][i]);
+                s[4 + i] = joined(a[2][i], a[3][i]);
+            }
+        } else {
+            f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+            auto all = [&](const f16x8 (&q)[8]) {
+#pragma unroll
+                for (int t = 0; t < 8; ++t) {
+                    a = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[0][t]), q[t], a, 0, 0, 0);
+                    b = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k[1][t]), q[t], b, 0, 0, 0);
+                }
+            };
+            all(ql);
+            all(qh);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[i] = a[i];
+                s[4 + i] = b[i];
+            }
         }
     }
     static __device__ __forceinline__ int row_of(int j, int g) { return 16 * (j >> 2) + 4 * g + (j & 3); }
@@ -238,7 +303,7 @@ struct Units {
 };
 template <typename T>
 __device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch& b, int groups, int lane) {
-    constexpr int kUnit = 4 * Tile<T>::kRows;
+    constexpr int kUnit = 4 * Tile<T, true>::kRows;
     Units u;
     // (the row past max_rows of a replayed call that its caller let run over)
     u.rows = lane < b.n ? min(pv.lens[b.seq[lane]] + 1, pv.max_rows) : 0;
@@ -253,14 +318,14 @@ __device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch&
     return u;
 }
 
-template <typename T>
+template <typename T, bool S>
 __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
                                                       const float* __restrict__ knew, const float* __restrict__ vnew,
                                                       const float* __restrict__ q_norm,
                                                       const float* __restrict__ k_norm, float* __restrict__ out,
                                                       float* __restrict__ part_o, float* __restrict__ part_ml, int hg,
                                                       int ng, float eps) {
-    using Tl = Tile<T>;
+    using Tl = Tile<T, S>;
     constexpr int R = Tl::kRows;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -377,8 +442,8 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
         }
         lds_barrier();
         {
-            const int r = min(n, hg - 1);        // columns from hg on are never read
-            tl.load_q(qbuf[r], r, g);
+            const int r = min(S ? n & 7 : n, hg - 1);      // columns from hg on are never read
+            tl.load_q(qbuf[r], r, lane);
         }
 
         float m_run = -INFINITY, l_run = 0.0f;
@@ -557,8 +622,11 @@ hipError_t launch_paged_decode(q35m_paged* p, int layer, const PagedBatch& b, co
                               part_ml, q_gate, out, hg, ng, nwg);
         return hipGetLastError();
     };
-    if (p->type == Q35M_KV_F16) return go(paged_decode<_Float16>, paged_decode_merge<_Float16>);
-    return go(paged_decode<float>, paged_decode_merge<float>);
+    if (p->type == Q35M_KV_F16)
+        return hg <= 8 ? go(paged_decode<_Float16, true>, paged_decode_merge<_Float16>)
+                       : go(paged_decode<_Float16, false>, paged_decode_merge<_Float16>);
+    return hg <= 8 ? go(paged_decode<float, true>, paged_decode_merge<float>)
+                   : go(paged_decode<float, false>, paged_decode_merge<float>);
 }
 
 }  // namespace q35
