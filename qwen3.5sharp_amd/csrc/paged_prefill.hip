@@ -20,8 +20,9 @@
 //
 // The products are the bound (4 x 256 flop a q head and visible row).
 // Scores are formed as S^T = K Q^T and the output as O^T = V^T P^T: P^T's operand
-// is S^T's own register layout, so P never crosses lanes, and the softmax's
-// statistics of a query row are one lane's (and its partner's) registers.
+// is S^T's own register layout, so weights cross no lanes (the two waves that share
+// query rows pass them on, or the halves of the scores, in that layout), and the
+// softmax's statistics of a query row are registers of its lanes.
 #include "paged_device.h"
 
 namespace q35 {
@@ -154,15 +155,11 @@ struct Walk {
 
 // ---- loads, and rows that not every query sees ----------------------------
 
-// 16 bytes a lane from global memory straight to LDS at address at + 16 lane (at
-// the same in every lane).  Complete once vmcnt says so: dma_wait() before the
-// barrier that publishes the rows.  The instruction is written out because the
-// compiler, told of it, waits for all such loads before the next LDS read, also
-// one of the other buffer.
+// Loads straight to LDS (dma_nth below): 16 bytes a lane, to address at + 16 lane.
+// Complete once vmcnt says so: dma_wait() before the barrier that publishes the
+// rows.  The instruction is written out because the compiler, told of it, waits for
+// all such loads before the next LDS read, also one of the other buffer.
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const lds_void*)p; }
-__device__ __forceinline__ void dma16(const void* p, uint32_t at) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(p) : "memory");
-}
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // V rows of a unit that not every query row of the tile sees.  Rows past the
@@ -372,20 +369,21 @@ typedef const __attribute__((address_space(3))) f16x8 lds_f16x8;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// The i-th of eight loads of dma16 for 16 rows of 512 bytes, two rows each: global
-// rows from `from` on, LDS rows from `at` on; off: the lane's place in two rows.
+// The i-th of eight loads for 8 KiB: global memory from `from` on, LDS
+// from `at` on, 1 KiB each; off: the lane's place in that KiB of global memory.
 // (The offset in the instruction counts on both sides.)
-__device__ __forceinline__ void dma_pair(int i, const void* from, uint32_t off, uint32_t at) {
-#define Q35_DMA_PAIR(imm)                                                                                     \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:" imm ::"s"(at), "v"(off), \
-                 "s"(from)                                                                                    \
-                 : "memory")
+template <int K>
+__device__ __forceinline__ void dma_kib(const void* from, uint32_t off, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(at), "v"(off), "s"(from),
+                 "n"(1024 * K)
+                 : "memory");
+}
+__device__ __forceinline__ void dma_nth(int i, const void* from, uint32_t off, uint32_t at) {
     if (i & 4) at += 4096, from = (const char*)from + 4096;
-    if ((i & 3) == 0) Q35_DMA_PAIR("0");
-    if ((i & 3) == 1) Q35_DMA_PAIR("1024");
-    if ((i & 3) == 2) Q35_DMA_PAIR("2048");
-    if ((i & 3) == 3) Q35_DMA_PAIR("3072");
-#undef Q35_DMA_PAIR
+    if ((i & 3) == 0) dma_kib<0>(from, off, at);
+    if ((i & 3) == 1) dma_kib<1>(from, off, at);
+    if ((i & 3) == 2) dma_kib<2>(from, off, at);
+    if ((i & 3) == 3) dma_kib<3>(from, off, at);
 }
 // A pointer that all lanes have the same, as the compiler cannot see.
 __device__ __forceinline__ const void* uniform(const void* p) {
@@ -453,8 +451,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         for (int r = 0; r < 16; r += 2) ko[r / 2] = 512u * h + 16u * (nn ^ h ^ r);
 #pragma unroll
         for (int r = 0; r < 4; r += 2) vo[r / 2] = 512u * h + 16u * (nn ^ (4 * (h + r)));
-        auto issue_k = [&](int i, const void* from, int buf) { dma_pair(i, from, ko[i], kaddr + buf * kBuf); };
-        auto issue_v = [&](int i, const void* from, int buf) { dma_pair(i, from, vo[i & 1], vaddr + buf * kBuf); };
+        auto issue_k = [&](int i, const void* from, int buf) { dma_nth(i, from, ko[i], kaddr + buf * kBuf); };
+        auto issue_v = [&](int i, const void* from, int buf) { dma_nth(i, from, vo[i & 1], vaddr + buf * kBuf); };
         auto k_from = [&](size_t at) { return uniform((const _Float16*)pv.k + at); };
         auto v_from = [&](size_t at) { return uniform((const _Float16*)pv.v + at); };
 
@@ -462,7 +460,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         const float4* const qs = reinterpret_cast<const float4*>(&st.v[0][0][0]);
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-            dma_pair(0, uniform(q_gate + row0 * 2 * kHd + from_row0(r) * 2 * kHd), 16 * (lane ^ (r & 31)),
+            dma_nth(0, uniform(q_gate + row0 * 2 * kHd + from_row0(r) * 2 * kHd), 16 * (lane ^ (r & 31)),
                      lds_address(&st.v[0][0][0]) + r * kHd * 4);
         // Where the wave's rows of the next units lie: found a unit before they are asked for.
         const size_t at0 = group_at(wk.t0);
@@ -530,7 +528,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
                     8 * (lane & 3);
             va[1][d] = va[0][d] + (half ? -32 * 512 : 32 * 512);   // the partner's rows
         }
-        auto k_at = [&](int s) { return *(lds_f16x8*)(ka[s & 7] + 256 * (s >> 3)); };
+        auto k_at = [&](int s) { return *(lds_f16x8*)(uintptr_t)(ka[s & 7] + 256 * (s >> 3)); };
         // Score products, K read four steps ahead (the first four by begin()), with
         // beside(s) among the products of step s.
         f16x8 kk[4];
@@ -621,8 +619,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 const uint32_t at = va[whose][d] + step * 16 * 512;
-                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * 512));
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at);
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(at + 8 * 512));
                 typedef short s16x8 __attribute__((ext_vector_type(8)));
                 v[d] = __builtin_bit_cast(f16x8, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
             }
@@ -921,8 +919,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         for (int i = 0; i < 8; ++i) ko[i] = 16u * (lane ^ ((8 * wave + i) & 15));
         vo[0] = 16u * lane;
         vo[1] = 16u * (lane ^ 8);
-        auto issue_k = [&](int i, const void* from, int buf) { dma_pair(i, from, ko[i], kaddr + buf * kBuf); };
-        auto issue_v = [&](int i, const void* from, int buf) { dma_pair(i, from, vo[i >> 2], vaddr + buf * kBuf); };
+        auto issue_k = [&](int i, const void* from, int buf) { dma_nth(i, from, ko[i], kaddr + buf * kBuf); };
+        auto issue_v = [&](int i, const void* from, int buf) { dma_nth(i, from, vo[i >> 2], vaddr + buf * kBuf); };
         auto k_from = [&](size_t at) { return uniform((const float*)pv.k + at); };
         auto v_from = [&](size_t at) { return uniform((const float*)pv.v + at); };
 
@@ -930,7 +928,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         const float4* const qs = reinterpret_cast<const float4*>(&st.v[0][0][0]);
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-            dma_pair(0, uniform(q_gate + row0 * 2 * kHd + from_row0(r) * 2 * kHd), 16 * (lane ^ (r & 31)),
+            dma_nth(0, uniform(q_gate + row0 * 2 * kHd + from_row0(r) * 2 * kHd), 16 * (lane ^ (r & 31)),
                      lds_address(&st.v[0][0][0]) + r * kHd * 4);
         const size_t at0 = group_at(s0);
 #pragma unroll
@@ -980,14 +978,14 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         auto k_read = [&](int s, float (&y)[8]) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const f32x4 a = *(lds_f32x4*)(ka[2 * (s & 3) + c] + 256 * (s >> 2));
+                const f32x4 a = *(lds_f32x4*)(uintptr_t)(ka[2 * (s & 3) + c] + 256 * (s >> 2));
 #pragma unroll
                 for (int k = 0; k < 4; ++k) y[4 * c + k] = a[k];
             }
         };
         auto v_read = [&](int row16, int d, float (&y)[8]) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = *(lds_float*)(va[d] + (row16 + (j & 3) + 8 * (j >> 2)) * kHd * 4);
+            for (int j = 0; j < 8; ++j) y[j] = *(lds_float*)(uintptr_t)(va[d] + (row16 + (j & 3) + 8 * (j >> 2)) * kHd * 4);
         };
         // The wave's half of a step's scores, to its partner; beside(s, i) behind the i-th
         // product of operand s.
