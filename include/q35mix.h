@@ -299,7 +299,8 @@ int q35m_paged_append(q35m_paged* p, int layer, int n, const int* seqs, const in
  * captured into a HIP graph on the context's stream, a replay decodes at the
  * lengths and pages of its time (the checks above are made when a call is
  * enqueued or captured: keep the pages of every row that a replay writes
- * mapped, and shared by nobody). */
+ * mapped, and shared by nobody).  An eager call leaves short sequences to one
+ * workgroup each, a replay does not, so the two may differ in the last bits. */
 int q35m_paged_attn_decode(q35m_paged* p, int layer, int n, const int* seqs, const float* q_gate, const float* k,
                            const float* v, float* out);
 /* q35m_attn_prefill over paged rows, for chunks of new tokens of n sequences

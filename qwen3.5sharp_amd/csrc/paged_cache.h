@@ -54,6 +54,11 @@ struct q35m_paged {
 
     q35m_paged(int n_seqs, int max_rows, int n_pages_, int page_rows)
         : map(n_seqs, max_rows, n_pages_, page_rows), n_pages(n_pages_) {}
+    // Whether the stream is being captured: a replay's lengths are not known now.
+    bool capturing() const {
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        return hipStreamIsCapturing(ctx->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
+    }
     size_t value_bytes() const { return type == Q35M_KV_F16 ? 2 : 4; }
     q35::PagedView view(int layer) const {
         return {k[layer], v[layer], dev_table, dev_len, rope, map.max_pages(), n_pages, page_shift,

@@ -296,18 +296,20 @@ struct Tile<_Float16, S> {
     }
 };
 
+// Rows of a unit.
+template <typename T>
+constexpr int kUnitRows = 4 * Tile<T, true>::kRows;
+
 // The units of a call's sequences, one sequence a lane: `end` is the number of
 // units up to and with the lane's.
 struct Units {
     int rows, tiles, end, total;
 };
-template <typename T>
-__device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch& b, int groups, int lane) {
-    constexpr int kUnit = 4 * Tile<T, true>::kRows;
+__device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch& b, int groups, int unit, int lane) {
     Units u;
     // (the row past max_rows of a replayed call that its caller let run over)
     u.rows = lane < b.n ? min(pv.lens[b.seq[lane]] + 1, pv.max_rows) : 0;
-    u.tiles = (u.rows + kUnit - 1) / kUnit;
+    u.tiles = (u.rows + unit - 1) / unit;
     u.end = u.tiles * groups;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
@@ -324,7 +326,7 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
                                                       const float* __restrict__ q_norm,
                                                       const float* __restrict__ k_norm, float* __restrict__ out,
                                                       float* __restrict__ part_o, float* __restrict__ part_ml, int hg,
-                                                      int ng, float eps) {
+                                                      int ng, int unit, float eps) {
     using Tl = Tile<T, S>;
     constexpr int R = Tl::kRows;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
     qw = make_float4(1.0f + qw.x, 1.0f + qw.y, 1.0f + qw.z, 1.0f + qw.w);
     const int qe = std::is_same_v<T, float> ? 0 : q_exponent(q_norm, lane);
     const float up = ldexpf(1.0f, qe), down = ldexpf(1.0f, -qe);
-    const Units un = units_of<T>(pv, b, groups, lane);
+    const Units un = units_of(pv, b, groups, unit, lane);
     const int per = (un.total + (int)gridDim.x - 1) / (int)gridDim.x;
     int u = blockIdx.x * per;
     const int u_end = min(u + per, un.total);
@@ -357,7 +359,7 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
         u += t1 - t0;
         const int kvh = y / ng, seq = b.seq[i], pos = rows - 1;
         const int* table = pv.table + (size_t)seq * pv.max_pages;
-        const int first = t0 * 4 * R + wave * R, stop = min(rows, t1 * 4 * R);
+        const int first = t0 * unit + wave * R, stop = min(rows, t1 * unit);
         const int last16 = pos & ~15;
 
         Tl tl;
@@ -537,7 +539,7 @@ __global__ __launch_bounds__(MW * kWave) void paged_decode_merge(PagedView pv, P
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int groups = pv.nkv * ng, nh = groups * hg;
     const int i = blockIdx.y, head = blockIdx.x, y = head / hg, h = head - y * hg;
-    const Units un = units_of<T>(pv, b, groups, lane);
+    const Units un = units_of(pv, b, groups, kUnitRows<T>, lane);
     const int per = (un.total + nwg - 1) / nwg;
     const int tiles = __builtin_amdgcn_readlane(un.tiles, i);
     const int s = __builtin_amdgcn_readlane(un.end, i) - tiles * groups + y * tiles;
@@ -609,14 +611,25 @@ hipError_t launch_paged_decode(q35m_paged* p, int layer, const PagedBatch& b, co
     float* part_ml = part_o + (size_t)2 * nwg * kPagedDecodeHeads * kHd;
     const PagedView pv = p->view(layer);
     const AttnLayer& L = c->full[layer];
+    // Short sequences that each get a workgroup are not cut, and nothing is to be
+    // joined, as the lengths known here say (not so those of a replay): up to 4 units
+    // of an fp16 cache (5.7 to 6.5 us against 8 to 10 for 1 to 4 sequences of up to 200
+    // rows, 7.6 against 8 at 400), up to 2 of an fp32 one (5.8 against 8.2 at 100 rows;
+    // no gain at 200).
+    const bool half = p->type == Q35M_KV_F16;
+    const int base = half ? kUnitRows<_Float16> : kUnitRows<float>, whole = base * (half ? 4 : 2);
+    bool cut = (long)b.n * c->d.nkv * ng > nwg;
+    for (int i = 0; i < b.n; ++i) cut |= p->map.length(b.seq[i]) >= whole;
+    cut = cut || p->capturing();
+    const int unit = cut ? base : whole;
     auto go = [&](auto part, auto merge) {
         {
             ProfScope ps(c, K_PAGED_DECODE);
             hipExtLaunchKernelGGL(part, dim3(nwg), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b, q_gate, k, v, L.q_norm,
-                                  L.k_norm, out, part_o, part_ml, hg, ng, c->d.eps);
+                                  L.k_norm, out, part_o, part_ml, hg, ng, unit, c->d.eps);
         }
         const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+        if (e != hipSuccess || !cut) return e;
         ProfScope ps(c, K_PAGED_DECODE_MERGE);
         hipExtLaunchKernelGGL(merge, dim3(c->d.nh, b.n), dim3(MW * kWave), 0, c->stream, ps.a, ps.b, 0, pv, b, part_o,
                               part_ml, q_gate, out, hg, ng, nwg);

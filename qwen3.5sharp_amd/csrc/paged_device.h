@@ -115,16 +115,10 @@ __device__ __forceinline__ void split16(const float* y, f16x8& hi, f16x8& lo) {
     }
 }
 
-// x times the output gate's sigmoid, 1 / (1 + e^-g).  The exponent's product is
-// rounded once, so e^-g is off by |g| 2^-24 of itself and two ulp more, and the
-// sigmoid by that much times 1 - sigmoid: 2^-21 at g = -8, less at positive g.
-// (The exact form, sigmoid_full, is twice the instructions: 64 of them a lane were
-// 5 us of a prompt's 99.)
-__device__ __forceinline__ float sigmoid(float g) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
-}
+// x times the output gate's sigmoid.
 __device__ __forceinline__ float4 gated(float4 x, float4 gate) {
-    return make_float4(x.x * sigmoid(gate.x), x.y * sigmoid(gate.y), x.z * sigmoid(gate.z), x.w * sigmoid(gate.w));
+    return make_float4(x.x * sigmoid_full(gate.x), x.y * sigmoid_full(gate.y), x.z * sigmoid_full(gate.z),
+                       x.w * sigmoid_full(gate.w));
 }
 
 // Four values rounded to the cache's type, stored as one vector.

@@ -23,6 +23,8 @@
 // is S^T's own register layout, so weights cross no lanes (the two waves that share
 // query rows pass them on, or the halves of the scores, in that layout), and the
 // softmax's statistics of a query row are registers of its lanes.
+#include <algorithm>
+
 #include "paged_device.h"
 
 namespace q35 {
@@ -39,13 +41,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 // if short, may count one more than it has rows for), which is
 // floor((q0 + j) / hg); sums of such floors are closed forms.
 struct Tiles {
-    int shift;             // log2 hg
+    int shift;             // log2 of tiles a unit
     int n;                 // tiles
     long q0;
-    __device__ __forceinline__ Tiles(int start, int tokens, int hg_shift) : shift(hg_shift) {
+    // more: log2 of what a unit is over 64 rows.
+    __device__ __forceinline__ Tiles(int start, int tokens, int hg_shift, int more) : shift(hg_shift + more) {
         const int tm_shift = 6 - hg_shift, tm = 1 << tm_shift;
         n = (tokens + tm - 1) >> tm_shift;
-        q0 = ((long)start + tm + kUnit - 1) >> tm_shift;
+        q0 = ((long)start + tm + (kUnit << more) - 1) >> tm_shift;
     }
     __device__ __forceinline__ long floors(long m) const {      // sum of floor(y / hg) over y < m
         const long k = m >> shift;
@@ -78,16 +81,19 @@ __device__ __forceinline__ long uniform(long v) {
 
 // Lane i: the units of the call's sequences up to and with the i-th.
 struct Units {
-    int start;
+    int start, more;
     long end, total;
 };
-__device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch& b, int groups, int hg_shift, int lane) {
+__device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch& b, int groups, int hg_shift, int more,
+                                          int lane) {
     Units u;
     u.start = 0;
     u.end = 0;
+    const int tokens = lane < b.n ? b.off[lane + 1] - b.off[lane] : 0;
+    u.more = more;
     if (lane < b.n) {
         u.start = pv.lens[b.seq[lane]];
-        const Tiles t(u.start, b.off[lane + 1] - b.off[lane], hg_shift);
+        const Tiles t(u.start, tokens, hg_shift, u.more);
         u.end = t.before(t.n) * groups;
     }
     for (int o = 1; o < b.n; o <<= 1) {
@@ -123,7 +129,7 @@ struct Walk {
             i = uniform((int)__popcll(__ballot(un.end <= u)));
             start = __builtin_amdgcn_readlane(un.start, i);
             tokens = b.off[i + 1] - b.off[i];
-            const Tiles ts(start, tokens, hg_shift);
+            const Tiles ts(start, tokens, hg_shift, un.more);
             n = ts.n;
             const long each = ts.before(n);
             long rest = u - (readlane_long(un.end, i) - each * groups);
@@ -140,7 +146,7 @@ struct Walk {
             }
             within = rest - ts.ordered(o);
         }
-        const Tiles ts(start, tokens, hg_shift);
+        const Tiles ts(start, tokens, hg_shift, un.more);
         y = uniform(y);
         o = uniform(o);
         n = uniform(n);
@@ -149,6 +155,7 @@ struct Walk {
         t0 = uniform((int)within);
         t1 = uniform((int)min((long)tiles, within + (u_end - u)));
         u = uniform(u + t1 - t0);
+        if (un.more) t1 = tiles = uniform((int)Tiles(start, tokens, hg_shift, 0).cnt(j));      // a whole tile, in 64s
         return true;
     }
 };
@@ -281,6 +288,14 @@ __device__ __forceinline__ void put_rows(float4* os, const f32x16 (&o)[4], int r
                 make_float4(o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]);
 }
 
+// 1 / (1 + e^-g).  The exponent's product is rounded once, so e^-g is off by |g|
+// 2^-24 of itself and two ulp more, and the sigmoid by that much times 1 - sigmoid:
+// 2^-21 at g = -8, less at positive g.  (sigmoid_full is twice the instructions: 64
+// of them a lane are 2500 cycles a segment.)
+__device__ __forceinline__ float sigmoid(float g) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
+}
+
 // From there a wave's 16 rows leave, one at a time: finished to out_row(row) (none
 // if null), or as parts.  l, m: sum and maximum of row 16 wave + lane % 16.
 template <typename F>
@@ -394,7 +409,7 @@ __device__ __forceinline__ const void* uniform(const void* p) {
 __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
                                                            const float* __restrict__ q_norm, float* __restrict__ out,
                                                            float* __restrict__ part_o, float* __restrict__ part_ml,
-                                                           int hg_shift, int ng, float eps) {
+                                                           int hg_shift, int ng, int more, float eps) {
     constexpr float kShift = 1.0f;                        // weights are e^{s - m} 2^kShift,
     constexpr float kMove = 14.0f;                        // so below 2^15: in fp16's range
     __shared__ __align__(16) F16Tile st;
@@ -410,7 +425,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
     st.w[tid] = 1.0f + q_norm[tid];                       // (read behind the first segment's first barrier)
     const int qe = q_exponent(q_norm, tid & 63);
     const float up = ldexpf(1.0f, qe), down = ldexpf(1.0f, -qe);
-    const Units un = units_of(pv, b, groups, hg_shift, tid & 63);
+    const Units un = units_of(pv, b, groups, hg_shift, more, tid & 63);
     Walk wk;
     wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
@@ -865,7 +880,7 @@ __device__ __forceinline__ f32x16 mul6(const Cut3& a, const Cut3& b, f32x16 c, F
 __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
                                                            const float* __restrict__ q_norm, float* __restrict__ out,
                                                            float* __restrict__ part_o, float* __restrict__ part_ml,
-                                                           int hg_shift, int ng, float eps) {
+                                                           int hg_shift, int ng, int more, float eps) {
     constexpr float kMove = 14.0f;
     __shared__ __align__(16) F32Tile st;
     const int tid = threadIdx.x;
@@ -878,7 +893,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
     const uint32_t kaddr = lds_address(&st.k[0][8 * wave][0]), vaddr = lds_address(&st.v[0][8 * wave][0]);
 
     st.w[tid] = 1.0f + q_norm[tid];                       // (read behind the first segment's first barrier)
-    const Units un = units_of(pv, b, groups, hg_shift, tid & 63);
+    const Units un = units_of(pv, b, groups, hg_shift, more, tid & 63);
     Walk wk;
     wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
@@ -1153,7 +1168,7 @@ __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBat
                                                           int hg_shift, int ng, int nwg) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int groups = pv.nkv * ng, nh = groups << hg_shift, tm = kPagedTileRows >> hg_shift;
-    const Units un = units_of(pv, b, groups, hg_shift, lane);
+    const Units un = units_of(pv, b, groups, hg_shift, 0, lane);
     const long per = (un.total + nwg - 1) / nwg;
     // The workgroup's tile: the sequences' tiles in order.
     int tile_end = lane < b.n ? ((b.off[lane + 1] - b.off[lane] + tm - 1) / tm) * groups : 0;
@@ -1164,7 +1179,7 @@ __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBat
     const int q = blockIdx.x >> 2;
     const int i = __popcll(__ballot(lane < b.n && tile_end <= q));
     const int tokens = b.off[i + 1] - b.off[i];
-    const Tiles ts(__builtin_amdgcn_readlane(un.start, i), tokens, hg_shift);
+    const Tiles ts(__builtin_amdgcn_readlane(un.start, i), tokens, hg_shift, un.more);
     const int local = q - (__builtin_amdgcn_readlane(tile_end, i) - ts.n * groups);
     const int y = local / ts.n, o = local - y * ts.n, j = ts.tile(o);
     const long each = ts.before(ts.n);
@@ -1244,18 +1259,31 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
     const PagedView pv = p->view(layer);
     const AttnLayer& L = c->full[layer];
     long tiles = 0;
-    for (int i = 0; i < b.n; ++i) tiles += (long)(b.off[i + 1] - b.off[i] + tm - 1) / tm * c->d.nkv * ng;
+    int longest = 0;                                       // rows that a query may see
+    for (int i = 0; i < b.n; ++i) {
+        const int tokens = b.off[i + 1] - b.off[i];
+        tiles += (long)(tokens + tm - 1) / tm * c->d.nkv * ng;
+        if (tokens) longest = std::max(longest, p->map.length(b.seq[i]) + tokens);
+    }
+    // Short tiles that each get a workgroup are not cut, and nothing is to be joined,
+    // as the lengths known here say (not so those of a replay): up to 4 units of an
+    // fp16 cache (30 tokens: 8.6 us against 11.0 with the joining; 230: 14.5 against
+    // 15.5), up to 2 of an fp32 one (13.7 against 15.4 for four sequences of 120 rows;
+    // 4 units are slower, 21 against 18).
+    const int shift = p->type == Q35M_KV_F16 ? 2 : 1;
+    const int more = tiles <= nwg && longest <= kUnit << shift && !p->capturing() ? shift : 0;
     {
         ProfScope ps(c, K_PAGED_PREFILL);
         auto go = [&](auto kern) {
             hipExtLaunchKernelGGL(kern, dim3(nwg), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b, q_gate, L.q_norm, out,
-                                  part_o, part_ml, hg_shift, ng, c->d.eps);
+                                  part_o, part_ml, hg_shift, ng, more, c->d.eps);
         };
         if (p->type == Q35M_KV_F16) go(paged_prefill_f16);
         else go(paged_prefill_f32);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    if (more) return hipSuccess;
     ProfScope ps(c, K_PAGED_PREFILL_MERGE);
     hipExtLaunchKernelGGL(paged_prefill_merge, dim3((unsigned)(4 * tiles)), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b,
                           part_o, part_ml, q_gate, out, hg_shift, ng, nwg);

@@ -651,6 +651,39 @@ def test_captured_calls_follow_lengths_and_pages(kv_type):
                 assert hip.hipGraphDestroy(g) == 0
 
 
+@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
+@pytest.mark.parametrize("rows", [100, 127, 128, 129, 255, 256, 257, 511, 512])
+def test_short_sequences_eager_and_replayed(kv_type, rows):
+    """Lengths at which an eager call stops leaving a sequence to one workgroup; a replayed call, captured at another
+    length, never does: both against the restatement."""
+    hip = q35mix.hip()
+    with Paged(kv_type, nh=8, nkv=2, n_seqs=2, max_rows=520, page_rows=32, salt=2) as p:
+        p.seed_rows([rows - 1, rows - 3], salt=4)
+        x1, x2 = p.inputs(2, salt=71), p.inputs(4, salt=72)
+        d1, d2 = p.dev(x1, "q_gate", "k", "v"), p.dev(x2, "q_gate", "k", "v")
+        o1, o2 = p.ctx.array((2, p.nh * HD)), p.ctx.array((4, p.nh * HD))
+        calls = [lambda: p.c.attn_decode(0, [0, 1], *d1, o1), lambda: p.c.attn_prefill(0, [0, 1], [1, 3], *d2, o2)]
+        p.c.truncate(0, 1)
+        p.c.truncate(1, 1)
+        graphs = [capture(p.ctx, c) for c in calls]
+        p.c.advance([0, 1], [rows - 2, rows - 4])
+        stream = ctypes.c_void_p(p.ctx.stream)
+        try:
+            for tokens, x, o, call, (_, exe) in (([1, 1], x1, o1, calls[0], graphs[0]), ([1, 3], x2, o2, calls[1], graphs[1])):
+                p.put([0, 1], tokens, x)
+                want = p.attend([0, 1], tokens, x)
+                for run in (call, lambda exe=exe: hip.hipGraphLaunch(exe, stream)) * 2:
+                    o.upload(np.zeros(o.shape, np.float32))
+                    assert run() in (None, 0)
+                    p.ctx.sync()
+                    close_to(o.download(), want)
+            p.check_pages()
+        finally:
+            for g, exe in graphs:
+                assert hip.hipGraphExecDestroy(exe) == 0
+                assert hip.hipGraphDestroy(g) == 0
+
+
 def test_changes_are_refused_while_capturing():
     hip = q35mix.hip()
     with Paged(KV_F32, max_rows=64) as p:
@@ -736,13 +769,20 @@ def test_refusals():
 
 
 def test_kernel_timers():
-    with Paged(KV_F16, max_rows=64) as p:
+    """Which kernels a call runs: parts are joined only where a sequence went to several workgroups."""
+    with Paged(KV_F16, n_seqs=2, max_rows=700) as p:
+        p.seed_rows([600, 5], salt=3)
         x = p.inputs(2)
         out = p.ctx.array((2, p.nh * HD))
-        p.ctx.profile(True)
-        p.c.attn_prefill(0, [0], [2], *p.dev(x, "q_gate", "k", "v"), out)
-        p.c.attn_decode(0, [0], *p.dev(x, "q_gate", "k", "v"), out)
-        ran = p.ctx.profile_read()
-        p.ctx.profile(False)
-        assert sorted(ran) == ["paged_append_rows", "paged_decode", "paged_decode_merge", "paged_prefill",
-                               "paged_prefill_merge"]
+        d = p.dev(x, "q_gate", "k", "v")
+
+        def ran(seq):
+            p.ctx.profile(True)
+            p.c.attn_prefill(0, [seq], [2], *d, out)
+            p.c.attn_decode(0, [seq], *d, out)
+            names = sorted(p.ctx.profile_read())
+            p.ctx.profile(False)
+            return names
+
+        assert ran(0) == ["paged_append_rows", "paged_decode", "paged_decode_merge", "paged_prefill", "paged_prefill_merge"]
+        assert ran(1) == ["paged_append_rows", "paged_decode", "paged_prefill"]
