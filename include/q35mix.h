@@ -253,7 +253,8 @@ typedef struct q35m_paged q35m_paged;
 
 /* A cache of n_pages pages for every full-attention layer of ctx and n_seqs
  * sequences of up to max_rows rows each (max_rows up to 2^24); page_rows is a
- * power of two from 16 to 1024.  Allocates here, and nothing afterwards.  At
+ * power of two from 16 to 1024.  Allocates here (the pages, and 512 bytes a row
+ * of max_rows for the rotation), and nothing afterwards.  At
  * first no page is mapped and every length is 0.  Destroy it before ctx. */
 int q35m_paged_create(q35m_ctx* ctx, int n_seqs, int max_rows, int n_pages, int page_rows, int kv_type,
                       q35m_paged** out);

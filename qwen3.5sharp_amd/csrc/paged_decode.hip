@@ -7,15 +7,16 @@
 // Every cached row is read once, so the bound is the cache's bytes over HBM's
 // rate; the products are a few operations a byte.
 //
-// Work is cut into units of kUnit rows of one (sequence, head group) and dealt
-// out evenly: workgroup w takes units [w per, (w + 1) per) of the units of all
+// Work is cut into units of 64 (fp32) or 128 (fp16) rows of one (sequence, head
+// group) and dealt out evenly: workgroup w takes units [w per, (w + 1) per) of the units of all
 // sequences in order, per = ceil(units / workgroups), both found on the device
 // from the lengths there, so batches of unequal lengths fill the card and a
 // captured launch fits any lengths.  A stretch of units of one (sequence, head
 // group) is a segment: whole ones are finished where they are, of the others
 // the maximum, the sum and the unnormalised output go to the workspace (two
 // segments of a workgroup at most are not whole, its first and its last), and
-// paged_decode_merge joins them.
+// paged_decode_merge joins them.  (Larger units where no sequence has to be cut:
+// launch_paged_decode.)
 //
 // A unit's rows go to the four waves, which keep an online softmax each and
 // meet at the segment's end.  All products are matrix instructions with the
@@ -48,8 +49,8 @@ constexpr float kPShift = 7.0f;
 // 120 us against 112 for 64 sequences of up to 4000 fp16 rows (709 MB, 6.3 TB/s),
 // 247 against 220 for 8 of up to 32768 fp32 rows (1.52 GB, 6.9 TB/s).  (Whole lines
 // and an exchange between lanes l and l ^ 8 in front of the products: 128 and 261.)
-// So up to 8 q heads (S) it is 8 rows x 128 bytes: a lane has row l % 8 and 16-byte chunk 2 g +
-// l / 8 % 2 of the line, g = l / 16.  As an operand these are 16 rows of which the
+// So up to 8 q heads (S) it is 8 rows x 128 bytes: a lane has row l % 8 and 16-byte
+// chunk 2 g + l / 8 % 2 of the line, g = l / 16.  As an operand these are 16 rows of which the
 // upper 8 are the lower ones' odd chunks; q's columns are as well: column n < 8 is
 // head n's even chunks, column n + 8 its odd ones.  The product's quarter (lower
 // rows, lower columns) is the even chunks' part of a score and the quarter (upper,

@@ -366,11 +366,11 @@ __device__ __forceinline__ void leave_rows(const float4* os, const uint32_t (*po
 // so what is the same every unit is a kept address, a scalar or an offset in the
 // instruction, the loads of the next unit are spread over the score products
 // (in one run of 16 they held the wave for 800 cycles), and every LDS read is a
-// step ahead.  2048 rows over as many: 98 us; 512 over 16384: 268 us.  Two
+// step ahead.  2048 rows over as many: 90 us; 512 over 16384: 257 to 265 us.  Two
 // workgroups a CU with half the registers each, partners splitting the dims and
 // exchanging scores (twice the exponentials): 133 and 318 us.
-// A segment's beginning and end are 30000 cycles of it: partners form half of q
-// each (9000 -> 5800 cycles), and the last rows' LDS reads and the gates come
+// A segment's beginning and end are 30000 cycles of it (40 % of a call of 2048 rows):
+// partners form half of q each (9000 -> 5800 cycles), and the last rows' LDS reads and the gates come
 // before the first store, whose end a later load's wait would wait for (16000 ->
 // 7000).
 struct F16Tile {
@@ -799,9 +799,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
 // (row / 4 % 2), and are cut up where they are read, 5.5 instructions a value, in
 // each wave for its 32 query rows: 7.3 a product, in the shadow of which they are
 // placed one stage a product (left to itself the compiler puts 40 in a row: 3050
-// cycles for 48 products instead of 2390).  133 rows over 8000: 133 us, 1000 over
-// as many: 82 us; the kernel of fp32 instructions took 165 and 112, its products
-// alone 131 and 61 at their rate.
+// cycles for 48 products instead of 2390).  133 rows over 8000: 130 us, 1000 over
+// as many: 72 us back to back; the kernel of fp32 instructions took 165 and 112.
 constexpr int kStep = 32;
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef const __attribute__((address_space(3))) f32x4 lds_f32x4;
@@ -1259,11 +1258,11 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
     const PagedView pv = p->view(layer);
     const AttnLayer& L = c->full[layer];
     long tiles = 0;
-    int longest = 0;                                       // rows that a query may see
+    long longest = 0;                                      // rows that a tile may see
     for (int i = 0; i < b.n; ++i) {
-        const int tokens = b.off[i + 1] - b.off[i];
-        tiles += (long)(tokens + tm - 1) / tm * c->d.nkv * ng;
-        if (tokens) longest = std::max(longest, p->map.length(b.seq[i]) + tokens);
+        const long n = ((long)b.off[i + 1] - b.off[i] + tm - 1) / tm;
+        tiles += n * c->d.nkv * ng;
+        if (n) longest = std::max(longest, p->map.length(b.seq[i]) + n * tm);
     }
     // Short tiles that each get a workgroup are not cut, and nothing is to be joined,
     // as the lengths known here say (not so those of a replay): up to 4 units of an

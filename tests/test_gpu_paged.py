@@ -411,6 +411,20 @@ def test_prefill_full_batch(kv_type):
 
 
 @pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
+@pytest.mark.parametrize("start,T", [(10, 113), (10, 118), (1, 127), (10, 241), (10, 246), (0, 256), (250, 7)])
+def test_prefill_tiles_past_the_rows(kv_type, start, T):
+    """A last tile whose 64 query rows reach past the chunk, and past the rows up to which tiles are not cut."""
+    with Paged(kv_type, n_seqs=1, max_rows=start + T, page_rows=16, salt=6) as p:
+        p.seed_rows([start], salt=1)
+        x = p.inputs(T, salt=73)
+        out = p.ctx.array((T, p.nh * HD))
+        p.c.attn_prefill(0, [0], [T], *p.dev(x, "q_gate", "k", "v"), out)
+        p.put([0], [T], x)
+        close_to(out.download(), p.attend([0], [T], x, sorted({0, T // 2, max(T - 17, 0), max(T - 2, 0), T - 1})))
+        p.check_pages()
+
+
+@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
 @pytest.mark.parametrize("max_rows", [117, 128])
 def test_a_sequence_filled_to_its_last_row(kv_type, max_rows):
     """A chunk and then single tokens up to row max_rows - 1; the next is refused."""
