@@ -180,6 +180,12 @@ __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINI
 __device__ __forceinline__ bool not_finite(_Float16 x) {
     return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
 }
+// The top bit of each value's place set where it is not finite: its exponent plus
+// one, of 32 bits of values.
+template <typename T>
+__device__ __forceinline__ uint32_t full_exponents(uint32_t x) {
+    return sizeof(T) == 2 ? (x & 0x7c007c00u) + 0x04000400u : (x & 0x7f800000u) + 0x00800000u;
+}
 // NaN in place of the values marked in `nan`, a bit a value.
 __device__ __forceinline__ float4 marked(float4 x, uint32_t nan) {
     auto one = [&](float v, int k) {
@@ -201,17 +207,16 @@ __device__ __forceinline__ void guard_rows(T* v, int base, int rows, uint32_t (*
     constexpr int count = COUNT, U = 4;        // U chunks a lane looks at together
 #pragma nounroll
     for (int x0 = max(0, first + 1 - base) * (kHd / E) + lane; x0 < count * (kHd / E); x0 += U * kWave) {
-        vec y[U];
-        bool look = false;
+        u32x4 y[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int x = min(x0 + u * kWave, count * (kHd / E) - 1);
-            y[u] = *reinterpret_cast<vec*>(v + x * E);
-            look |= base + x / (kHd / E) >= rows;
+        for (int u = 0; u < U; ++u) y[u] = *reinterpret_cast<u32x4*>(v + min(x0 + u * kWave, count * (kHd / E) - 1) * E);
+        uint32_t full = 0;
 #pragma unroll
-            for (int k = 0; k < E; ++k) look |= not_finite(y[u][k]);
-        }
-        if (!look) continue;
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) full |= full_exponents<T>(y[u][k]);
+        const int end = base + min(x0 + (U - 1) * kWave, count * (kHd / E) - 1) / (kHd / E);     // the last one's row
+        if (end < rows && !(full & (sizeof(T) == 2 ? 0x80008000u : 0x80000000u))) continue;
 #pragma nounroll
         for (int x = x0; x < min(x0 + U * kWave, count * (kHd / E)); x += kWave) {
             const int r = base + x / (kHd / E);
@@ -296,8 +301,8 @@ __device__ __forceinline__ float sigmoid(float g) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
 }
 
-// From there a wave's 16 rows leave, one at a time: finished to out_row(row) (none
-// if null), or as parts.  l, m: sum and maximum of row 16 wave + lane % 16.
+// From there a wave's 16 rows leave, one at a time: finished to out_row(row), the
+// lane's place (none if null), or as parts.  l, m: sum and maximum of row 16 wave + lane % 16.
 template <typename F>
 __device__ __forceinline__ void leave_rows(const float4* os, const uint32_t (*poison)[kHd / 32], float l, float m, bool whole,
                                            float4 (&gate)[16], float* part_o, float* part_ml, int wave, int lane, F out_row) {
@@ -325,7 +330,7 @@ __device__ __forceinline__ void leave_rows(const float4* os, const uint32_t (*po
             const float inv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv_l), k));
             const float4 g = gate[k];
             x = make_float4(x.x * inv * g.x, x.y * inv * g.y, x.z * inv * g.z, x.w * inv * g.w);
-            if (float* to = out_row(16 * wave + k)) reinterpret_cast<float4*>(to)[lane] = x;
+            if (char* to = out_row(16 * wave + k)) *reinterpret_cast<float4*>(to) = x;
         };
         rows8(0, put);
         rows8(8, put);
@@ -422,10 +427,11 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
     constexpr int kBuf = kUnit * kHd * 2;                 // bytes of a buffer
     const uint32_t kaddr = lds_address(&st.k[0][16 * wave][0]), vaddr = lds_address(&st.v[0][16 * wave][0]);
 
-    st.w[tid] = 1.0f + q_norm[tid];                       // (read behind the first segment's first barrier)
+    const float w = q_norm[tid];
     const int qe = q_exponent(q_norm, tid & 63);
     const float up = ldexpf(1.0f, qe), down = ldexpf(1.0f, -qe);
     const Units un = units_of(pv, b, groups, hg_shift, more, tid & 63);
+    st.w[tid] = 1.0f + w;                                 // (read behind the first segment's first barrier)
     Walk wk;
     wk.begin(un, wg, gridDim.x);
     while (wk.next(b, un, groups, hg_shift)) {
@@ -443,9 +449,12 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         const int first = uniform(start + wk.j * tm);          // position of the tile's first token
         const int mine = min(start + min(wk.j * tm + ((32 * rg + nn) >> hg_shift), tokens - 1), pv.max_rows - 1);
         // Query row r of the tile is row row0 + from_row0(r) of q and out (the last
-        // token's for rows past the `left` tokens).
+        // token's for rows past the `left` tokens): a 64-bit base a tile and 32 bits from
+        // there.
         const int left = uniform(tokens - wk.j * tm);
         const long row0 = uniform((long)(uniform(b.off[wk.i]) + wk.j * tm) * nh + (wk.y << hg_shift));
+        const char* const q_tile = (const char*)uniform(q_gate + row0 * 2 * kHd);
+        char* const out_tile = (char*)uniform(out + row0 * kHd);
         auto from_row0 = [&](int r) { return min(r >> hg_shift, left - 1) * nh + (r & (hg - 1)); };
 
         // A wave brings its 16 rows of a unit's K or V.  It holds 64 entries of the
@@ -475,7 +484,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         const float4* const qs = reinterpret_cast<const float4*>(&st.v[0][0][0]);
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-            dma_nth(0, uniform(q_gate + row0 * 2 * kHd + from_row0(r) * 2 * kHd), 16 * (lane ^ (r & 31)),
+            dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 16 * (lane ^ (r & 31)),
                      lds_address(&st.v[0][0][0]) + r * kHd * 4);
         // Where the wave's rows of the next units lie: found a unit before they are asked for.
         const size_t at0 = group_at(wk.t0);
@@ -750,8 +759,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         if (whole) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                gate[r] = reinterpret_cast<const float4*>(
-                    uniform(q_gate + row0 * 2 * kHd + from_row0(16 * wave + r) * 2 * kHd + kHd))[lane];
+                gate[r] = *reinterpret_cast<const float4*>(
+                    q_tile + (uint32_t)(from_row0(16 * wave + r) * (2 * kHd * 4) + 4 * kHd + 16 * lane));
         }
         guard();
         add(v1, h1, l1);
@@ -779,7 +788,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         leave_rows(
             os, st.poison, st.mx[1][row >> 5][row & 31] + st.mx[1][2 + (row >> 5)][row & 31], st.mx[0][row >> 5][row & 31],
             whole, gate, part_o + (size_t)slot * kPagedTileRows * kHd, part_ml + (size_t)2 * slot * kPagedTileRows, wave,
-            lane, [&](int r) { return r >> hg_shift < left ? out + row0 * kHd + from_row0(r) * kHd : nullptr; });
+            lane, [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; });
         lds_barrier();                                     // (the stores need no wait)
     }
 }
@@ -907,9 +916,12 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         const int first = uniform(start + wk.j * tm);     // position of the tile's first token
         const int mine = min(start + min(wk.j * tm + ((32 * rg + nn) >> hg_shift), tokens - 1), pv.max_rows - 1);
         // Query row r of the tile is row row0 + from_row0(r) of q and out (the last
-        // token's for rows past the `left` tokens).
+        // token's for rows past the `left` tokens): a 64-bit base a tile and 32 bits from
+        // there.
         const int left = uniform(tokens - wk.j * tm);
         const long row0 = uniform((long)(uniform(b.off[wk.i]) + wk.j * tm) * nh + (wk.y << hg_shift));
+        const char* const q_tile = (const char*)uniform(q_gate + row0 * 2 * kHd);
+        char* const out_tile = (char*)uniform(out + row0 * kHd);
         auto from_row0 = [&](int r) { return min(r >> hg_shift, left - 1) * nh + (r & (hg - 1)); };
 
         // A wave brings 8 rows of a step's K and V; it holds 64 entries of the page
@@ -942,7 +954,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         const float4* const qs = reinterpret_cast<const float4*>(&st.v[0][0][0]);
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-            dma_nth(0, uniform(q_gate + row0 * 2 * kHd + from_row0(r) * 2 * kHd), 16 * (lane ^ (r & 31)),
+            dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 16 * (lane ^ (r & 31)),
                      lds_address(&st.v[0][0][0]) + r * kHd * 4);
         const size_t at0 = group_at(s0);
 #pragma unroll
@@ -1128,8 +1140,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         if (whole) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                gate[r] = reinterpret_cast<const float4*>(
-                    uniform(q_gate + row0 * 2 * kHd + from_row0(16 * wave + r) * 2 * kHd + kHd))[lane];
+                gate[r] = *reinterpret_cast<const float4*>(
+                    q_tile + (uint32_t)(from_row0(16 * wave + r) * (2 * kHd * 4) + 4 * kHd + 16 * lane));
         }
         guard(s0 + steps - 1);
         weigh(s0 + steps - 1);
@@ -1149,7 +1161,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         leave_rows(
             os, st.poison, st.ss[row >> 5][row & 31], st.ss[2 + (row >> 5)][row & 31], whole, gate,
             part_o + (size_t)slot * kPagedTileRows * kHd, part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane,
-            [&](int r) { return r >> hg_shift < left ? out + row0 * kHd + from_row0(r) * kHd : nullptr; });
+            [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; });
         lds_barrier();                                     // (the stores need no wait)
     }
 }
