@@ -415,8 +415,13 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
                                                            const float* __restrict__ q_norm, float* __restrict__ out,
                                                            float* __restrict__ part_o, float* __restrict__ part_ml,
                                                            int hg_shift, int ng, int more, float eps) {
-    constexpr float kShift = 1.0f;                        // weights are e^{s - m} 2^kShift,
-    constexpr float kMove = 14.0f;                        // so below 2^15: in fp16's range
+    // Weights are e^{s - m} 2^kShift, and m is behind the largest score by up to kMove
+    // (in log2): below 2^15.9, in fp16's range, and in steps of 2^-24, 2^-30 of the largest
+    // weight or finer.  Half a step, 2^-31, is less than what adding 16 rows to an fp32
+    // sum rounds off a row (2^-25 / 16).  A smaller kMove scales the output more often:
+    // 2048 rows 92.7 us at (7, 8), 90.4 here, 88.5 at (1, 14), whose steps lose rows 18
+    // nats below the largest.
+    constexpr float kShift = 6.0f, kMove = 9.9f;
     __shared__ __align__(16) F16Tile st;
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -618,11 +623,13 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
             sub = kShift - (m_run == -INFINITY ? 0.0f : m_run);
         };
         f16x8 ph[2], pl[2];
-        float p_even = 0.0f;
+        float p_even = 0.0f, p_sum = 0.0f;                 // (of the unit: one small weight at a time would be lost
+                                                           // beside a large sum)
         auto weight = [&](int k) {
             const float p = __builtin_amdgcn_exp2f(fmaf(sc[k], down, sub));
-            l_run += p;
-            asm volatile("" : "+v"(l_run));                 // here, among the products
+            p_sum = k ? p_sum + p : p;
+            if (k == 15) l_run += p_sum;
+            asm volatile("" : "+v"(p_sum));                 // here, among the products
             if (k & 1) {
                 f16x2 hi, lo;
                 split16(p_even, p, hi, lo);
@@ -1077,11 +1084,13 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
                 pin();
             }
             const float sub = m_run == -INFINITY ? 0.0f : m_run;
+            float sum = 0.0f;                              // (of the step, as the fp16 kernel's of a unit)
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
                 sc[k] = __builtin_amdgcn_exp2f(sc[k] - sub);
-                l_run += sc[k];
+                sum += sc[k];
             }
+            l_run += sum;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float y[8];
