@@ -3,9 +3,8 @@ restatement in 64 bits of test_gpu_paged.py.  Each test states its own tolerance
 import numpy as np
 import pytest
 
-import q35mix
 from q35mix import KV_F16, KV_F32
-from test_gpu_paged import HD, TOL, Paged, cast, close_to, say
+from test_gpu_paged import HD, TOL, Paged, cast, say
 
 pytestmark = pytest.mark.gpu
 
@@ -67,115 +66,3 @@ def test_prefill_weights_far_below_the_largest(kv_type):
         e = np.abs(out.download()[some] - want).max()
         say(f"weights of 2^-26.7, type {kv_type}: {e:.1e} of {np.abs(want).max():.2f}")
         assert e <= TOL
-
-
-# ------------------------------------------------------------------ infinities
-
-def same_kind(got, want, tol):
-    """Infinities of the same sign, NaN where NaN, the rest within tol of the largest."""
-    assert np.array_equal(np.isnan(got), np.isnan(want))
-    inf = np.isinf(want)
-    assert np.array_equal(np.isinf(got), inf) and np.array_equal(got[inf] > 0, want[inf] > 0)
-    ok = np.isfinite(want)
-    e = np.abs(got[ok] - want[ok]).max() / np.abs(want[ok]).max()
-    assert e <= tol, e
-    return int(inf.sum()), int(np.isnan(want).sum())
-
-
-@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
-@pytest.mark.parametrize("n,T,sharp", [(0, 30, 1), (90, 40, 1), (1700, 70, 1), (1700, 70, 8), (300, 1, 1), (2500, 1, 8)])
-def test_infinite_values(kv_type, n, T, sharp):
-    """A V of +-inf makes the output of every token that sees it that infinity in its dim and heads, however small its
-    weight; infinities of both signs, or a NaN, make it NaN.  T = 1 runs the one-token kernels and a chunk of one.
-    (sharp: cached K times 8, scores of deviation 32 nats.  TOL as in test_gpu_paged.py, scores 8 times the size.)"""
-    with Paged(kv_type, n_seqs=2, max_rows=n + T, page_rows=32) as p:
-        rs = np.random.RandomState(n + T)
-        x = {k: v.copy() for k, v in p.inputs(T, salt=75).items()}
-        xv = x["v"].reshape(T, p.nkv, HD)
-        if n:
-            K, V = (rs.standard_normal((n, p.nkv, HD)).astype(np.float32) for _ in range(2))
-            K *= sharp
-            V[n // 13, 0, 3] = np.inf                # seen by all
-            V[n - 1, 1, 255] = -np.inf
-            V[n // 2, 2, 9], V[n - 2, 2, 9] = np.inf, -np.inf
-            V[n // 3, 3, 77] = np.nan
-            V[3, 3, 200] = -1e6                      # infinite in fp16
-            put_rows(p, 0, 0, K)
-            put_rows(p, 0, 1, V)
-            start(p, n)
-        xv[T // 2, 1, 130] = np.inf                  # seen by some, of the other heads' rows by none
-        xv[T - 1, 0, 4] = -np.inf
-        xv[0, 2, 64], xv[T // 3, 2, 64] = -np.inf, np.inf if T > 1 else -np.inf
-        xv[T // 4, 3, 8] = np.nan
-        xv[T // 2, 3, 201] = 1e6
-        args = p.dev(x, "q_gate", "k", "v")
-        out = p.ctx.array((T, p.nh * HD))
-        calls = [lambda: p.c.attn_prefill(0, [0], [T], *args, out)]
-        if T == 1:
-            calls.append(lambda: p.c.attn_decode(0, [0], *args, out))
-        p.put([0], [T], x)
-        with np.errstate(invalid="ignore"):
-            want = p.attend([0], [T], x)
-        # beside them what is finite, which for an fp32 cache holds values of 1e6 too
-        big = np.abs(want) > 1e3
-        for call in calls:
-            out.upload(np.zeros(out.shape, np.float32))
-            call()
-            got = out.download()
-            counts = same_kind(np.where(big & np.isfinite(want), 0, got), np.where(big & np.isfinite(want), 0, want), TOL * sharp)
-            ok = big & np.isfinite(want)
-            assert not ok.any() or np.abs(got[ok] - want[ok]).max() <= TOL * sharp * np.abs(want[ok]).max()
-            say(f"infinities {T} behind {n} type {kv_type}: {counts[0]} infinite, {counts[1]} NaN")
-            assert counts[0] and counts[1]
-        p.check_pages()
-
-
-# ------------------------------------------------------------------ the output gate
-
-@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
-@pytest.mark.parametrize("T", [1, 3, 40])
-def test_gate_keeps_fp32_precision(kv_type, T):
-    """V of ones, a first token that sees one row: its output is the gate's sigmoid, at -80 to 20.
-
-    Tolerance, relative: the sigmoid's exponential is an ulp off, 2^-23, its reciprocal, the two products with it and
-    the division by the sum 2^-24 each, and as much again for what the compensated argument leaves: 2^-21."""
-    with Paged(kv_type, max_rows=64) as p:
-        x = {k: v.copy() for k, v in p.inputs(T, salt=76).items()}
-        x["v"][:] = 1
-        g = np.linspace(-80, 20, p.nh * HD).astype(np.float32).reshape(p.nh, HD)
-        x["q_gate"].reshape(T, p.nh, 2, HD)[:, :, 1] = g
-        args, out = p.dev(x, "q_gate", "k", "v"), p.ctx.array((T, p.nh * HD))
-        want = (1 / (1 + np.exp(-g.astype(np.float64)))).ravel()
-        calls = [lambda: p.c.attn_prefill(0, [0], [T], *args, out)]
-        if T == 1:
-            calls.append(lambda: p.c.attn_decode(0, [0], *args, out))
-        for call in calls:
-            call()
-            e = np.abs(out.download()[0] / want - 1).max()
-            say(f"gate, {T} tokens, type {kv_type}: {e / 2.0 ** -24:.2f} half steps")
-            assert e <= 2.0 ** -21
-
-
-# ------------------------------------------------------------------ fp32's range
-
-def test_fp32_values_near_the_largest():
-    """V of 2^119 over 230 rows (their sum with weights up to one stays below 2^127), in rows whose scores rise 9 nats
-    past those of the rows before.  Tolerance: test_gpu_paged.py's."""
-    n, T = 230, 3
-    with Paged(KV_F32, max_rows=n + T, page_rows=16) as p:
-        score = np.zeros(n)
-        score[70:] = 9.0
-        x = levels(p, n, T, score, salt=77)
-        rs = np.random.RandomState(2)
-        V = rs.uniform(1.0, 2.0, (n, p.nkv, HD)).astype(np.float32) * np.float32(2.0 ** 118)
-        put_rows(p, 0, 1, V)
-        start(p, n)
-        x["v"][:] = rs.uniform(1.0, 2.0, x["v"].shape).astype(np.float32) * np.float32(2.0 ** 118)
-        args = p.dev(x, "q_gate", "k", "v")
-        out, one = p.ctx.array((T, p.nh * HD)), p.ctx.array((1, p.nh * HD))
-        p.c.attn_decode(0, [0], *args, one)
-        p.c.attn_prefill(0, [0], [T], *args, out)
-        p.put([0], [T], x)
-        want = p.attend([0], [T], x)
-        close_to(one.download().astype(np.float64), want[:1])
-        close_to(out.download().astype(np.float64), want)
