@@ -293,14 +293,6 @@ __device__ __forceinline__ void put_rows(float4* os, const f32x16 (&o)[4], int r
                 make_float4(o[d][k], o[d][k + 1], o[d][k + 2], o[d][k + 3]);
 }
 
-// 1 / (1 + e^-g).  The exponent's product is rounded once, so e^-g is off by |g|
-// 2^-24 of itself and two ulp more, and the sigmoid by that much times 1 - sigmoid:
-// 2^-21 at g = -8, less at positive g.  (sigmoid_full is twice the instructions: 64
-// of them a lane are 2500 cycles a segment.)
-__device__ __forceinline__ float sigmoid(float g) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
-}
-
 // From there a wave's 16 rows leave, one at a time: finished to out_row(row), the
 // lane's place (none if null), or as parts.  l, m: sum and maximum of row 16 wave + lane % 16.
 template <typename F>
@@ -323,7 +315,7 @@ __device__ __forceinline__ void leave_rows(const float4* os, const uint32_t (*po
         // (all gates before the first store: a wait for a load waits for the stores before it)
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-            gate[k] = make_float4(sigmoid(gate[k].x), sigmoid(gate[k].y), sigmoid(gate[k].z), sigmoid(gate[k].w));
+            gate[k] = gate_sigmoid(gate[k]);
             asm volatile("" : "+v"(gate[k].x), "+v"(gate[k].y), "+v"(gate[k].z), "+v"(gate[k].w));
         }
         auto put = [&](int k, float4 x) {

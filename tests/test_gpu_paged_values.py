@@ -3,8 +3,9 @@ restatement in 64 bits of test_gpu_paged.py.  Each test states its own tolerance
 import numpy as np
 import pytest
 
+import q35mix
 from q35mix import KV_F16, KV_F32
-from test_gpu_paged import HD, TOL, Paged, cast, say
+from test_gpu_paged import HD, TOL, Paged, cast, close_to, say
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +67,48 @@ def test_prefill_weights_far_below_the_largest(kv_type):
         e = np.abs(out.download()[some] - want).max()
         say(f"weights of 2^-26.7, type {kv_type}: {e:.1e} of {np.abs(want).max():.2f}")
         assert e <= TOL
+
+
+# ------------------------------------------------------------------ the output gate
+
+@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_gate_keeps_fp32_precision(kv_type, T):
+    """V of ones, a first token that sees one row: its output is the gate's sigmoid, at -80 to 20.
+
+    Tolerance, relative: the sigmoid's exponential and its reciprocal are an ulp off, 2^-23 each, the two sums between
+    them, the product with it and the division by the sum of weights 2^-24 each: 2^-21."""
+    with Paged(kv_type, max_rows=64) as p:
+        x = {k: v.copy() for k, v in p.inputs(T, salt=76).items()}
+        x["v"][:] = 1
+        g = np.linspace(-80, 20, p.nh * HD).astype(np.float32).reshape(p.nh, HD)
+        x["q_gate"].reshape(T, p.nh, 2, HD)[:, :, 1] = g
+        args, out = p.dev(x, "q_gate", "k", "v"), p.ctx.array((T, p.nh * HD))
+        want = (1 / (1 + np.exp(-g.astype(np.float64)))).ravel()
+        calls = [lambda: p.c.attn_prefill(0, [0], [T], *args, out)]
+        if T == 1:
+            calls.append(lambda: p.c.attn_decode(0, [0], *args, out))
+        for call in calls:
+            call()
+            e = np.abs(out.download()[0] / want - 1).max()
+            say(f"gate, {T} tokens, type {kv_type}: {e / 2.0 ** -24:.2f} half steps")
+            assert e <= 2.0 ** -21
+
+
+@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
+def test_gates_without_bounds(kv_type):
+    """Gates whose exponential overflows, infinite ones and NaN: 0, 1 and NaN."""
+    gates = np.array([-np.inf, np.inf, np.nan, -1e30, 1e30, -3e38, 3e38, -200, 200, -1e5, 1e5, 0], np.float32)
+    sig = np.array([0, 1, np.nan, 0, 1, 0, 1, 0, 1, 0, 1, 0.5], np.float32)
+    for T in (1, 20):
+        with Paged(kv_type, max_rows=32) as p:
+            x = {k: v.copy() for k, v in p.inputs(T, salt=78).items()}
+            x["v"][:] = 1
+            x["q_gate"].reshape(T, p.nh, 2, HD)[:, :, 1] = np.resize(gates, HD)
+            args, out = p.dev(x, "q_gate", "k", "v"), p.ctx.array((T, p.nh * HD))
+            calls = [lambda: p.c.attn_prefill(0, [0], [T], *args, out)]
+            if T == 1:
+                calls.append(lambda: p.c.attn_decode(0, [0], *args, out))
+            for call in calls:
+                call()
+                assert np.allclose(out.download().reshape(T, p.nh, HD), np.resize(sig, HD), rtol=2e-6, atol=1e-38, equal_nan=True)
