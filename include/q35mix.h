@@ -250,6 +250,10 @@ typedef struct q35m_paged q35m_paged;
  * q35m_paged_attn_prefill takes the bits of an fp32 value below 2^-126 as 0). */
 #define Q35M_KV_F32 0
 #define Q35M_KV_F16 1
+/* Values that are not finite reach the outputs of the tokens that see their row and
+ * no other: an infinite V value makes its dim of the output that infinity, whatever
+ * the row's weight, and V infinities of both signs or a NaN make it NaN; an infinite
+ * or NaN K value may make every dim NaN. */
 
 /* A cache of n_pages pages for every full-attention layer of ctx and n_seqs
  * sequences of up to max_rows rows each (max_rows up to 2^24); page_rows is a

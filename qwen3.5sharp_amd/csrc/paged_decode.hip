@@ -498,10 +498,8 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
             if (whole && wave + 4 * k < hg)
                 gate[k] = *reinterpret_cast<const float4*>(q_rows + (size_t)(wave + 4 * k) * 2 * kHd + kHd);
         lds_barrier();
-#pragma unroll
-        for (int k = 0; k < kPagedDecodeHeads / 4; ++k) {
-            const int r = wave + 4 * k;
-            if (r >= hg) break;
+        bool look = false;                                 // at an output that is not finite
+        auto join = [&](int r, float4 gt, bool settle, uint32_t found) {
             float M = -INFINITY, l = 0.0f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -514,15 +512,32 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
                 l += e * ml[w][r][1];
                 o.x += e * x.x; o.y += e * x.y; o.z += e * x.z; o.w += e * x.w;
             }
+            look |= not_finite(o);
+            if (settle) o = settled(o, found);
             if (whole) {
                 const float inv = 1.0f / l;
                 *reinterpret_cast<float4*>(out + ((size_t)i * nh + y * hg + r) * kHd + 4 * lane) =
-                    gated(make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), gate[k]);
+                    gated(make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), gt);
             } else {
                 const size_t at = (size_t)slot * kPagedDecodeHeads + r;
                 *reinterpret_cast<float4*>(part_o + at * kHd + 4 * lane) = o;
                 if (lane == 0) *reinterpret_cast<float2*>(part_ml + 2 * at) = make_float2(M, l);
             }
+        };
+#pragma unroll
+        for (int k = 0; k < kPagedDecodeHeads / 4; ++k) {
+            if (wave + 4 * k >= hg) break;
+            join(wave + 4 * k, gate[k], false, 0);
+        }
+        if (__builtin_expect(__any(look), 0)) {            // once more, with the infinities among the rows
+            uint32_t found = infinite_rows<T>(pv, table, kvh, t0 * unit, min(stop, pos), lane);
+            if (pos < stop) {                              // the new row, as the cache holds it
+                const float4 x = *reinterpret_cast<const float4*>(vnew + ((size_t)i * pv.nkv + kvh) * kHd + 4 * lane);
+                found |= infinite(make_float4((float)(T)x.x, (float)(T)x.y, (float)(T)x.z, (float)(T)x.w));
+            }
+#pragma nounroll
+            for (int r = wave; r < hg; r += 4)
+                join(r, *reinterpret_cast<const float4*>(q_rows + (size_t)r * 2 * kHd + kHd), true, found);
         }
         lds_barrier();
     }
@@ -586,6 +601,14 @@ __global__ __launch_bounds__(MW * kWave) void paged_decode_merge(PagedView pv, P
             const float4 x = obuf[w][lane];
             o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
             l += lbuf[w];
+        }
+        if (__builtin_expect(__any(not_finite(o)), 0)) {       // an infinity outlasts a weight of 0
+            o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma nounroll
+            for (int w = w0; w <= w1; ++w) {
+                const size_t at = part(w);
+                o = plus_weighted(o, __builtin_amdgcn_exp2f(part_ml[2 * at] - mu), reinterpret_cast<const float4*>(part_o + at * kHd)[lane]);
+            }
         }
         const float inv = 1.0f / l;
         *reinterpret_cast<float4*>(out + row * kHd + 4 * lane) = gated(make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), gate);

@@ -142,4 +142,61 @@ __device__ __forceinline__ void store_row4(_Float16* p, float4 v) {
     *reinterpret_cast<f16x4*>(p) = f16x4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
 }
 
+// ---- V values that are not finite -------------------------------------------
+//
+// The output of a token that sees an infinite V is that infinity, however small the
+// weight, and NaN if it sees both or a NaN.  The matrix products cannot say so (0 and
+// the low part of a weight times an infinity are NaN, and so are the parts of one), so
+// they only have to leave something that is not finite: then, once a segment, the rows
+// that its queries see are looked through.  Bits 0 .. 3 of `found`: an infinity or NaN
+// in dim 4 lane + bit; bits 4 .. 7: a negative infinity or NaN.
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
+__device__ __forceinline__ bool not_finite(_Float16 x) {
+    return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
+}
+__device__ __forceinline__ bool not_finite(float4 x) {
+    return not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w);
+}
+__device__ __forceinline__ uint32_t infinite(float4 x) {
+    auto one = [](float v, int k) { return (v < INFINITY ? 0u : 1u << k) | (v > -INFINITY ? 0u : 16u << k); };
+    return one(x.x, 0) | one(x.y, 1) | one(x.z, 2) | one(x.w, 3);
+}
+__device__ __forceinline__ float4 load_row4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load_row4(const _Float16* p) {
+    const f16x4 x = *reinterpret_cast<const f16x4*>(p);
+    return make_float4((float)x[0], (float)x[1], (float)x[2], (float)x[3]);
+}
+// Rows [from, to) of kv head kvh of the sequence whose row of the page table `table` is.
+template <typename T>
+__device__ __forceinline__ uint32_t infinite_rows(const PagedView& pv, const int* __restrict__ table, int kvh, int from,
+                                                  int to, int lane) {
+    constexpr int U = 8;       // rows whose loads are in flight together
+    uint32_t found = 0;
+#pragma nounroll
+    for (int r = from; r < to; r += U) {
+        float4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int row = min(r + u, to - 1);
+            const int page = page_of(table, row >> pv.page_shift, pv.max_pages, pv.n_pages);
+            x[u] = load_row4((const T*)pv.v + row_offset<T>(pv, page, kvh, row) + 4 * lane);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) found |= infinite(x[u]);
+    }
+    return found;
+}
+__device__ __forceinline__ float4 settled(float4 x, uint32_t found) {
+    auto one = [&](float v, int k) {
+        const bool up = found >> k & 1, down = found >> k & 16;
+        return up ? (!down ? INFINITY : v != v ? v : NAN) : down ? -INFINITY : v;
+    };
+    return make_float4(one(x.x, 0), one(x.y, 1), one(x.z, 2), one(x.w, 3));
+}
+// o + f x of a part x of an output, whose infinities stay where f underflows.
+__device__ __forceinline__ float4 plus_weighted(float4 o, float f, float4 x) {
+    auto one = [&](float a, float v) { return a + (not_finite(v) ? v : f * v); };
+    return make_float4(one(o.x, x.x), one(o.y, x.y), one(o.z, x.z), one(o.w, x.w));
+}
+
 }  // namespace q35

@@ -172,31 +172,17 @@ __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" :
 // V rows of a unit that not every query row of the tile sees.  Rows past the
 // tile's last row hold anything and become zeros; a value that is not finite
 // becomes zero too (0 x inf is NaN in the products of the query rows that do not
-// see it), and the outputs of the query rows that do are marked in `poison`, a
-// bit a (query row, dim), which turns them to NaN at the segment's end.  A wave
-// takes COUNT rows of kHd values from v on; base: their first row's position.
-// (Rows up to `first` are seen by all of the tile.)
-__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
-__device__ __forceinline__ bool not_finite(_Float16 x) {
-    return (__builtin_bit_cast(unsigned short, x) & 0x7c00) == 0x7c00;
-}
+// see it), and `found` is set, upon which the outputs of the query rows that do are
+// settled at the segment's end.  A wave takes COUNT rows of kHd values from v on;
+// base: their first row's position.  (Rows up to `first` are seen by all of the tile.)
 // The top bit of each value's place set where it is not finite: its exponent plus
 // one, of 32 bits of values.
 template <typename T>
 __device__ __forceinline__ uint32_t full_exponents(uint32_t x) {
     return sizeof(T) == 2 ? (x & 0x7c007c00u) + 0x04000400u : (x & 0x7f800000u) + 0x00800000u;
 }
-// NaN in place of the values marked in `nan`, a bit a value.
-__device__ __forceinline__ float4 marked(float4 x, uint32_t nan) {
-    auto one = [&](float v, int k) {
-        return __builtin_bit_cast(float, __builtin_bit_cast(int, v) | ((int)(nan << (31 - k)) >> 31));
-    };
-    return make_float4(one(x.x, 0), one(x.y, 1), one(x.z, 2), one(x.w, 3));
-}
-// 16-byte chunks are permuted by row: chunk ^ S ((row >> H) & M).
-template <int COUNT, int S, int H, int M, typename T>
-__device__ __forceinline__ void guard_rows(T* v, int base, int rows, uint32_t (*poison)[kHd / 32], int first,
-                                           int tokens_left, int hg_shift, int lane) {
+template <int COUNT, typename T>
+__device__ __forceinline__ void guard_rows(T* v, int base, int rows, int* found, int first, int lane) {
     constexpr int E = 16 / sizeof(T);          // values of 16 bytes
     typedef T vec __attribute__((ext_vector_type(E)));
     if (base >= rows) {
@@ -219,22 +205,16 @@ __device__ __forceinline__ void guard_rows(T* v, int base, int rows, uint32_t (*
         if (end < rows && !(full & (sizeof(T) == 2 ? 0x80008000u : 0x80000000u))) continue;
 #pragma nounroll
         for (int x = x0; x < min(x0 + U * kWave, count * (kHd / E)); x += kWave) {
-            const int r = base + x / (kHd / E);
-            if (r >= rows) {
+            if (base + x / (kHd / E) >= rows) {
                 *reinterpret_cast<vec*>(v + x * E) = vec{};
                 continue;
             }
 #pragma nounroll
-            for (int k = 0; k < E; ++k) {
-                const T one = v[x * E + k];
-                if (!not_finite(one)) continue;
-                const int d = (x % (kHd / E) ^ (S * ((r >> H) & M))) * E + k;
-                // query row q: token min(q >> hg_shift, tokens_left - 1) of the tile, at first + that
-#pragma nounroll
-                for (int q = 0; q < kPagedTileRows; ++q)
-                    if (r <= first + min(q >> hg_shift, tokens_left - 1)) atomicOr(&poison[q][d >> 5], 1u << (d & 31));
-                v[x * E + k] = (T)0.0f;
-            }
+            for (int k = 0; k < E; ++k)
+                if (not_finite(v[x * E + k])) {
+                    v[x * E + k] = (T)0.0f;
+                    *found = 1;
+                }
         }
     }
 }
@@ -295,20 +275,24 @@ __device__ __forceinline__ void put_rows(float4* os, const f32x16 (&o)[4], int r
 
 // From there a wave's 16 rows leave, one at a time: finished to out_row(row), the
 // lane's place (none if null), or as parts.  l, m: sum and maximum of row 16 wave + lane % 16.
+// Whether a value of theirs is not finite.
 template <typename F>
-__device__ __forceinline__ void leave_rows(const float4* os, const uint32_t (*poison)[kHd / 32], float l, float m, bool whole,
-                                           float4 (&gate)[16], float* part_o, float* part_ml, int wave, int lane, F out_row) {
+__device__ __forceinline__ bool leave_rows(const float4* os, float l, float m, bool whole, float4 (&gate)[16], float* part_o,
+                                           float* part_ml, int wave, int lane, F out_row) {
+    float nan[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     auto rows8 = [&](int k0, auto&& put) {
         float4 x[8];
-        uint32_t nan[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int r = 16 * wave + k0 + k;
             x[k] = os[r * (kHd / 4) + (lane ^ (r & 31))];
-            nan[k] = poison[r][lane >> 3] >> (4 * (lane & 7));
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) put(k0 + k, marked(x[k], nan[k]));
+        for (int k = 0; k < 8; ++k) {
+            nan[0] = fmaf(x[k].x, 0.0f, nan[0]); nan[1] = fmaf(x[k].y, 0.0f, nan[1]);
+            nan[2] = fmaf(x[k].z, 0.0f, nan[2]); nan[3] = fmaf(x[k].w, 0.0f, nan[3]);
+            put(k0 + k, x[k]);
+        }
     };
     if (whole) {
         const float inv_l = 1.0f / l;
@@ -332,6 +316,31 @@ __device__ __forceinline__ void leave_rows(const float4* os, const uint32_t (*po
         rows8(0, put);
         rows8(8, put);
         if (lane < 16) reinterpret_cast<float2*>(part_ml)[16 * wave + lane] = make_float2(m, l);
+    }
+    return __any((nan[0] + nan[1]) + (nan[2] + nan[3]) != 0.0f);      // (0 x inf is NaN)
+}
+
+// The wave's rows once more, with the infinities that their tokens see among the
+// segment's rows [from, to) (query row q: up to first + min(q >> hg_shift, left - 1)).
+// gate_row(row): the lane's place of the gate.
+template <typename T, typename G, typename F>
+__device__ __forceinline__ void settle_rows(const float4* os, const PagedView& pv, const int* table, int kvh, int from,
+                                            int to, int first, int left, int hg_shift, float l, bool whole, float* part_o,
+                                            int wave, int lane, G gate_row, F out_row) {
+    uint32_t found = 0;
+#pragma nounroll
+    for (int k = 0; k < 16; ++k) {
+        const int q = 16 * wave + k, end = min(to, first + min(q >> hg_shift, left - 1) + 1);
+        found |= infinite_rows<T>(pv, table, kvh, from, end, lane);
+        from = max(from, end);
+        float4 x = settled(os[q * (kHd / 4) + (lane ^ (q & 31))], found);
+        if (whole) {
+            const float inv = 1.0f / __shfl(l, k, kWave);
+            x = gated(make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), *reinterpret_cast<const float4*>(gate_row(q)));
+            if (char* to_row = out_row(q)) *reinterpret_cast<float4*>(to_row) = x;
+        } else {
+            reinterpret_cast<float4*>(part_o + q * kHd)[lane] = x;
+        }
     }
 }
 
@@ -374,8 +383,8 @@ struct F16Tile {
     _Float16 k[2][kUnit][kHd], v[2][kUnit][kHd];
     f16x8 p[4][4][kWave];                 // a wave's weights: operands (hi, lo) of its two 16-row steps
     float mx[2][4][32];                   // maxima of a unit's halves; at the end sums and maxima
-    uint32_t poison[kPagedTileRows][kHd / 32];
     float w[kHd];                         // 1 + the norm's weights
+    int found;                            // values that are not finite
 };
 typedef const __attribute__((address_space(3))) f16x8 lds_f16x8;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -488,7 +497,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
 #pragma unroll
         for (int i = 0; i < 8; ++i) issue_k(i, k_from(at0), 0);
         size_t at1 = group_at(wk.t0 + 1), at2 = group_at(wk.t0 + 2);
-        for (int x = tid; x < kPagedTileRows * (kHd / 32); x += NT) (&st.poison[0][0])[x] = 0;
+        if (tid == 0) st.found = 0;
 
         // q: lane (row nn, h) forms dims 128 half + 16 s + 8 h + j of its row, s < 8:
         // norm (which the rotation leaves), rotation, scale and the two halves, which
@@ -704,8 +713,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         // unit), every wave is past the buffers that the next rows go to.
         auto guard = [&]() {
             if (masked(t)) {
-                guard_rows<16, 4, 0, 3>(&st.v[buf][16 * wave][0], t * kUnit + 16 * wave, rows, st.poison, first,
-                              left, hg_shift, lane);
+                guard_rows<16>(&st.v[buf][16 * wave][0], t * kUnit + 16 * wave, rows, &st.found, first, lane);
                 lds_barrier();
             }
         };
@@ -784,10 +792,15 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         put_rows(os, o, rg, half, lane);
         lds_barrier();
         const int row = 16 * wave + (lane & 15);           // a row's sum and maximum in lane row % 16
-        leave_rows(
-            os, st.poison, st.mx[1][row >> 5][row & 31] + st.mx[1][2 + (row >> 5)][row & 31], st.mx[0][row >> 5][row & 31],
-            whole, gate, part_o + (size_t)slot * kPagedTileRows * kHd, part_ml + (size_t)2 * slot * kPagedTileRows, wave,
-            lane, [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; });
+        const float l = st.mx[1][row >> 5][row & 31] + st.mx[1][2 + (row >> 5)][row & 31];
+        float* const to_part = part_o + (size_t)slot * kPagedTileRows * kHd;
+        auto gate_row = [&](int r) { return q_tile + (uint32_t)(from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane); };
+        auto out_row = [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; };
+        const bool look = leave_rows(os, l, st.mx[0][row >> 5][row & 31], whole, gate, to_part,
+                                     part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane, out_row);
+        if (__builtin_expect(look || uniform(st.found), 0))
+            settle_rows<_Float16>(os, pv, table, kvh, wk.t0 * kUnit, min(rows, wk.t1 * kUnit), first, left, hg_shift, l, whole,
+                            to_part, wave, lane, gate_row, out_row);
         lds_barrier();                                     // (the stores need no wait)
     }
 }
@@ -817,8 +830,8 @@ struct F32Tile {
     float k[2][kStep][kHd], v[2][kStep][kHd];
     float4 x[4][4][kWave];                // a wave's half of the scores
     float ss[4][32];                      // q's sums of squares; at the end sums and maxima
-    uint32_t poison[kPagedTileRows][kHd / 32];
     float w[kHd];
+    int found;
 };
 
 struct Cut3 {
@@ -959,7 +972,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
 #pragma unroll
         for (int i = 0; i < 8; ++i) issue_k(i, k_from(at0), 0);
         size_t at1 = group_at(s0 + 1), at2 = group_at(s0 + 2);
-        for (int x = tid; x < kPagedTileRows * (kHd / 32); x += NT) (&st.poison[0][0])[x] = 0;
+        if (tid == 0) st.found = 0;
 
         // q: lane (row nn, h) has dims 128 half + 16 s + 8 h + j of its row, s < 8.
         Cut3 q[8];
@@ -1108,8 +1121,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         };
         auto guard = [&](int s) {
             if (s * kStep + kStep - 1 > first)
-                guard_rows<8, 8, 2, 1>(&st.v[buf][8 * wave][0], s * kStep + 8 * wave, rows, st.poison, first,
-                                    left, hg_shift, lane);
+                guard_rows<8>(&st.v[buf][8 * wave][0], s * kStep + 8 * wave, rows, &st.found, first, lane);
         };
 #pragma nounroll
         for (int s = s0; s + 1 < s0 + steps; ++s) {
@@ -1159,10 +1171,15 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         put_rows(os, o, rg, half, lane);
         lds_barrier();
         const int row = 16 * wave + (lane & 15);
-        leave_rows(
-            os, st.poison, st.ss[row >> 5][row & 31], st.ss[2 + (row >> 5)][row & 31], whole, gate,
-            part_o + (size_t)slot * kPagedTileRows * kHd, part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane,
-            [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; });
+        const float l = st.ss[row >> 5][row & 31];
+        float* const to_part = part_o + (size_t)slot * kPagedTileRows * kHd;
+        auto gate_row = [&](int r) { return q_tile + (uint32_t)(from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane); };
+        auto out_row = [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; };
+        const bool look = leave_rows(os, l, st.ss[2 + (row >> 5)][row & 31], whole, gate, to_part,
+                                     part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane, out_row);
+        if (__builtin_expect(look || uniform(st.found), 0))
+            settle_rows<float>(os, pv, table, kvh, wk.t0 * kUnit, min(rows, wk.t1 * kUnit), first, left, hg_shift, l, whole,
+                            to_part, wave, lane, gate_row, out_row);
         lds_barrier();                                     // (the stores need no wait)
     }
 }
@@ -1243,6 +1260,17 @@ __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBat
         }
     }
     const float inv_l = 1.0f / row_sum(l);
+    if (__builtin_expect(__any(not_finite(x[0]) || not_finite(x[1]) || not_finite(x[2]) || not_finite(x[3])), 0)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {                      // an infinity outlasts a weight of 0
+            const float top = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mu), 16 * r));
+            x[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma nounroll
+            for (int w = w0; w <= w1; ++w)
+                x[r] = plus_weighted(x[r], __builtin_amdgcn_exp2f(part_ml[2 * part(w, r)] - top),
+                                     reinterpret_cast<const float4*>(part_o + part(w, r) * kHd)[lane]);
+        }
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const float inv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv_l), 16 * r));

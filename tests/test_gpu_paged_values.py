@@ -69,6 +69,67 @@ def test_prefill_weights_far_below_the_largest(kv_type):
         assert e <= TOL
 
 
+# ------------------------------------------------------------------ infinities
+
+def same_kind(got, want, tol):
+    """Infinities of the same sign, NaN where NaN, the rest within tol of the largest."""
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    inf = np.isinf(want)
+    assert np.array_equal(np.isinf(got), inf) and np.array_equal(got[inf] > 0, want[inf] > 0)
+    ok = np.isfinite(want)
+    e = np.abs(got[ok] - want[ok]).max() / np.abs(want[ok]).max()
+    assert e <= tol, e
+    return int(inf.sum()), int(np.isnan(want).sum())
+
+
+@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
+@pytest.mark.parametrize("n,T,sharp", [(0, 30, 1), (90, 40, 1), (1700, 70, 1), (1700, 70, 8), (300, 1, 1), (2500, 1, 8)])
+def test_infinite_values(kv_type, n, T, sharp):
+    """A V of +-inf makes the output of every token that sees it that infinity in its dim and heads, however small its
+    weight; infinities of both signs, or a NaN, make it NaN.  T = 1 runs the one-token kernels and a chunk of one.
+    (sharp: cached K times 8, scores of deviation 32 nats.  TOL as in test_gpu_paged.py, scores 8 times the size.)"""
+    with Paged(kv_type, n_seqs=2, max_rows=n + T, page_rows=32) as p:
+        rs = np.random.RandomState(n + T)
+        x = {k: v.copy() for k, v in p.inputs(T, salt=75).items()}
+        xv = x["v"].reshape(T, p.nkv, HD)
+        if n:
+            K, V = (rs.standard_normal((n, p.nkv, HD)).astype(np.float32) for _ in range(2))
+            K *= sharp
+            V[n // 13, 0, 3] = np.inf                # seen by all
+            V[n - 1, 1, 255] = -np.inf
+            V[n // 2, 2, 9], V[n - 2, 2, 9] = np.inf, -np.inf
+            V[n // 3, 3, 77] = np.nan
+            V[3, 3, 200] = -1e6                      # infinite in fp16
+            put_rows(p, 0, 0, K)
+            put_rows(p, 0, 1, V)
+            start(p, n)
+        xv[T // 2, 1, 130] = np.inf                  # seen by some, of the other heads' rows by none
+        xv[T - 1, 0, 4] = -np.inf
+        xv[0, 2, 64], xv[T // 3, 2, 64] = -np.inf, np.inf if T > 1 else -np.inf
+        xv[T // 4, 3, 8] = np.nan
+        xv[T // 2, 3, 201] = 1e6
+        args = p.dev(x, "q_gate", "k", "v")
+        out = p.ctx.array((T, p.nh * HD))
+        calls = [lambda: p.c.attn_prefill(0, [0], [T], *args, out)]
+        if T == 1:
+            calls.append(lambda: p.c.attn_decode(0, [0], *args, out))
+        p.put([0], [T], x)
+        with np.errstate(invalid="ignore"):
+            want = p.attend([0], [T], x)
+        # beside them what is finite, which for an fp32 cache holds values of 1e6 too
+        big = np.abs(want) > 1e3
+        for call in calls:
+            out.upload(np.zeros(out.shape, np.float32))
+            call()
+            got = out.download()
+            counts = same_kind(np.where(big & np.isfinite(want), 0, got), np.where(big & np.isfinite(want), 0, want), TOL * sharp)
+            ok = big & np.isfinite(want)
+            assert not ok.any() or np.abs(got[ok] - want[ok]).max() <= TOL * sharp * np.abs(want[ok]).max()
+            say(f"infinities {T} behind {n} type {kv_type}: {counts[0]} infinite, {counts[1]} NaN")
+            assert counts[0] and counts[1]
+        p.check_pages()
+
+
 # ------------------------------------------------------------------ the output gate
 
 @pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
