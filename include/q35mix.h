@@ -247,7 +247,9 @@ typedef struct q35m_paged q35m_paged;
  * the values of an fp32 cache, rounded to nearest even when their row is
  * written, beyond the range of fp16 to infinities; activations and outputs are
  * fp32, and the attention adds no rounding beyond fp32's, but that
- * q35m_paged_attn_prefill takes the bits of an fp32 value below 2^-126 as 0). */
+ * q35m_paged_attn_prefill takes bits of a weight's product with a V value below 2^-126
+ * as 0, weights of 2^-14 for the largest: V values below 2^-96 begin to lose bits).
+ * An output is finite where the sum of |V| over the rows that its token sees is. */
 #define Q35M_KV_F32 0
 #define Q35M_KV_F16 1
 /* Values that are not finite reach the outputs of the tokens that see their row and

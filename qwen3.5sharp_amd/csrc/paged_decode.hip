@@ -40,9 +40,12 @@ namespace {
 
 constexpr int NT = 256;
 constexpr float kLog2e = 1.4426950408889634f;
-// P is formed as e^{s - m} 2^kPShift, so that its low fp16 half loses nothing
-// that fp32 holds (the normalisation divides the factor out).
-constexpr float kPShift = 7.0f;
+// P is formed as e^{s - m} 2^kPShift (the normalisation divides the factor out).  fp16:
+// the largest weight is at the upper end of the range, so that the steps of a weight's
+// low half, 2^-24, are 2^-39 of it.  fp32: weights up to one, so that an output overflows
+// only where the sum of |V| over the rows does.
+template <typename T>
+constexpr float kPShift = std::is_same_v<T, float> ? 0.0f : 15.0f;
 
 // How a wave reads K.  The operand's own shape, 16 rows x 64 bytes an instruction,
 // takes half a cache line of a row at a time, which reads slower than whole lines:
@@ -471,7 +474,7 @@ __global__ __launch_bounds__(NT, 1) void paged_decode(PagedView pv, PagedBatch b
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < Tl::kScores; ++j) {
-                s[j] = __builtin_amdgcn_exp2f(s[j] - mu + kPShift);
+                s[j] = __builtin_amdgcn_exp2f(s[j] - mu + kPShift<T>);
                 sum += s[j];
             }
             l_run = l_run * alpha + sum;

@@ -811,8 +811,9 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
 // as three bf16 values, 8 bits of its mantissa each (exact), and the six products
 // of an operand pair that reach 2^-16 of it: 24 bits, with fp32's range, at six
 // bf16 instructions, 192 cycles where the fp32 instruction takes 512 for the same
-// 32 x 32 x 16.  Those instructions take parts below 2^-126 as 0, so a value below
-// 2^-110 loses its last bits (2^-16 of it at 2^-118).
+// 32 x 32 x 16.  Those instructions take what is below 2^-126 as 0, parts and
+// products: weights being up to one, the largest at 2^-14 or more, an output is off by up
+// to 2^-112 a row, so values below 2^-96 begin to lose bits.
 // Wave (rg, half) has query rows 32 rg ..; partners split the dims: each forms the
 // scores' products of dims 128 half .. and hands them to the other, both form the
 // weights, and each adds the output dims 128 half ...
@@ -901,6 +902,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
                                                            const float* __restrict__ q_norm, float* __restrict__ out,
                                                            float* __restrict__ part_o, float* __restrict__ part_ml,
                                                            int hg_shift, int ng, int more, float eps) {
+    // Weights are e^{s - m} with m up to kMove (in log2) above the largest score: at most
+    // one, so that an output overflows only where the sum of |V| over the rows does.
     constexpr float kMove = 14.0f;
     __shared__ __align__(16) F32Tile st;
     const int tid = threadIdx.x;
@@ -1078,8 +1081,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
 #pragma unroll
             for (int k = 2; k < 16; ++k) mx = fmaxf(mx, sc[k]);
             mx = xor32_max(mx);
-            if (__builtin_expect_with_probability(__any(mx > m_run + kMove), 0, 0.99)) {   // (m_run is -inf at first)
-                const float m_new = fmaxf(m_run, mx);
+            if (__builtin_expect_with_probability(__any(mx > m_run), 0, 0.99)) {   // (m_run is -inf at first)
+                const float m_new = mx > m_run ? mx + kMove : m_run;
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
                 m_run = m_new;
                 l_run *= alpha;

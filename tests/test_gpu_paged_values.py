@@ -173,3 +173,28 @@ def test_gates_without_bounds(kv_type):
             for call in calls:
                 call()
                 assert np.allclose(out.download().reshape(T, p.nh, HD), np.resize(sig, HD), rtol=2e-6, atol=1e-38, equal_nan=True)
+
+
+# ------------------------------------------------------------------ fp32's range
+
+def test_fp32_values_near_the_largest():
+    """V of 2^119 over 230 rows (their sum with weights up to one stays below 2^127), in rows whose scores rise 9 nats
+    past those of the rows before.  Tolerance: test_gpu_paged.py's."""
+    n, T = 230, 3
+    with Paged(KV_F32, max_rows=n + T, page_rows=16) as p:
+        score = np.zeros(n)
+        score[70:] = 9.0
+        x = levels(p, n, T, score, salt=77)
+        rs = np.random.RandomState(2)
+        V = rs.uniform(1.0, 2.0, (n, p.nkv, HD)).astype(np.float32) * np.float32(2.0 ** 118)
+        put_rows(p, 0, 1, V)
+        start(p, n)
+        x["v"][:] = rs.uniform(1.0, 2.0, x["v"].shape).astype(np.float32) * np.float32(2.0 ** 118)
+        args = p.dev(x, "q_gate", "k", "v")
+        out, one = p.ctx.array((T, p.nh * HD)), p.ctx.array((1, p.nh * HD))
+        p.c.attn_decode(0, [0], *args, one)
+        p.c.attn_prefill(0, [0], [T], *args, out)
+        p.put([0], [T], x)
+        want = p.attend([0], [T], x)
+        close_to(one.download().astype(np.float64), want[:1])
+        close_to(out.download().astype(np.float64), want)
