@@ -29,7 +29,10 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
+// (HIP keeps an error for the thread's next hipGetLastError, which is that of a later
+// launch: it is taken back once it is reported.)
 int hip_fail(hipError_t e, const char* what) {
+    (void)hipGetLastError();
     if (e == hipErrorOutOfMemory) return fail(Q35M_ERR_OOM, "%s: %s", what, hipGetErrorString(e));
     return fail(Q35M_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }

@@ -26,7 +26,10 @@ int pfail(int code, const char* fmt, ...) {
     return q35_set_error(code, buf);
 }
 
+// (HIP keeps an error for the thread's next hipGetLastError, which is that of a later
+// launch: it is taken back once it is reported.)
 int phip(hipError_t e, const char* what) {
+    (void)hipGetLastError();
     return pfail(e == hipErrorOutOfMemory ? Q35M_ERR_OOM : Q35M_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
@@ -36,10 +39,13 @@ int phip(hipError_t e, const char* what) {
         if (e_ != hipSuccess) return phip(e_, what);  \
     } while (0)
 
-// The context's device made current for a call, and the caller's put back.
+// The context's device made current for a call, and the caller's put back.  An error
+// that an earlier call of the thread left is not this call's: a launch that succeeded
+// would be reported as failed, and its change of lengths or pages not be kept.
 class DeviceScope {
 public:
     explicit DeviceScope(int device) {
+        (void)hipGetLastError();
         if (hipGetDevice(&before_) != hipSuccess) before_ = device;
         if (before_ != device) (void)hipSetDevice(device);
         else before_ = -1;
