@@ -258,8 +258,8 @@ typedef struct q35m_paged q35m_paged;
  * or NaN K value may make every dim NaN. */
 
 /* A cache of n_pages pages for every full-attention layer of ctx and n_seqs
- * sequences of up to max_rows rows each (max_rows up to 2^24); page_rows is a
- * power of two from 16 to 1024.  Allocates here (the pages, and 512 bytes a row
+ * sequences of up to max_rows rows each (max_rows up to 2^24, 2^30 counted once a
+ * q head, of up to 4096); page_rows is a power of two from 16 to 1024.  Allocates here (the pages, and 512 bytes a row
  * of max_rows for the rotation), and nothing afterwards.  At
  * first no page is mapped and every length is 0.  Destroy it before ctx. */
 int q35m_paged_create(q35m_ctx* ctx, int n_seqs, int max_rows, int n_pages, int page_rows, int kv_type,
@@ -297,7 +297,7 @@ int q35m_paged_device_ptr(q35m_paged* p, int layer, int kind, void** dptr, size_
  * whose attention nobody reads (all of a prompt but its last token, in the
  * model's last layer).  Rows past the last sequence's are not read.  Pages
  * must be mapped up to the last new row (Q35M_ERR_CAPACITY otherwise, as past
- * max_rows). */
+ * max_rows).  A call brings up to 2^24 rows (Q35M_ERR_UNSUPPORTED). */
 int q35m_paged_append(q35m_paged* p, int layer, int n, const int* seqs, const int* tokens, const float* k,
                       const float* v);
 /* q35m_attn_decode over paged rows: one new token of each of n sequences.
@@ -314,7 +314,8 @@ int q35m_paged_attn_decode(q35m_paged* p, int layer, int n, const int* seqs, con
  * at once: tokens[i] >= 0 rows of sequence seqs[i], in the sequences' order,
  * row j of a sequence at position length + j attending over the rows up to its
  * own.  q_gate [sum][heads*2*head_dim], k, v [sum][kv_heads*head_dim], out
- * [sum][heads*head_dim]; rows past the sum are neither read nor written.
+ * [sum][heads*head_dim]; rows past the sum are neither read nor written.  A call
+ * brings up to 2^24 rows, and 2^27 counted once a head (Q35M_ERR_UNSUPPORTED).
  * Captured and replayed as q35m_paged_attn_decode.
  * The attention calls on one cache share its workspace: graphs that hold them
  * are replayed in order, on one stream. */

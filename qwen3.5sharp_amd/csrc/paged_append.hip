@@ -50,14 +50,14 @@ __global__ __launch_bounds__(256) void paged_rope_fill(double* __restrict__ tabl
     table[row * kRopeDim + kRopeHalf + i] = sin(angle);
 }
 
-// One wave per (new row, kv head), four a workgroup.  Reads 2 KiB and writes 2
-// rows a wave: a copy with a reduction of one wave in between.
+// One wave per (new row, kv head), four a workgroup, from unit0 on.  Reads 2 KiB and
+// writes 2 rows a wave: a copy with a reduction of one wave in between.
 template <typename T>
 __global__ __launch_bounds__(256) void paged_append_rows(PagedView pv, PagedBatch b, const float* __restrict__ k,
                                                          const float* __restrict__ v, const float* __restrict__ k_norm,
-                                                         double eps) {
+                                                         double eps, long unit0) {
     const int lane = threadIdx.x & 63;
-    const long unit = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long unit = unit0 + (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = (int)(unit / pv.nkv), kvh = (int)(unit % pv.nkv);
     if (row >= b.off[b.n]) return;
     const size_t at = ((size_t)row * pv.nkv + kvh) * kHd + 4 * lane;
@@ -111,15 +111,22 @@ hipError_t launch_paged_lengths(q35m_ctx* c, int* lens, int n, const int* seq, c
 
 hipError_t launch_paged_append(q35m_paged* p, int layer, const PagedBatch& b, const float* k, const float* v) {
     q35m_ctx* c = p->ctx;
+    // (a grid holds fewer than 2^32 threads, 2^26 units)
+    constexpr long kMost = 1L << 22;
     const long units = (long)b.off[b.n] * c->d.nkv;
-    ProfScope ps(c, K_PAGED_APPEND);
-    auto go = [&](auto kern) {
-        hipExtLaunchKernelGGL(kern, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, c->stream, ps.a, ps.b, 0,
-                              p->view(layer), b, k, v, c->full[layer].k_norm, (double)c->d.eps);
-    };
-    if (p->type == Q35M_KV_F16) go(paged_append_rows<_Float16>);
-    else go(paged_append_rows<float>);
-    return hipGetLastError();
+    for (long u = 0; u < units; u += kMost) {
+        ProfScope ps(c, K_PAGED_APPEND);
+        auto go = [&](auto kern) {
+            const long n = units - u < kMost ? units - u : kMost;
+            hipExtLaunchKernelGGL(kern, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, c->stream, ps.a, ps.b, 0,
+                                  p->view(layer), b, k, v, c->full[layer].k_norm, (double)c->d.eps, u);
+        };
+        if (p->type == Q35M_KV_F16) go(paged_append_rows<_Float16>);
+        else go(paged_append_rows<float>);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace q35

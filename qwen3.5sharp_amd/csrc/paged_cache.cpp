@@ -4,6 +4,7 @@
 // the kernels read; a change of the host copy enqueues the same change of the
 // device copy on the context's stream, so calls enqueued before it see the old
 // state and calls after it the new one.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -109,8 +110,10 @@ int check_seqs(const q35m_paged* p, int n, const int* seqs) {
     return Q35M_OK;
 }
 
-// The batch of a call that writes tokens[i] rows (null: one) of each sequence.
-int build_batch(const q35m_paged* p, int n, const int* seqs, const int* tokens, bool need_tokens, q35::PagedBatch* b) {
+// The batch of a call that writes tokens[i] rows (null: one) of each sequence, up to
+// `most` in all.
+int build_batch(const q35m_paged* p, int n, const int* seqs, const int* tokens, bool need_tokens, long most,
+                q35::PagedBatch* b) {
     int r = check_seqs(p, n, seqs);
     if (r) return r;
     if (need_tokens && !tokens) return pfail(Q35M_ERR_INVALID, "null tokens");
@@ -120,15 +123,22 @@ int build_batch(const q35m_paged* p, int n, const int* seqs, const int* tokens, 
     for (int i = 0; i < n; ++i) {
         const int t = need_tokens ? tokens[i] : 1;
         if (t < 0) return pfail(Q35M_ERR_INVALID, "sequence %d: %d tokens", seqs[i], t);
-        const q35::PageMap::Result m = p->map.usable(seqs[i], t);
-        if (m != q35::PageMap::kOk) return map_fail(p, m, seqs[i]);
         sum += t;
-        if (sum > (1L << 24)) return pfail(Q35M_ERR_UNSUPPORTED, "more than 2^24 new rows in one call");
+        if (sum > most) return pfail(Q35M_ERR_UNSUPPORTED, "more than %ld new rows in one call", most);
         b->seq[i] = seqs[i];
         b->off[i + 1] = (int)sum;
     }
+    for (int i = 0; i < n; ++i) {
+        const q35::PageMap::Result m = p->map.usable(seqs[i], b->off[i + 1] - b->off[i]);
+        if (m != q35::PageMap::kOk) return map_fail(p, m, seqs[i]);
+    }
     return Q35M_OK;
 }
+
+// New rows of one call: an append, and a prefill, whose query rows (of all heads) are
+// what the grids count: of more than 2^27, q_gate and out would not fit the device.
+constexpr long kMostRows = 1L << 24, kMostQueryRows = 1L << 27;
+constexpr int kMostHeads = 4096;    // a tile's rows are within 2^31 bytes of its first
 
 int not_capturing(const q35m_paged* p, const char* what) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
@@ -193,6 +203,7 @@ int q35m_paged_create(q35m_ctx* ctx, int n_seqs, int max_rows, int n_pages, int 
     if (max_rows > (1 << 24)) return pfail(Q35M_ERR_UNSUPPORTED, "max_rows %d: up to 2^24", max_rows);
     if ((long)max_rows * ctx->d.nh > (1L << 30))     // the kernels count units of 64 rows and head groups in 32 bits
         return pfail(Q35M_ERR_UNSUPPORTED, "max_rows %d: up to 2^30 over the %d q heads", max_rows, ctx->d.nh);
+    if (ctx->d.nh > kMostHeads) return pfail(Q35M_ERR_UNSUPPORTED, "%d q heads: up to %d", ctx->d.nh, kMostHeads);
     int shift = 4;
     while (shift <= 10 && (1 << shift) != page_rows) ++shift;
     if (shift > 10) return pfail(Q35M_ERR_UNSUPPORTED, "page_rows %d: a power of two from 16 to 1024", page_rows);
@@ -300,7 +311,7 @@ int q35m_paged_append(q35m_paged* p, int layer, int n, const int* seqs, const in
     if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
     int r = check_layer(p, layer, true);
     q35::PagedBatch b;
-    if (!r) r = build_batch(p, n, seqs, tokens, true, &b);
+    if (!r) r = build_batch(p, n, seqs, tokens, true, kMostRows, &b);
     if (!r) r = check_pointers({k, v});
     if (r || b.off[n] == 0) return r;
     DeviceScope dev(p->ctx->device);
@@ -313,7 +324,7 @@ int q35m_paged_attn_decode(q35m_paged* p, int layer, int n, const int* seqs, con
     if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
     int r = check_layer(p, layer, true);
     q35::PagedBatch b;
-    if (!r) r = build_batch(p, n, seqs, nullptr, false, &b);
+    if (!r) r = build_batch(p, n, seqs, nullptr, false, kMostRows, &b);
     if (!r) r = check_pointers({q_gate, k, v, out});
     if (r) return r;
     DeviceScope dev(p->ctx->device);
@@ -326,7 +337,7 @@ int q35m_paged_attn_prefill(q35m_paged* p, int layer, int n, const int* seqs, co
     if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
     int r = check_layer(p, layer, true);
     q35::PagedBatch b;
-    if (!r) r = build_batch(p, n, seqs, tokens, true, &b);
+    if (!r) r = build_batch(p, n, seqs, tokens, true, std::min(kMostRows, kMostQueryRows / p->ctx->d.nh), &b);
     if (!r) r = check_pointers({q_gate, k, v, out});
     if (r || b.off[n] == 0) return r;
     DeviceScope dev(p->ctx->device);
