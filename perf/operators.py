@@ -11,6 +11,11 @@ Sequence i holds `rows` cached rows (fewer, unequally many, where `ragged`) and 
 pages of `page` rows lie in a random order in the pool, whose free pages and unwritten rows hold other conversations'
 stale values.  `half` is a cache of 16-bit floats, else of 32-bit ones; a row is rounded to it once.
 
+Streams: the library works on its context's own stream, which does not wait for torch's nor torch's for it.  prepare()
+waits for the card before it takes memory that an earlier state's calls may still read, and after it has made the
+inputs; run() enqueues, as a serving loop does, whose calls follow each other on that stream, and whoever takes its
+outputs elsewhere synchronises first.
+
 Where `own` is false, run() computes the same with elementary torch operations: 32 bits, with 64 for the rotation and
 the norm (whose K rows are rounded to 16 bits).  Where it is true it calls the library's front end, on buffers of the
 same shape and contents.
@@ -192,6 +197,8 @@ class _Buf:
 
 
 def prepare(case, seed):
+    if own:
+        torch.cuda.synchronize()
     x, lens, counts, per, pool, table = _inputs(case, seed)
     n, nkv, half = case["n"], case["nkv"], case["half"]
     shape = (pool, nkv, case["page"], HD)
@@ -212,6 +219,7 @@ def prepare(case, seed):
         s["args"] = [_Buf(x[k]) for k in (("k", "v") if case["kind"] == "append" else ("q_gate", "k", "v"))]
         if case["kind"] != "append":
             s["args"].append(_Buf(s["out"]))
+        torch.cuda.synchronize()
         return s
     # Plan of the plain form: each new row's sequence, place in its chunk and position.
     seq = np.repeat(np.arange(n), counts)
