@@ -83,12 +83,13 @@ def same_kind(got, want, tol):
 
 
 @pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
-@pytest.mark.parametrize("n,T,sharp", [(0, 30, 1), (90, 40, 1), (1700, 70, 1), (1700, 70, 8), (300, 1, 1), (2500, 1, 8)])
-def test_infinite_values(kv_type, n, T, sharp):
+@pytest.mark.parametrize("n,T,sharp,nh", [(0, 30, 1, 16), (90, 40, 1, 16), (90, 40, 1, 4), (1700, 70, 1, 16), (1700, 70, 8, 16),
+                                          (600, 20, 1, 64), (300, 1, 1, 16), (300, 1, 1, 4), (2500, 1, 8, 16), (2500, 1, 1, 64)])
+def test_infinite_values(kv_type, n, T, sharp, nh):
     """A V of +-inf makes the output of every token that sees it that infinity in its dim and heads, however small its
     weight; infinities of both signs, or a NaN, make it NaN.  T = 1 runs the one-token kernels and a chunk of one.
     (sharp: cached K times 8, scores of deviation 32 nats.  TOL as in test_gpu_paged.py, scores 8 times the size.)"""
-    with Paged(kv_type, n_seqs=2, max_rows=n + T, page_rows=32) as p:
+    with Paged(kv_type, nh=nh, n_seqs=2, max_rows=n + T, page_rows=32) as p:
         rs = np.random.RandomState(n + T)
         x = {k: v.copy() for k, v in p.inputs(T, salt=75).items()}
         xv = x["v"].reshape(T, p.nkv, HD)
@@ -198,3 +199,26 @@ def test_fp32_values_near_the_largest():
         want = p.attend([0], [T], x)
         close_to(one.download().astype(np.float64), want[:1])
         close_to(out.download().astype(np.float64), want)
+
+
+# ------------------------------------------------------------------ prompts of many tiles
+
+@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
+@pytest.mark.parametrize("n,T,page", [(0, 2048, 64), (0, 1031, 16), (700, 1500, 128)])
+def test_prompts_of_whole_and_cut_tiles(kv_type, n, T, page):
+    """16 q heads on 4 kv heads: 2048 rows are two whole tiles a workgroup, paired first with last; the others are cut.
+    Rows of tiles at both ends and in the middle.  Tolerance: test_gpu_paged.py's."""
+    with Paged(kv_type, max_rows=n + T, page_rows=page, salt=7) as p:
+        rs = np.random.RandomState(n + T)
+        for which in range(2):
+            put_rows(p, 0, which, rs.standard_normal((n, p.nkv, HD)).astype(np.float32))
+        start(p, n)
+        x = p.inputs(T, salt=79)
+        out = p.ctx.array((T, p.nh * HD))
+        p.c.attn_prefill(0, [0], [T], *p.dev(x, "q_gate", "k", "v"), out)
+        p.put([0], [T], x)
+        mid = T // 2 // 16 * 16
+        some = sorted({*range(18), *range(mid - 2, mid + 18, 3), *range(T // 3, T // 3 + 33, 8), *range(T - 18, T)})
+        e = close_to(out.download().astype(np.float64), p.attend([0], [T], x, some))
+        say(f"prompt of {T} behind {n} type {kv_type}: {e:.1e}")
+        p.check_pages()
