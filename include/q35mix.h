@@ -245,23 +245,28 @@ typedef struct q35m_paged q35m_paged;
 
 /* How a cache holds K and V: fp32, or fp16 (half the memory and the traffic:
  * the values of an fp32 cache, rounded to nearest even when their row is
- * written, beyond the range of fp16 to infinities; activations and outputs are
- * fp32, and the attention adds no rounding beyond fp32's, but that
- * q35m_paged_attn_prefill takes bits of a weight's product with a V value below 2^-126
- * as 0, weights of 2^-14 for the largest: V values below 2^-96 begin to lose bits).
+ * written, beyond the range of fp16 to infinities); activations and outputs are
+ * fp32.  What the attention rounds beyond fp32's half steps of 2^-24:
+ *  - over an fp16 cache the normed q and the softmax weights are held to 2^-23 of
+ *    themselves, q values to no less than 2^-39 of 16 max |1 + w|, weights to no less
+ *    than 2^-31 (q35m_paged_attn_decode: 2^-40) of the row's largest;
+ *  - over an fp32 cache q35m_paged_attn_prefill takes the bits below 2^-126 of a
+ *    weight's product with a V value as 0, the largest weight being 2^-14 or more: V
+ *    values below 2^-96 begin to lose bits.
  * An output is finite where the sum of |V| over the rows that its token sees is. */
 #define Q35M_KV_F32 0
 #define Q35M_KV_F16 1
 /* Values that are not finite reach the outputs of the tokens that see their row and
  * no other: an infinite V value makes its dim of the output that infinity, whatever
  * the row's weight, and V infinities of both signs or a NaN make it NaN; an infinite
- * or NaN K value may make every dim NaN. */
+ * or NaN K value may make every dim NaN.  (Such a call takes up to twelve times as long.) */
 
 /* A cache of n_pages pages for every full-attention layer of ctx and n_seqs
  * sequences of up to max_rows rows each (max_rows up to 2^24, 2^30 counted once a
  * q head, of up to 4096); page_rows is a power of two from 16 to 1024.  Allocates here (the pages, and 512 bytes a row
  * of max_rows for the rotation), and nothing afterwards.  At
- * first no page is mapped and every length is 0.  Destroy it before ctx. */
+ * first no page is mapped and every length is 0.  Destroy it before ctx, and replay no
+ * graph that holds its calls afterwards. */
 int q35m_paged_create(q35m_ctx* ctx, int n_seqs, int max_rows, int n_pages, int page_rows, int kv_type,
                       q35m_paged** out);
 int q35m_paged_destroy(q35m_paged* p);

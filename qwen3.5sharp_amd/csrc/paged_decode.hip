@@ -27,7 +27,7 @@
 //   order; so neither P nor V crosses lanes.
 // fp32 caches use the fp32 instruction (16 x 16 x 4).  fp16 caches use
 // 16 x 16 x 32 on fp16 with the fp32 operands q and P as two fp16 values each
-// (hi + lo, 22 bits; q's row and P scaled by powers of two into the range),
+// (hi + lo, to 2^-23 of the value; q's row and P scaled by powers of two into the range),
 // and a register transpose of V (8 rows x 8 dims a lane).
 // The waves share the forming of q rows through LDS: formed in every wave, behind
 // K and V in the queue of loads, they cost a call over 8192 rows 2 of its 13 us
@@ -618,7 +618,7 @@ __global__ __launch_bounds__(MW * kWave) void paged_decode_merge(PagedView pv, P
     }
 }
 
-// One workgroup a CU (300 registers a lane).
+// One workgroup a CU: up to 256 vector and 216 accumulation registers a lane.
 int decode_workgroups(const q35m_ctx* c) { return c->n_cu; }
 
 }  // namespace

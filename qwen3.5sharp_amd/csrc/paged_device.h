@@ -80,8 +80,9 @@ __device__ __forceinline__ float4 paged_key_row(float4 x, const double* __restri
 }
 
 // Exponent e such that every value of a normed q row, times log2(e) / 16 and
-// 2^e, is below 2^15: its fp16 halves are in range whatever the norm weights,
-// and values 2^-10 of the largest keep all 22 bits.  |q_d| <= 16 |1 + w_d|.
+// 2^e, is below 2^15: its fp16 halves are in range whatever the norm weights, and
+// hold values from 2^-16 of the bound on to 2^-23 of themselves, smaller ones to 2^-39 of
+// it.  |q_d| <= 16 |1 + w_d|.
 __device__ __forceinline__ int q_exponent(const float* __restrict__ w, int lane) {
     const float4 a = *reinterpret_cast<const float4*>(w + 4 * lane);
     const float m = fmaxf(fmaxf(fabsf(1.0f + a.x), fabsf(1.0f + a.y)), fmaxf(fabsf(1.0f + a.z), fabsf(1.0f + a.w)));
@@ -89,7 +90,7 @@ __device__ __forceinline__ int q_exponent(const float* __restrict__ w, int lane)
     return 15 - __builtin_amdgcn_readfirstlane(max(min(e, 100), -100));
 }
 
-// (a, b) = hi + lo to 22 bits each: one conversion of the pair and a fused
+// (a, b) = hi + lo to 2^-23 of each: one conversion of the pair and a fused
 // multiply-add for each remainder (a - hi, exact, rounded to fp16).  hi is made a
 // value of its own before it is used: where a is a product, the compiler would
 // otherwise round it to fp16 in one step for one use and in two for another,

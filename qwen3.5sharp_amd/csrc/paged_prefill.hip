@@ -352,7 +352,8 @@ __device__ __forceinline__ void settle_rows(const float4* os, const PagedView& p
 // ..; so a row's q is in both waves' registers (128 of them) but its output in
 // one's (64), and the two never have to be joined.
 // 32 x 32 x 16 instructions on fp16 with the fp32 operands q and P as two fp16
-// values each: hi + lo, 22 bits, two products an operand pair.  K and V units
+// values each: hi + lo, to 2^-23 of the value, two products an operand pair (three parts
+// would be half as many products again; one part is 2^-11 off).  K and V units
 // are double-buffered in LDS by loads that bypass the registers, 16-byte chunks
 // permuted by row so that the rows that one read touches fall into different
 // banks (K: chunk ^ row % 16, V: chunk ^ 4 (row % 4)); V is transposed as it is
@@ -364,17 +365,17 @@ __device__ __forceinline__ void settle_rows(const float4* os, const PagedView& p
 // maximum a row that the weights refer to; the maxima of a unit's two halves meet
 // with the weights of the unit before, and it moves only when a score passes it by
 // kMove.
-// What bounds it: the matrix instructions' power.  64 a unit and SIMD are 2048
-// cycles, at which random operands pull the clock to 1.55 GHz (20 ns each where
-// zeros take 15): 1.3 us a unit.  It takes 3400 cycles at 1.8 GHz: a single wave a
-// SIMD issues everything in order, about four vector instructions in a matrix
-// instruction's shadow (16.4 ns a product with up to 4, 22.9 with 6, 34 with 12),
-// so what is the same every unit is a kept address, a scalar or an offset in the
-// instruction, the loads of the next unit are spread over the score products
-// (in one run of 16 they held the wave for 800 cycles), and every LDS read is a
-// step ahead.  2048 rows over as many: 90 us; 512 over 16384: 257 to 265 us.  Two
-// workgroups a CU with half the registers each, partners splitting the dims and
-// exchanging scores (twice the exponentials): 133 and 318 us.
+// What bounds it: issue.  The 64 matrix instructions of a unit and SIMD are 2048
+// cycles, of the 3400 that it takes at 1.8 GHz: a single wave a SIMD issues everything
+// in order, about four vector instructions in a matrix instruction's shadow (16.4 ns a
+// product with up to 4, 22.9 with 6, 34 with 12), so what is the same every unit is a
+// kept address, a scalar or an offset in the instruction, the loads of the next unit
+// are spread over the score products (in one run of 16 they held the wave for 800
+// cycles), and every LDS read is a step ahead.  (Closer feeding gains less than it
+// counts: on random operands the pipe pulls the clock to 1.55 GHz, 20 ns a product or
+// 1.3 us a unit, where zeros take 15.)  2048 rows over as many: 92 us; 512 over 16384:
+// 265 to 268 us.  Two workgroups a CU with half the registers each, partners splitting
+// the dims and exchanging scores (twice the exponentials): 133 and 318 us.
 // A segment's beginning and end are 30000 cycles of it (40 % of a call of 2048 rows):
 // partners form half of q each (9000 -> 5800 cycles), and the last rows' LDS reads and the gates come
 // before the first store, whose end a later load's wait would wait for (16000 ->

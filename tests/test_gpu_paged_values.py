@@ -1,5 +1,10 @@
 """Paged K/V cache on the GPU: values at which an output could lose bits, range or its sign, against the plain
-restatement in 64 bits of test_gpu_paged.py.  Each test states its own tolerance."""
+restatement in 64 bits of test_gpu_paged.py.  Each test states its own tolerance.
+
+That file's bound of 2e-5 of the largest output counts fp32's roundings, a deviation of 9e-6.  Over an fp16 cache two
+more belong to it, q and the weights to 2^-23 of themselves: 256 products of about 2 (a score of 32 in size) each off by
+2^-23 of itself with random signs move the score by 16 * 2^-23 * 2 / sqrt(3) = 2.2e-6, and a weight's own rounding is
+1.2e-7 of it.  In squares that is 9.3e-6, twice which the bound still covers."""
 import numpy as np
 import pytest
 
