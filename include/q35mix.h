@@ -256,6 +256,15 @@ typedef struct q35m_paged q35m_paged;
  * An output is finite where the sum of |V| over the rows that its token sees is. */
 #define Q35M_KV_F32 0
 #define Q35M_KV_F16 1
+/* In 4 bits (a quarter of fp16's memory and traffic, 17 bytes for 32 values): MX blocks of
+ * 32 consecutive dims of a row, which share a power of two 2^s, each value one of 0, 1/2, 1,
+ * 3/2, 2, 3, 4, 6 times it, with a sign.  s is the smallest with the block's largest value at most
+ * 7 2^s, within -23 .. 13; values are rounded to the nearest of these, ties to the even
+ * code, and beyond the last one to it: K rows as an fp32 cache holds them, V rows as they
+ * come.  Beyond what an fp16 cache's attention rounds (see above), nothing is: the
+ * held values take part as they are, and q in a 4-bit cache's scores is held to 2^-19 of
+ * the largest value of its 32 dims.  A block with a value that is not finite is NaN, in all of its dims. */
+#define Q35M_KV_MXFP4 4
 /* Values that are not finite reach the outputs of the tokens that see their row and
  * no other: an infinite V value makes its dim of the output that infinity, whatever
  * the row's weight, and V infinities of both signs or a NaN make it NaN; an infinite
@@ -290,7 +299,10 @@ int q35m_paged_truncate(q35m_paged* p, int seq, int length);
 int q35m_paged_len(const q35m_paged* p, int seq, int* length);
 /* Device address and size of one layer's pages, for zero-copy callers: kind
  * Q35M_STATE_KEYS or Q35M_STATE_VALUES, [n_pages][kv_heads][page_rows]
- * [head_dim] values of the cache's type. */
+ * [head_dim] values of the cache's type.  In 4 bits each [n_pages][kv_heads] is
+ * 136 page_rows bytes: the codes [page_rows][128], dim 2 i in the lower half of byte i (the sign
+ * its top bit), then the scales, s + 127 or 255 for NaN, of K [page_rows][8], of V
+ * [page_rows / 16][8][16]. */
 int q35m_paged_device_ptr(q35m_paged* p, int layer, int kind, void** dptr, size_t* bytes);
 
 /* The rows of new tokens of n sequences put into their pages: for each
@@ -305,6 +317,13 @@ int q35m_paged_device_ptr(q35m_paged* p, int layer, int kind, void** dptr, size_
  * max_rows).  A call brings up to 2^24 rows (Q35M_ERR_UNSUPPORTED). */
 int q35m_paged_append(q35m_paged* p, int layer, int n, const int* seqs, const int* tokens, const float* k,
                       const float* v);
+/* Rows as the cache holds them, in fp32: for each sequence seqs[i] the rows first[i]
+ * .. first[i] + count[i] - 1 (HOST arrays; seqs distinct, up to 64; up to 2^24 rows), in
+ * the sequences' order, to k and v [sum of counts][kv_heads*head_dim].  Any rows whose
+ * pages are mapped, beyond the length too (Q35M_ERR_CAPACITY otherwise, as past
+ * max_rows); after a plan (below) rows of pages that are not mapped are zeros. */
+int q35m_paged_rows(q35m_paged* p, int layer, int n, const int* seqs, const int* first, const int* count, float* k,
+                    float* v);
 /* q35m_attn_decode over paged rows: one new token of each of n sequences.
  * q_gate [n][heads*2*head_dim], k, v [n][kv_heads*head_dim], out
  * [n][heads*head_dim].  The lengths and page tables are read on the device:
@@ -326,6 +345,34 @@ int q35m_paged_attn_decode(q35m_paged* p, int layer, int n, const int* seqs, con
  * are replayed in order, on one stream. */
 int q35m_paged_attn_prefill(q35m_paged* p, int layer, int n, const int* seqs, const int* tokens,
                             const float* q_gate, const float* k, const float* v, float* out);
+
+/* Page tables and slots from request lengths that the device has, in one launch and
+ * without the host, for serving loops that are captured whole or learn the lengths on
+ * the device.  All arrays are DEVICE memory.  Request i is sequence i of the cache, i < n: it holds
+ * rows[i] rows and brings tokens[i] more.  Its length becomes rows[i]; the pages of its
+ * rows stay; the pages that its tokens need beyond them come from free_pages [n_free],
+ * in the requests' order, all of them or, where the list is too short up to and with
+ * this request, none; its entries behind these become -1.  taken[i] is how many it took, or -1
+ * where it got none of those it needs.  slots (row of the page times page_rows added to
+ * by the row in it: page * page_rows + row; -1 where the token has no page) come for the
+ * tokens of all requests in order, up to n_slots of them; what is behind stays.  Up to
+ * 65535 requests.
+ * rows and tokens are taken within 0 and max_rows, in that order; page ids of the list
+ * outside [0, n_pages) count as no page.
+ * A first call gives the lengths and tables over to the device: q35m_paged_map, _advance,
+ * _truncate and _len are refused from then on (Q35M_ERR_INVALID), the operators above
+ * no longer check lengths or pages but bring up to max_rows rows a sequence, leave out rows
+ * that have no page, and what they give for a token whose rows are not all mapped is
+ * undefined (no other token's is).  Which pages requests share is the caller's
+ * to keep: no page that is taken may be in another's rows.  Capturable; replays plan the
+ * lengths of their time. */
+int q35m_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
+                    int64_t* slots, size_t n_slots, int* taken);
+/* Device addresses of the tables [n_seqs][*max_pages] (page ids, -1: not mapped) and
+ * the lengths [n_seqs], which the calls on the context's stream read and a plan writes.
+ * A caller may set entries of the tables before a plan (a shared prefix's pages); the lengths are
+ * to be read only. */
+int q35m_paged_tables(q35m_paged* p, int** table, int** lens, int* max_pages);
 
 /* ---- one decode step of every layer, captured once, replayed per token ---- */
 

@@ -205,7 +205,8 @@ const char* kernel_name(int id) {
         "linear_qt<1>", "attn_decode_partial<4,16>", "attn_decode_partial<8,16>", "q6k_gemm_blk",
         "linear_gemm<5>", "linear_gemm<14>", "linear_gemm<2>", "linear_gemm<1>",
         "attn_split_prep", "attn_split_flash", "attn_split_merge", "linear_gemm<4>", "linear_gemm<6>",
-        "paged_append_rows", "paged_decode", "paged_decode_merge", "paged_prefill", "paged_prefill_merge"};
+        "paged_append_rows", "paged_decode", "paged_decode_merge", "paged_prefill", "paged_prefill_merge",
+        "paged_rows", "paged_plan"};
     return (id >= 0 && id < K_COUNT) ? names[id] : nullptr;
 }
 

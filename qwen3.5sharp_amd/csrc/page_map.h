@@ -75,6 +75,16 @@ public:
         return kOk;
     }
 
+    // Whether rows [first, first + n) of seq may be read; `bound`: as far as max_rows goes, mapped or not.
+    Result readable(int seq, int first, int n, bool bound) const {
+        if (!has(seq)) return kBadSeq;
+        if (first > max_rows_ - n) return kTooLong;
+        if (!bound && n > 0)
+            for (int i = first / page_rows_; i <= (first + n - 1) / page_rows_; ++i)
+                if (page(seq, i) < 0) return kUnmapped;
+        return kOk;
+    }
+
 private:
     int n_seqs_, max_rows_, max_pages_, n_pages_, page_rows_;
     std::vector<int> table_;

@@ -71,9 +71,47 @@ __global__ __launch_bounds__(256) void paged_append_rows(PagedView pv, PagedBatc
     const int page = page_of(pv.table + (size_t)seq * pv.max_pages, pos >> pv.page_shift, pv.max_pages, pv.n_pages);
     if (page < 0) return;
     const float4 y = paged_key_row(xk, pv.rope + (size_t)pos * kRopeDim, k_norm, lane, eps);
-    const size_t to = row_offset<T>(pv, page, kvh, pos) + 4 * lane;
-    store_row4((T*)pv.k + to, y);
-    store_row4((T*)pv.v + to, xv);
+    if constexpr (std::is_same_v<T, Mx4>) {
+        const int in = pos & ((1 << pv.page_shift) - 1);
+        mx_put_key((uint8_t*)pv.k + mx_page(pv, page, kvh), pv, in, mx_round(y), lane);
+        mx_put_value((uint8_t*)pv.v + mx_page(pv, page, kvh), pv, in, mx_round(xv), lane);
+    } else {
+        const size_t to = row_offset<T>(pv, page, kvh, pos) + 4 * lane;
+        store_row4((T*)pv.k + to, y);
+        store_row4((T*)pv.v + to, xv);
+    }
+}
+
+// Rows read back, one wave per (row, kv head): row `row` of the call is row first + (its
+// place) of its sequence.  Rows of pages that are not mapped are zeros.
+template <typename T>
+__global__ __launch_bounds__(256) void paged_rows(PagedView pv, PagedBatch b, PagedFirst first, float* __restrict__ k,
+                                                  float* __restrict__ v, long unit0) {
+    const int lane = threadIdx.x & 63;
+    const long unit = unit0 + (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = (int)(unit / pv.nkv), kvh = (int)(unit % pv.nkv);
+    if (row >= b.off[b.n]) return;
+    const int i = __popcll(__ballot(lane < b.n && b.off[min(lane, b.n)] <= row)) - 1;
+    const int pos = first.row[i] + row - b.off[i];
+    const int page = page_of(pv.table + (size_t)b.seq[i] * pv.max_pages, pos >> pv.page_shift, pv.max_pages, pv.n_pages);
+    float4 xk = make_float4(0.f, 0.f, 0.f, 0.f), xv = xk;
+    if (page >= 0) {
+        if constexpr (std::is_same_v<T, Mx4>) {
+            const int in = pos & ((1 << pv.page_shift) - 1);
+            const uint8_t* const kp = (const uint8_t*)pv.k + mx_page(pv, page, kvh);
+            const uint8_t* const vp = (const uint8_t*)pv.v + mx_page(pv, page, kvh);
+            const uint32_t at = (uint32_t)in * kMxCodes + 2 * lane;
+            xk = mx_values({*reinterpret_cast<const uint16_t*>(kp + at), kp[mx_key_scale(pv, in) + (lane >> 3)]});
+            xv = mx_values({*reinterpret_cast<const uint16_t*>(vp + at), vp[mx_value_scale(pv, in, lane >> 3)]});
+        } else {
+            const size_t at = row_offset<T>(pv, page, kvh, pos) + 4 * lane;
+            xk = load_row4((const T*)pv.k + at);
+            xv = load_row4((const T*)pv.v + at);
+        }
+    }
+    const size_t to = ((size_t)row * pv.nkv + kvh) * kHd + 4 * lane;
+    *reinterpret_cast<float4*>(k + to) = xk;
+    *reinterpret_cast<float4*>(v + to) = xv;
 }
 
 }  // namespace
@@ -121,8 +159,29 @@ hipError_t launch_paged_append(q35m_paged* p, int layer, const PagedBatch& b, co
             hipExtLaunchKernelGGL(kern, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, c->stream, ps.a, ps.b, 0,
                                   p->view(layer), b, k, v, c->full[layer].k_norm, (double)c->d.eps, u);
         };
-        if (p->type == Q35M_KV_F16) go(paged_append_rows<_Float16>);
+        if (p->type == Q35M_KV_MXFP4) go(paged_append_rows<Mx4>);
+        else if (p->type == Q35M_KV_F16) go(paged_append_rows<_Float16>);
         else go(paged_append_rows<float>);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+hipError_t launch_paged_rows(q35m_paged* p, int layer, const PagedBatch& b, const PagedFirst& first, float* k, float* v) {
+    q35m_ctx* c = p->ctx;
+    constexpr long kMost = 1L << 22;
+    const long units = (long)b.off[b.n] * c->d.nkv;
+    for (long u = 0; u < units; u += kMost) {
+        ProfScope ps(c, K_PAGED_ROWS);
+        auto go = [&](auto kern) {
+            const long n = units - u < kMost ? units - u : kMost;
+            hipExtLaunchKernelGGL(kern, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, c->stream, ps.a, ps.b, 0,
+                                  p->view(layer), b, first, k, v, u);
+        };
+        if (p->type == Q35M_KV_MXFP4) go(paged_rows<Mx4>);
+        else if (p->type == Q35M_KV_F16) go(paged_rows<_Float16>);
+        else go(paged_rows<float>);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -129,7 +129,10 @@ int build_batch(const q35m_paged* p, int n, const int* seqs, const int* tokens, 
         b->off[i + 1] = (int)sum;
     }
     for (int i = 0; i < n; ++i) {
-        const q35::PageMap::Result m = p->map.usable(seqs[i], b->off[i + 1] - b->off[i]);
+        const int t = b->off[i + 1] - b->off[i];
+        // (after a plan the kernels keep to the pages and lengths that they find)
+        const q35::PageMap::Result m = !p->planned ? p->map.usable(seqs[i], t)
+                                       : t > p->map.max_rows() ? q35::PageMap::kTooLong : q35::PageMap::kOk;
         if (m != q35::PageMap::kOk) return map_fail(p, m, seqs[i]);
     }
     return Q35M_OK;
@@ -146,6 +149,11 @@ int not_capturing(const q35m_paged* p, const char* what) {
     if (st != hipStreamCaptureStatusNone)
         return pfail(Q35M_ERR_INVALID, "%s: the stream is being captured (a replay would repeat the change)", what);
     return Q35M_OK;
+}
+
+// The host's tables and lengths are the device's until a plan.
+int not_planned(const q35m_paged* p, const char* what) {
+    return p->planned ? pfail(Q35M_ERR_INVALID, "%s: the cache's lengths and tables are planned on the device", what) : Q35M_OK;
 }
 
 void release(q35m_paged* p) {
@@ -168,7 +176,7 @@ int fill(q35m_paged* p, int page_rows) {
     p->k.assign(layers, nullptr);
     p->v.assign(layers, nullptr);
     p->allocations.reserve(2 * (size_t)layers + 4);
-    p->layer_bytes = (size_t)p->n_pages * c->d.nkv * page_rows * q35::kHd * p->value_bytes();
+    p->layer_bytes = (size_t)p->n_pages * c->d.nkv * page_rows * p->row_bytes();
     const size_t entries = (size_t)p->map.n_seqs() * p->map.max_pages();
     int r = Q35M_OK;
     for (int l = 0; l < layers && !r; ++l) {
@@ -207,7 +215,8 @@ int q35m_paged_create(q35m_ctx* ctx, int n_seqs, int max_rows, int n_pages, int 
     int shift = 4;
     while (shift <= 10 && (1 << shift) != page_rows) ++shift;
     if (shift > 10) return pfail(Q35M_ERR_UNSUPPORTED, "page_rows %d: a power of two from 16 to 1024", page_rows);
-    if (kv_type != Q35M_KV_F32 && kv_type != Q35M_KV_F16) return pfail(Q35M_ERR_INVALID, "unknown cache type %d", kv_type);
+    if (kv_type != Q35M_KV_F32 && kv_type != Q35M_KV_F16 && kv_type != Q35M_KV_MXFP4)
+        return pfail(Q35M_ERR_INVALID, "unknown cache type %d", kv_type);
     bool any = false;
     for (int l = 0; l < ctx->cfg.num_layers; ++l) any |= ctx->is_recurrent[l] == 0;
     if (!any) return pfail(Q35M_ERR_INVALID, "the context has no full-attention layer");
@@ -244,7 +253,8 @@ int q35m_paged_destroy(q35m_paged* p) {
 int q35m_paged_map(q35m_paged* p, int seq, int first, int n, const int* pages) {
     if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
     DeviceScope dev(p->ctx->device);
-    int r = not_capturing(p, "paged_map");
+    int r = not_planned(p, "paged_map");
+    if (!r) r = not_capturing(p, "paged_map");
     if (r) return r;
     const q35::PageMap::Result m = p->map.can_map(seq, first, n, pages);
     if (m != q35::PageMap::kOk) return map_fail(p, m, seq);
@@ -260,7 +270,7 @@ int q35m_paged_advance(q35m_paged* p, int n, const int* seqs, const int* tokens)
     int r = check_seqs(p, n, seqs);
     if (r) return r;
     if (!tokens) return pfail(Q35M_ERR_INVALID, "null tokens");
-    if ((r = not_capturing(p, "paged_advance"))) return r;
+    if ((r = not_planned(p, "paged_advance")) || (r = not_capturing(p, "paged_advance"))) return r;
     int len[q35::kMaxBatch];
     for (int i = 0; i < n; ++i) {
         if (tokens[i] < 0) return pfail(Q35M_ERR_INVALID, "negative advance %d", tokens[i]);
@@ -277,6 +287,7 @@ int q35m_paged_truncate(q35m_paged* p, int seq, int length) {
     if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
     DeviceScope dev(p->ctx->device);
     if (!p->map.has(seq)) return map_fail(p, q35::PageMap::kBadSeq, seq);
+    if (int planned = not_planned(p, "paged_truncate")) return planned;
     if (length < 0) return pfail(Q35M_ERR_INVALID, "negative length %d", length);
     if (length > p->map.length(seq))
         return pfail(Q35M_ERR_RANGE, "cannot extend sequence %d from %d to %d", seq, p->map.length(seq), length);
@@ -291,6 +302,7 @@ int q35m_paged_len(const q35m_paged* p, int seq, int* length) {
     if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
     if (!p->map.has(seq)) return map_fail(p, q35::PageMap::kBadSeq, seq);
     if (!length) return pfail(Q35M_ERR_INVALID, "null length");
+    if (int planned = not_planned(p, "paged_len")) return planned;
     *length = p->map.length(seq);
     return Q35M_OK;
 }
@@ -343,6 +355,59 @@ int q35m_paged_attn_prefill(q35m_paged* p, int layer, int n, const int* seqs, co
     DeviceScope dev(p->ctx->device);
     PHIP_TRY(q35::launch_paged_append(p, layer, b, k, v), "paged_attn_prefill rows");
     PHIP_TRY(q35::launch_paged_prefill(p, layer, b, q_gate, out), "paged_attn_prefill");
+    return Q35M_OK;
+}
+
+int q35m_paged_rows(q35m_paged* p, int layer, int n, const int* seqs, const int* first, const int* count, float* k,
+                    float* v) {
+    if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
+    int r = check_layer(p, layer, false);
+    if (!r) r = check_seqs(p, n, seqs);
+    if (r) return r;
+    if (!first || !count) return pfail(Q35M_ERR_INVALID, "null first or count");
+    q35::PagedBatch b;
+    q35::PagedFirst f;
+    long sum = 0;
+    b.n = n;
+    b.off[0] = 0;
+    for (int i = 0; i < n; ++i) {
+        if (first[i] < 0 || count[i] < 0)
+            return pfail(Q35M_ERR_INVALID, "sequence %d: %d rows from row %d", seqs[i], count[i], first[i]);
+        if ((sum += count[i]) > kMostRows) return pfail(Q35M_ERR_UNSUPPORTED, "more than %ld rows in one call", kMostRows);
+        const q35::PageMap::Result m = p->map.readable(seqs[i], first[i], count[i], p->planned);
+        if (m != q35::PageMap::kOk) return map_fail(p, m, seqs[i]);
+        b.seq[i] = seqs[i];
+        f.row[i] = first[i];
+        b.off[i + 1] = (int)sum;
+    }
+    if ((r = check_pointers({k, v})) || sum == 0) return r;
+    DeviceScope dev(p->ctx->device);
+    PHIP_TRY(q35::launch_paged_rows(p, layer, b, f, k, v), "paged_rows");
+    return Q35M_OK;
+}
+
+int q35m_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
+                    int64_t* slots, size_t n_slots, int* taken) {
+    if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
+    if (n < 1 || n > p->map.n_seqs())
+        return pfail(Q35M_ERR_CAPACITY, "%d requests (1..%d, the cache's sequences)", n, p->map.n_seqs());
+    if (n > 65535) return pfail(Q35M_ERR_UNSUPPORTED, "%d requests: up to 65535 in one plan", n);
+    if (n_free < 0) return pfail(Q35M_ERR_INVALID, "%d free pages", n_free);
+    if (!rows || !tokens || !taken || (!free_pages && n_free) || (!slots && n_slots))
+        return pfail(Q35M_ERR_INVALID, "null array of a plan");
+    if (((uintptr_t)rows | (uintptr_t)tokens | (uintptr_t)taken | (uintptr_t)free_pages) & 3 || (uintptr_t)slots & 7)
+        return pfail(Q35M_ERR_INVALID, "arrays of a plan must be aligned to their values");
+    DeviceScope dev(p->ctx->device);
+    PHIP_TRY(q35::launch_paged_plan(p, n, rows, tokens, free_pages, n_free, slots, n_slots, taken), "paged_plan");
+    p->planned = true;
+    return Q35M_OK;
+}
+
+int q35m_paged_tables(q35m_paged* p, int** table, int** lens, int* max_pages) {
+    if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
+    if (table) *table = p->dev_table;
+    if (lens) *lens = p->dev_len;
+    if (max_pages) *max_pages = p->map.max_pages();
     return Q35M_OK;
 }
 

@@ -20,7 +20,8 @@ struct PagedBatch {
 };
 
 // What the kernels know of one layer's pages.  A page holds page_rows rows of
-// every kv head, head-major: [page][kv_head][row][head_dim].
+// every kv head, head-major: [page][kv_head][row][head_dim] (4 bits: kMxRow bytes a
+// row instead, see paged_device.h).
 struct PagedView {
     void* k;
     void* v;
@@ -36,12 +37,16 @@ struct PagedView {
 constexpr int kPagedDecodeHeads = 16;    // q heads a decode workgroup takes at most
 constexpr int kPagedTileRows = 64;       // query rows of a prefill workgroup
 
+// A row of a kv head in 4 bits: 128 bytes of codes, dim 2 i in the lower half of byte
+// i, and 8 block scales, one of 32 dims each.
+constexpr int kMxCodes = kHd / 2, kMxBlock = 32, kMxBlocks = kHd / kMxBlock, kMxRow = kMxCodes + kMxBlocks;
+
 }  // namespace q35
 
 struct q35m_paged {
     q35m_ctx* ctx = nullptr;
     q35::PageMap map;
-    int type = 0;                        // Q35M_KV_F32, Q35M_KV_F16
+    int type = 0;                        // Q35M_KV_F32, Q35M_KV_F16, Q35M_KV_MXFP4
     int n_pages = 0, page_shift = 0;
     std::vector<void*> k, v;             // by layer (null for DeltaNet layers)
     size_t layer_bytes = 0;              // of K, and of V, of one layer
@@ -51,6 +56,7 @@ struct q35m_paged {
     float* work = nullptr;               // partial results of one attention call
     size_t work_bytes = 0;
     std::vector<void*> allocations;
+    bool planned = false;                // q35m_paged_plan has run: lengths and tables are the device's alone
 
     q35m_paged(int n_seqs, int max_rows, int n_pages_, int page_rows)
         : map(n_seqs, max_rows, n_pages_, page_rows), n_pages(n_pages_) {}
@@ -59,7 +65,11 @@ struct q35m_paged {
         hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
         return hipStreamIsCapturing(ctx->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
     }
-    size_t value_bytes() const { return type == Q35M_KV_F16 ? 2 : 4; }
+    // Whether the lengths of a call are known now: not those of a replay or a plan.
+    bool lengths_known() const { return !planned && !capturing(); }
+    size_t row_bytes() const {
+        return type == Q35M_KV_MXFP4 ? (size_t)q35::kMxRow : (size_t)q35::kHd * (type == Q35M_KV_F16 ? 2 : 4);
+    }
     q35::PagedView view(int layer) const {
         return {k[layer], v[layer], dev_table, dev_len, rope, map.max_pages(), n_pages, page_shift,
                 map.max_rows(), ctx->d.nkv};
@@ -76,9 +86,18 @@ hipError_t launch_paged_table(q35m_ctx* c, int* table, size_t at, const int* ids
 hipError_t launch_paged_lengths(q35m_ctx* c, int* lens, int n, const int* seq, const int* len);
 
 hipError_t launch_paged_append(q35m_paged* p, int layer, const PagedBatch& b, const float* k, const float* v);
+// Rows first[i] .. first[i] + (b.off[i + 1] - b.off[i]) - 1 of b.seq[i] as fp32.
+struct PagedFirst {
+    int row[kMaxBatch];
+};
+hipError_t launch_paged_rows(q35m_paged* p, int layer, const PagedBatch& b, const PagedFirst& first, float* k, float* v);
+hipError_t launch_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
+                             int64_t* slots, size_t n_slots, int* taken);
 size_t paged_decode_work_bytes(const q35m_ctx* c);
 hipError_t launch_paged_decode(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, const float* k,
                                const float* v, float* out);
+hipError_t launch_paged_decode_mx4(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, const float* k,
+                                   const float* v, float* out);
 size_t paged_prefill_work_bytes(const q35m_ctx* c);
 hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, float* out);
 

@@ -1,0 +1,472 @@
+// Paged K/V cache in 4 bits: attention of one new token per sequence (paged_decode.hip
+// says what is computed and how the rows are dealt out; here as well a unit is 128
+// rows, 32 a wave).
+//
+// S^T = K Q^T takes K as it lies in the cache: the matrix instruction for 4-, 6- and
+// 8-bit floats multiplies blocks of 32 values that share a power of two, which is how a
+// row is held.  q takes part in the 6-bit type (3 bits of mantissa, up to 7.5): each
+// block of 32 dims is cut into six digits of base 16, x = sum d_k 2^{e - 4 k}, |d_k| <= 8, which
+// reach 2^-24 of the block's largest value, one power of two each.  The digits are columns
+// of the operand: 16 of them are four heads by four digits, so a second product brings
+// the last two, and the columns of a head are added at the end: a score to fp32 precision
+// at two products of 16 x 16 x 128 a head quad, and no K value is converted.
+// O^T = V^T P^T takes V as fp16, which holds every value of the cache: a conversion of two
+// values an instruction, with the row's power of two in it, and a transposition in
+// registers; a block's power of two is per row, along this product's sum, so the
+// matrix instruction's own cannot serve here.  P is two fp16 values (hi + lo, to 2^-23 of
+// it), which are columns too up to 8 heads.
+#include "paged_decode.h"
+
+namespace q35 {
+namespace {
+
+constexpr int NT = 256;
+constexpr int kTileRows = 32;                    // of a wave
+constexpr int kUnitRows4 = 4 * kTileRows;
+constexpr int kDigits = 6;
+constexpr int kDigitWords = 50;                  // 48 words of 6-bit codes, and 2 for the banks
+constexpr float kPShift4 = 15.0f;                // P is e^{s - m} 2^15 (see paged_decode.hip)
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// c += A B for 16 x 16 x 128: A in 4 bits (16 bytes a lane: row l % 16, values 32 (l / 16) ..),
+// B in 6 (24 bytes), byte T of the scales.
+template <int T>
+__device__ __forceinline__ f32x4 scaled_product(u32x4 a, const uint32_t (&b)[6], f32x4 c, uint32_t sa, uint32_t sb) {
+    const i32x8 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    const i32x8 y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], (int)b[4], (int)b[5], 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 2, T, (int)sa, T, (int)sb);
+}
+
+// NQ: quads of q heads a workgroup takes, 1, 2 or 4.
+template <int NQ>
+struct Tile4 {
+    static constexpr int kHeads = 4 * NQ;
+    uint32_t q[NQ][2][2][6];   // [quad][digits 0 .. 3, 4 ..][t]: head 4 quad + n % 4, digit n / 4 of these, dims 64 g + 32 t ..
+    uint32_t qs[NQ][2];        // their scales, byte t
+    u32x4 kc[2][2];            // row 16 kb + n, dims 64 g + 32 t ..
+    uint32_t ks[2];            // its scales of blocks 2 g and 2 g + 1
+    uint2 vc[8];               // row 16 (j / 4) + 4 g + j % 4, dims 16 n ..
+    uint32_t vs[2];            // scales of rows 16 kb + 4 g .., block n / 2
+    f32x4 o[16];               // dims 64 g + 16 i + x at [x][i]
+
+    __device__ __forceinline__ void load_q(const uint32_t (*codes)[kDigits][kDigitWords], const uint8_t (*scales)[kDigits][kMxBlocks],
+                                           int hg, int lane) {
+        const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int a = 0; a < NQ; ++a)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int head = min(4 * a + (n & 3), hg - 1), digit = 4 * s + (n >> 2);      // heads from hg on are never read
+                const int d = min(digit, kDigits - 1);
+                const uint32_t sc = *reinterpret_cast<const uint16_t*>(&scales[head][d][2 * g]);
+                qs[a][s] = digit < kDigits ? sc : 0x7f7fu;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int w = 0; w < 6; ++w) q[a][s][t][w] = digit < kDigits ? codes[head][d][12 * g + 6 * t + w] : 0u;
+            }
+    }
+    // codes: the 16 rows' first byte in the page; in: their first row's place there.
+    __device__ __forceinline__ void load_k(const uint8_t* page, const PagedView& pv, int in, int kb, int lane) {
+        const int n = lane & 15, g = lane >> 4;
+        const uint8_t* const at = page + (uint32_t)(in + n) * kMxCodes + 32 * g;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) kc[kb][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + 16 * t));
+        ks[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(page + mx_key_scale(pv, in + n) + 2 * g));
+    }
+    __device__ __forceinline__ void load_v(const uint8_t* page, const PagedView& pv, int in, int kb, int lane) {
+        const int n = lane & 15, g = lane >> 4;
+        const uint8_t* const at = page + (uint32_t)(in + 4 * g) * kMxCodes + 8 * n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(at + i * kMxCodes));
+            vc[4 * kb + i] = make_uint2(x[0], x[1]);
+        }
+        vs[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(page + mx_value_scale(pv, in, n >> 1) + 4 * g));
+    }
+    // Row `at` of the tile (none if negative) is the new one (its codes and scales at kn, vn);
+    // rows from `rows` on are masked: what they hold must not be NaN.
+    __device__ __forceinline__ void fix(const uint8_t* kn, const uint8_t* vn, int at, int rows, int lane) {
+        const int n = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            if (16 * kb + n == at) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) kc[kb][t] = *reinterpret_cast<const u32x4*>(kn + 32 * g + 16 * t);
+                ks[kb] = *reinterpret_cast<const uint16_t*>(kn + kMxCodes + 2 * g);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 16 * kb + 4 * g + i;
+                const uint32_t keep = ~(0xffu << 8 * i);
+                if (r == at) {
+                    vc[4 * kb + i] = *reinterpret_cast<const uint2*>(vn + 8 * n);
+                    vs[kb] = (vs[kb] & keep) | (uint32_t)vn[kMxCodes + (n >> 1)] << 8 * i;
+                }
+                if (r >= rows) vs[kb] = (vs[kb] & keep) | 127u << 8 * i;
+            }
+        }
+    }
+    // Scores of rows row_of(j, g) and the lane's head, n % kHeads.
+    __device__ __forceinline__ void scores(float (&s)[8], int lane) const {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            f32x4 c[NQ];
+#pragma unroll
+            for (int a = 0; a < NQ; ++a) {
+                c[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int d = 1; d >= 0; --d) {             // the last digits' products first
+                    c[a] = scaled_product<0>(kc[kb][0], q[a][d][0], c[a], ks[kb], qs[a][d]);
+                    c[a] = scaled_product<1>(kc[kb][1], q[a][d][1], c[a], ks[kb], qs[a][d]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float x[NQ];
+#pragma unroll
+                for (int a = 0; a < NQ; ++a) {             // the digits' columns n, n ^ 4, n ^ 8, n ^ 12
+                    x[a] = c[a][i];
+                    x[a] += row_xor<8>(x[a]);
+                    x[a] += row_ror4(x[a]);
+                }
+                const bool odd = lane & 4, upper = lane & 8;
+                if constexpr (NQ == 1) s[4 * kb + i] = x[0];
+                if constexpr (NQ == 2) s[4 * kb + i] = odd ? x[1] : x[0];
+                if constexpr (NQ == 4) s[4 * kb + i] = upper ? (odd ? x[3] : x[2]) : (odd ? x[1] : x[0]);
+            }
+        }
+    }
+    static __device__ __forceinline__ int row_of(int j, int g) { return 16 * (j >> 2) + 4 * g + (j & 3); }
+    __device__ __forceinline__ void pv(const float (&p)[8], int lane) {
+        f16x8 ph, pl;
+        split16(p, ph, pl);
+        if constexpr (NQ < 4) {                            // columns kHeads .. 2 kHeads - 1 are the low parts
+            const u32x4 h = __builtin_bit_cast(u32x4, ph), l = __builtin_bit_cast(u32x4, pl);
+            u32x4 b;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) b[w] = lane & kHeads ? l[w] : h[w];
+            ph = __builtin_bit_cast(f16x8, b);
+        }
+        float unit[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) unit[j] = __uint_as_float((vs[j >> 2] >> 8 * (j & 3) & 0xffu) << 23);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            auto byte = [&](auto B) {
+                constexpr int b = decltype(B)::value;
+                uint32_t x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w ? vc[j].y : vc[j].x, unit[j], b));
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+                    const u32x4 a = {__builtin_amdgcn_perm(x[1], x[0], sel), __builtin_amdgcn_perm(x[3], x[2], sel),
+                                     __builtin_amdgcn_perm(x[5], x[4], sel), __builtin_amdgcn_perm(x[7], x[6], sel)};
+                    const f16x8 av = __builtin_bit_cast(f16x8, a);
+                    f32x4& to = o[8 * w + 2 * b + e];
+                    if constexpr (NQ == 4) to = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pl, to, 0, 0, 0);
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, ph, to, 0, 0, 0);
+                }
+            };
+            byte(std::integral_constant<int, 0>{});
+            byte(std::integral_constant<int, 1>{});
+            byte(std::integral_constant<int, 2>{});
+            byte(std::integral_constant<int, 3>{});
+        }
+    }
+    // The lane's output values, 4 consecutive dims at a time.
+    template <typename F>
+    __device__ __forceinline__ void each4(int g, F f) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int x = 0; x < 16; x += 4) {
+                float y[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    y[k] = o[x + k][i];
+                    if constexpr (NQ == 1) y[k] += row_ror4(y[k]);         // (columns n and n + 8 agree)
+                    if constexpr (NQ == 2) y[k] += row_xor<8>(y[k]);
+                }
+                f(64 * g + 16 * i + x, make_float4(y[0], y[1], y[2], y[3]));
+            }
+    }
+};
+
+// Digits of a q row's dims 4 l .., as 6-bit codes (sign, 2 bits of exponent, 3 of mantissa)
+// of half a digit, packed along the row, and each block's scales.
+__device__ __forceinline__ void put_digits(uint32_t (*codes)[kDigitWords], uint8_t (*scales)[kMxBlocks], float4 x, int lane) {
+    auto mag = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+    uint32_t m = max(max(mag(x.x), mag(x.y)), max(mag(x.z), mag(x.w)));
+    m = max(m, row_xor_bits<1>(m));
+    m = max(m, row_xor_bits<2>(m));
+    m = max(m, row_xor_bits<4>(m));
+    const int e = max((int)(m >> 23), 40);                 // every |x| is below 2^{e - 126}
+    const float up = __uint_as_float((uint32_t)(256 - e) << 23);
+    float t[4] = {x.x * up, x.y * up, x.z * up, x.w * up};
+#pragma unroll
+    for (int k = 0; k < kDigits; ++k) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float d = rintf(t[i]);
+            t[i] = (t[i] - d) * 16.0f;
+            const uint32_t a = (uint32_t)fabsf(d);         // a / 2: codes 4 a up to 2, 8 + 2 a from there to 4
+            c |= (min(4 * a, 8 + 2 * a) | (d < 0.0f ? 32u : 0u)) << 6 * i;
+        }
+        // Four lanes' 24 bits are three words.
+        const uint32_t next = row_move<0xF9>(c);           // quad_perm 1 2 3 3
+        const int at = lane & 3;
+        const uint32_t w = c >> 8 * at | next << (24 - 8 * at);
+        if (at < 3) codes[k][3 * (lane >> 2) + at] = w;
+        if ((lane & 7) == 0) scales[k][lane >> 3] = m >= 0x7f800000u ? (uint8_t)kMxNan : (uint8_t)(e - 1 - 4 * k);
+    }
+}
+
+template <int NQ>
+__global__ __launch_bounds__(NT, 1) void paged_decode_mx4(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
+                                                          const float* __restrict__ knew, const float* __restrict__ vnew,
+                                                          const float* __restrict__ q_norm,
+                                                          const float* __restrict__ k_norm, float* __restrict__ out,
+                                                          float* __restrict__ part_o, float* __restrict__ part_ml, int hg,
+                                                          int ng, int unit, float eps) {
+    constexpr int R = kTileRows, H = 4 * NQ, HW = H / 4;   // HW: heads a wave forms and joins
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int groups = pv.nkv * ng, nh = groups * hg;
+
+    __shared__ __align__(16) float obuf[4][H][kHd];
+    __shared__ float ml[4][H][2];
+    __shared__ __align__(16) uint8_t newrow[4][2][kMxRow + 8];
+    __shared__ __align__(16) uint32_t qcodes[H][kDigits][kDigitWords];
+    __shared__ __align__(8) uint8_t qscales[H][kDigits][kMxBlocks];
+
+    float4 qw = *reinterpret_cast<const float4*>(q_norm + 4 * lane);
+    const float4 kw = *reinterpret_cast<const float4*>(k_norm + 4 * lane);
+    qw = make_float4(1.0f + qw.x, 1.0f + qw.y, 1.0f + qw.z, 1.0f + qw.w);
+    const Units un = units_of(pv, b, groups, unit, lane);
+    const int per = (un.total + (int)gridDim.x - 1) / (int)gridDim.x;
+    int u = blockIdx.x * per;
+    const int u_end = min(u + per, un.total);
+
+    while (u < u_end) {
+        const int i = __popcll(__ballot(un.end <= u));            // the unit's sequence in the batch
+        const int tiles = __builtin_amdgcn_readlane(un.tiles, i);
+        const int rows = __builtin_amdgcn_readlane(un.rows, i);
+        const int local = u - (__builtin_amdgcn_readlane(un.end, i) - tiles * groups);
+        const int y = local / tiles, t0 = local - y * tiles;      // head group, first unit of the segment
+        const int t1 = min(tiles, t0 + (u_end - u));
+        u += t1 - t0;
+        const int kvh = y / ng, seq = b.seq[i], pos = rows - 1;
+        const int* table = pv.table + (size_t)seq * pv.max_pages;
+        const int first = t0 * unit + wave * R, stop = min(rows, t1 * unit);
+        const int last16 = pos & ~15, in_page = (1 << pv.page_shift) - 1;
+
+        Tile4<NQ> tl;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) tl.o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        int pg[2];
+        auto pages = [&](int base) {     // of the 16-row groups at base (the last one past the end)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                pg[kb] = page_of(table, min(base + 16 * kb, last16) >> pv.page_shift, pv.max_pages, pv.n_pages);
+        };
+        auto load_k = [&](int base, const int (&p)[2]) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                tl.load_k((const uint8_t*)pv.k + mx_page(pv, p[kb], kvh), pv, min(base + 16 * kb, last16) & in_page, kb, lane);
+        };
+        auto load_v = [&](int base, const int (&p)[2]) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+                tl.load_v((const uint8_t*)pv.v + mx_page(pv, p[kb], kvh), pv, min(base + 16 * kb, last16) & in_page, kb, lane);
+        };
+        // What q's rows and the new row are made of is asked for before K and V, so
+        // that they are formed while those are on their way; a wave forms every
+        // fourth q row, for all.
+        const bool has_new = first <= pos / R * R && pos / R * R < stop && (pos / R * R - first) % (4 * R) == 0;
+        if (first < stop) pages(first);
+        float4 xq[HW], xk{}, xv{};
+        const float* const q_rows = q_gate + ((size_t)i * nh + y * hg) * 2 * kHd + 4 * lane;
+#pragma unroll
+        for (int k = 0; k < HW; ++k)
+            if (wave + 4 * k < hg) xq[k] = *reinterpret_cast<const float4*>(q_rows + (size_t)(wave + 4 * k) * 2 * kHd);
+        if (has_new) {
+            const size_t at = ((size_t)i * pv.nkv + kvh) * kHd + 4 * lane;
+            xk = *reinterpret_cast<const float4*>(knew + at);
+            xv = *reinterpret_cast<const float4*>(vnew + at);
+        }
+        double cs[4], sn[4];                     // the rotation of dims 4 (lane % 8) ..
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            cs[k] = pv.rope[(size_t)pos * kRopeDim + 4 * (lane & 7) + k];
+            sn[k] = pv.rope[(size_t)pos * kRopeDim + kRopeHalf + 4 * (lane & 7) + k];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (first < stop) {
+            load_k(first, pg);
+            load_v(first, pg);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+
+        // q: the rotation, the norm, the scale 1/16 (and log2 e, for exp2).
+#pragma unroll
+        for (int k = 0; k < HW; ++k) {
+            const int r = wave + 4 * k;
+            if (r >= hg) break;
+            float x[4] = {xq[k].x, xq[k].y, xq[k].z, xq[k].w}, ss = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float a = x[c], z = row_xor<8>(a), co = (float)cs[c], si = (float)sn[c];
+                x[c] = lane < 8 ? a * co - z * si : lane < 16 ? z * si + a * co : a;
+                ss += x[c] * x[c];
+            }
+            const float scale = (kLog2e / 16.0f) / sqrtf(wave_sum(ss) / (float)kHd + eps);
+            put_digits(qcodes[r], qscales[r],
+                       make_float4(x[0] * (scale * qw.x), x[1] * (scale * qw.y), x[2] * (scale * qw.z), x[3] * (scale * qw.w)),
+                       lane);
+        }
+        // The wave that holds the new row makes it (every head group needs it;
+        // one writes it to the page, and none reads it from there).
+        if (has_new) {
+            const MxLane yk = mx_round(paged_key_row(xk, cs, sn, kw, lane, (double)eps)), yv = mx_round(xv);
+            uint8_t* const kn = newrow[wave][0];
+            uint8_t* const vn = newrow[wave][1];
+            reinterpret_cast<uint16_t*>(kn)[lane] = (uint16_t)yk.codes;
+            reinterpret_cast<uint16_t*>(vn)[lane] = (uint16_t)yv.codes;
+            if ((lane & 7) == 0) {
+                kn[kMxCodes + (lane >> 3)] = (uint8_t)yk.scale;
+                vn[kMxCodes + (lane >> 3)] = (uint8_t)yv.scale;
+            }
+            const int pnew = page_of(table, pos >> pv.page_shift, pv.max_pages, pv.n_pages);
+            if (y % ng == 0 && pnew >= 0 && pv.lens[seq] < pv.max_rows) {
+                mx_put_key((uint8_t*)pv.k + mx_page(pv, pnew, kvh), pv, pos & in_page, yk, lane);
+                mx_put_value((uint8_t*)pv.v + mx_page(pv, pnew, kvh), pv, pos & in_page, yv, lane);
+            }
+        }
+        lds_barrier();
+        tl.load_q(qcodes, qscales, hg, lane);
+
+        float m_run = -INFINITY, l_run = 0.0f;
+        for (int base = first; base < stop; base += 4 * R) {
+            const int next = base + 4 * R;
+            const bool more = next < stop;
+            if (more) pages(next);
+            if (base + R > pos) tl.fix(newrow[wave][0], newrow[wave][1], pos - base, rows - base, lane);
+            float s[8];
+            tl.scores(s, lane);
+            if (more) load_k(next, pg);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                s[j] = base + tl.row_of(j, g) < rows ? s[j] : -INFINITY;
+                mx = fmaxf(mx, s[j]);
+            }
+            mx = fmaxf(m_run, xor16_max(xor32_max(mx)));
+            const float mu = mx == -INFINITY ? 0.0f : mx;
+            const float alpha = __builtin_amdgcn_exp2f(m_run - mu);
+            m_run = mx;
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                s[j] = __builtin_amdgcn_exp2f(s[j] - mu + kPShift4);
+                sum += s[j];
+            }
+            l_run = l_run * alpha + sum;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) tl.o[x] *= alpha;
+            tl.pv(s, lane);
+            if (more) load_v(next, pg);
+        }
+
+        // The four waves of the segment join.
+        l_run = xor16_sum(xor32_sum(l_run));
+        tl.each4(g, [&](int d, float4 x) {
+            if (n < hg) *reinterpret_cast<float4*>(&obuf[wave][n][d]) = x;
+        });
+        if (n < hg && g == 0) {
+            ml[wave][n][0] = m_run;
+            ml[wave][n][1] = l_run;
+        }
+        const bool whole = t0 == 0 && t1 == tiles;
+        const int slot = 2 * blockIdx.x + (t0 == 0);
+        float4 gate[HW];
+#pragma unroll
+        for (int k = 0; k < HW; ++k)
+            if (whole && wave + 4 * k < hg)
+                gate[k] = *reinterpret_cast<const float4*>(q_rows + (size_t)(wave + 4 * k) * 2 * kHd + kHd);
+        lds_barrier();
+        // (A value of the cache that is not finite is NaN, and NaN times any weight is, so
+        // nothing is to be settled here.)
+#pragma unroll
+        for (int k = 0; k < HW; ++k) {
+            const int r = wave + 4 * k;
+            if (r >= hg) break;
+            float M = -INFINITY, l = 0.0f;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][r][0]);
+            const float mu = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float e = __builtin_amdgcn_exp2f(ml[w][r][0] - mu);
+                const float4 x = *reinterpret_cast<const float4*>(&obuf[w][r][4 * lane]);
+                l += e * ml[w][r][1];
+                o.x += e * x.x; o.y += e * x.y; o.z += e * x.z; o.w += e * x.w;
+            }
+            if (whole) {
+                const float inv = 1.0f / l;
+                *reinterpret_cast<float4*>(out + ((size_t)i * nh + y * hg + r) * kHd + 4 * lane) =
+                    gated(make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), gate[k]);
+            } else {
+                const size_t at = (size_t)slot * kPagedDecodeHeads + r;
+                *reinterpret_cast<float4*>(part_o + at * kHd + 4 * lane) = o;
+                if (lane == 0) *reinterpret_cast<float2*>(part_ml + 2 * at) = make_float2(M, l);
+            }
+        }
+        lds_barrier();
+    }
+}
+
+}  // namespace
+
+// One workgroup a CU.
+hipError_t launch_paged_decode_mx4(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, const float* k,
+                                   const float* v, float* out) {
+    q35m_ctx* c = p->ctx;
+    const int per_kv = c->d.nh / c->d.nkv;
+    const int hg = per_kv <= 16 ? per_kv : per_kv % 16 == 0 ? 16 : 8;
+    const int ng = per_kv / hg, nwg = c->n_cu;
+    float* part_o = p->work;
+    float* part_ml = part_o + (size_t)2 * nwg * kPagedDecodeHeads * kHd;
+    const PagedView pv = p->view(layer);
+    const AttnLayer& L = c->full[layer];
+    // Short sequences that each get a workgroup are not cut (see launch_paged_decode).
+    const int whole = 4 * kUnitRows4;
+    bool cut = (long)b.n * c->d.nkv * ng > nwg || !p->lengths_known();
+    for (int i = 0; i < b.n && !cut; ++i) cut = p->map.length(b.seq[i]) >= whole;
+    const int unit = cut ? kUnitRows4 : whole;
+    {
+        ProfScope ps(c, K_PAGED_DECODE);
+        auto go = [&](auto kern) {
+            hipExtLaunchKernelGGL(kern, dim3(nwg), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b, q_gate, k, v, L.q_norm,
+                                  L.k_norm, out, part_o, part_ml, hg, ng, unit, c->d.eps);
+        };
+        if (hg <= 4) go(paged_decode_mx4<1>);
+        else if (hg <= 8) go(paged_decode_mx4<2>);
+        else go(paged_decode_mx4<4>);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !cut) return e;
+    ProfScope ps(c, K_PAGED_DECODE_MERGE);
+    hipExtLaunchKernelGGL(paged_decode_merge<kUnitRows4>, dim3(c->d.nh, b.n), dim3(MW * kWave), 0, c->stream, ps.a, ps.b, 0, pv, b,
+                          part_o, part_ml, q_gate, out, hg, ng, nwg);
+    return hipGetLastError();
+}
+
+}  // namespace q35

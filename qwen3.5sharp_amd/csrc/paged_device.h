@@ -31,6 +31,66 @@ __device__ __forceinline__ size_t row_offset(const PagedView& pv, int page, int 
     return ((((size_t)max(page, 0) * pv.nkv + kvh) << pv.page_shift) + in) * kHd;
 }
 
+// ---- rows in 4 bits ---------------------------------------------------------
+//
+// The MX format of 4-bit floats: 32 values share a power of two 2^s, held as s + 127,
+// and each has a sign and one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 in units of it.  s is the
+// smallest with the block's largest value at most 7 2^s: that one is then within half
+// a step of 6, the last code (from there on it would be cut by up to a quarter).  s is
+// kept from -23 to 13, the range in which every value held is an fp16 value, which the
+// attention's products rely on: smaller values are 0, larger ones +-6 2^13.  A block with a
+// value that is not finite is NaN, scale 255 (one code cannot say infinity).
+//
+// Of each (page, kv head): the rows' codes [page_rows][128], then their scales, as the
+// attention reads them: K [page_rows][8], V [page_rows / 16][8][16], 16 rows of a block
+// together.
+struct Mx4 {};
+constexpr uint32_t kMxNan = 255;
+__device__ __forceinline__ size_t mx_page(const PagedView& pv, int page, int kvh) {     // its first byte
+    return ((size_t)max(page, 0) * pv.nkv + kvh) * ((size_t)kMxRow << pv.page_shift);
+}
+__device__ __forceinline__ uint32_t mx_key_scale(const PagedView& pv, int in) {         // of row `in` of the page
+    return ((uint32_t)kMxCodes << pv.page_shift) + (uint32_t)in * kMxBlocks;
+}
+__device__ __forceinline__ uint32_t mx_value_scale(const PagedView& pv, int in, int block) {
+    return ((uint32_t)kMxCodes << pv.page_shift) + (uint32_t)(in >> 4) * (16 * kMxBlocks) + 16 * block + (in & 15);
+}
+// Lane l's dims 4 l .. of a row: four codes, and its block's scale (the same in 8 lanes).
+struct MxLane {
+    uint32_t codes, scale;
+};
+__device__ __forceinline__ MxLane mx_round(float4 x) {
+    auto mag = [](float v) { return __float_as_uint(v) & 0x7fffffffu; };                // (an order, with NaN on top)
+    uint32_t m = max(max(mag(x.x), mag(x.y)), max(mag(x.z), mag(x.w)));
+    m = max(m, row_xor_bits<1>(m));
+    m = max(m, row_xor_bits<2>(m));
+    m = max(m, row_xor_bits<4>(m));
+    MxLane r{0, kMxNan};
+    if (m >= 0x7f800000u) return r;
+    // m = f 2^e: 7 2^s >= m from s = e - 2 on where f <= 7/4, else from e - 1 on.
+    const int s = (int)((m + 0x1fffffu) >> 23) - 2;
+    r.scale = (uint32_t)min(max(s, 127 - 23), 127 + 13);
+    const float unit = __uint_as_float(r.scale << 23);
+    r.codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x.x, x.y, unit, 0);           // nearest, ties to even, up to 6
+    r.codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r.codes, x.z, x.w, unit, 1) & 0xffffu;
+    return r;
+}
+__device__ __forceinline__ void mx_put_key(uint8_t* page, const PagedView& pv, int in, MxLane x, int lane) {
+    *reinterpret_cast<uint16_t*>(page + (uint32_t)in * kMxCodes + 2 * lane) = (uint16_t)x.codes;
+    if ((lane & 7) == 0) page[mx_key_scale(pv, in) + (lane >> 3)] = (uint8_t)x.scale;
+}
+__device__ __forceinline__ void mx_put_value(uint8_t* page, const PagedView& pv, int in, MxLane x, int lane) {
+    *reinterpret_cast<uint16_t*>(page + (uint32_t)in * kMxCodes + 2 * lane) = (uint16_t)x.codes;
+    if ((lane & 7) == 0) page[mx_value_scale(pv, in, lane >> 3)] = (uint8_t)x.scale;
+}
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float4 mx_values(MxLane x) {
+    const float unit = __uint_as_float(x.scale << 23);
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x.codes, unit, 0);
+    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(x.codes, unit, 1);
+    return x.scale == kMxNan ? make_float4(NAN, NAN, NAN, NAN) : make_float4(a.x, a.y, b.x, b.y);
+}
+
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
@@ -169,6 +229,16 @@ __device__ __forceinline__ float4 load_row4(const _Float16* p) {
 }
 // Rows [from, to) of kv head kvh of the sequence whose row of the page table `table` is.
 template <typename T>
+__device__ __forceinline__ float4 value_row4(const PagedView& pv, int page, int kvh, int row, int lane) {
+    if constexpr (std::is_same_v<T, Mx4>) {                // (a block is NaN or finite)
+        const int in = row & ((1 << pv.page_shift) - 1);
+        const uint8_t* const at = (const uint8_t*)pv.v + mx_page(pv, page, kvh);
+        return at[mx_value_scale(pv, in, lane >> 3)] == kMxNan ? make_float4(NAN, NAN, NAN, NAN) : make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+        return load_row4((const T*)pv.v + row_offset<T>(pv, page, kvh, row) + 4 * lane);
+    }
+}
+template <typename T>
 __device__ __forceinline__ uint32_t infinite_rows(const PagedView& pv, const int* __restrict__ table, int kvh, int from,
                                                   int to, int lane) {
     constexpr int U = 8;       // rows whose loads are in flight together
@@ -180,7 +250,7 @@ __device__ __forceinline__ uint32_t infinite_rows(const PagedView& pv, const int
         for (int u = 0; u < U; ++u) {
             const int row = min(r + u, to - 1);
             const int page = page_of(table, row >> pv.page_shift, pv.max_pages, pv.n_pages);
-            x[u] = load_row4((const T*)pv.v + row_offset<T>(pv, page, kvh, row) + 4 * lane);
+            x[u] = value_row4<T>(pv, page, kvh, row, lane);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) found |= infinite(x[u]);

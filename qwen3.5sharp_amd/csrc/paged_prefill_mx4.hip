@@ -1,0 +1,530 @@
+// Paged K/V cache in 4 bits: attention of chunks of new tokens (paged_prefill.hip says
+// what is computed, how the work is divided and how the fp16 kernel, whose shape this
+// one has, pipelines its units).
+//
+// The scores take K as it lies in the cache, from global memory to registers: the
+// matrix instruction for 4-, 6- and 8-bit floats, 32 x 32 x 64, multiplies blocks of 32
+// values with a power of two each, and runs four times as many products a cycle as the
+// fp16 one.  q is cut into kParts parts of the 6-bit type (3 bits of mantissa), each
+// the rounding of what the ones before it left, a power of 16 below: five reach 2^-20 of
+// the block's largest value, at 5 / 4 of one fp16 product's time where two would be taken.
+// The output's products are fp16's, with P as hi + lo: a block's power of two is a row's,
+// along that product's sum.  V is converted into LDS, once a workgroup, beside products.
+#include <type_traits>
+
+#include "paged_prefill.h"
+
+namespace q35 {
+namespace {
+
+constexpr int NT = 256;
+constexpr int kParts = 5;
+
+struct Mx4Tile {
+    _Float16 v[2][kUnit][kHd];            // (first q's parts)
+    float4 q[kPagedTileRows * kHd / 4];   // q rows; at the end the output's
+    f16x8 p[4][4][kWave];                 // a wave's weights: operands (hi, lo) of its two 16-row steps
+    float mx[2][4][32];                   // maxima of a unit's halves; at the end sums and maxima
+    float w[kHd];                         // 1 + the norm's weights
+    uint8_t qscale[2][4][kWave];          // the first part's scales
+    int found;                            // values that are not finite
+};
+static_assert(2 * 4 * kParts * 3 * kWave * sizeof(uint2) <= sizeof(Mx4Tile::v), "the parts' room");
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+
+// c += A B for 32 x 32 x 64: A in 4 bits (16 bytes a lane: row l % 32, values 32 (l / 32) ..),
+// B in 6 (24 bytes), byte S of A's scales and of B's.
+template <int S>
+__device__ __forceinline__ f32x16 scaled_product32(u32x4 a, const uint32_t (&b)[6], f32x16 c, uint32_t sa, uint32_t sb) {
+    const i32x8 x = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    const i32x8 y = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], (int)b[4], (int)b[5], 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 2, S, (int)sa, S, (int)sb);
+}
+
+// A block of q as parts of 6 bits, three 8-byte words each at to[word][lane]; returned is
+// the first part's scale, of which a later one's is 4 less than the one's before.  The
+// conversions are written out because their results come while they still read: the
+// compiler lets the two share registers.
+__device__ __forceinline__ uint32_t cut_block(float (&x)[kMxBlock], uint2* to) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kMxBlock; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    const uint32_t e = max(m >> 23, 40u);                  // every |x| is below 2^{e - 126}, 8 times 2^{e - 129}
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) {
+        const float unit = __uint_as_float((e - 2 - 4 * k) << 23);
+        f32x16 even, odd;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            even[i] = x[2 * i];
+            odd[i] = x[2 * i + 1];
+        }
+        u32x6 part;
+        asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3" : "=&v"(part) : "v"(even), "v"(odd), "v"(unit));
+#pragma unroll
+        for (int w = 0; w < 3; ++w) to[(3 * k + w) * kWave] = make_uint2(part[2 * w], part[2 * w + 1]);
+        if (k + 1 == kParts) break;
+        f32x32 back;
+        asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2" : "=&v"(back) : "v"(part), "v"(unit));
+#pragma unroll
+        for (int i = 0; i < kMxBlock; ++i) x[i] -= back[i];
+    }
+    return m >= 0x7f800000u ? kMxNan : e - 2;
+}
+
+__global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
+                                                           const float* __restrict__ q_norm, float* __restrict__ out,
+                                                           float* __restrict__ part_o, float* __restrict__ part_ml,
+                                                           int hg_shift, int ng, int more, float eps) {
+    // (as in the fp16 kernel)
+    constexpr float kShift = 6.0f, kMove = 9.9f;
+    __shared__ __align__(16) Mx4Tile st;
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rg = wave & 1, half = wave >> 1;
+    const int hg = 1 << hg_shift, tm = kPagedTileRows >> hg_shift;
+    const int groups = pv.nkv * ng, nh = groups << hg_shift;
+    const int wg = xcd_remap(blockIdx.x, gridDim.x);      // neighbours, which share K and V, on one XCD's L2
+    constexpr int kBuf = kUnit * kHd * 2;                 // bytes of a V buffer
+
+    const float w = q_norm[tid];
+    const Units un = units_of(pv, b, groups, hg_shift, more, tid & 63);
+    st.w[tid] = 1.0f + w;                                 // (read behind the first segment's first barrier)
+    Walk wk;
+    wk.begin(un, wg, gridDim.x);
+    while (wk.next(b, un, groups, hg_shift)) {
+        const int start = uniform(wk.start), tokens = uniform(wk.tokens);
+        const int seq = b.seq[wk.i], kvh = wk.y / ng;
+        const int* table = pv.table + (size_t)seq * pv.max_pages;
+        // (the lane's own places as values of this segment: addresses made of them
+        // would else be kept over all segments)
+        int lane = tid & 63, nn = lane & 31;
+        asm volatile("" : "+v"(lane), "+v"(nn));
+        const int h = lane >> 5;
+        // Rows the tile's tokens see: [0, rows); the lane's query row sees [0, mine].
+        const int rows = uniform(min(start + min((wk.j + 1) * tm, tokens), pv.max_rows));
+        const int last16 = (rows - 1) & ~15;
+        const int first = uniform(start + wk.j * tm);          // position of the tile's first token
+        const int mine = min(start + min(wk.j * tm + ((32 * rg + nn) >> hg_shift), tokens - 1), pv.max_rows - 1);
+        // Query row r of the tile is row row0 + from_row0(r) of q and out (the last
+        // token's for rows past the `left` tokens): a 64-bit base a tile and 32 bits from
+        // there.
+        const int left = uniform(tokens - wk.j * tm);
+        const long row0 = uniform((long)(uniform(b.off[wk.i]) + wk.j * tm) * nh + (wk.y << hg_shift));
+        const char* const q_tile = (const char*)uniform(q_gate + row0 * 2 * kHd);
+        char* const out_tile = (char*)uniform(out + row0 * kHd);
+        auto from_row0 = [&](int r) { return min(r >> hg_shift, left - 1) * nh + (r & (hg - 1)); };
+
+        // A wave takes rows 32 half .. of a unit's K and brings rows 16 wave .. of its V,
+        // the rg-th 16 of those.  It holds 64 entries of the page table, one a lane, from
+        // entry `held` on; a unit's two pages are found a unit before they are asked for.
+        int held = 0, ids = 0;
+        auto hold = [&](int entry) {
+            held = entry;
+            ids = page_of(table, entry + lane, pv.max_pages, pv.n_pages);
+        };
+        hold(min(wk.t0 * kUnit + 32 * half, last16) >> pv.page_shift);
+        struct Place {
+            size_t page[2];          // first bytes of the pages of the two groups of 16 rows
+            int in[2];               // their first rows' places there
+        };
+        auto place = [&](int t) {
+            Place p;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int r = uniform(min(t * kUnit + 32 * half + 16 * g, last16)), entry = r >> pv.page_shift;
+                if (__builtin_expect(uniform(entry - held) >= kWave, 0)) hold(entry);
+                p.page[g] = mx_page(pv, __builtin_amdgcn_readlane(ids, uniform(entry - held)), kvh);
+                p.in[g] = r & ((1 << pv.page_shift) - 1);
+            }
+            return p;
+        };
+        // K: lane (row nn, h) takes blocks 4 h .. of its row; V: 16-byte pieces of two rows,
+        // 8 i + lane / 8, block lane % 8.
+        u32x4 kc[4], vc[2];
+        uint32_t ks, vs[2];
+        auto key_row = [&](const Place& p) {
+            const uint8_t* const a = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[0] + (uint32_t)p.in[0] * kMxCodes);
+            const uint8_t* const b = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[1] + (uint32_t)p.in[1] * kMxCodes);
+            return (nn & 16 ? b : a) + (uint32_t)((nn & 15) * kMxCodes + 64 * h);
+        };
+        auto key_scales = [&](const Place& p) {
+            const uint8_t* const a = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[0] + mx_key_scale(pv, p.in[0]));
+            const uint8_t* const b = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[1] + mx_key_scale(pv, p.in[1]));
+            return *reinterpret_cast<const uint32_t*>((nn & 16 ? b : a) + (uint32_t)((nn & 15) * kMxBlocks + 4 * h));
+        };
+        auto load_values = [&](const Place& p) {
+            const size_t page = rg ? p.page[1] : p.page[0];
+            const int in = rg ? p.in[1] : p.in[0];
+            const uint8_t* const at = (const uint8_t*)uniform((const uint8_t*)pv.v + page + (uint32_t)in * kMxCodes);
+            const uint8_t* const sc = (const uint8_t*)uniform((const uint8_t*)pv.v + page + mx_value_scale(pv, in, 0));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                vc[i] = *reinterpret_cast<const u32x4*>(at + (uint32_t)(1024 * i + 16 * lane));
+                vs[i] = sc[(uint32_t)(16 * (lane & 7) + 8 * i + (lane >> 3))];
+            }
+        };
+
+        // q rows, 16-byte chunks permuted by row (chunk ^ row % 32).
+#pragma unroll 4
+        for (int r = 16 * wave; r < 16 * wave + 16; ++r)
+            dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 16 * (lane ^ (r & 31)), lds_address(&st.q[0]) + r * kHd * 4);
+        Place at1 = place(wk.t0);
+        {
+            const uint8_t* const from = key_row(at1);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) kc[s] = *reinterpret_cast<const u32x4*>(from + 16 * s);
+            ks = key_scales(at1);
+            load_values(at1);
+        }
+        at1 = place(wk.t0 + 1);
+        Place at2 = place(wk.t0 + 2);
+        if (tid == 0) st.found = 0;
+
+        // q: the norm's rows in fp32, then partners cut half of each row's blocks into parts
+        // and hand them over: lane (row nn, h) blocks 4 h + s, s = 2 half and 2 half + 1.
+        {
+            float4* const at = st.q + (32 * rg + nn) * (kHd / 4);
+            float x[8][8];
+            const float scale = q_row(x, at, pv.rope + (size_t)mine * kRopeDim, st.mx[0], rg, half, lane, eps);
+            const float* const w = &st.w[128 * half + 8 * h];
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+#pragma unroll
+                for (int c = 0; c < 8; c += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(&w[16 * s + c]);
+                    at[(32 * half + 4 * s + 2 * h + c / 4) ^ nn] = make_float4(x[s][c] * (scale * v.x), x[s][c + 1] * (scale * v.y),
+                                                                              x[s][c + 2] * (scale * v.z), x[s][c + 3] * (scale * v.w));
+                }
+        }
+        lds_barrier();
+        uint2* const parts = reinterpret_cast<uint2*>(&st.v[0][0][0]) + rg * (4 * kParts * 3 * kWave) + lane;
+#pragma nounroll
+        for (int s = 2 * half; s < 2 * half + 2; ++s) {
+            const float4* const at = st.q + (32 * rg + nn) * (kHd / 4);
+            float x[kMxBlock];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float4 v = at[(8 * (4 * h + s) + c) ^ nn];
+                x[4 * c] = v.x; x[4 * c + 1] = v.y; x[4 * c + 2] = v.z; x[4 * c + 3] = v.w;
+            }
+            st.qscale[rg][s][lane] = (uint8_t)cut_block(x, parts + s * (kParts * 3 * kWave));
+        }
+        lds_barrier();
+        uint32_t q[4][kParts][6], qs[kParts];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int k = 0; k < kParts; ++k)
+#pragma unroll
+                for (int w = 0; w < 3; ++w) {
+                    const uint2 v = parts[((s * kParts + k) * 3 + w) * kWave];
+                    q[s][k][2 * w] = v.x;
+                    q[s][k][2 * w + 1] = v.y;
+                }
+        qs[0] = st.qscale[rg][0][lane] | st.qscale[rg][1][lane] << 8 | st.qscale[rg][2][lane] << 16 | (uint32_t)st.qscale[rg][3][lane] << 24;
+#pragma unroll
+        for (int k = 1; k < kParts; ++k) qs[k] = qs[k - 1] - 0x04040404u;      // (no borrow: a scale is 38 or more)
+        lds_barrier();                                     // the parts are read
+
+        // The output stays in accumulation registers all along: pin() is a use there,
+        // without which the compiler moves all of it to vector registers and back on
+        // every unit, for the rare branch that scales it.
+        f32x16 o[4];                                       // dims 128 half + 32 d + row at [d]
+        auto pin = [&]() { asm volatile("" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3])); };
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[d][k] = 0.0f;
+        pin();
+        float m_run = -INFINITY, l_run = 0.0f, mx = -INFINITY;
+        float sc[16];                                      // the wave's scores of a unit
+
+        // V operands of 16 rows and 32 dims: lane (dim nn, h), rows 4 h + {0..3, 8..11},
+        // which the transposing read gathers from lanes of 4 rows x 16 dims.
+        uint32_t va[2][4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            va[0][d] = lds_address(&st.v[0][32 * half + 4 * h + ((lane >> 2) & 3)][0]) + 32 * (8 * half + ((2 * d + ((lane >> 4) & 1)) ^ (2 * ((lane >> 2) & 3)))) +
+                    8 * (lane & 3);
+            va[1][d] = va[0][d] + (half ? -32 * 512 : 32 * 512);   // the partner's rows
+        }
+        // Where the lane's converted V goes: row 16 wave + 8 i + lane / 8, chunks 4 (lane % 8) ..
+        // of 16 bytes, permuted by row (chunk ^ 4 (row % 4)).
+        _Float16* const vto = &st.v[0][16 * wave + (lane >> 3)][32 * ((lane & 7) ^ ((lane >> 3) & 3))];
+        float unit[2];
+        // The rows' powers of two; rows that not every query row of the tile sees: see guard_rows
+        // (a scale of 0 makes the row's values 0).
+        auto units = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (__builtin_expect(t * kUnit + kUnit - 1 > first, 0)) {
+                    const int r = t * kUnit + 16 * wave + 8 * i + (lane >> 3);
+                    if (r >= rows) vs[i] = 0;
+                    if (r > first && vs[i] == kMxNan) {
+                        vs[i] = 0;
+                        st.found = 1;
+                    }
+                }
+                unit[i] = __uint_as_float(vs[i] << 23);
+            }
+        };
+        auto convert = [&](int c, int buf) {               // the c-th of eight chunks
+            const uint32_t x = vc[c >> 2][c & 3];
+            const float u = unit[c >> 2];
+            const u32x4 y = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, u, 0)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, u, 1)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, u, 2)),
+                             __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, u, 3))};
+            *reinterpret_cast<u32x4*>(vto + buf * (kUnit * kHd) + (c >> 2) * (8 * kHd) + (c & 3) * 8) = y;
+        };
+        // Score products, with beside(i) behind the i-th of 20; a block's codes are
+        // replaced by the next unit's once it is done.
+        f32x16 x;
+        auto scores = [&](const uint8_t* next, auto beside) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[k] = 0.0f;
+            auto step = [&](auto S) {
+                constexpr int s = decltype(S)::value;
+#pragma unroll
+                for (int k = kParts - 1; k >= 0; --k) {
+                    x = scaled_product32<s>(kc[s], q[s][k], x, ks, qs[k]);
+                    beside(kParts * s + kParts - 1 - k);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                kc[s] = *reinterpret_cast<const u32x4*>(next + 16 * s);
+            };
+            step(std::integral_constant<int, 0>{});
+            step(std::integral_constant<int, 1>{});
+            step(std::integral_constant<int, 2>{});
+            step(std::integral_constant<int, 3>{});
+        };
+        auto take = [&]() {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                sc[k] = x[k];
+                asm volatile("" : "+v"(sc[k]));            // moved once, to vector registers
+            }
+        };
+        // Whether some row of the tile does not see some row of unit t.
+        auto masked = [&](int t) { return t * kUnit + kUnit - 1 > first; };
+        auto mask = [&](int t) {
+            const int lim = mine - (t * kUnit + 32 * half) - 4 * h;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) sc[k] = 8 * (k >> 2) + (k & 3) <= lim ? sc[k] : -INFINITY;
+        };
+        // Posts the maximum of the unit's scores.
+        auto post = [&]() {
+            mx = fmaxf(sc[0], sc[1]);
+#pragma unroll
+            for (int k = 2; k < 16; ++k) mx = fmaxf(mx, sc[k]);
+            mx = xor32_max(mx);
+            if (h == 0) st.mx[0][wave][nn] = mx;
+        };
+        // The row's maximum over both halves of the unit, which may move the one the
+        // weights refer to (known a while before it is done).
+        bool moves;
+        float sub;                                         // what the weights' exponents have added
+        auto meet = [&](float other) {
+            mx = fmaxf(mx, other);
+            moves = __any(mx > m_run + kMove);             // (m_run is -inf at first)
+        };
+        auto move = [&]() {
+            if (__builtin_expect_with_probability(moves, 0, 0.99)) {
+                const float m_new = fmaxf(m_run, mx);
+                const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
+                m_run = m_new;
+                l_run *= alpha;
+                pin();
+#pragma unroll
+                for (int d = 0; d < 4; ++d) o[d] *= alpha;
+                pin();
+            }
+            sub = kShift - (m_run == -INFINITY ? 0.0f : m_run);
+        };
+        f16x8 ph[2], pl[2];
+        float p_even = 0.0f, p_sum = 0.0f;                 // (of the unit: one small weight at a time would be lost
+                                                           // beside a large sum)
+        auto weight = [&](int k) {
+            const float p = __builtin_amdgcn_exp2f(sc[k] + sub);
+            p_sum = k ? p_sum + p : p;
+            if (k == 15) l_run += p_sum;
+            asm volatile("" : "+v"(p_sum));                 // here, among the products
+            if (k & 1) {
+                f16x2 hi, lo;
+                split16(p_even, p, hi, lo);
+                ph[k >> 3][(k & 7) - 1] = hi.x; ph[k >> 3][k & 7] = hi.y;
+                pl[k >> 3][(k & 7) - 1] = lo.x; pl[k >> 3][k & 7] = lo.y;
+            } else {
+                p_even = p;
+            }
+        };
+        auto hand_over = [&]() {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                st.p[wave][2 * c][lane] = ph[c];
+                st.p[wave][2 * c + 1][lane] = pl[c];
+            }
+        };
+        auto v_read = [&](int whose, int step, f16x8 (&v)[4]) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const uint32_t at = va[whose][d] + step * 16 * 512;
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at);
+                const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(at + 8 * 512));
+                typedef short s16x8 __attribute__((ext_vector_type(8)));
+                v[d] = __builtin_bit_cast(f16x8, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
+            }
+        };
+        auto add = [&](const f16x8 (&v)[4], f16x8 hi, f16x8 lo, auto beside) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], lo, o[d], 0, 0, 0);
+                beside(d);
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], hi, o[d], 0, 0, 0);
+                beside(4 + d);
+            }
+        };
+        auto nothing = [](int) {};
+
+        {
+            const uint8_t* const next = key_row(at1);
+            scores(next, nothing);
+            ks = key_scales(at1);
+            units(wk.t0);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) convert(c, 0);
+            load_values(at1);
+        }
+        take();
+        if (masked(wk.t0)) mask(wk.t0);
+        post();
+        int t = wk.t0, buf = 0;
+        lds_barrier();
+        meet(st.mx[0][wave ^ 2][nn]);
+        // Output products of unit t: the wave's own 32 rows, whose first 16 rows of V
+        // are read by now, then its partner's.  The last 16 rows' wait, read, for the
+        // next unit's beginning.  behind() runs among the first products, ahead() with
+        // the partner's maxima.
+        f16x8 v0[4], v1[4], h1, l1;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            h1[k] = l1[k] = (_Float16)0.0f;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) v1[d][k] = (_Float16)0.0f;
+        }
+        auto output = [&](auto behind, auto ahead) {
+            hand_over();
+            v_read(0, 1, v1);
+            __builtin_amdgcn_sched_barrier(0);
+            behind();
+            __builtin_amdgcn_sched_barrier(0);
+            lds_barrier();                                 // the partner's weights and maxima
+            const float other = st.mx[0][wave ^ 2][nn];
+            const f16x8 h0 = st.p[wave ^ 2][0][lane], l0 = st.p[wave ^ 2][1][lane];
+            h1 = st.p[wave ^ 2][2][lane];
+            l1 = st.p[wave ^ 2][3][lane];
+            v_read(1, 0, v0);
+            __builtin_amdgcn_sched_barrier(0);
+            add(v1, ph[1], pl[1], nothing);
+            ahead(other);
+            __builtin_amdgcn_sched_barrier(0);
+            v_read(1, 1, v1);
+            add(v0, h0, l0, nothing);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // A unit begins once its V is there and every wave is past the buffer that the next
+        // one's goes to, and with what the unit before left: eight products, beside which the
+        // next unit's V is converted.
+#pragma nounroll
+        for (; t + 1 < wk.t1; ++t) {
+            lds_barrier();
+            const int flip = buf ? -kBuf : kBuf;
+            const uint8_t* const next_k = key_row(at2);
+            units(t + 1);
+            add(v1, h1, l1, [&](int c) {
+                convert(c, buf ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            load_values(at2);
+            at1 = at2;
+            at2 = place(t + 3);
+            move();
+            scores(next_k, [&](int i) {
+                if (i < 16) weight(i);
+                if (i == 16) v_read(0, 0, v0);
+            });
+            ks = key_scales(at1);
+            output(
+                [&]() {
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0[d], pl[0], o[d], 0, 0, 0);
+                    take();
+                    if (masked(t + 1)) {
+                        asm volatile("");                  // a branch, not selects
+                        mask(t + 1);
+                    }
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0[d], ph[0], o[d], 0, 0, 0);
+                    post();
+                },
+                meet);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) va[0][d] += flip, va[1][d] += flip;
+            buf ^= 1;
+        }
+        lds_barrier();
+        const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
+        float4 gate[16];                                   // of the wave's rows 16 wave ..
+        if (whole) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                gate[r] = *reinterpret_cast<const float4*>(
+                    q_tile + (uint32_t)(from_row0(16 * wave + r) * (2 * kHd * 4) + 4 * kHd + 16 * lane));
+        }
+        add(v1, h1, l1, nothing);
+        move();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) weight(k);
+        v_read(0, 0, v0);
+        output([&]() { add(v0, ph[0], pl[0], nothing); }, [](float) {});
+        add(v1, h1, l1, nothing);
+        pin();
+
+        // The tile's rows to LDS, then a row a wave at a time: finished, or as a part
+        // to the workspace.  (Places again as values of this part: kept from the
+        // segment's beginning they would be in registers all the while.)
+        asm volatile("" : "+v"(lane), "+v"(nn));
+        const int slot = 2 * wg + (wk.t0 == 0);
+        l_run = xor32_sum(l_run);
+        if (lane < 32) st.mx[1][wave][nn] = l_run;
+        if (half == 0 && lane < 32) st.mx[0][rg][nn] = m_run;
+        lds_barrier();                                     // the last maxima are read
+        float4* const os = st.q;
+        put_rows(os, o, rg, half, lane);
+        lds_barrier();
+        const int row = 16 * wave + (lane & 15);           // a row's sum and maximum in lane row % 16
+        const float l = st.mx[1][row >> 5][row & 31] + st.mx[1][2 + (row >> 5)][row & 31];
+        float* const to_part = part_o + (size_t)slot * kPagedTileRows * kHd;
+        auto gate_row = [&](int r) { return q_tile + (uint32_t)(from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane); };
+        auto out_row = [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; };
+        const bool look = leave_rows(os, l, st.mx[0][row >> 5][row & 31], whole, gate, to_part,
+                                     part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane, out_row);
+        if (__builtin_expect(look || uniform(st.found), 0))
+            settle_rows<Mx4>(os, pv, table, kvh, wk.t0 * kUnit, min(rows, wk.t1 * kUnit), first, left, hg_shift, l, whole,
+                            to_part, wave, lane, gate_row, out_row);
+        lds_barrier();                                     // (the stores need no wait)
+    }
+}
+
+}  // namespace
+
+PagedPrefillKernel paged_prefill_mx4_kernel() { return paged_prefill_mx4; }
+
+}  // namespace q35

@@ -105,6 +105,8 @@ enum KernelId {
     K_PAGED_DECODE_MERGE,
     K_PAGED_PREFILL,
     K_PAGED_PREFILL_MERGE,
+    K_PAGED_ROWS,
+    K_PAGED_PLAN,
     K_COUNT
 };
 const char* kernel_name(int id);

@@ -22,7 +22,7 @@ ERR_INVALID, ERR_UNSUPPORTED, ERR_CAPACITY, ERR_NO_DEVICE, ERR_HIP, ERR_OOM, ERR
     -1, -2, -3, -4, -5, -6, -7
 STATE_RECURRENT, STATE_CONV, STATE_KEYS, STATE_VALUES = 0, 1, 2, 3
 PROJ_REFERENCE, PROJ_BLOCK = 0, 1
-KV_F32, KV_F16 = 0, 1
+KV_F32, KV_F16, KV_MXFP4 = 0, 1, 4
 
 _lib = None
 _hip = None
@@ -109,6 +109,9 @@ def lib() -> ctypes.CDLL:
         _lib.q35m_paged_len.argtypes = [vp, ci, ip]
         _lib.q35m_paged_device_ptr.argtypes = [vp, ci, ci, ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_size_t)]
         _lib.q35m_paged_append.argtypes = [vp, ci, ci, ip, ip, vp, vp]
+        _lib.q35m_paged_rows.argtypes = [vp, ci, ci, ip, ip, ip, vp, vp]
+        _lib.q35m_paged_plan.argtypes = [vp, ci, vp, vp, vp, ci, vp, ctypes.c_size_t, vp]
+        _lib.q35m_paged_tables.argtypes = [vp, ctypes.POINTER(vp), ctypes.POINTER(vp), ip]
         _lib.q35m_paged_attn_decode.argtypes = [vp, ci, ci, ip, vp, vp, vp, vp]
         _lib.q35m_paged_attn_prefill.argtypes = [vp, ci, ci, ip, ip, vp, vp, vp, vp]
     return _lib
@@ -567,7 +570,8 @@ class PagedCache:
 
     def device_ptr(self, layer: int, kind: int):
         """(address, bytes) of one layer's key or value pages,
-        [n_pages][kv_heads][page_rows][256]."""
+        [n_pages][kv_heads][page_rows][256] (in 4 bits 136 bytes a row: codes,
+        then scales, of each [n_pages][kv_heads])."""
         p = ctypes.c_void_p()
         n = ctypes.c_size_t()
         check(lib().q35m_paged_device_ptr(self.handle, layer, kind, ctypes.byref(p), ctypes.byref(n)))
@@ -577,6 +581,25 @@ class PagedCache:
         """tokens[i] new rows of sequence seqs[i] from k, v [sum(tokens)][kv_heads*256]."""
         assert len(seqs) == len(tokens)
         check(lib().q35m_paged_append(self.handle, layer, len(seqs), _seqs(seqs), _seqs(tokens), k.ptr, v.ptr))
+
+    def rows(self, layer, seqs, first, count, k, v) -> None:
+        """Rows first[i], ... (count[i] of them) of sequence seqs[i] as the cache holds
+        them, in fp32, to k, v [sum(count)][kv_heads*256]."""
+        assert len(seqs) == len(first) == len(count)
+        check(lib().q35m_paged_rows(self.handle, layer, len(seqs), _seqs(seqs), _seqs(first), _seqs(count), k.ptr, v.ptr))
+
+    def plan(self, n, rows, tokens, free, slots, taken) -> None:
+        """Tables and lengths of sequences 0 .. n - 1 from device arrays (.ptr, .nbytes): rows,
+        tokens [n] int32, free pages int32; slots int64, taken [n] int32 are written."""
+        assert min(rows.nbytes, tokens.nbytes, taken.nbytes) >= 4 * n
+        check(lib().q35m_paged_plan(self.handle, n, rows.ptr, tokens.ptr, free.ptr, free.nbytes // 4, slots.ptr,
+                                    slots.nbytes // 8, taken.ptr))
+
+    def tables(self):
+        """(device address of the tables [n_seqs][max_pages], of the lengths [n_seqs], max_pages)."""
+        t, n, m = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_int()
+        check(lib().q35m_paged_tables(self.handle, ctypes.byref(t), ctypes.byref(n), ctypes.byref(m)))
+        return t.value, n.value, m.value
 
     def attn_decode(self, layer, seqs, q_gate, k, v, out) -> None:
         check(lib().q35m_paged_attn_decode(self.handle, layer, len(seqs), _seqs(seqs), q_gate.ptr, k.ptr, v.ptr,
