@@ -257,10 +257,10 @@ __device__ __forceinline__ void put_rows(float4* os, const f32x16 (&o)[4], int r
 }
 
 // From there a wave's 16 rows leave, one at a time: finished to out_row(row), the
-// lane's place (none if null), or as parts.  l, m: sum and maximum of row 16 wave + lane % 16.
+// lane's place (none if null), or as parts.  gate_of(k): the gate of the wave's k-th row, if whole.  l, m: sum and maximum of row 16 wave + lane % 16.
 // Whether a value of theirs is not finite.
-template <typename F>
-__device__ __forceinline__ bool leave_rows(const float4* os, float l, float m, bool whole, float4 (&gate)[16], float* part_o,
+template <typename G, typename F>
+__device__ __forceinline__ bool leave_rows(const float4* os, float l, float m, bool whole, G gate_of, float* part_o,
                                            float* part_ml, int wave, int lane, F out_row) {
     float nan[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     auto rows8 = [&](int k0, auto&& put) {
@@ -280,16 +280,17 @@ __device__ __forceinline__ bool leave_rows(const float4* os, float l, float m, b
     if (whole) {
         const float inv_l = 1.0f / l;
         // (all gates before the first store: a wait for a load waits for the stores before it)
+        float4 gate[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-            gate[k] = gate_sigmoid(gate[k]);
+            gate[k] = gate_sigmoid(gate_of(k));
             asm volatile("" : "+v"(gate[k].x), "+v"(gate[k].y), "+v"(gate[k].z), "+v"(gate[k].w));
         }
         auto put = [&](int k, float4 x) {
             const float inv = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv_l), k));
             const float4 g = gate[k];
             x = make_float4(x.x * inv * g.x, x.y * inv * g.y, x.z * inv * g.z, x.w * inv * g.w);
-            if (char* to = out_row(16 * wave + k)) *reinterpret_cast<float4*>(to) = x;
+            if (char* to = out_row(16 * wave + k)) to_global(to, x);
         };
         rows8(0, put);
         rows8(8, put);

@@ -459,7 +459,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         float* const to_part = part_o + (size_t)slot * kPagedTileRows * kHd;
         auto gate_row = [&](int r) { return q_tile + (uint32_t)(from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane); };
         auto out_row = [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; };
-        const bool look = leave_rows(os, l, st.mx[0][row >> 5][row & 31], whole, gate, to_part,
+        const bool look = leave_rows(os, l, st.mx[0][row >> 5][row & 31], whole, [&](int k) { return gate[k]; }, to_part,
                                      part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane, out_row);
         if (__builtin_expect(look || uniform(st.found), 0))
             settle_rows<_Float16>(os, pv, table, kvh, wk.t0 * kUnit, min(rows, wk.t1 * kUnit), first, left, hg_shift, l, whole,
@@ -841,7 +841,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
         float* const to_part = part_o + (size_t)slot * kPagedTileRows * kHd;
         auto gate_row = [&](int r) { return q_tile + (uint32_t)(from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane); };
         auto out_row = [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; };
-        const bool look = leave_rows(os, l, st.ss[2 + (row >> 5)][row & 31], whole, gate, to_part,
+        const bool look = leave_rows(os, l, st.ss[2 + (row >> 5)][row & 31], whole, [&](int k) { return gate[k]; }, to_part,
                                      part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane, out_row);
         if (__builtin_expect(look || uniform(st.found), 0))
             settle_rows<float>(os, pv, table, kvh, wk.t0 * kUnit, min(rows, wk.t1 * kUnit), first, left, hg_shift, l, whole,

@@ -21,8 +21,8 @@ constexpr int NT = 256;
 constexpr int kParts = 5;
 
 struct Mx4Tile {
-    _Float16 v[2][kUnit][kHd];            // (first q's parts)
-    float4 q[kPagedTileRows * kHd / 4];   // q rows; at the end the output's
+    _Float16 v[2][kUnit][kHd];            // (first q's parts, at the end the output's rows)
+    float4 q[kPagedTileRows * kHd / 4];   // q rows, then their gates
     f16x8 p[4][4][kWave];                 // a wave's weights: operands (hi, lo) of its two 16-row steps
     float mx[2][4][32];                   // maxima of a unit's halves; at the end sums and maxima
     float w[kHd];                         // 1 + the norm's weights
@@ -144,8 +144,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         };
         // K: lane (row nn, h) takes blocks 4 h .. of its row; V: 16-byte pieces of two rows,
         // 8 i + lane / 8, block lane % 8.
-        u32x4 kc[4], vc[2];
-        uint32_t ks, vs[2];
+        u32x4 kc[4], vc[2][2];
+        uint32_t ks, vs[2][2];                             // (V of two units: they are waited for longest)
         auto key_row = [&](const Place& p) {
             const uint8_t* const a = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[0] + (uint32_t)p.in[0] * kMxCodes);
             const uint8_t* const b = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[1] + (uint32_t)p.in[1] * kMxCodes);
@@ -154,17 +154,17 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         auto key_scales = [&](const Place& p) {
             const uint8_t* const a = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[0] + mx_key_scale(pv, p.in[0]));
             const uint8_t* const b = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[1] + mx_key_scale(pv, p.in[1]));
-            return *reinterpret_cast<const uint32_t*>((nn & 16 ? b : a) + (uint32_t)((nn & 15) * kMxBlocks + 4 * h));
+            return from_global<uint32_t>((nn & 16 ? b : a) + (uint32_t)((nn & 15) * kMxBlocks + 4 * h));
         };
-        auto load_values = [&](const Place& p) {
+        auto load_values = [&](const Place& p, u32x4 (&vc)[2], uint32_t (&vs)[2]) {
             const size_t page = rg ? p.page[1] : p.page[0];
             const int in = rg ? p.in[1] : p.in[0];
             const uint8_t* const at = (const uint8_t*)uniform((const uint8_t*)pv.v + page + (uint32_t)in * kMxCodes);
             const uint8_t* const sc = (const uint8_t*)uniform((const uint8_t*)pv.v + page + mx_value_scale(pv, in, 0));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                vc[i] = *reinterpret_cast<const u32x4*>(at + (uint32_t)(1024 * i + 16 * lane));
-                vs[i] = sc[(uint32_t)(16 * (lane & 7) + 8 * i + (lane >> 3))];
+                vc[i] = from_global<u32x4>(at + (uint32_t)(1024 * i + 16 * lane));
+                vs[i] = from_global<uint8_t>(sc + (uint32_t)(16 * (lane & 7) + 8 * i + (lane >> 3)));
             }
         };
 
@@ -176,12 +176,12 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         {
             const uint8_t* const from = key_row(at1);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) kc[s] = *reinterpret_cast<const u32x4*>(from + 16 * s);
+            for (int s = 0; s < 4; ++s) kc[s] = from_global<u32x4>(from + 16 * s);
             ks = key_scales(at1);
-            load_values(at1);
+            load_values(at1, vc[0], vs[0]);
+            at1 = place(wk.t0 + 1);
+            load_values(at1, vc[1], vs[1]);
         }
-        at1 = place(wk.t0 + 1);
-        Place at2 = place(wk.t0 + 2);
         if (tid == 0) st.found = 0;
 
         // q: the norm's rows in fp32, then partners cut half of each row's blocks into parts
@@ -229,6 +229,13 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
 #pragma unroll
         for (int k = 1; k < kParts; ++k) qs[k] = qs[k - 1] - 0x04040404u;      // (no borrow: a scale is 38 or more)
         lds_barrier();                                     // the parts are read
+        // The gates of the wave's rows 16 wave .. take q's place.
+        const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
+        if (whole) {
+#pragma unroll 4
+            for (int r = 16 * wave; r < 16 * wave + 16; ++r)
+                dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane, lds_address(&st.q[0]) + r * kHd * 4);
+        }
 
         // The output stays in accumulation registers all along: pin() is a use there,
         // without which the compiler moves all of it to vector registers and back on
@@ -241,24 +248,29 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
             for (int k = 0; k < 16; ++k) o[d][k] = 0.0f;
         pin();
         float m_run = -INFINITY, l_run = 0.0f, mx = -INFINITY;
-        float sc[16];                                      // the wave's scores of a unit
+        f32x16 sc[2];                                      // the wave's scores of two units
 
         // V operands of 16 rows and 32 dims: lane (dim nn, h), rows 4 h + {0..3, 8..11},
         // which the transposing read gathers from lanes of 4 rows x 16 dims.
         uint32_t va[2][4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            va[0][d] = lds_address(&st.v[0][32 * half + 4 * h + ((lane >> 2) & 3)][0]) + 32 * (8 * half + ((2 * d + ((lane >> 4) & 1)) ^ (2 * ((lane >> 2) & 3)))) +
-                    8 * (lane & 3);
+            va[0][d] = lds_address(&st.v[0][32 * half + 4 * h + ((lane >> 2) & 3)][0]) +
+                       32 * (8 * half + ((2 * d + ((lane >> 4) & 1)) ^ (2 * ((lane >> 2) & 3)) ^ ((lane >> 2) & 1))) + 8 * ((lane & 3) ^ (2 * half));
             va[1][d] = va[0][d] + (half ? -32 * 512 : 32 * 512);   // the partner's rows
         }
-        // Where the lane's converted V goes: row 16 wave + 8 i + lane / 8, chunks 4 (lane % 8) ..
-        // of 16 bytes, permuted by row (chunk ^ 4 (row % 4)).
-        _Float16* const vto = &st.v[0][16 * wave + (lane >> 3)][32 * ((lane & 7) ^ ((lane >> 3) & 3))];
+        // Where the lane's converted V goes: row 16 wave + 8 i + lane / 8, chunks 4 (lane % 8) + c
+        // of 16 bytes, in place chunk ^ 4 (row % 4) ^ 2 (row % 2) ^ (chunk / 16): the rows that one
+        // read touches fall into different banks, and so do the 16 lanes that write together.
+        uint32_t vto[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            vto[c] = lds_address(&st.v[0][16 * wave + (lane >> 3)][0]) + 64 * ((lane & 7) ^ ((lane >> 3) & 3)) +
+                     16 * (c ^ ((lane >> 2) & 1) ^ (2 * ((lane >> 3) & 1)));
         float unit[2];
         // The rows' powers of two; rows that not every query row of the tile sees: see guard_rows
         // (a scale of 0 makes the row's values 0).
-        auto units = [&](int t) {
+        auto units = [&](int t, uint32_t (&vs)[2]) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 if (__builtin_expect(t * kUnit + kUnit - 1 > first, 0)) {
@@ -272,22 +284,22 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
                 unit[i] = __uint_as_float(vs[i] << 23);
             }
         };
-        auto convert = [&](int c, int buf) {               // the c-th of eight chunks
+        auto convert = [&](int c, const u32x4 (&vc)[2], int buf) {     // the c-th of eight chunks
             const uint32_t x = vc[c >> 2][c & 3];
             const float u = unit[c >> 2];
             const u32x4 y = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, u, 0)),
                              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, u, 1)),
                              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, u, 2)),
                              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(x, u, 3))};
-            *reinterpret_cast<u32x4*>(vto + buf * (kUnit * kHd) + (c >> 2) * (8 * kHd) + (c & 3) * 8) = y;
+            typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+            *(lds_u32x4*)(uintptr_t)(vto[c & 3] + buf * kBuf + (c >> 2) * (8 * kHd * 2)) = y;
         };
         // Score products, with beside(i) behind the i-th of 20; a block's codes are
         // replaced by the next unit's once it is done.
-        f32x16 x;
-        auto scores = [&](const uint8_t* next, auto beside) {
+        auto scores = [&](f32x16& x, const uint8_t* next, auto beside) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) x[k] = 0.0f;
-            auto step = [&](auto S) {
+            auto step = [&](auto S) __attribute__((always_inline)) {
                 constexpr int s = decltype(S)::value;
 #pragma unroll
                 for (int k = kParts - 1; k >= 0; --k) {
@@ -295,29 +307,22 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
                     beside(kParts * s + kParts - 1 - k);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                kc[s] = *reinterpret_cast<const u32x4*>(next + 16 * s);
+                kc[s] = from_global<u32x4>(next + 16 * s);
             };
             step(std::integral_constant<int, 0>{});
             step(std::integral_constant<int, 1>{});
             step(std::integral_constant<int, 2>{});
             step(std::integral_constant<int, 3>{});
         };
-        auto take = [&]() {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                sc[k] = x[k];
-                asm volatile("" : "+v"(sc[k]));            // moved once, to vector registers
-            }
-        };
         // Whether some row of the tile does not see some row of unit t.
         auto masked = [&](int t) { return t * kUnit + kUnit - 1 > first; };
-        auto mask = [&](int t) {
+        auto mask = [&](int t, f32x16& sc) {
             const int lim = mine - (t * kUnit + 32 * half) - 4 * h;
 #pragma unroll
             for (int k = 0; k < 16; ++k) sc[k] = 8 * (k >> 2) + (k & 3) <= lim ? sc[k] : -INFINITY;
         };
         // Posts the maximum of the unit's scores.
-        auto post = [&]() {
+        auto post = [&](const f32x16& sc) {
             mx = fmaxf(sc[0], sc[1]);
 #pragma unroll
             for (int k = 2; k < 16; ++k) mx = fmaxf(mx, sc[k]);
@@ -348,7 +353,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         f16x8 ph[2], pl[2];
         float p_even = 0.0f, p_sum = 0.0f;                 // (of the unit: one small weight at a time would be lost
                                                            // beside a large sum)
-        auto weight = [&](int k) {
+        auto weight = [&](int k, const f32x16& sc) {
             const float p = __builtin_amdgcn_exp2f(sc[k] + sub);
             p_sum = k ? p_sum + p : p;
             if (k == 15) l_run += p_sum;
@@ -369,10 +374,10 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
                 st.p[wave][2 * c + 1][lane] = pl[c];
             }
         };
-        auto v_read = [&](int whose, int step, f16x8 (&v)[4]) {
+        auto v_read = [&](int buf, int whose, int step, f16x8 (&v)[4]) {
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                const uint32_t at = va[whose][d] + step * 16 * 512;
+                const uint32_t at = va[whose][d] + buf * kBuf + step * 16 * 512;
                 const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at);
                 const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(at + 8 * 512));
                 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -394,18 +399,20 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         auto nothing = [](int) {};
 
         {
+            // (V's loads before K's, as in the loop: they are waited for in order)
             const uint8_t* const next = key_row(at1);
-            scores(next, nothing);
-            ks = key_scales(at1);
-            units(wk.t0);
+            units(wk.t0, vs[0]);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) convert(c, 0);
-            load_values(at1);
+            for (int c = 0; c < 8; ++c) convert(c, vc[0], 0);
+            const Place at2 = place(wk.t0 + 2);
+            load_values(at2, vc[0], vs[0]);
+            scores(sc[0], next, nothing);
+            ks = key_scales(at1);
+            at1 = at2;
         }
-        take();
-        if (masked(wk.t0)) mask(wk.t0);
-        post();
-        int t = wk.t0, buf = 0;
+        if (masked(wk.t0)) mask(wk.t0, sc[0]);
+        post(sc[0]);
+        int t = wk.t0;
         lds_barrier();
         meet(st.mx[0][wave ^ 2][nn]);
         // Output products of unit t: the wave's own 32 rows, whose first 16 rows of V
@@ -419,9 +426,9 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
 #pragma unroll
             for (int d = 0; d < 4; ++d) v1[d][k] = (_Float16)0.0f;
         }
-        auto output = [&](auto behind, auto ahead) {
+        auto output = [&](int buf, auto behind, auto ahead) __attribute__((always_inline)) {
             hand_over();
-            v_read(0, 1, v1);
+            v_read(buf, 0, 1, v1);
             __builtin_amdgcn_sched_barrier(0);
             behind();
             __builtin_amdgcn_sched_barrier(0);
@@ -430,71 +437,79 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
             const f16x8 h0 = st.p[wave ^ 2][0][lane], l0 = st.p[wave ^ 2][1][lane];
             h1 = st.p[wave ^ 2][2][lane];
             l1 = st.p[wave ^ 2][3][lane];
-            v_read(1, 0, v0);
+            v_read(buf, 1, 0, v0);
             __builtin_amdgcn_sched_barrier(0);
             add(v1, ph[1], pl[1], nothing);
             ahead(other);
             __builtin_amdgcn_sched_barrier(0);
-            v_read(1, 1, v1);
+            v_read(buf, 1, 1, v1);
             add(v0, h0, l0, nothing);
             __builtin_amdgcn_sched_barrier(0);
         };
         // A unit begins once its V is there and every wave is past the buffer that the next
         // one's goes to, and with what the unit before left: eight products, beside which the
-        // next unit's V is converted.
-#pragma nounroll
-        for (; t + 1 < wk.t1; ++t) {
+        // next unit's V is converted.  (B: the unit's V buffer and place among the scores; units
+        // in pairs, so that what one leaves to the next stays where it is.)
+        auto go_on = [&](auto B) __attribute__((always_inline)) {
+            constexpr int b = decltype(B)::value;
             lds_barrier();
-            const int flip = buf ? -kBuf : kBuf;
-            const uint8_t* const next_k = key_row(at2);
-            units(t + 1);
+            const uint8_t* const next_k = key_row(at1);
+            units(t + 1, vs[b ^ 1]);
             add(v1, h1, l1, [&](int c) {
-                convert(c, buf ^ 1);
+                convert(c, vc[b ^ 1], b ^ 1);
                 __builtin_amdgcn_sched_barrier(0);
             });
-            load_values(at2);
-            at1 = at2;
-            at2 = place(t + 3);
+            const Place at2 = place(t + 3);
+            load_values(at2, vc[b ^ 1], vs[b ^ 1]);
             move();
-            scores(next_k, [&](int i) {
-                if (i < 16) weight(i);
-                if (i == 16) v_read(0, 0, v0);
+            scores(sc[b ^ 1], next_k, [&](int i) {
+                if (i < 16) weight(i, sc[b]);
+                if (i == 16) v_read(b, 0, 0, v0);
             });
             ks = key_scales(at1);
+            at1 = at2;
             output(
+                b,
                 [&]() {
 #pragma unroll
                     for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0[d], pl[0], o[d], 0, 0, 0);
-                    take();
+                    asm volatile("" : "+v"(sc[b ^ 1]));    // in vector registers, where the weights want them
                     if (masked(t + 1)) {
                         asm volatile("");                  // a branch, not selects
-                        mask(t + 1);
+                        mask(t + 1, sc[b ^ 1]);
                     }
 #pragma unroll
                     for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0[d], ph[0], o[d], 0, 0, 0);
-                    post();
+                    post(sc[b ^ 1]);
                 },
                 meet);
+        };
+        auto finish = [&](auto B) __attribute__((always_inline)) {
+            constexpr int b = decltype(B)::value;
+            lds_barrier();
+            add(v1, h1, l1, nothing);
+            move();
 #pragma unroll
-            for (int d = 0; d < 4; ++d) va[0][d] += flip, va[1][d] += flip;
-            buf ^= 1;
+            for (int k = 0; k < 16; ++k) weight(k, sc[b]);
+            v_read(b, 0, 0, v0);
+            output(b, [&]() { add(v0, ph[0], pl[0], nothing); }, [](float) {});
+            add(v1, h1, l1, nothing);
+        };
+#pragma nounroll
+        for (;; t += 2) {
+            if (t + 1 == wk.t1) {
+                finish(std::integral_constant<int, 0>{});
+                break;
+            }
+            go_on(std::integral_constant<int, 0>{});
+            if (t + 2 == wk.t1) {
+                finish(std::integral_constant<int, 1>{});
+                break;
+            }
+            ++t;
+            go_on(std::integral_constant<int, 1>{});
+            --t;
         }
-        lds_barrier();
-        const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
-        float4 gate[16];                                   // of the wave's rows 16 wave ..
-        if (whole) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                gate[r] = *reinterpret_cast<const float4*>(
-                    q_tile + (uint32_t)(from_row0(16 * wave + r) * (2 * kHd * 4) + 4 * kHd + 16 * lane));
-        }
-        add(v1, h1, l1, nothing);
-        move();
-#pragma unroll
-        for (int k = 0; k < 16; ++k) weight(k);
-        v_read(0, 0, v0);
-        output([&]() { add(v0, ph[0], pl[0], nothing); }, [](float) {});
-        add(v1, h1, l1, nothing);
         pin();
 
         // The tile's rows to LDS, then a row a wave at a time: finished, or as a part
@@ -505,8 +520,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         l_run = xor32_sum(l_run);
         if (lane < 32) st.mx[1][wave][nn] = l_run;
         if (half == 0 && lane < 32) st.mx[0][rg][nn] = m_run;
-        lds_barrier();                                     // the last maxima are read
-        float4* const os = st.q;
+        lds_barrier();                                     // V and the last maxima are read
+        float4* const os = reinterpret_cast<float4*>(&st.v[0][0][0]);
         put_rows(os, o, rg, half, lane);
         lds_barrier();
         const int row = 16 * wave + (lane & 15);           // a row's sum and maximum in lane row % 16
@@ -514,7 +529,9 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         float* const to_part = part_o + (size_t)slot * kPagedTileRows * kHd;
         auto gate_row = [&](int r) { return q_tile + (uint32_t)(from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane); };
         auto out_row = [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; };
-        const bool look = leave_rows(os, l, st.mx[0][row >> 5][row & 31], whole, gate, to_part,
+        dma_wait();                                        // (the gates, which the wave itself has brought)
+        auto gate_of = [&](int k) { return st.q[(16 * wave + k) * (kHd / 4) + lane]; };
+        const bool look = leave_rows(os, l, st.mx[0][row >> 5][row & 31], whole, gate_of, to_part,
                                      part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane, out_row);
         if (__builtin_expect(look || uniform(st.found), 0))
             settle_rows<Mx4>(os, pv, table, kvh, wk.t0 * kUnit, min(rows, wk.t1 * kUnit), first, left, hg_shift, l, whole,
