@@ -119,52 +119,49 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         auto from_row0 = [&](int r) { return min(r >> hg_shift, left - 1) * nh + (r & (hg - 1)); };
 
         // A wave takes rows 32 half .. of a unit's K and brings rows 16 wave .. of its V,
-        // the rg-th 16 of those.  It holds 64 entries of the page table, one a lane, from
-        // entry `held` on; a unit's two pages are found a unit before they are asked for.
-        int held = 0, ids = 0;
+        // the rg-th 16 of those.  It holds where 64 entries of the page table lie, one a lane,
+        // from entry `held` on (one instruction fewer counts here: see above).
+        int held = 0;
+        uint32_t at_lo = 0, at_hi = 0;                     // of the K page; V's is v_behind further
+        const uint64_t v_behind = (uint64_t)pv.v - (uint64_t)pv.k;
+        const int in_page = (1 << pv.page_shift) - 1, scales = kMxCodes << pv.page_shift;
         auto hold = [&](int entry) {
             held = entry;
-            ids = page_of(table, entry + lane, pv.max_pages, pv.n_pages);
+            const uint64_t at = (uint64_t)pv.k + mx_page(pv, page_of(table, entry + lane, pv.max_pages, pv.n_pages), kvh);
+            at_lo = (uint32_t)at;
+            at_hi = (uint32_t)(at >> 32);
         };
-        hold(min(wk.t0 * kUnit + 32 * half, last16) >> pv.page_shift);
-        struct Place {
-            size_t page[2];          // first bytes of the pages of the two groups of 16 rows
-            int in[2];               // their first rows' places there
+        // First row of the g-th 16 rows of unit t that the wave takes (the last 16, past the end).
+        auto group = [&](int t, int g) { return min(t * kUnit + 32 * half + 16 * g, last16); };
+        auto hold_unit = [&](int t) {
+            if (__builtin_expect(uniform((group(t, 1) >> pv.page_shift) - held) >= kWave, 0)) hold(uniform(group(t, 0) >> pv.page_shift));
         };
-        auto place = [&](int t) {
-            Place p;
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const int r = uniform(min(t * kUnit + 32 * half + 16 * g, last16)), entry = r >> pv.page_shift;
-                if (__builtin_expect(uniform(entry - held) >= kWave, 0)) hold(entry);
-                p.page[g] = mx_page(pv, __builtin_amdgcn_readlane(ids, uniform(entry - held)), kvh);
-                p.in[g] = r & ((1 << pv.page_shift) - 1);
-            }
-            return p;
-        };
+        hold(uniform(group(wk.t0, 0) >> pv.page_shift));
         // K: lane (row nn, h) takes blocks 4 h .. of its row; V: 16-byte pieces of two rows,
         // 8 i + lane / 8, block lane % 8.
         u32x4 kc[4], vc[2][2];
-        uint32_t ks, vs[2][2];                             // (V of two units: they are waited for longest)
-        auto key_row = [&](const Place& p) {
-            const uint8_t* const a = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[0] + (uint32_t)p.in[0] * kMxCodes);
-            const uint8_t* const b = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[1] + (uint32_t)p.in[1] * kMxCodes);
-            return (nn & 16 ? b : a) + (uint32_t)((nn & 15) * kMxCodes + 64 * h);
+        uint32_t ks[2], vs[2][2];                          // (V of two units: they are waited for longest)
+        struct Keys {
+            const uint8_t *row, *scale;
         };
-        auto key_scales = [&](const Place& p) {
-            const uint8_t* const a = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[0] + mx_key_scale(pv, p.in[0]));
-            const uint8_t* const b = (const uint8_t*)uniform((const uint8_t*)pv.k + p.page[1] + mx_key_scale(pv, p.in[1]));
-            return from_global<uint32_t>((nn & 16 ? b : a) + (uint32_t)((nn & 15) * kMxBlocks + 4 * h));
+        auto keys = [&](int t) {
+            const int r = min(t * kUnit + 32 * half + (nn & 16), last16), in = r & in_page;
+            const int from = 4 * ((r >> pv.page_shift) - held);
+            const uint32_t lo = __builtin_amdgcn_ds_bpermute(from, (int)at_lo), hi = __builtin_amdgcn_ds_bpermute(from, (int)at_hi);
+            const uint8_t* const at = (const uint8_t*)((uint64_t)hi << 32 | lo);
+            return Keys{at + (uint32_t)((in + (nn & 15)) * kMxCodes + 64 * h),
+                        at + (uint32_t)(scales + (in + (nn & 15)) * kMxBlocks + 4 * h)};
         };
-        auto load_values = [&](const Place& p, u32x4 (&vc)[2], uint32_t (&vs)[2]) {
-            const size_t page = rg ? p.page[1] : p.page[0];
-            const int in = rg ? p.in[1] : p.in[0];
-            const uint8_t* const at = (const uint8_t*)uniform((const uint8_t*)pv.v + page + (uint32_t)in * kMxCodes);
-            const uint8_t* const sc = (const uint8_t*)uniform((const uint8_t*)pv.v + page + mx_value_scale(pv, in, 0));
+        auto load_values = [&](int t, u32x4 (&vc)[2], uint32_t (&vs)[2]) {
+            const int r = uniform(group(t, rg)), from = uniform((r >> pv.page_shift) - held), in = r & in_page;
+            const uint64_t at = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)at_hi, from) << 32 |
+                                 (uint32_t)__builtin_amdgcn_readlane((int)at_lo, from)) + v_behind;
+            const uint32_t code = (uint32_t)(in * kMxCodes + 16 * lane);
+            const uint32_t scale = (uint32_t)(scales + in * kMxBlocks + 16 * (lane & 7) + (lane >> 3));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                vc[i] = from_global<u32x4>(at + (uint32_t)(1024 * i + 16 * lane));
-                vs[i] = from_global<uint8_t>(sc + (uint32_t)(16 * (lane & 7) + 8 * i + (lane >> 3)));
+                vc[i] = from_global<u32x4>((const uint8_t*)at + code + 1024 * i);
+                vs[i] = from_global<uint8_t>((const uint8_t*)at + scale + 8 * i);
             }
         };
 
@@ -172,15 +169,14 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
             dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 16 * (lane ^ (r & 31)), lds_address(&st.q[0]) + r * kHd * 4);
-        Place at1 = place(wk.t0);
         {
-            const uint8_t* const from = key_row(at1);
+            const Keys k = keys(wk.t0);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) kc[s] = from_global<u32x4>(from + 16 * s);
-            ks = key_scales(at1);
-            load_values(at1, vc[0], vs[0]);
-            at1 = place(wk.t0 + 1);
-            load_values(at1, vc[1], vs[1]);
+            for (int s = 0; s < 4; ++s) kc[s] = from_global<u32x4>(k.row + 16 * s);
+            ks[0] = from_global<uint32_t>(k.scale);
+            load_values(wk.t0, vc[0], vs[0]);
+            hold_unit(wk.t0 + 1);
+            load_values(wk.t0 + 1, vc[1], vs[1]);
         }
         if (tid == 0) st.found = 0;
 
@@ -296,7 +292,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         };
         // Score products, with beside(i) behind the i-th of 20; a block's codes are
         // replaced by the next unit's once it is done.
-        auto scores = [&](f32x16& x, const uint8_t* next, auto beside) __attribute__((always_inline)) {
+        auto scores = [&](f32x16& x, uint32_t ks, const uint8_t* next, auto beside) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) x[k] = 0.0f;
             auto step = [&](auto S) __attribute__((always_inline)) {
@@ -327,7 +323,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
 #pragma unroll
             for (int k = 2; k < 16; ++k) mx = fmaxf(mx, sc[k]);
             mx = xor32_max(mx);
-            if (h == 0) st.mx[0][wave][nn] = mx;
+            st.mx[0][wave][nn] = mx;                       // (both halves the same)
         };
         // The row's maximum over both halves of the unit, which may move the one the
         // weights refer to (known a while before it is done).
@@ -353,8 +349,14 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         f16x8 ph[2], pl[2];
         float p_even = 0.0f, p_sum = 0.0f;                 // (of the unit: one small weight at a time would be lost
                                                            // beside a large sum)
+        // The k-th weight is begun, and the one before, whose exponential is there by now, summed
+        // and cut; 17 steps are 16 weights.
+        float p_next = 0.0f;
         auto weight = [&](int k, const f32x16& sc) {
-            const float p = __builtin_amdgcn_exp2f(sc[k] + sub);
+            const float p = p_next;
+            if (k < 16) p_next = __builtin_amdgcn_exp2f(sc[k] + sub);
+            if (k == 0) return;
+            --k;
             p_sum = k ? p_sum + p : p;
             if (k == 15) l_run += p_sum;
             asm volatile("" : "+v"(p_sum));                 // here, among the products
@@ -400,15 +402,14 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
 
         {
             // (V's loads before K's, as in the loop: they are waited for in order)
-            const uint8_t* const next = key_row(at1);
+            const Keys next = keys(wk.t0 + 1);
             units(wk.t0, vs[0]);
 #pragma unroll
             for (int c = 0; c < 8; ++c) convert(c, vc[0], 0);
-            const Place at2 = place(wk.t0 + 2);
-            load_values(at2, vc[0], vs[0]);
-            scores(sc[0], next, nothing);
-            ks = key_scales(at1);
-            at1 = at2;
+            hold_unit(wk.t0 + 2);
+            load_values(wk.t0 + 2, vc[0], vs[0]);
+            scores(sc[0], ks[0], next.row, nothing);
+            ks[1] = from_global<uint32_t>(next.scale);
         }
         if (masked(wk.t0)) mask(wk.t0, sc[0]);
         post(sc[0]);
@@ -453,21 +454,20 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         auto go_on = [&](auto B) __attribute__((always_inline)) {
             constexpr int b = decltype(B)::value;
             lds_barrier();
-            const uint8_t* const next_k = key_row(at1);
+            const Keys next = keys(t + 2);
             units(t + 1, vs[b ^ 1]);
             add(v1, h1, l1, [&](int c) {
                 convert(c, vc[b ^ 1], b ^ 1);
                 __builtin_amdgcn_sched_barrier(0);
             });
-            const Place at2 = place(t + 3);
-            load_values(at2, vc[b ^ 1], vs[b ^ 1]);
+            hold_unit(t + 3);
+            load_values(t + 3, vc[b ^ 1], vs[b ^ 1]);
             move();
-            scores(sc[b ^ 1], next_k, [&](int i) {
-                if (i < 16) weight(i, sc[b]);
-                if (i == 16) v_read(b, 0, 0, v0);
+            scores(sc[b ^ 1], ks[b ^ 1], next.row, [&](int i) {
+                if (i < 17) weight(i, sc[b]);
+                if (i == 17) v_read(b, 0, 0, v0);
             });
-            ks = key_scales(at1);
-            at1 = at2;
+            ks[b] = from_global<uint32_t>(next.scale);
             output(
                 b,
                 [&]() {
@@ -490,25 +490,22 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
             add(v1, h1, l1, nothing);
             move();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) weight(k, sc[b]);
+            for (int k = 0; k < 17; ++k) weight(k, sc[b]);
             v_read(b, 0, 0, v0);
             output(b, [&]() { add(v0, ph[0], pl[0], nothing); }, [](float) {});
             add(v1, h1, l1, nothing);
         };
 #pragma nounroll
-        for (;; t += 2) {
-            if (t + 1 == wk.t1) {
-                finish(std::integral_constant<int, 0>{});
-                break;
-            }
+        for (; t + 2 < wk.t1; ++t) {
             go_on(std::integral_constant<int, 0>{});
-            if (t + 2 == wk.t1) {
-                finish(std::integral_constant<int, 1>{});
-                break;
-            }
             ++t;
             go_on(std::integral_constant<int, 1>{});
-            --t;
+        }
+        if (t + 1 < wk.t1) {
+            go_on(std::integral_constant<int, 0>{});
+            finish(std::integral_constant<int, 1>{});
+        } else {
+            finish(std::integral_constant<int, 0>{});
         }
         pin();
 
