@@ -21,10 +21,12 @@ constexpr int NT = 256;
 constexpr int kParts = 5;
 
 struct Mx4Tile {
-    _Float16 v[2][kUnit][kHd];            // (first q's parts, at the end the output's rows)
-    float4 q[kPagedTileRows * kHd / 4];   // q rows, then their gates
-    f16x8 p[4][4][kWave];                 // a wave's weights: operands (hi, lo) of its two 16-row steps
-    float mx[2][4][32];                   // maxima of a unit's halves; at the end sums and maxima
+    _Float16 v[2][kUnit][kHd];            // (first q's parts, at the end the gates)
+    union {
+        float4 q[kPagedTileRows * kHd / 4];   // q rows, at the end the output's
+        f16x8 p[2][4][4][kWave];          // a wave's weights of two units: operands (hi, lo) of two 16-row steps
+    };
+    float mx[2][4][32];                   // maxima of two units' halves; at the end sums and maxima
     float w[kHd];                         // 1 + the norm's weights
     uint8_t qscale[2][4][kWave];          // the first part's scales
     int found;                            // values that are not finite
@@ -225,14 +227,6 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
 #pragma unroll
         for (int k = 1; k < kParts; ++k) qs[k] = qs[k - 1] - 0x04040404u;      // (no borrow: a scale is 38 or more)
         lds_barrier();                                     // the parts are read
-        // The gates of the wave's rows 16 wave .. take q's place.
-        const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
-        if (whole) {
-#pragma unroll 4
-            for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-                dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane, lds_address(&st.q[0]) + r * kHd * 4);
-        }
-
         // The output stays in accumulation registers all along: pin() is a use there,
         // without which the compiler moves all of it to vector registers and back on
         // every unit, for the rare branch that scales it.
@@ -290,17 +284,29 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
             typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
             *(lds_u32x4*)(uintptr_t)(vto[c & 3] + buf * kBuf + (c >> 2) * (8 * kHd * 2)) = y;
         };
-        // Score products, with beside(i) behind the i-th of 20; a block's codes are
-        // replaced by the next unit's once it is done.
-        auto scores = [&](f32x16& x, uint32_t ks, const uint8_t* next, auto beside) __attribute__((always_inline)) {
+        // The products between two barriers, with beside(i) behind the i-th slot of 40: 20 of
+        // scores, of which each waits for the one before (23 ns, where independent ones take
+        // 18), and between them, if `left`, the 16 that the unit before has left.  A block's
+        // codes are replaced by the next unit's once it is done.
+        f16x8 v0[4], v1[4], w0[4], w1[4], h0, l0, h1, l1;
+        auto left_over = [&](int i) {
+            const f16x8 &a = i < 8 ? v0[i & 3] : v1[i & 3], &b = i < 8 ? (i & 4 ? h0 : l0) : (i & 4 ? h1 : l1);
+            o[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, o[i & 3], 0, 0, 0);
+        };
+        auto scores = [&](f32x16& x, uint32_t ks, const uint8_t* next, auto left, auto beside) __attribute__((always_inline)) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) x[k] = 0.0f;
             auto step = [&](auto S) __attribute__((always_inline)) {
                 constexpr int s = decltype(S)::value;
 #pragma unroll
                 for (int k = kParts - 1; k >= 0; --k) {
+                    const int i = kParts * s + kParts - 1 - k;
                     x = scaled_product32<s>(kc[s], q[s][k], x, ks, qs[k]);
-                    beside(kParts * s + kParts - 1 - k);
+                    asm volatile("" : "+a"(x));            // here: left to itself the compiler moves it to its use
+                    beside(2 * i);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (decltype(left)::value && i < 16) left_over(i);
+                    beside(2 * i + 1);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 kc[s] = from_global<u32x4>(next + 16 * s);
@@ -318,12 +324,12 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
             for (int k = 0; k < 16; ++k) sc[k] = 8 * (k >> 2) + (k & 3) <= lim ? sc[k] : -INFINITY;
         };
         // Posts the maximum of the unit's scores.
-        auto post = [&](const f32x16& sc) {
+        auto post = [&](int buf, const f32x16& sc) {
             mx = fmaxf(sc[0], sc[1]);
 #pragma unroll
             for (int k = 2; k < 16; ++k) mx = fmaxf(mx, sc[k]);
             mx = xor32_max(mx);
-            st.mx[0][wave][nn] = mx;                       // (both halves the same)
+            st.mx[buf][wave][nn] = mx;                      // (both halves the same)
         };
         // The row's maximum over both halves of the unit, which may move the one the
         // weights refer to (known a while before it is done).
@@ -333,18 +339,24 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
             mx = fmaxf(mx, other);
             moves = __any(mx > m_run + kMove);             // (m_run is -inf at first)
         };
+        float alpha;
         auto move = [&]() {
+            alpha = 1.0f;
             if (__builtin_expect_with_probability(moves, 0, 0.99)) {
                 const float m_new = fmaxf(m_run, mx);
-                const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
+                alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
                 m_run = m_new;
                 l_run *= alpha;
+            }
+            sub = kShift - (m_run == -INFINITY ? 0.0f : m_run);
+        };
+        auto scale = [&]() {                               // (once what refers to the maximum before is added)
+            if (__builtin_expect_with_probability(moves, 0, 0.99)) {
                 pin();
 #pragma unroll
                 for (int d = 0; d < 4; ++d) o[d] *= alpha;
                 pin();
             }
-            sub = kShift - (m_run == -INFINITY ? 0.0f : m_run);
         };
         f16x8 ph[2], pl[2];
         float p_even = 0.0f, p_sum = 0.0f;                 // (of the unit: one small weight at a time would be lost
@@ -369,12 +381,18 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
                 p_even = p;
             }
         };
-        auto hand_over = [&]() {
+        auto hand_over = [&](int buf) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                st.p[wave][2 * c][lane] = ph[c];
-                st.p[wave][2 * c + 1][lane] = pl[c];
+                st.p[buf][wave][2 * c][lane] = ph[c];
+                st.p[buf][wave][2 * c + 1][lane] = pl[c];
             }
+        };
+        auto take_over = [&](int buf) {
+            h0 = st.p[buf][wave ^ 2][0][lane];
+            l0 = st.p[buf][wave ^ 2][1][lane];
+            h1 = st.p[buf][wave ^ 2][2][lane];
+            l1 = st.p[buf][wave ^ 2][3][lane];
         };
         auto v_read = [&](int buf, int whose, int step, f16x8 (&v)[4]) {
 #pragma unroll
@@ -386,114 +404,114 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
                 v[d] = __builtin_bit_cast(f16x8, s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]});
             }
         };
-        auto add = [&](const f16x8 (&v)[4], f16x8 hi, f16x8 lo, auto beside) {
+        auto add = [&](const f16x8 (&v)[4], f16x8 hi, f16x8 lo) {
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], lo, o[d], 0, 0, 0);
-                beside(d);
-            }
+            for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], lo, o[d], 0, 0, 0);
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], hi, o[d], 0, 0, 0);
-                beside(4 + d);
-            }
+            for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d], hi, o[d], 0, 0, 0);
         };
-        auto nothing = [](int) {};
 
         {
             // (V's loads before K's, as in the loop: they are waited for in order)
             const Keys next = keys(wk.t0 + 1);
-            units(wk.t0, vs[0]);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) convert(c, vc[0], 0);
-            hold_unit(wk.t0 + 2);
-            load_values(wk.t0 + 2, vc[0], vs[0]);
-            scores(sc[0], ks[0], next.row, nothing);
             ks[1] = from_global<uint32_t>(next.scale);
+            units(wk.t0, vs[0]);
+            scores(sc[0], ks[0], next.row, std::false_type{}, [&](int i) {
+                if (i % 2 == 0 && i < 16) convert(i / 2, vc[0], 0);
+                if (i == 16) {
+                    hold_unit(wk.t0 + 2);
+                    load_values(wk.t0 + 2, vc[0], vs[0]);
+                }
+            });
         }
         if (masked(wk.t0)) mask(wk.t0, sc[0]);
-        post(sc[0]);
+        post(1, sc[0]);
         int t = wk.t0;
         lds_barrier();
-        meet(st.mx[0][wave ^ 2][nn]);
-        // Output products of unit t: the wave's own 32 rows, whose first 16 rows of V
-        // are read by now, then its partner's.  The last 16 rows' wait, read, for the
-        // next unit's beginning.  behind() runs among the first products, ahead() with
-        // the partner's maxima.
-        f16x8 v0[4], v1[4], h1, l1;
+        meet(st.mx[1][wave ^ 2][nn]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            h1[k] = l1[k] = (_Float16)0.0f;
+            h0[k] = l0[k] = h1[k] = l1[k] = (_Float16)0.0f;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) v1[d][k] = (_Float16)0.0f;
+            for (int d = 0; d < 4; ++d) v0[d][k] = v1[d][k] = (_Float16)0.0f;
         }
+        // Unit t's own rows' products, and all that its partner's need but the weights, which
+        // come behind the barrier: those products are left to the next unit, between the
+        // scores.  behind() runs among the first products, ahead() with the partner's maxima.
         auto output = [&](int buf, auto behind, auto ahead) __attribute__((always_inline)) {
-            hand_over();
-            v_read(buf, 0, 1, v1);
+            hand_over(buf);
+            scale();
             __builtin_amdgcn_sched_barrier(0);
             behind();
             __builtin_amdgcn_sched_barrier(0);
             lds_barrier();                                 // the partner's weights and maxima
-            const float other = st.mx[0][wave ^ 2][nn];
-            const f16x8 h0 = st.p[wave ^ 2][0][lane], l0 = st.p[wave ^ 2][1][lane];
-            h1 = st.p[wave ^ 2][2][lane];
-            l1 = st.p[wave ^ 2][3][lane];
-            v_read(buf, 1, 0, v0);
+            const float other = st.mx[buf][wave ^ 2][nn];
+            take_over(buf);
             __builtin_amdgcn_sched_barrier(0);
-            add(v1, ph[1], pl[1], nothing);
+            add(w1, ph[1], pl[1]);
             ahead(other);
             __builtin_amdgcn_sched_barrier(0);
-            v_read(buf, 1, 1, v1);
-            add(v0, h0, l0, nothing);
-            __builtin_amdgcn_sched_barrier(0);
         };
-        // A unit begins once its V is there and every wave is past the buffer that the next
-        // one's goes to, and with what the unit before left: eight products, beside which the
-        // next unit's V is converted.  (B: the unit's V buffer and place among the scores; units
-        // in pairs, so that what one leaves to the next stays where it is.)
+        // One barrier a unit: behind it a unit's V, weights and maxima are there, and every wave
+        // has read the V before, whose buffer the next one's goes to.  (B: the unit's V buffer and
+        // place among the scores; units in pairs, so that what one leaves to the next stays
+        // where it is.)
         auto go_on = [&](auto B) __attribute__((always_inline)) {
             constexpr int b = decltype(B)::value;
-            lds_barrier();
             const Keys next = keys(t + 2);
-            units(t + 1, vs[b ^ 1]);
-            add(v1, h1, l1, [&](int c) {
-                convert(c, vc[b ^ 1], b ^ 1);
-                __builtin_amdgcn_sched_barrier(0);
-            });
-            hold_unit(t + 3);
-            load_values(t + 3, vc[b ^ 1], vs[b ^ 1]);
-            move();
-            scores(sc[b ^ 1], ks[b ^ 1], next.row, [&](int i) {
-                if (i < 17) weight(i, sc[b]);
-                if (i == 17) v_read(b, 0, 0, v0);
-            });
             ks[b] = from_global<uint32_t>(next.scale);
+            units(t + 1, vs[b ^ 1]);
+            move();
+            scores(sc[b ^ 1], ks[b ^ 1], next.row, std::true_type{}, [&](int i) {
+                if (i % 2 == 0 && i < 34) weight(i / 2, sc[b]);
+                if (i % 4 == 1 && i < 32) convert(i / 4, vc[b ^ 1], b ^ 1);
+                if (i == 17) v_read(b, 1, 0, v0);
+                if (i == 21) v_read(b, 0, 0, w0);
+                if (i == 25) v_read(b, 0, 1, w1);
+                if (i == 33) v_read(b, 1, 1, v1);
+                if (i == 34) {
+                    hold_unit(t + 3);
+                    load_values(t + 3, vc[b ^ 1], vs[b ^ 1]);
+                }
+            });
             output(
                 b,
                 [&]() {
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0[d], pl[0], o[d], 0, 0, 0);
+                    for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w0[d], pl[0], o[d], 0, 0, 0);
                     asm volatile("" : "+v"(sc[b ^ 1]));    // in vector registers, where the weights want them
                     if (masked(t + 1)) {
                         asm volatile("");                  // a branch, not selects
                         mask(t + 1, sc[b ^ 1]);
                     }
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0[d], ph[0], o[d], 0, 0, 0);
-                    post(sc[b ^ 1]);
+                    for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(w0[d], ph[0], o[d], 0, 0, 0);
+                    post(b, sc[b ^ 1]);
                 },
                 meet);
         };
+        const bool whole = wk.t0 == 0 && wk.t1 == wk.tiles;
         auto finish = [&](auto B) __attribute__((always_inline)) {
             constexpr int b = decltype(B)::value;
-            lds_barrier();
-            add(v1, h1, l1, nothing);
             move();
+            v_read(b, 0, 0, w0);
+            v_read(b, 0, 1, w1);
 #pragma unroll
-            for (int k = 0; k < 17; ++k) weight(k, sc[b]);
-            v_read(b, 0, 0, v0);
-            output(b, [&]() { add(v0, ph[0], pl[0], nothing); }, [](float) {});
-            add(v1, h1, l1, nothing);
+            for (int i = 0; i < 17; ++i) {
+                if (i < 16) left_over(i);
+                weight(i, sc[b]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            v_read(b, 1, 0, v0);
+            v_read(b, 1, 1, v1);
+            output(b, [&]() { add(w0, ph[0], pl[0]); }, [](float) {});
+            if (whole) {                                   // the gates of the wave's rows 16 wave .. take V's place
+#pragma unroll 4
+                for (int r = 16 * wave; r < 16 * wave + 16; ++r)
+                    dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane, lds_address(&st.v[0][0][0]) + r * kHd * 4);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) left_over(i);
         };
 #pragma nounroll
         for (; t + 2 < wk.t1; ++t) {
@@ -517,8 +535,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         l_run = xor32_sum(l_run);
         if (lane < 32) st.mx[1][wave][nn] = l_run;
         if (half == 0 && lane < 32) st.mx[0][rg][nn] = m_run;
-        lds_barrier();                                     // V and the last maxima are read
-        float4* const os = reinterpret_cast<float4*>(&st.v[0][0][0]);
+        lds_barrier();                                     // the weights are read
+        float4* const os = st.q;
         put_rows(os, o, rg, half, lane);
         lds_barrier();
         const int row = 16 * wave + (lane & 15);           // a row's sum and maximum in lane row % 16
@@ -527,7 +545,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         auto gate_row = [&](int r) { return q_tile + (uint32_t)(from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane); };
         auto out_row = [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; };
         dma_wait();                                        // (the gates, which the wave itself has brought)
-        auto gate_of = [&](int k) { return st.q[(16 * wave + k) * (kHd / 4) + lane]; };
+        auto gate_of = [&](int k) { return reinterpret_cast<const float4*>(&st.v[0][0][0])[(16 * wave + k) * (kHd / 4) + lane]; };
         const bool look = leave_rows(os, l, st.mx[0][row >> 5][row & 31], whole, gate_of, to_part,
                                      part_ml + (size_t)2 * slot * kPagedTileRows, wave, lane, out_row);
         if (__builtin_expect(look || uniform(st.found), 0))
