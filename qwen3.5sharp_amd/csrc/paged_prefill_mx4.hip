@@ -31,7 +31,7 @@ struct Mx4Tile {
     uint8_t qscale[2][4][kWave];          // the first part's scales
     int found;                            // values that are not finite
 };
-static_assert(2 * 4 * kParts * 3 * kWave * sizeof(uint2) <= sizeof(Mx4Tile::v), "the parts' room");
+static_assert(2 * 4 * kParts * kWave * (sizeof(uint4) + sizeof(uint2)) <= sizeof(Mx4Tile::v), "the parts' room");
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
@@ -46,33 +46,31 @@ __device__ __forceinline__ f32x16 scaled_product32(u32x4 a, const uint32_t (&b)[
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, c, 4, 2, S, (int)sa, S, (int)sb);
 }
 
-// A block of q as parts of 6 bits, three 8-byte words each at to[word][lane]; returned is
-// the first part's scale, of which a later one's is 4 less than the one's before.  The
-// conversions are written out because their results come while they still read: the
-// compiler lets the two share registers.
-__device__ __forceinline__ uint32_t cut_block(float (&x)[kMxBlock], uint2* to) {
+// A block of q, dims 2 i and 2 i + 1 in even[i] and odd[i], as parts of 6 bits, 16 and 8
+// bytes each at to[16-byte word][lane] and behind; returned is the first part's scale, of
+// which a later one's is 4 less than the one's before.  The conversions are written out
+// because their results come while they still read: the compiler lets the two share
+// registers.
+__device__ __forceinline__ uint32_t cut_block(f32x16 even, f32x16 odd, uint4* to, uint2* to2) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < kMxBlock; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int i = 0; i < kMxBlock / 2; ++i) m = max(m, max(__float_as_uint(even[i]) & 0x7fffffffu, __float_as_uint(odd[i]) & 0x7fffffffu));
     const uint32_t e = max(m >> 23, 40u);                  // every |x| is below 2^{e - 126}, 8 times 2^{e - 129}
 #pragma unroll
     for (int k = 0; k < kParts; ++k) {
         const float unit = __uint_as_float((e - 2 - 4 * k) << 23);
-        f32x16 even, odd;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            even[i] = x[2 * i];
-            odd[i] = x[2 * i + 1];
-        }
         u32x6 part;
         asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3" : "=&v"(part) : "v"(even), "v"(odd), "v"(unit));
-#pragma unroll
-        for (int w = 0; w < 3; ++w) to[(3 * k + w) * kWave] = make_uint2(part[2 * w], part[2 * w + 1]);
+        to[k * kWave] = make_uint4(part[0], part[1], part[2], part[3]);
+        to2[k * kWave] = make_uint2(part[4], part[5]);
         if (k + 1 == kParts) break;
         f32x32 back;
         asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2" : "=&v"(back) : "v"(part), "v"(unit));
 #pragma unroll
-        for (int i = 0; i < kMxBlock; ++i) x[i] -= back[i];
+        for (int i = 0; i < kMxBlock / 2; ++i) {
+            even[i] -= back[2 * i];
+            odd[i] -= back[2 * i + 1];
+        }
     }
     return m >= 0x7f800000u ? kMxNan : e - 2;
 }
@@ -138,7 +136,6 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         auto hold_unit = [&](int t) {
             if (__builtin_expect(uniform((group(t, 1) >> pv.page_shift) - held) >= kWave, 0)) hold(uniform(group(t, 0) >> pv.page_shift));
         };
-        hold(uniform(group(wk.t0, 0) >> pv.page_shift));
         // K: lane (row nn, h) takes blocks 4 h .. of its row; V: 16-byte pieces of two rows,
         // 8 i + lane / 8, block lane % 8.
         u32x4 kc[4], vc[2][2];
@@ -167,10 +164,11 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
             }
         };
 
-        // q rows, 16-byte chunks permuted by row (chunk ^ row % 32).
+        // q rows, which have the longest way, 16-byte chunks permuted by row (chunk ^ row % 32).
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
             dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 16 * (lane ^ (r & 31)), lds_address(&st.q[0]) + r * kHd * 4);
+        hold(uniform(group(wk.t0, 0) >> pv.page_shift));
         {
             const Keys k = keys(wk.t0);
 #pragma unroll
@@ -199,30 +197,31 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
                 }
         }
         lds_barrier();
-        uint2* const parts = reinterpret_cast<uint2*>(&st.v[0][0][0]) + rg * (4 * kParts * 3 * kWave) + lane;
+        uint4* const parts = reinterpret_cast<uint4*>(&st.v[0][0][0]) + rg * (4 * kParts * kWave) + lane;
+        uint2* const parts2 = reinterpret_cast<uint2*>(reinterpret_cast<uint4*>(&st.v[0][0][0]) + 2 * 4 * kParts * kWave) +
+                              rg * (4 * kParts * kWave) + lane;
 #pragma nounroll
         for (int s = 2 * half; s < 2 * half + 2; ++s) {
             const float4* const at = st.q + (32 * rg + nn) * (kHd / 4);
-            float x[kMxBlock];
+            f32x16 even, odd;
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 const float4 v = at[(8 * (4 * h + s) + c) ^ nn];
-                x[4 * c] = v.x; x[4 * c + 1] = v.y; x[4 * c + 2] = v.z; x[4 * c + 3] = v.w;
+                even[2 * c] = v.x; odd[2 * c] = v.y; even[2 * c + 1] = v.z; odd[2 * c + 1] = v.w;
             }
-            st.qscale[rg][s][lane] = (uint8_t)cut_block(x, parts + s * (kParts * 3 * kWave));
+            st.qscale[rg][s][lane] = (uint8_t)cut_block(even, odd, parts + s * (kParts * kWave), parts2 + s * (kParts * kWave));
         }
         lds_barrier();
         uint32_t q[4][kParts][6], qs[kParts];
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int k = 0; k < kParts; ++k)
-#pragma unroll
-                for (int w = 0; w < 3; ++w) {
-                    const uint2 v = parts[((s * kParts + k) * 3 + w) * kWave];
-                    q[s][k][2 * w] = v.x;
-                    q[s][k][2 * w + 1] = v.y;
-                }
+            for (int k = 0; k < kParts; ++k) {
+                const uint4 x = parts[(s * kParts + k) * kWave];
+                const uint2 y = parts2[(s * kParts + k) * kWave];
+                q[s][k][0] = x.x; q[s][k][1] = x.y; q[s][k][2] = x.z; q[s][k][3] = x.w;
+                q[s][k][4] = y.x; q[s][k][5] = y.y;
+            }
         qs[0] = st.qscale[rg][0][lane] | st.qscale[rg][1][lane] << 8 | st.qscale[rg][2][lane] << 16 | (uint32_t)st.qscale[rg][3][lane] << 24;
 #pragma unroll
         for (int k = 1; k < kParts; ++k) qs[k] = qs[k - 1] - 0x04040404u;      // (no borrow: a scale is 38 or more)
