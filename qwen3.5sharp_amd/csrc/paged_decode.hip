@@ -531,7 +531,8 @@ int decode_workgroups(const q35m_ctx* c) { return c->n_cu; }
 }  // namespace
 
 size_t paged_decode_work_bytes(const q35m_ctx* c) {
-    return (size_t)2 * decode_workgroups(c) * kPagedDecodeHeads * (kHd + 2) * sizeof(float);
+    // (two a CU over a cache in 4 bits)
+    return (size_t)2 * 2 * decode_workgroups(c) * kPagedDecodeHeads * (kHd + 2) * sizeof(float);
 }
 
 hipError_t launch_paged_decode(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, const float* k,

@@ -25,7 +25,11 @@ constexpr int kTileRows = 32;                    // of a wave
 constexpr int kUnitRows4 = 4 * kTileRows;
 constexpr int kDigits = 6;
 constexpr int kDigitWords = 50;                  // 48 words of 6-bit codes, and 2 for the banks
-constexpr float kPShift4 = 15.0f;                // P is e^{s - m} 2^15 (see paged_decode.hip)
+// P is e^{s - m} 2^kShift4, and m is behind the largest score by up to kMove4 (in log2): the
+// output is scaled (128 instructions of the tile's 370) only when a score passes m by that.
+// Weights are below 2^15.9, in fp16's range, and their low halves in steps of 2^-30 of the
+// largest weight or finer.
+constexpr float kShift4 = 6.0f, kMove4 = 9.9f;
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -67,24 +71,24 @@ struct Tile4 {
                     for (int w = 0; w < 6; ++w) q[a][s][t][w] = digit < kDigits ? codes[head][d][12 * g + 6 * t + w] : 0u;
             }
     }
-    // codes: the 16 rows' first byte in the page; in: their first row's place there.
-    __device__ __forceinline__ void load_k(const uint8_t* page, const PagedView& pv, int in, int kb, int lane) {
+    // 16 rows, whose codes begin at `codes` and scales at `scales` (the same for all lanes).
+    __device__ __forceinline__ void load_k(const uint8_t* codes, const uint8_t* scales, int kb, int lane) {
         const int n = lane & 15, g = lane >> 4;
-        const uint8_t* const at = page + (uint32_t)(in + n) * kMxCodes + 32 * g;
+        const uint32_t at = n * kMxCodes + 32 * g, sc = n * kMxBlocks + 2 * g;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) kc[kb][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at + 16 * t));
-        ks[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(page + mx_key_scale(pv, in + n) + 2 * g));
+        for (int t = 0; t < 2; ++t) kc[kb][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(codes + at + 16 * t));
+        ks[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(scales + sc));
     }
-    __device__ __forceinline__ void load_v(const uint8_t* page, const PagedView& pv, int in, int kb, int lane) {
+    __device__ __forceinline__ void load_v(const uint8_t* codes, const uint8_t* scales, int kb, int lane) {
         const int n = lane & 15, g = lane >> 4;
-        const uint8_t* const at = page + (uint32_t)(in + 4 * g) * kMxCodes + 8 * n;
+        const uint32_t at = 4 * g * kMxCodes + 8 * n, sc = 16 * (n >> 1) + 4 * g;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(at + i * kMxCodes));
+            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(codes + at + i * kMxCodes));
             vc[4 * kb + i] = make_uint2(x[0], x[1]);
         }
-        vs[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(page + mx_value_scale(pv, in, n >> 1) + 4 * g));
+        vs[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(scales + sc));
     }
     // Row `at` of the tile (none if negative) is the new one (its codes and scales at kn, vn);
     // rows from `rows` on are masked: what they hold must not be NaN.
@@ -178,6 +182,18 @@ struct Tile4 {
             byte(std::integral_constant<int, 3>{});
         }
     }
+    // The output stays in accumulation registers: without a use there the compiler moves all
+    // of it back and forth for the rare scaling.
+    __device__ __forceinline__ void pin() {
+        asm volatile("" : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]), "+a"(o[6]), "+a"(o[7]));
+        asm volatile("" : "+a"(o[8]), "+a"(o[9]), "+a"(o[10]), "+a"(o[11]), "+a"(o[12]), "+a"(o[13]), "+a"(o[14]), "+a"(o[15]));
+    }
+    __device__ __forceinline__ void scale(float by) {
+        pin();
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[x] *= by;
+        pin();
+    }
     // The lane's output values, 4 consecutive dims at a time.
     template <typename F>
     __device__ __forceinline__ void each4(int g, F f) const {
@@ -228,7 +244,7 @@ __device__ __forceinline__ void put_digits(uint32_t (*codes)[kDigitWords], uint8
 }
 
 template <int NQ>
-__global__ __launch_bounds__(NT, 1) void paged_decode_mx4(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
+__global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
                                                           const float* __restrict__ knew, const float* __restrict__ vnew,
                                                           const float* __restrict__ q_norm,
                                                           const float* __restrict__ k_norm, float* __restrict__ out,
@@ -270,21 +286,27 @@ __global__ __launch_bounds__(NT, 1) void paged_decode_mx4(PagedView pv, PagedBat
         Tile4<NQ> tl;
 #pragma unroll
         for (int x = 0; x < 16; ++x) tl.o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-        int pg[2];
-        auto pages = [&](int base) {     // of the 16-row groups at base (the last one past the end)
+        size_t pg[2];
+        auto pages = [&](int base) {     // where the 16-row groups at base lie (the last one past the end)
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
-                pg[kb] = page_of(table, min(base + 16 * kb, last16) >> pv.page_shift, pv.max_pages, pv.n_pages);
+                pg[kb] = mx_page(pv, page_of(table, min(base + 16 * kb, last16) >> pv.page_shift, pv.max_pages, pv.n_pages), kvh);
         };
-        auto load_k = [&](int base, const int (&p)[2]) {
+        auto load_k = [&](int base, const size_t (&p)[2]) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                tl.load_k((const uint8_t*)pv.k + mx_page(pv, p[kb], kvh), pv, min(base + 16 * kb, last16) & in_page, kb, lane);
+            for (int kb = 0; kb < 2; ++kb) {
+                const int in = min(base + 16 * kb, last16) & in_page;
+                const uint8_t* const page = (const uint8_t*)pv.k + p[kb];
+                tl.load_k(page + (uint32_t)in * kMxCodes, page + mx_key_scale(pv, in), kb, lane);
+            }
         };
-        auto load_v = [&](int base, const int (&p)[2]) {
+        auto load_v = [&](int base, const size_t (&p)[2]) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                tl.load_v((const uint8_t*)pv.v + mx_page(pv, p[kb], kvh), pv, min(base + 16 * kb, last16) & in_page, kb, lane);
+            for (int kb = 0; kb < 2; ++kb) {
+                const int in = min(base + 16 * kb, last16) & in_page;
+                const uint8_t* const page = (const uint8_t*)pv.v + p[kb];
+                tl.load_v(page + (uint32_t)in * kMxCodes, page + mx_value_scale(pv, in, 0), kb, lane);
+            }
         };
         // What q's rows and the new row are made of is asked for before K and V, so
         // that they are formed while those are on their way; a wave forms every
@@ -367,19 +389,22 @@ __global__ __launch_bounds__(NT, 1) void paged_decode_mx4(PagedView pv, PagedBat
                 s[j] = base + tl.row_of(j, g) < rows ? s[j] : -INFINITY;
                 mx = fmaxf(mx, s[j]);
             }
-            mx = fmaxf(m_run, xor16_max(xor32_max(mx)));
-            const float mu = mx == -INFINITY ? 0.0f : mx;
-            const float alpha = __builtin_amdgcn_exp2f(m_run - mu);
-            m_run = mx;
+            mx = xor16_max(xor32_max(mx));
+            if (__builtin_expect(__any(mx > m_run + kMove4), 0)) {         // (m_run is -inf at first)
+                const float m_new = fmaxf(m_run, mx);
+                const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
+                m_run = m_new;
+                l_run *= alpha;
+                tl.scale(alpha);
+            }
+            const float sub = kShift4 - (m_run == -INFINITY ? 0.0f : m_run);
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                s[j] = __builtin_amdgcn_exp2f(s[j] - mu + kPShift4);
+                s[j] = __builtin_amdgcn_exp2f(s[j] + sub);
                 sum += s[j];
             }
-            l_run = l_run * alpha + sum;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) tl.o[x] *= alpha;
+            l_run += sum;
             tl.pv(s, lane);
             if (more) load_v(next, pg);
         }
@@ -435,13 +460,12 @@ __global__ __launch_bounds__(NT, 1) void paged_decode_mx4(PagedView pv, PagedBat
 
 }  // namespace
 
-// One workgroup a CU.
 hipError_t launch_paged_decode_mx4(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, const float* k,
                                    const float* v, float* out) {
     q35m_ctx* c = p->ctx;
     const int per_kv = c->d.nh / c->d.nkv;
     const int hg = per_kv <= 16 ? per_kv : per_kv % 16 == 0 ? 16 : 8;
-    const int ng = per_kv / hg, nwg = c->n_cu;
+    const int ng = per_kv / hg, nwg = c->n_cu * (hg <= 8 ? 2 : 1);
     float* part_o = p->work;
     float* part_ml = part_o + (size_t)2 * nwg * kPagedDecodeHeads * kHd;
     const PagedView pv = p->view(layer);
