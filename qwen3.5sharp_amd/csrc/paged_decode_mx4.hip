@@ -48,10 +48,12 @@ struct Tile4 {
     static constexpr int kHeads = 4 * NQ;
     uint32_t q[NQ][2][2][6];   // [quad][digits 0 .. 3, 4 ..][t]: head 4 quad + n % 4, digit n / 4 of these, dims 64 g + 32 t ..
     uint32_t qs[NQ][2];        // their scales, byte t
-    u32x4 kc[2][2];            // row 16 kb + n, dims 64 g + 32 t ..
-    uint32_t ks[2];            // its scales of blocks 2 g and 2 g + 1
-    uint2 vc[8];               // row 16 (j / 4) + 4 g + j % 4, dims 16 n ..
-    uint32_t vs[2];            // scales of rows 16 kb + 4 g .., block n / 2
+    struct Rows {
+        u32x4 kc[2][2];        // row 16 kb + n, dims 64 g + 32 t ..
+        uint32_t ks[2];        // its scales of blocks 4 (g / 2) ..
+        uint2 vc[8];           // row 16 (j / 4) + 4 g + j % 4, dims 16 n ..
+        uint32_t vs[2];        // scales of rows 16 kb + 4 g .., block n / 2
+    };
     f32x4 o[16];               // dims 64 g + 16 i + x at [x][i]
 
     __device__ __forceinline__ void load_q(const uint32_t (*codes)[kDigits][kDigitWords], const uint8_t (*scales)[kDigits][kMxBlocks],
@@ -71,60 +73,63 @@ struct Tile4 {
                     for (int w = 0; w < 6; ++w) q[a][s][t][w] = digit < kDigits ? codes[head][d][12 * g + 6 * t + w] : 0u;
             }
     }
+    // (K without the hint that it is read once: an instruction takes half of each line, 44.2 us
+    // against 47.9 for 64 sequences of up to 4000 rows.)
     // 16 rows, whose codes begin at `codes` and scales at `scales` (the same for all lanes).
-    __device__ __forceinline__ void load_k(const uint8_t* codes, const uint8_t* scales, int kb, int lane) {
+    static __device__ __forceinline__ void load_k(Rows& r, const uint8_t* codes, const uint8_t* scales, int kb, int lane) {
         const int n = lane & 15, g = lane >> 4;
-        const uint32_t at = n * kMxCodes + 32 * g, sc = n * kMxBlocks + 2 * g;
+        const uint32_t at = n * kMxCodes + 32 * g, sc = n * kMxBlocks + 4 * (g >> 1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) kc[kb][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(codes + at + 16 * t));
-        ks[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(scales + sc));
+        for (int t = 0; t < 2; ++t) r.kc[kb][t] = *reinterpret_cast<const u32x4*>(codes + at + 16 * t);
+        r.ks[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(scales + sc));
     }
-    __device__ __forceinline__ void load_v(const uint8_t* codes, const uint8_t* scales, int kb, int lane) {
+    static __device__ __forceinline__ void load_v(Rows& r, const uint8_t* codes, const uint8_t* scales, int kb, int lane) {
         const int n = lane & 15, g = lane >> 4;
         const uint32_t at = 4 * g * kMxCodes + 8 * n, sc = 16 * (n >> 1) + 4 * g;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
             const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(codes + at + i * kMxCodes));
-            vc[4 * kb + i] = make_uint2(x[0], x[1]);
+            r.vc[4 * kb + i] = make_uint2(x[0], x[1]);
         }
-        vs[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(scales + sc));
+        r.vs[kb] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(scales + sc));
     }
     // Row `at` of the tile (none if negative) is the new one (its codes and scales at kn, vn);
     // rows from `rows` on are masked: what they hold must not be NaN.
-    __device__ __forceinline__ void fix(const uint8_t* kn, const uint8_t* vn, int at, int rows, int lane) {
+    static __device__ __forceinline__ void fix(Rows& x, const uint8_t* kn, const uint8_t* vn, int at, int rows, int lane) {
         const int n = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             if (16 * kb + n == at) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) kc[kb][t] = *reinterpret_cast<const u32x4*>(kn + 32 * g + 16 * t);
-                ks[kb] = *reinterpret_cast<const uint16_t*>(kn + kMxCodes + 2 * g);
+                for (int t = 0; t < 2; ++t) x.kc[kb][t] = *reinterpret_cast<const u32x4*>(kn + 32 * g + 16 * t);
+                x.ks[kb] = *reinterpret_cast<const uint32_t*>(kn + kMxCodes + 4 * (g >> 1));
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 16 * kb + 4 * g + i;
                 const uint32_t keep = ~(0xffu << 8 * i);
                 if (r == at) {
-                    vc[4 * kb + i] = *reinterpret_cast<const uint2*>(vn + 8 * n);
-                    vs[kb] = (vs[kb] & keep) | (uint32_t)vn[kMxCodes + (n >> 1)] << 8 * i;
+                    x.vc[4 * kb + i] = *reinterpret_cast<const uint2*>(vn + 8 * n);
+                    x.vs[kb] = (x.vs[kb] & keep) | (uint32_t)vn[kMxCodes + (n >> 1)] << 8 * i;
                 }
-                if (r >= rows) vs[kb] = (vs[kb] & keep) | 127u << 8 * i;
+                if (r >= rows) x.vs[kb] = (x.vs[kb] & keep) | 127u << 8 * i;
             }
         }
     }
     // Scores of rows row_of(j, g) and the lane's head, n % kHeads.
-    __device__ __forceinline__ void scores(float (&s)[8], int lane) const {
+    __device__ __forceinline__ void scores(const Rows& r, float (&s)[8], int lane) const {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             f32x4 c[NQ];
+            const uint32_t ks = r.ks[kb] >> (lane & 16);   // blocks 2 g and 2 g + 1
 #pragma unroll
             for (int a = 0; a < NQ; ++a) {
                 c[a] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int d = 1; d >= 0; --d) {             // the last digits' products first
-                    c[a] = scaled_product<0>(kc[kb][0], q[a][d][0], c[a], ks[kb], qs[a][d]);
-                    c[a] = scaled_product<1>(kc[kb][1], q[a][d][1], c[a], ks[kb], qs[a][d]);
+                    c[a] = scaled_product<0>(r.kc[kb][0], q[a][d][0], c[a], ks, qs[a][d]);
+                    c[a] = scaled_product<1>(r.kc[kb][1], q[a][d][1], c[a], ks, qs[a][d]);
                 }
             }
 #pragma unroll
@@ -144,7 +149,7 @@ struct Tile4 {
         }
     }
     static __device__ __forceinline__ int row_of(int j, int g) { return 16 * (j >> 2) + 4 * g + (j & 3); }
-    __device__ __forceinline__ void pv(const float (&p)[8], int lane) {
+    __device__ __forceinline__ void pv(const Rows& r, const float (&p)[8], int lane) {
         f16x8 ph, pl;
         split16(p, ph, pl);
         if constexpr (NQ < 4) {                            // columns kHeads .. 2 kHeads - 1 are the low parts
@@ -156,7 +161,7 @@ struct Tile4 {
         }
         float unit[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) unit[j] = __uint_as_float((vs[j >> 2] >> 8 * (j & 3) & 0xffu) << 23);
+        for (int j = 0; j < 8; ++j) unit[j] = __uint_as_float((r.vs[j >> 2] >> 8 * (j & 3) & 0xffu) << 23);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             auto byte = [&](auto B) {
@@ -164,7 +169,7 @@ struct Tile4 {
                 uint32_t x[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    x[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w ? vc[j].y : vc[j].x, unit[j], b));
+                    x[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w ? r.vc[j].y : r.vc[j].x, unit[j], b));
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t sel = e ? 0x07060302u : 0x05040100u;
@@ -251,6 +256,7 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
                                                           float* __restrict__ part_o, float* __restrict__ part_ml, int hg,
                                                           int ng, int unit, float eps) {
     constexpr int R = kTileRows, H = 4 * NQ, HW = H / 4;   // HW: heads a wave forms and joins
+    constexpr int D = NQ == 4 ? 2 : 1;                     // tiles a wave asks for ahead
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
@@ -286,33 +292,50 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
         Tile4<NQ> tl;
 #pragma unroll
         for (int x = 0; x < 16; ++x) tl.o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-        size_t pg[2];
-        auto pages = [&](int base) {     // where the 16-row groups at base lie (the last one past the end)
+        // Tiles of the wave: k at first + 4 R k.  All but the last are cached rows alone; the
+        // last one may hold the new row, and rows past it.
+        const int tiles_mine = first < stop ? (stop - first + 4 * R - 1) / (4 * R) : 0;
+        const bool ends = tiles_mine && first + (tiles_mine - 1) * 4 * R + R > pos;
+        typename Tile4<NQ>::Rows held[D];                  // tiles whose rows are on their way
+        // Rows of tile k (past the wave's last one that again, which costs no traffic: loads that
+        // are sometimes left out would all be waited for); their pages are asked for a
+        // tile before, by scalar loads, which the vector ones are not waited for with.
+        typedef const __attribute__((address_space(4))) int const_int;
+        const_int* const ids = (const_int*)(uintptr_t)table;
+        int id[2];
+        auto group = [&](int k, int kb) { return min(first + 4 * R * min(k, tiles_mine - 1) + 16 * kb, last16); };
+        auto ask = [&](int k) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-                pg[kb] = mx_page(pv, page_of(table, min(base + 16 * kb, last16) >> pv.page_shift, pv.max_pages, pv.n_pages), kvh);
+            for (int kb = 0; kb < 2; ++kb) id[kb] = ids[group(k, kb) >> pv.page_shift];
         };
-        auto load_k = [&](int base, const size_t (&p)[2]) {
+        size_t at[2];
+        int in[2];
+        auto place = [&](int k) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                const int in = min(base + 16 * kb, last16) & in_page;
-                const uint8_t* const page = (const uint8_t*)pv.k + p[kb];
-                tl.load_k(page + (uint32_t)in * kMxCodes, page + mx_key_scale(pv, in), kb, lane);
+                at[kb] = mx_page(pv, id[kb] < pv.n_pages ? id[kb] : -1, kvh);
+                in[kb] = group(k, kb) & in_page;
             }
         };
-        auto load_v = [&](int base, const size_t (&p)[2]) {
+        auto load_k = [&](typename Tile4<NQ>::Rows& r) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                const int in = min(base + 16 * kb, last16) & in_page;
-                const uint8_t* const page = (const uint8_t*)pv.v + p[kb];
-                tl.load_v(page + (uint32_t)in * kMxCodes, page + mx_value_scale(pv, in, 0), kb, lane);
+                const uint8_t* const page = (const uint8_t*)pv.k + at[kb];
+                Tile4<NQ>::load_k(r, page + (uint32_t)in[kb] * kMxCodes, page + mx_key_scale(pv, in[kb]), kb, lane);
+            }
+        };
+        auto load_v = [&](typename Tile4<NQ>::Rows& r) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const uint8_t* const page = (const uint8_t*)pv.v + at[kb];
+                Tile4<NQ>::load_v(r, page + (uint32_t)in[kb] * kMxCodes, page + mx_value_scale(pv, in[kb], 0), kb, lane);
             }
         };
         // What q's rows and the new row are made of is asked for before K and V, so
         // that they are formed while those are on their way; a wave forms every
         // fourth q row, for all.
         const bool has_new = first <= pos / R * R && pos / R * R < stop && (pos / R * R - first) % (4 * R) == 0;
-        if (first < stop) pages(first);
+        if (tiles_mine) ask(0);
         float4 xq[HW], xk{}, xv{};
         const float* const q_rows = q_gate + ((size_t)i * nh + y * hg) * 2 * kHd + 4 * lane;
 #pragma unroll
@@ -330,9 +353,14 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
             sn[k] = pv.rope[(size_t)pos * kRopeDim + kRopeHalf + 4 * (lane & 7) + k];
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (first < stop) {
-            load_k(first, pg);
-            load_v(first, pg);
+        if (tiles_mine) {
+#pragma unroll
+            for (int k = 0; k < D; ++k) {
+                place(k);
+                ask(k + 1);
+                load_k(held[k]);
+                load_v(held[k]);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);
 
@@ -375,18 +403,19 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
         tl.load_q(qcodes, qscales, hg, lane);
 
         float m_run = -INFINITY, l_run = 0.0f;
-        for (int base = first; base < stop; base += 4 * R) {
-            const int next = base + 4 * R;
-            const bool more = next < stop;
-            if (more) pages(next);
-            if (base + R > pos) tl.fix(newrow[wave][0], newrow[wave][1], pos - base, rows - base, lane);
+        // Tile k, whose rows are r; the ones of tile k + D take their place if `more`.
+        auto tile = [&](int k, typename Tile4<NQ>::Rows& r, auto more, int visible) __attribute__((always_inline)) {
+            if (decltype(more)::value) {
+                place(k + D);
+                ask(k + D + 1);
+            }
             float s[8];
-            tl.scores(s, lane);
-            if (more) load_k(next, pg);
+            tl.scores(r, s, lane);
+            if (decltype(more)::value) load_k(r);
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                s[j] = base + tl.row_of(j, g) < rows ? s[j] : -INFINITY;
+                if (!decltype(more)::value) s[j] = tl.row_of(j, g) < visible ? s[j] : -INFINITY;
                 mx = fmaxf(mx, s[j]);
             }
             mx = xor16_max(xor32_max(mx));
@@ -405,8 +434,27 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
                 sum += s[j];
             }
             l_run += sum;
-            tl.pv(s, lane);
-            if (more) load_v(next, pg);
+            tl.pv(r, s, lane);
+            if (decltype(more)::value) load_v(r);
+        };
+        const int plain = tiles_mine - (ends ? 1 : 0);
+        int k = 0;
+#pragma nounroll
+        for (; k + D <= plain; k += D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) tile(k + d, held[d], std::true_type{}, 0);
+        }
+        auto last = [&](typename Tile4<NQ>::Rows& r) __attribute__((always_inline)) {
+            const int base = first + 4 * R * k;
+            Tile4<NQ>::fix(r, newrow[wave][0], newrow[wave][1], pos - base, rows - base, lane);
+            tile(k, r, std::false_type{}, rows - base);
+        };
+        if (D == 2 && k < plain) {
+            tile(k, held[0], std::true_type{}, 0);
+            ++k;
+            if (ends) last(held[D - 1]);
+        } else if (ends) {
+            last(held[0]);
         }
 
         // The four waves of the segment join.

@@ -63,8 +63,9 @@ __device__ __forceinline__ size_t row_offset(const PagedView& pv, int page, int 
 // together.
 struct Mx4 {};
 constexpr uint32_t kMxNan = 255;
+// (A pool of 2^32 pages times heads, of 2 KiB at least, would not fit the device.)
 __device__ __forceinline__ size_t mx_page(const PagedView& pv, int page, int kvh) {     // its first byte
-    return ((size_t)max(page, 0) * pv.nkv + kvh) * ((size_t)kMxRow << pv.page_shift);
+    return (size_t)((uint32_t)max(page, 0) * (uint32_t)pv.nkv + (uint32_t)kvh) * ((uint32_t)kMxRow << pv.page_shift);
 }
 __device__ __forceinline__ uint32_t mx_key_scale(const PagedView& pv, int in) {         // of row `in` of the page
     return ((uint32_t)kMxCodes << pv.page_shift) + (uint32_t)in * kMxBlocks;
