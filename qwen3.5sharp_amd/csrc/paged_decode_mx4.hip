@@ -268,10 +268,11 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
     __shared__ __align__(16) uint32_t qcodes[H][kDigits][kDigitWords];
     __shared__ __align__(8) uint8_t qscales[H][kDigits][kMxBlocks];
 
-    float4 qw = *reinterpret_cast<const float4*>(q_norm + 4 * lane);
-    const float4 kw = *reinterpret_cast<const float4*>(k_norm + 4 * lane);
-    qw = make_float4(1.0f + qw.x, 1.0f + qw.y, 1.0f + qw.z, 1.0f + qw.w);
+    __shared__ __align__(16) float norms[2][kHd];          // 1 + q's weights, k's
+    norms[0][tid] = 1.0f + q_norm[tid];
+    norms[1][tid] = k_norm[tid];
     const Units un = units_of(pv, b, groups, unit, lane);
+    lds_barrier();
     const int per = (un.total + (int)gridDim.x - 1) / (int)gridDim.x;
     int u = blockIdx.x * per;
     const int u_end = min(u + per, un.total);
@@ -303,7 +304,7 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
         typedef const __attribute__((address_space(4))) int const_int;
         const_int* const ids = (const_int*)(uintptr_t)table;
         int id[2];
-        auto group = [&](int k, int kb) { return min(first + 4 * R * min(k, tiles_mine - 1) + 16 * kb, last16); };
+        auto group = [&](int k, int kb) { return min(first + 4 * R * min(k, max(tiles_mine, 1) - 1) + 16 * kb, last16); };
         auto ask = [&](int k) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) id[kb] = ids[group(k, kb) >> pv.page_shift];
@@ -335,17 +336,20 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
         // that they are formed while those are on their way; a wave forms every
         // fourth q row, for all.
         const bool has_new = first <= pos / R * R && pos / R * R < stop && (pos / R * R - first) % (4 * R) == 0;
-        if (tiles_mine) ask(0);
-        float4 xq[HW], xk{}, xv{};
+        // (Asked for by all waves, needed or not: a load that some path leaves out is waited for
+        // with those behind it.)
+        ask(0);
+        float4 xq[HW], xk, xv;
         const float* const q_rows = q_gate + ((size_t)i * nh + y * hg) * 2 * kHd + 4 * lane;
 #pragma unroll
         for (int k = 0; k < HW; ++k)
-            if (wave + 4 * k < hg) xq[k] = *reinterpret_cast<const float4*>(q_rows + (size_t)(wave + 4 * k) * 2 * kHd);
-        if (has_new) {
-            const size_t at = ((size_t)i * pv.nkv + kvh) * kHd + 4 * lane;
-            xk = *reinterpret_cast<const float4*>(knew + at);
-            xv = *reinterpret_cast<const float4*>(vnew + at);
+            xq[k] = *reinterpret_cast<const float4*>(q_rows + (size_t)min(wave + 4 * k, hg - 1) * 2 * kHd);
+        {
+            const size_t from = ((size_t)i * pv.nkv + kvh) * kHd + 4 * lane;
+            xk = *reinterpret_cast<const float4*>(knew + from);
+            xv = *reinterpret_cast<const float4*>(vnew + from);
         }
+        const int id_new = ids[pos >> pv.page_shift], len = ((const_int*)(uintptr_t)pv.lens)[seq];
         double cs[4], sn[4];                     // the rotation of dims 4 (lane % 8) ..
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -353,18 +357,17 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
             sn[k] = pv.rope[(size_t)pos * kRopeDim + kRopeHalf + 4 * (lane & 7) + k];
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (tiles_mine) {
 #pragma unroll
-            for (int k = 0; k < D; ++k) {
-                place(k);
-                ask(k + 1);
-                load_k(held[k]);
-                load_v(held[k]);
-            }
+        for (int k = 0; k < D; ++k) {
+            place(k);
+            ask(k + 1);
+            load_k(held[k]);
+            load_v(held[k]);
         }
         __builtin_amdgcn_sched_barrier(0);
 
         // q: the rotation, the norm, the scale 1/16 (and log2 e, for exp2).
+        const float4 qw = reinterpret_cast<const float4*>(norms[0])[lane];
 #pragma unroll
         for (int k = 0; k < HW; ++k) {
             const int r = wave + 4 * k;
@@ -384,7 +387,7 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
         // The wave that holds the new row makes it (every head group needs it;
         // one writes it to the page, and none reads it from there).
         if (has_new) {
-            const MxLane yk = mx_round(paged_key_row(xk, cs, sn, kw, lane, (double)eps)), yv = mx_round(xv);
+            const MxLane yk = mx_round(paged_key_row(xk, cs, sn, reinterpret_cast<const float4*>(norms[1])[lane], lane, (double)eps)), yv = mx_round(xv);
             uint8_t* const kn = newrow[wave][0];
             uint8_t* const vn = newrow[wave][1];
             reinterpret_cast<uint16_t*>(kn)[lane] = (uint16_t)yk.codes;
@@ -393,8 +396,8 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
                 kn[kMxCodes + (lane >> 3)] = (uint8_t)yk.scale;
                 vn[kMxCodes + (lane >> 3)] = (uint8_t)yv.scale;
             }
-            const int pnew = page_of(table, pos >> pv.page_shift, pv.max_pages, pv.n_pages);
-            if (y % ng == 0 && pnew >= 0 && pv.lens[seq] < pv.max_rows) {
+            const int pnew = id_new < pv.n_pages ? id_new : -1;
+            if (y % ng == 0 && pnew >= 0 && len < pv.max_rows) {
                 mx_put_key((uint8_t*)pv.k + mx_page(pv, pnew, kvh), pv, pos & in_page, yk, lane);
                 mx_put_value((uint8_t*)pv.v + mx_page(pv, pnew, kvh), pv, pos & in_page, yv, lane);
             }
