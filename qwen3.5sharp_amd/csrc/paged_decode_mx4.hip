@@ -370,8 +370,7 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
         const float4 qw = reinterpret_cast<const float4*>(norms[0])[lane];
 #pragma unroll
         for (int k = 0; k < HW; ++k) {
-            const int r = wave + 4 * k;
-            if (r >= hg) break;
+            const int r = wave + 4 * k;                    // (rows from hg on: the last one again)
             float x[4] = {xq[k].x, xq[k].y, xq[k].z, xq[k].w}, ss = 0.0f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
