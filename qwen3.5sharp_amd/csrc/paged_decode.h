@@ -9,6 +9,20 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Sums over lanes 0 .. l, by moves within rows of 16 lanes and then of rows' last values.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int scan_step(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = scan_step<0x111, 0xf>(v);          // row_shr 1, 2, 4, 8
+    v = scan_step<0x112, 0xf>(v);
+    v = scan_step<0x114, 0xf>(v);
+    v = scan_step<0x118, 0xf>(v);
+    v = scan_step<0x142, 0xa>(v);          // row_bcast 15, to rows 1 and 3
+    return scan_step<0x143, 0xc>(v);       // row_bcast 31, to rows 2 and 3
+}
+
 // The units of a call's sequences, one sequence a lane: `end` is the number of
 // units up to and with the lane's.
 struct Units {
@@ -20,11 +34,7 @@ __device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch&
     u.rows = lane < b.n ? min(pv.lens[b.seq[lane]] + 1, pv.max_rows) : 0;
     u.tiles = (u.rows + unit - 1) / unit;
     u.end = u.tiles * groups;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const int x = __shfl_up(u.end, o, kWave);
-        if (lane >= o) u.end += x;
-    }
+    u.end = wave_scan(u.end);
     u.total = __builtin_amdgcn_readlane(u.end, kWave - 1);
     return u;
 }

@@ -8,6 +8,7 @@ stream.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 import subprocess
@@ -315,8 +316,9 @@ class DeviceBytes(DeviceArray):
 
 
 def _seqs(seqs):
-    arr = (ctypes.c_int * len(seqs))(*seqs)
-    return arr
+    if len(seqs) < 8:
+        return (ctypes.c_int * len(seqs))(*seqs)
+    return (ctypes.c_int * len(seqs)).from_buffer(array.array("i", seqs))
 
 
 class Context:
