@@ -151,6 +151,31 @@ int not_capturing(const q35m_paged* p, const char* what) {
     return Q35M_OK;
 }
 
+// Whether what a plan writes is also what it reads, or writes elsewhere: requests are planned
+// side by side.  (rows may be the lengths themselves, which it leaves as it reads them.)
+struct Span {
+    const void* at;
+    size_t bytes;
+    bool meets(const Span& o) const {
+        const uintptr_t a = (uintptr_t)at, b = (uintptr_t)o.at;
+        return bytes && o.bytes && (a < b ? b - a < bytes : a - b < o.bytes);
+    }
+};
+bool plan_overlaps(const q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
+                   const int64_t* slots, size_t n_slots, const int* taken) {
+    const size_t seqs = (size_t)p->map.n_seqs(), most = (size_t)n * p->map.max_rows();
+    const Span in[] = {{rows, n * sizeof(int)}, {tokens, n * sizeof(int)}, {free_pages, n_free * sizeof(int)}};
+    const Span out[] = {{slots, std::min(n_slots, most) * sizeof(int64_t)}, {taken, n * sizeof(int)},
+                        {p->dev_table, seqs * p->map.max_pages() * sizeof(int)}, {p->dev_len, seqs * sizeof(int)}};
+    for (const Span& o : out) {
+        for (const Span& i : in)
+            if (o.meets(i) && !(&i == &in[0] && &o == &out[3] && i.at == o.at)) return true;
+        for (const Span& x : out)
+            if (&o != &x && o.meets(x)) return true;
+    }
+    return false;
+}
+
 // The host's tables and lengths are the device's until a plan.
 int not_planned(const q35m_paged* p, const char* what) {
     return p->planned ? pfail(Q35M_ERR_INVALID, "%s: the cache's lengths and tables are planned on the device", what) : Q35M_OK;
@@ -397,6 +422,8 @@ int q35m_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, co
         return pfail(Q35M_ERR_INVALID, "null array of a plan");
     if (((uintptr_t)rows | (uintptr_t)tokens | (uintptr_t)taken | (uintptr_t)free_pages) & 3 || (uintptr_t)slots & 7)
         return pfail(Q35M_ERR_INVALID, "arrays of a plan must be aligned to their values");
+    if (plan_overlaps(p, n, rows, tokens, free_pages, n_free, slots, n_slots, taken))
+        return pfail(Q35M_ERR_INVALID, "an array that a plan writes overlaps another one");
     DeviceScope dev(p->ctx->device);
     PHIP_TRY(q35::launch_paged_plan(p, n, rows, tokens, free_pages, n_free, slots, n_slots, taken), "paged_plan");
     p->planned = true;

@@ -296,3 +296,28 @@ def test_refusals():
         p.c.plan(4, good, good, none, none, Ints(p.ctx, [0] * 4))
         refused(q35mix.ERR_INVALID, lambda: p.c.map(0, 0, [1]), "planned")
         p.ctx.sync()
+
+
+def test_arrays_that_overlap():
+    """Requests are planned side by side: nothing that a plan writes may be what it reads or writes elsewhere, but the
+    lengths, which are left as they are read."""
+    with Planner(4, 64, 16, 20) as p:
+        n = Ints(p.ctx, [0] * 16)
+        def part(at, count, size=4):
+            return type("Part", (), {"ptr": n.ptr + 4 * at, "nbytes": size * count})()
+        rows, tokens, free, taken = part(0, 4), part(4, 4), part(8, 4), part(12, 4)
+        slots = Ints(p.ctx, [0] * 8, np.int64)
+        far = Ints(p.ctx, [0] * 4)
+        inside = lambda ptr, size=16: type("Inside", (), {"ptr": ptr, "nbytes": size})()
+        for bad in (dict(taken=part(3, 4)), dict(taken=rows), dict(taken=part(5, 4)), dict(taken=part(9, 4)),
+                    dict(slots=inside(n.ptr)), dict(slots=inside(n.ptr + 24)), dict(slots=inside(n.ptr + 40)),
+                    dict(slots=inside(n.ptr + 56)), dict(tokens=inside(p.lens_ptr)), dict(taken=inside(p.lens_ptr)),
+                    dict(rows=inside(p.lens_ptr + 4)), dict(rows=inside(p.lens_ptr - 4)), dict(free=inside(p.lens_ptr)),
+                    dict(free=inside(p.table_ptr + 60)), dict(rows=inside(p.table_ptr)), dict(slots=inside(p.table_ptr)),
+                    dict(taken=inside(p.table_ptr + 48))):
+            a = dict(rows=rows, tokens=tokens, free=free, slots=slots, taken=taken) | bad
+            refused(q35mix.ERR_INVALID, lambda: p.c.plan(4, a["rows"], a["tokens"], a["free"], a["slots"], a["taken"]), "overlap")
+        p.c.map(0, 0, [1])                                             # nothing was planned
+        p.c.plan(4, rows, rows, rows, slots, taken)                    # what is only read may be one array
+        p.c.plan(4, inside(p.lens_ptr), tokens, free, slots, far)
+        p.ctx.sync()
