@@ -28,17 +28,23 @@ struct Tiles {
     int n;                 // tiles
     long q0;
     // more: log2 of what a unit is over 64 rows.
-    __device__ __forceinline__ Tiles(int start, int tokens, int hg_shift, int more) : shift(hg_shift + more) {
+    __host__ __device__ __forceinline__ Tiles(int start, int tokens, int hg_shift, int more) : shift(hg_shift + more) {
         const int tm_shift = 6 - hg_shift, tm = 1 << tm_shift;
         n = (tokens + tm - 1) >> tm_shift;
         q0 = ((long)start + tm + (kUnit << more) - 1) >> tm_shift;
     }
-    __device__ __forceinline__ long floors(long m) const {      // sum of floor(y / hg) over y < m
+    __host__ __device__ __forceinline__ long floors(long m) const {      // sum of floor(y / hg) over y < m
         const long k = m >> shift;
         return ((k * (k - 1)) >> 1 << shift) + k * (m - (k << shift));
     }
-    __device__ __forceinline__ long cnt(int j) const { return (q0 + j) >> shift; }
-    __device__ __forceinline__ long before(int j) const { return floors(q0 + j) - floors(q0); }   // tiles < j
+    __host__ __device__ __forceinline__ long cnt(int j) const { return (q0 + j) >> shift; }
+    __host__ __device__ __forceinline__ long before(int j) const { return floors(q0 + j) - floors(q0); }   // tiles < j
+    // Units of tiles j and n - 1 - j together, if all of them are in pairs of as many (else 0): two
+    // numbers whose sum is hg - 1 modulo hg have remainders that add up to hg - 1.
+    __host__ __device__ __forceinline__ long pair() const {
+        const long sum = 2 * q0 + n - 1, last = (1L << shift) - 1;
+        return n % 2 == 0 && (sum & last) == last ? (sum - last) >> shift : 0;
+    }
     // In the paired order: the tile at place o, and the units of the places before o.
     __device__ __forceinline__ int tile(int o) const { return o & 1 ? n - 1 - (o >> 1) : o >> 1; }
     __device__ __forceinline__ long ordered(int o) const {

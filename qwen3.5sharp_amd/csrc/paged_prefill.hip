@@ -964,12 +964,19 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
     float* part_ml = part_o + (size_t)2 * nwg * kPagedTileRows * kHd;
     const PagedView pv = p->view(layer);
     const AttnLayer& L = c->full[layer];
-    long tiles = 0;
+    long tiles = 0, units = 0;
     long longest = 0;                                      // rows that a tile may see
+    long pair = 0;                                         // units of every pair of tiles (-1: they differ)
     for (int i = 0; i < b.n; ++i) {
-        const long n = ((long)b.off[i + 1] - b.off[i] + tm - 1) / tm;
-        tiles += n * c->d.nkv * ng;
-        if (n) longest = std::max(longest, p->map.length(b.seq[i]) + n * tm);
+        const int tokens = b.off[i + 1] - b.off[i];
+        if (!tokens) continue;
+        const long start = p->map.length(b.seq[i]);
+        const Tiles ts((int)start, tokens, hg_shift, 0);
+        tiles += (long)ts.n * c->d.nkv * ng;
+        units += ts.before(ts.n) * c->d.nkv * ng;
+        longest = std::max(longest, start + (long)ts.n * tm);
+        const long both = ts.pair();
+        pair = both && (!pair || pair == both) ? both : -1;
     }
     // Short tiles that each get a workgroup are not cut, and nothing is to be joined,
     // as the lengths known here say (not so those of a replay): up to 4 units of an
@@ -977,7 +984,11 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
     // 15.5), up to 2 of an fp32 one (13.7 against 15.4 for four sequences of 120 rows;
     // 4 units are slower, 21 against 18).
     const int shift = p->type == Q35M_KV_F32 ? 1 : 2;
-    const int more = tiles <= nwg && longest <= kUnit << shift && p->lengths_known() ? shift : 0;
+    const bool known = p->lengths_known();
+    const int more = known && tiles <= nwg && longest <= kUnit << shift ? shift : 0;
+    // Nor is a tile where each workgroup's share is a number of whole pairs (2048 tokens of
+    // a new sequence in 4 bits: 102 us instead of 105).
+    const bool cut = !more && !(known && pair > 0 && (units + nwg - 1) / nwg % pair == 0);
     {
         ProfScope ps(c, K_PAGED_PREFILL);
         auto go = [&](auto kern) {
@@ -990,7 +1001,7 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (more) return hipSuccess;
+    if (!cut) return hipSuccess;
     ProfScope ps(c, K_PAGED_PREFILL_MERGE);
     hipExtLaunchKernelGGL(paged_prefill_merge, dim3((unsigned)(4 * tiles)), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b,
                           part_o, part_ml, q_gate, out, hg_shift, ng, nwg);
