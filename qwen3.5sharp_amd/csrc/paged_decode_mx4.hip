@@ -15,6 +15,8 @@
 // registers; a block's power of two is per row, along this product's sum, so the
 // matrix instruction's own cannot serve here.  P is two fp16 values (hi + lo, to 2^-23 of
 // it), which are columns too up to 8 heads.
+#include <algorithm>
+
 #include "paged_decode.h"
 
 namespace q35 {
@@ -520,11 +522,19 @@ hipError_t launch_paged_decode_mx4(q35m_paged* p, int layer, const PagedBatch& b
     float* part_ml = part_o + (size_t)2 * nwg * kPagedDecodeHeads * kHd;
     const PagedView pv = p->view(layer);
     const AttnLayer& L = c->full[layer];
-    // Short sequences that each get a workgroup are not cut (see launch_paged_decode).
-    const int whole = 4 * kUnitRows4;
-    bool cut = (long)b.n * c->d.nkv * ng > nwg || !p->lengths_known();
-    for (int i = 0; i < b.n && !cut; ++i) cut = p->map.length(b.seq[i]) >= whole;
-    const int unit = cut ? kUnitRows4 : whole;
+    // Sequences are not cut, and nothing is to be joined, where that leaves the busiest CU up to 3
+    // units more, as the lengths known here say (not so those of a replay): a launch against
+    // 1.1 us a unit.  450 rows, 4 units for 1: 10.3 us against 11.3; 16 sequences of 600, 5 for
+    // 2: 12.9 against 14.3, of 1000, 8 for 2: 16.1 against 14.5; 64 of 3000, as many: 37 against 41.
+    long units = 0, longest = 0;
+    for (int i = 0; i < b.n; ++i) {
+        const long n = p->map.length(b.seq[i]) / kUnitRows4 + 1;
+        units += n * c->d.nkv * ng;
+        longest = std::max(longest, n);
+    }
+    const long groups = (long)b.n * c->d.nkv * ng, rounds = (groups + c->n_cu - 1) / c->n_cu;
+    const bool cut = groups > nwg || rounds * longest > (units + c->n_cu - 1) / c->n_cu + 3 || !p->lengths_known();
+    const int unit = kUnitRows4 * (cut ? 1 : (int)longest);
     {
         ProfScope ps(c, K_PAGED_DECODE);
         auto go = [&](auto kern) {

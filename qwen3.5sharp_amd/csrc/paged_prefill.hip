@@ -966,7 +966,7 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
     const AttnLayer& L = c->full[layer];
     long tiles = 0, units = 0;
     long longest = 0;                                      // rows that a tile may see
-    long pair = 0;                                         // units of every pair of tiles (-1: they differ)
+    long pair = 0, most = 0;                               // units of every pair of tiles (-1: they differ); of the largest pair
     for (int i = 0; i < b.n; ++i) {
         const int tokens = b.off[i + 1] - b.off[i];
         if (!tokens) continue;
@@ -977,15 +977,29 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
         longest = std::max(longest, start + (long)ts.n * tm);
         const long both = ts.pair();
         pair = both && (!pair || pair == both) ? both : -1;
+        most = std::max(most, ts.cnt(0) + ts.cnt(ts.n - 1) + 1);
     }
     // Short tiles that each get a workgroup are not cut, and nothing is to be joined,
     // as the lengths known here say (not so those of a replay): up to 4 units of an
     // fp16 cache (30 tokens: 8.6 us against 11.0 with the joining; 230: 14.5 against
     // 15.5), up to 2 of an fp32 one (13.7 against 15.4 for four sequences of 120 rows;
     // 4 units are slower, 21 against 18).
-    const int shift = p->type == Q35M_KV_F32 ? 1 : 2;
     const bool known = p->lengths_known();
-    const int more = known && tiles <= nwg && longest <= kUnit << shift ? shift : 0;
+    int more = 0;
+    if (p->type != Q35M_KV_MXFP4) {
+        const int shift = p->type == Q35M_KV_F32 ? 1 : 2;
+        if (known && tiles <= nwg && longest <= kUnit << shift) more = shift;
+    } else if (known) {
+        // In 4 bits, whole tiles dealt out evenly (in pairs, which are alike) where that leaves
+        // the busiest workgroup up to 12 units more than cutting: a cut tile is begun and ended
+        // once more, 14 us at 1.55 a unit, and joined.  1000 tokens, 16 units for 9: 47 us
+        // against 66; 2000, 34 for 32: 88 against 106; 800 behind 1000, 29 for 18: 67 against 70;
+        // 512 behind 1000, 24 for 11: 59 against 55.
+        const long rounds = (tiles + nwg - 1) / nwg;
+        const long whole = rounds / 2 * most + rounds % 2 * ((longest + kUnit - 1) / kUnit);
+        if (whole * nwg <= units + 12 * nwg)
+            for (more = 1; kUnit << more < longest;) ++more;
+    }
     // Nor is a tile where each workgroup's share is a number of whole pairs (2048 tokens of
     // a new sequence in 4 bits: 102 us instead of 105).
     const bool cut = !more && !(known && pair > 0 && (units + nwg - 1) / nwg % pair == 0);

@@ -186,9 +186,10 @@ def test_a_pool_of_more_than_4_gib():
 
 # ------------------------------------------------------------------ prompts of whole and cut tiles
 
-@pytest.mark.parametrize("n,T,page", [(0, 2048, 64), (64, 2048, 16), (700, 1500, 128)])
+@pytest.mark.parametrize("n,T,page", [(0, 2048, 64), (64, 2048, 16), (700, 1500, 128), (0, 1000, 32), (0, 1100, 64), (2000, 1500, 256),
+                                      (30, 2500, 1024), (3000, 64, 16)])
 def test_prompts_of_whole_and_cut_tiles(n, T, page):
-    """16 q heads on 4 kv heads: 2048 rows are two whole tiles a workgroup, paired first with last; the others are cut."""
+    """16 q heads on 4 kv heads: one to three whole tiles a workgroup, in pairs of first and last, or tiles cut anywhere."""
     with Mx4(max_rows=n + T, page_rows=page, salt=7) as p:
         p.seed_rows([n], salt=n)
         mid = T // 2 // 16 * 16
@@ -200,7 +201,9 @@ def test_prompts_of_whole_and_cut_tiles(n, T, page):
 @pytest.mark.parametrize("lens,tokens", [([0], [2048]), ([0, 0], [1024, 1024]), ([0, 64], [1024, 1024]), ([32, 32], [1024, 1024]),
                                          ([0, 0, 0], [1024, 0, 1023]), ([17, 17], [1024, 1024])])
 def test_prompts_joined_or_not(kv_type, lens, tokens):
-    """A call whose tiles all come out whole ends with them; a replay, which cannot know, joins what is cut: the same."""
+    """A call whose tiles all come out whole ends with them; a replay, which cannot know, joins what is cut: the same.  A
+    4-bit cache's call also leaves tiles whole that a replay cuts (here the two lengths that differ): as near as any
+    two orders of the sums."""
     with make(kv_type, n_seqs=len(lens), max_rows=2112, page_rows=64) as p:
         p.seed_rows(lens, salt=1)
         seqs, rows = list(range(len(lens))), sum(tokens)
@@ -212,9 +215,28 @@ def test_prompts_joined_or_not(kv_type, lens, tokens):
         want = out.download()
         for _ in range(3):
             launch()
-            assert np.array_equal(again.download(), want)
+            if kv_type == KV_MXFP4 and lens == [0, 64]:
+                close_to(again.download(), want)
+            else:
+                assert np.array_equal(again.download(), want)
         end()
         assert np.isfinite(want).all()
+
+
+@pytest.mark.parametrize("lens", [[600] * 16, [511, 0, 700], [1100] * 40 + [7] * 24, [3000] * 3, [2000] * 20, [130, 500, 900, 1300]])
+def test_sequences_joined_or_not(lens):
+    """One new token: sequences left whole and cut, and a replay's, which are always cut."""
+    with Mx4(n_seqs=len(lens), max_rows=max(lens) + 1, page_rows=128, nh=8, nkv=4) as p:
+        p.seed_rows(lens, salt=2)
+        decode(p, range(len(lens)), lens, 9)
+        x, n = p.inputs(len(lens), salt=9), len(lens)
+        d, out, again = p.dev(x, "q_gate", "k", "v"), p.ctx.array((n, p.nh * HD)), p.ctx.array((n, p.nh * HD))
+        p.c.attn_decode(0, list(range(n)), *d, out)
+        launch, end = capture(p, lambda: p.c.attn_decode(0, list(range(n)), *d, again))
+        for _ in range(2):
+            launch()
+            close_to(again.download(), out.download())
+        end()
 
 
 # ------------------------------------------------------------------ graphs in turn
