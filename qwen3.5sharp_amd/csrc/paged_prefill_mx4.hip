@@ -83,9 +83,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
     constexpr float kShift = 6.0f, kMove = 9.9f;
     __shared__ __align__(16) Mx4Tile st;
     const int tid = threadIdx.x;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rg = wave & 1, half = wave >> 1;
-    const int hg = 1 << hg_shift, tm = kPagedTileRows >> hg_shift;
+    const int tm = kPagedTileRows >> hg_shift;
     const int groups = pv.nkv * ng, nh = groups << hg_shift;
     const int wg = xcd_remap(blockIdx.x, gridDim.x);      // neighbours, which share K and V, on one XCD's L2
     constexpr int kBuf = kUnit * kHd * 2;                 // bytes of a V buffer
@@ -99,11 +97,11 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         const int start = uniform(wk.start), tokens = uniform(wk.tokens);
         const int seq = b.seq[wk.i], kvh = wk.y / ng;
         const int* table = pv.table + (size_t)seq * pv.max_pages;
-        // (the lane's own places as values of this segment: addresses made of them
-        // would else be kept over all segments)
-        int lane = tid & 63, nn = lane & 31;
-        asm volatile("" : "+v"(lane), "+v"(nn));
-        const int h = lane >> 5;
+        // (the lane's and the wave's own places as values of this segment: addresses made of them
+        // would else be kept over all segments, moved out of the registers and back)
+        int lane = tid & 63, nn = lane & 31, wave = uniform(tid >> 6);
+        asm volatile("" : "+v"(lane), "+v"(nn), "+s"(wave));
+        const int h = lane >> 5, rg = wave & 1, half = wave >> 1;
         // Rows the tile's tokens see: [0, rows); the lane's query row sees [0, mine].
         const int rows = uniform(min(start + min((wk.j + 1) * tm, tokens), pv.max_rows));
         const int last16 = (rows - 1) & ~15;
@@ -116,7 +114,12 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         const long row0 = uniform((long)(uniform(b.off[wk.i]) + wk.j * tm) * nh + (wk.y << hg_shift));
         const char* const q_tile = (const char*)uniform(q_gate + row0 * 2 * kHd);
         char* const out_tile = (char*)uniform(out + row0 * kHd);
-        auto from_row0 = [&](int r) { return min(r >> hg_shift, left - 1) * nh + (r & (hg - 1)); };
+        // (Made anew for each use, for the same reason.)
+        auto rows_from = [&]() {
+            int shift = hg_shift;
+            asm volatile("" : "+s"(shift));
+            return [=](int r) { return min(r >> shift, left - 1) * nh + (r & ((1 << shift) - 1)); };
+        };
 
         // A wave takes rows 32 half .. of a unit's K and brings rows 16 wave .. of its V,
         // the rg-th 16 of those.  It holds where 64 entries of the page table lie, one a lane,
@@ -165,9 +168,10 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         };
 
         // q rows, which have the longest way, 16-byte chunks permuted by row (chunk ^ row % 32).
+        const auto q_from = rows_from();
 #pragma unroll 4
         for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-            dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 16 * (lane ^ (r & 31)), lds_address(&st.q[0]) + r * kHd * 4);
+            dma_nth(0, q_tile, q_from(r) * (2 * kHd * 4) + 16 * (lane ^ (r & 31)), lds_address(&st.q[0]) + r * kHd * 4);
         hold(uniform(group(wk.t0, 0) >> pv.page_shift));
         {
             const Keys k = keys(wk.t0);
@@ -505,9 +509,10 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
             v_read(b, 1, 1, v1);
             output(b, [&]() { add(w0, ph[0], pl[0]); }, [](float) {});
             if (whole) {                                   // the gates of the wave's rows 16 wave .. take V's place
+                const auto gate_from = rows_from();
 #pragma unroll 4
                 for (int r = 16 * wave; r < 16 * wave + 16; ++r)
-                    dma_nth(0, q_tile, from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane, lds_address(&st.v[0][0][0]) + r * kHd * 4);
+                    dma_nth(0, q_tile, gate_from(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane, lds_address(&st.v[0][0][0]) + r * kHd * 4);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) left_over(i);
@@ -529,7 +534,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         // The tile's rows to LDS, then a row a wave at a time: finished, or as a part
         // to the workspace.  (Places again as values of this part: kept from the
         // segment's beginning they would be in registers all the while.)
-        asm volatile("" : "+v"(lane), "+v"(nn));
+        asm volatile("" : "+v"(lane), "+v"(nn), "+s"(wave));
         const int slot = 2 * wg + (wk.t0 == 0);
         l_run = xor32_sum(l_run);
         if (lane < 32) st.mx[1][wave][nn] = l_run;
@@ -541,6 +546,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         const int row = 16 * wave + (lane & 15);           // a row's sum and maximum in lane row % 16
         const float l = st.mx[1][row >> 5][row & 31] + st.mx[1][2 + (row >> 5)][row & 31];
         float* const to_part = part_o + (size_t)slot * kPagedTileRows * kHd;
+        const auto from_row0 = rows_from();
         auto gate_row = [&](int r) { return q_tile + (uint32_t)(from_row0(r) * (2 * kHd * 4) + 4 * kHd + 16 * lane); };
         auto out_row = [&](int r) { return r >> hg_shift < left ? out_tile + (uint32_t)(from_row0(r) * (kHd * 4) + 16 * lane) : nullptr; };
         dma_wait();                                        // (the gates, which the wave itself has brought)
