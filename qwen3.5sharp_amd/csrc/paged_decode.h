@@ -39,19 +39,44 @@ __device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch&
     return u;
 }
 
+// Whether a 4-bit cache's sequences are left whole, each (sequence, head group) to a
+// workgroup, so that nothing is to be joined: where the busiest CU gets up to 3 units
+// more than if they are dealt out (a launch against 1.1 us a unit).  450 rows, 4
+// units for 1: 10.3 us against 11.3; 16 sequences of 600, 5 for 2: 12.9 against 14.3, of
+// 1000, 8 for 2: 16.1 against 14.5; 64 of 3000, as many: 37 against 41.
+__host__ __device__ __forceinline__ bool left_whole(int groups, int units, int longest, int n_cu, int nwg) {
+    const int each = (groups <= n_cu ? 1 : 2) * longest;   // (nwg: one or two a CU)
+    return groups <= nwg && (each - 4) * n_cu < units;
+}
+// The units of such a cache, and how many rows one has.
+__device__ __forceinline__ Units units_or_whole(const PagedView& pv, const PagedBatch& b, int groups, int& unit, int n_cu,
+                                                int nwg, int lane) {
+    Units u = units_of(pv, b, groups, unit, lane);
+    const int longest = __builtin_amdgcn_readfirstlane((int)wave_max((float)u.tiles));
+    if (left_whole(b.n * groups, u.total, longest, n_cu, nwg)) {
+        unit *= longest;
+        u.tiles = lane < b.n;
+        u.end = min(lane + 1, b.n) * groups;
+        u.total = b.n * groups;
+    }
+    return u;
+}
+
 // The parts of one (sequence, q head), where its units went to several
-// workgroups: waves take parts in turn, a lane four dims.
+// workgroups: waves take parts in turn, a lane four dims.  n_cu: 0, or the CUs of a call
+// whose sequences may be whole.
 constexpr int MW = 8;      // waves
 template <int UNIT>
 __global__ __launch_bounds__(MW * kWave) void paged_decode_merge(PagedView pv, PagedBatch b,
                                                                  const float* __restrict__ part_o,
                                                                  const float* __restrict__ part_ml,
                                                                  const float* __restrict__ q_gate,
-                                                                 float* __restrict__ out, int hg, int ng, int nwg) {
+                                                                 float* __restrict__ out, int hg, int ng, int nwg, int n_cu) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int groups = pv.nkv * ng, nh = groups * hg;
     const int i = blockIdx.y, head = blockIdx.x, y = head / hg, h = head - y * hg;
-    const Units un = units_of(pv, b, groups, UNIT, lane);
+    int unit = UNIT;
+    const Units un = n_cu ? units_or_whole(pv, b, groups, unit, n_cu, nwg, lane) : units_of(pv, b, groups, UNIT, lane);
     const int per = (un.total + nwg - 1) / nwg;
     const int tiles = __builtin_amdgcn_readlane(un.tiles, i);
     const int s = __builtin_amdgcn_readlane(un.end, i) - tiles * groups + y * tiles;

@@ -567,7 +567,7 @@ hipError_t launch_paged_decode(q35m_paged* p, int layer, const PagedBatch& b, co
         if (e != hipSuccess || !cut) return e;
         ProfScope ps(c, K_PAGED_DECODE_MERGE);
         hipExtLaunchKernelGGL(merge, dim3(c->d.nh, b.n), dim3(MW * kWave), 0, c->stream, ps.a, ps.b, 0, pv, b, part_o,
-                              part_ml, q_gate, out, hg, ng, nwg);
+                              part_ml, q_gate, out, hg, ng, nwg, 0);
         return hipGetLastError();
     };
     if (p->type == Q35M_KV_F16)

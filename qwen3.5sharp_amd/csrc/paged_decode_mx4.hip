@@ -256,7 +256,7 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
                                                           const float* __restrict__ q_norm,
                                                           const float* __restrict__ k_norm, float* __restrict__ out,
                                                           float* __restrict__ part_o, float* __restrict__ part_ml, int hg,
-                                                          int ng, int unit, float eps) {
+                                                          int ng, int n_cu, float eps) {
     constexpr int R = kTileRows, H = 4 * NQ, HW = H / 4;   // HW: heads a wave forms and joins
     constexpr int D = NQ == 4 ? 2 : 1;                     // tiles a wave asks for ahead
     const int tid = threadIdx.x, lane = tid & 63;
@@ -273,7 +273,8 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
     __shared__ __align__(16) float norms[2][kHd];          // 1 + q's weights, k's
     norms[0][tid] = 1.0f + q_norm[tid];
     norms[1][tid] = k_norm[tid];
-    const Units un = units_of(pv, b, groups, unit, lane);
+    int unit = kUnitRows4;
+    const Units un = units_or_whole(pv, b, groups, unit, n_cu, gridDim.x, lane);
     lds_barrier();
     const int per = (un.total + (int)gridDim.x - 1) / (int)gridDim.x;
     int u = blockIdx.x * per;
@@ -522,24 +523,19 @@ hipError_t launch_paged_decode_mx4(q35m_paged* p, int layer, const PagedBatch& b
     float* part_ml = part_o + (size_t)2 * nwg * kPagedDecodeHeads * kHd;
     const PagedView pv = p->view(layer);
     const AttnLayer& L = c->full[layer];
-    // Sequences are not cut, and nothing is to be joined, where that leaves the busiest CU up to 3
-    // units more, as the lengths known here say (not so those of a replay): a launch against
-    // 1.1 us a unit.  450 rows, 4 units for 1: 10.3 us against 11.3; 16 sequences of 600, 5 for
-    // 2: 12.9 against 14.3, of 1000, 8 for 2: 16.1 against 14.5; 64 of 3000, as many: 37 against 41.
-    long units = 0, longest = 0;
+    // Whether anything is to be joined, as far as the lengths are known here (not a replay's).
+    int units = 0, longest = 0;
     for (int i = 0; i < b.n; ++i) {
-        const long n = p->map.length(b.seq[i]) / kUnitRows4 + 1;
+        const int n = p->map.length(b.seq[i]) / kUnitRows4 + 1;
         units += n * c->d.nkv * ng;
         longest = std::max(longest, n);
     }
-    const long groups = (long)b.n * c->d.nkv * ng, rounds = (groups + c->n_cu - 1) / c->n_cu;
-    const bool cut = groups > nwg || rounds * longest > (units + c->n_cu - 1) / c->n_cu + 3 || !p->lengths_known();
-    const int unit = kUnitRows4 * (cut ? 1 : (int)longest);
+    const bool cut = !left_whole(b.n * c->d.nkv * ng, units, longest, c->n_cu, nwg) || !p->lengths_known();
     {
         ProfScope ps(c, K_PAGED_DECODE);
         auto go = [&](auto kern) {
             hipExtLaunchKernelGGL(kern, dim3(nwg), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b, q_gate, k, v, L.q_norm,
-                                  L.k_norm, out, part_o, part_ml, hg, ng, unit, c->d.eps);
+                                  L.k_norm, out, part_o, part_ml, hg, ng, c->n_cu, c->d.eps);
         };
         if (hg <= 4) go(paged_decode_mx4<1>);
         else if (hg <= 8) go(paged_decode_mx4<2>);
@@ -549,7 +545,7 @@ hipError_t launch_paged_decode_mx4(q35m_paged* p, int layer, const PagedBatch& b
     if (e != hipSuccess || !cut) return e;
     ProfScope ps(c, K_PAGED_DECODE_MERGE);
     hipExtLaunchKernelGGL(paged_decode_merge<kUnitRows4>, dim3(c->d.nh, b.n), dim3(MW * kWave), 0, c->stream, ps.a, ps.b, 0, pv, b,
-                          part_o, part_ml, q_gate, out, hg, ng, nwg);
+                          part_o, part_ml, q_gate, out, hg, ng, nwg, c->n_cu);
     return hipGetLastError();
 }
 
