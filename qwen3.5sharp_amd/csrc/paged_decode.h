@@ -64,7 +64,7 @@ __device__ __forceinline__ Units units_or_whole(const PagedView& pv, const Paged
 
 // The parts of one (sequence, q head), where its units went to several
 // workgroups: waves take parts in turn, a lane four dims.  n_cu: 0, or the CUs of a call
-// whose sequences may be whole.
+// whose sequences may turn out to be whole.
 constexpr int MW = 8;      // waves
 template <int UNIT>
 __global__ __launch_bounds__(MW * kWave) void paged_decode_merge(PagedView pv, PagedBatch b,

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
                                                           const float* __restrict__ q_norm,
                                                           const float* __restrict__ k_norm, float* __restrict__ out,
                                                           float* __restrict__ part_o, float* __restrict__ part_ml, int hg,
-                                                          int ng, int n_cu, float eps) {
+                                                          int ng, int unit, int n_cu, float eps) {
     constexpr int R = kTileRows, H = 4 * NQ, HW = H / 4;   // HW: heads a wave forms and joins
     constexpr int D = NQ == 4 ? 2 : 1;                     // tiles a wave asks for ahead
     const int tid = threadIdx.x, lane = tid & 63;
@@ -273,8 +273,8 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
     __shared__ __align__(16) float norms[2][kHd];          // 1 + q's weights, k's
     norms[0][tid] = 1.0f + q_norm[tid];
     norms[1][tid] = k_norm[tid];
-    int unit = kUnitRows4;
-    const Units un = units_or_whole(pv, b, groups, unit, n_cu, gridDim.x, lane);
+    const Units un = unit ? units_of(pv, b, groups, unit, lane)
+                          : units_or_whole(pv, b, groups, unit = kUnitRows4, n_cu, gridDim.x, lane);
     lds_barrier();
     const int per = (un.total + (int)gridDim.x - 1) / (int)gridDim.x;
     int u = blockIdx.x * per;
@@ -523,29 +523,31 @@ hipError_t launch_paged_decode_mx4(q35m_paged* p, int layer, const PagedBatch& b
     float* part_ml = part_o + (size_t)2 * nwg * kPagedDecodeHeads * kHd;
     const PagedView pv = p->view(layer);
     const AttnLayer& L = c->full[layer];
-    // Whether anything is to be joined, as far as the lengths are known here (not a replay's).
+    // (Where the lengths are known here, nothing is launched to join sequences left whole; else the
+    // kernels find it: unit 0.)
     int units = 0, longest = 0;
     for (int i = 0; i < b.n; ++i) {
         const int n = p->map.length(b.seq[i]) / kUnitRows4 + 1;
         units += n * c->d.nkv * ng;
         longest = std::max(longest, n);
     }
-    const bool cut = !left_whole(b.n * c->d.nkv * ng, units, longest, c->n_cu, nwg) || !p->lengths_known();
+    const bool known = p->lengths_known(), whole = left_whole(b.n * c->d.nkv * ng, units, longest, c->n_cu, nwg);
+    const int unit = !known ? 0 : whole ? kUnitRows4 * longest : kUnitRows4;
     {
         ProfScope ps(c, K_PAGED_DECODE);
         auto go = [&](auto kern) {
             hipExtLaunchKernelGGL(kern, dim3(nwg), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b, q_gate, k, v, L.q_norm,
-                                  L.k_norm, out, part_o, part_ml, hg, ng, c->n_cu, c->d.eps);
+                                  L.k_norm, out, part_o, part_ml, hg, ng, unit, c->n_cu, c->d.eps);
         };
         if (hg <= 4) go(paged_decode_mx4<1>);
         else if (hg <= 8) go(paged_decode_mx4<2>);
         else go(paged_decode_mx4<4>);
     }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !cut) return e;
+    if (e != hipSuccess || (known && whole)) return e;
     ProfScope ps(c, K_PAGED_DECODE_MERGE);
     hipExtLaunchKernelGGL(paged_decode_merge<kUnitRows4>, dim3(c->d.nh, b.n), dim3(MW * kWave), 0, c->stream, ps.a, ps.b, 0, pv, b,
-                          part_o, part_ml, q_gate, out, hg, ng, nwg, c->n_cu);
+                          part_o, part_ml, q_gate, out, hg, ng, nwg, known ? 0 : c->n_cu);
     return hipGetLastError();
 }
 

@@ -94,6 +94,56 @@ __device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch&
     return u;
 }
 
+// In 4 bits tiles are left whole, dealt out in pairs of first and last, which are alike,
+// where that leaves the busiest workgroup up to 12 units more than cutting: a cut tile
+// is begun and ended once more, 14 us at 1.55 a unit, and joined.  1000 tokens, 16 units
+// for 9: 47 us against 66; 2000, 34 for 32: 88 against 106; 800 behind 1000, 29 for 18: 67
+// against 70; 512 behind 1000, 24 for 11: 59 against 55.
+// Returned is log2 of what a unit is over 64 rows then, of which a tile has one (0: cut).
+// longest: rows that a tile may see; pair: units of a sequence's first and last tile.
+__host__ __device__ __forceinline__ int whole_tiles(long tiles, long units, int longest, int pair, int nwg) {
+    const unsigned rounds = (unsigned)((unsigned)tiles + nwg - 1) / (unsigned)nwg;
+    const long most = (long)(rounds >> 1) * (pair + 1) + (rounds & 1) * ((longest + kUnit - 1) / kUnit);
+    if ((most - 12) * nwg > units) return 0;
+    const unsigned more = (unsigned)(longest - 1) / kUnit;
+    return more < 2 ? 1 : 32 - __builtin_clz(more);
+}
+__device__ __forceinline__ Units units_or_whole(const PagedView& pv, const PagedBatch& b, int groups, int hg_shift, int nwg,
+                                                int lane) {
+    Units u;
+    u.start = 0;
+    u.end = 0;
+    int tiles = 0, longest = 1, pair = 0;                  // (the last two: of this and the sequences before)
+    const int tokens = lane < b.n ? b.off[lane + 1] - b.off[lane] : 0;
+    if (lane < b.n) u.start = pv.lens[b.seq[lane]];
+    if (tokens) {
+        const Tiles t(u.start, tokens, hg_shift, 0);
+        u.end = t.before(t.n) * groups;
+        tiles = t.n * groups;
+        longest = u.start + (t.n << (6 - hg_shift));
+        pair = (int)(t.cnt(0) + t.cnt(t.n - 1));
+    }
+    for (int o = 1; o < b.n; o <<= 1) {
+        const long x = shfl_up_long(u.end, o);
+        const int y = __shfl_up(tiles, o, kWave), z = __shfl_up(longest, o, kWave), p = __shfl_up(pair, o, kWave);
+        if (lane >= o) {
+            u.end += x;
+            tiles += y;
+            longest = max(longest, z);
+            pair = max(pair, p);
+        }
+    }
+    auto all = [&](int v) { return __builtin_amdgcn_readlane(v, b.n - 1); };
+    u.total = readlane_long(u.end, b.n - 1);
+    u.more = whole_tiles(all(tiles), u.total, all(longest), all(pair), nwg);
+    if (u.more) {
+        u.end = tiles;
+        u.total = all(tiles);
+    }
+    if (lane >= b.n) u.end = u.total;
+    return u;
+}
+
 // A workgroup's walk over its units, segment by segment.
 struct Walk {
     long u, u_end;

@@ -860,10 +860,12 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f32(PagedView pv, PagedBa
 __global__ __launch_bounds__(NT) void paged_prefill_merge(PagedView pv, PagedBatch b, const float* __restrict__ part_o,
                                                           const float* __restrict__ part_ml,
                                                           const float* __restrict__ q_gate, float* __restrict__ out,
-                                                          int hg_shift, int ng, int nwg) {
+                                                          int hg_shift, int ng, int nwg, int more) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int groups = pv.nkv * ng, nh = groups << hg_shift, tm = kPagedTileRows >> hg_shift;
-    const Units un = units_of(pv, b, groups, hg_shift, 0, lane);
+    const Units un = more < 0 ? units_or_whole(pv, b, groups, hg_shift, nwg, lane)
+                              : units_of(pv, b, groups, hg_shift, 0, lane);
+    if (un.more) return;
     const long per = (un.total + nwg - 1) / nwg;
     // The workgroup's tile: the sequences' tiles in order.
     int tile_end = lane < b.n ? ((b.off[lane + 1] - b.off[lane] + tm - 1) / tm) * groups : 0;
@@ -966,7 +968,8 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
     const AttnLayer& L = c->full[layer];
     long tiles = 0, units = 0;
     long longest = 0;                                      // rows that a tile may see
-    long pair = 0, most = 0;                               // units of every pair of tiles (-1: they differ); of the largest pair
+    long pair = 0;                                         // units of every pair of tiles (-1: they differ)
+    int most = 0;                                          // of the largest first and last tile
     for (int i = 0; i < b.n; ++i) {
         const int tokens = b.off[i + 1] - b.off[i];
         if (!tokens) continue;
@@ -977,7 +980,7 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
         longest = std::max(longest, start + (long)ts.n * tm);
         const long both = ts.pair();
         pair = both && (!pair || pair == both) ? both : -1;
-        most = std::max(most, ts.cnt(0) + ts.cnt(ts.n - 1) + 1);
+        most = std::max(most, (int)(ts.cnt(0) + ts.cnt(ts.n - 1)));
     }
     // Short tiles that each get a workgroup are not cut, and nothing is to be joined,
     // as the lengths known here say (not so those of a replay): up to 4 units of an
@@ -989,20 +992,12 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
     if (p->type != Q35M_KV_MXFP4) {
         const int shift = p->type == Q35M_KV_F32 ? 1 : 2;
         if (known && tiles <= nwg && longest <= kUnit << shift) more = shift;
-    } else if (known) {
-        // In 4 bits, whole tiles dealt out evenly (in pairs, which are alike) where that leaves
-        // the busiest workgroup up to 12 units more than cutting: a cut tile is begun and ended
-        // once more, 14 us at 1.55 a unit, and joined.  1000 tokens, 16 units for 9: 47 us
-        // against 66; 2000, 34 for 32: 88 against 106; 800 behind 1000, 29 for 18: 67 against 70;
-        // 512 behind 1000, 24 for 11: 59 against 55.
-        const long rounds = (tiles + nwg - 1) / nwg;
-        const long whole = rounds / 2 * most + rounds % 2 * ((longest + kUnit - 1) / kUnit);
-        if (whole * nwg <= units + 12 * nwg)
-            for (more = 1; kUnit << more < longest;) ++more;
+    } else {
+        more = known ? whole_tiles(tiles, units, (int)longest, most, nwg) : -1;      // (-1: the kernels find it)
     }
     // Nor is a tile where each workgroup's share is a number of whole pairs (2048 tokens of
     // a new sequence in 4 bits: 102 us instead of 105).
-    const bool cut = !more && !(known && pair > 0 && (units + nwg - 1) / nwg % pair == 0);
+    const bool cut = more <= 0 && !(known && pair > 0 && (units + nwg - 1) / nwg % pair == 0);
     {
         ProfScope ps(c, K_PAGED_PREFILL);
         auto go = [&](auto kern) {
@@ -1018,7 +1013,7 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
     if (!cut) return hipSuccess;
     ProfScope ps(c, K_PAGED_PREFILL_MERGE);
     hipExtLaunchKernelGGL(paged_prefill_merge, dim3((unsigned)(4 * tiles)), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b,
-                          part_o, part_ml, q_gate, out, hg_shift, ng, nwg);
+                          part_o, part_ml, q_gate, out, hg_shift, ng, nwg, more);
     return hipGetLastError();
 }
 

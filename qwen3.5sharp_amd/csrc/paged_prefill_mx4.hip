@@ -89,7 +89,8 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
     constexpr int kBuf = kUnit * kHd * 2;                 // bytes of a V buffer
 
     const float w = q_norm[tid];
-    const Units un = units_of(pv, b, groups, hg_shift, more, tid & 63);
+    const Units un = more < 0 ? units_or_whole(pv, b, groups, hg_shift, gridDim.x, tid & 63)
+                              : units_of(pv, b, groups, hg_shift, more, tid & 63);
     st.w[tid] = 1.0f + w;                                 // (read behind the first segment's first barrier)
     Walk wk;
     wk.begin(un, wg, gridDim.x);

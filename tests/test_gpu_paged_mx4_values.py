@@ -201,9 +201,8 @@ def test_prompts_of_whole_and_cut_tiles(n, T, page):
 @pytest.mark.parametrize("lens,tokens", [([0], [2048]), ([0, 0], [1024, 1024]), ([0, 64], [1024, 1024]), ([32, 32], [1024, 1024]),
                                          ([0, 0, 0], [1024, 0, 1023]), ([17, 17], [1024, 1024])])
 def test_prompts_joined_or_not(kv_type, lens, tokens):
-    """A call whose tiles all come out whole ends with them; a replay, which cannot know, joins what is cut: the same.  A
-    4-bit cache's call also leaves tiles whole that a replay cuts (here the two lengths that differ): as near as any
-    two orders of the sums."""
+    """A call whose tiles all come out whole ends with them; a replay, whose host cannot know, launches the joining too:
+    the same."""
     with make(kv_type, n_seqs=len(lens), max_rows=2112, page_rows=64) as p:
         p.seed_rows(lens, salt=1)
         seqs, rows = list(range(len(lens))), sum(tokens)
@@ -215,10 +214,7 @@ def test_prompts_joined_or_not(kv_type, lens, tokens):
         want = out.download()
         for _ in range(3):
             launch()
-            if kv_type == KV_MXFP4 and lens == [0, 64]:
-                close_to(again.download(), want)
-            else:
-                assert np.array_equal(again.download(), want)
+            assert np.array_equal(again.download(), want)
         end()
         assert np.isfinite(want).all()
 
@@ -289,3 +285,23 @@ def test_timers_name_the_kernels():
         p.ctx.profile(False)
         assert sorted(ran) == ["paged_append_rows", "paged_decode", "paged_decode_merge", "paged_prefill", "paged_prefill_merge",
                                "paged_rows"]
+
+
+@pytest.mark.parametrize("lens,tokens", [([0], [300]), ([0], [1500]), ([900, 3, 0, 40], [100, 0, 700, 33]), ([1700], [16]),
+                                         ([1000, 1900], [1, 2]), ([0] * 6, [290, 301, 16, 1, 205, 300])])
+def test_replayed_chunks_are_divided_alike(lens, tokens):
+    """Tiles are left whole or cut by a rule on the lengths, which a replay reads where they are."""
+    with Mx4(n_seqs=len(lens), max_rows=2000, page_rows=64, nh=16, nkv=4) as p:
+        p.seed_rows(lens, salt=1)
+        seqs, rows = list(range(len(lens))), sum(tokens)
+        x = p.inputs(rows, salt=81)
+        d = p.dev(x, "q_gate", "k", "v")
+        out, again = p.ctx.array((rows, p.nh * HD)), p.ctx.array((rows, p.nh * HD))
+        launch, end = capture(p, lambda: p.c.attn_prefill(0, seqs, tokens, *d, again))
+        for shorter in (1, 3):
+            p.c.attn_prefill(0, seqs, tokens, *d, out)
+            launch()
+            assert np.array_equal(again.download(), out.download()) and np.isfinite(out.download()).all()
+            for s, n in enumerate(lens):
+                p.c.truncate(s, n // 3)
+        end()
