@@ -52,8 +52,8 @@ __global__ __launch_bounds__(256) void paged_rope_fill(double* __restrict__ tabl
 
 // One wave per (new row, kv head), four a workgroup, from unit0 on.  Reads 2 KiB and
 // writes 2 rows a wave: a copy with a reduction of one wave in between.
-template <typename T>
-__global__ __launch_bounds__(256) void paged_append_rows(PagedView pv, PagedBatch b, const float* __restrict__ k,
+template <typename T, int N>
+__global__ __launch_bounds__(256) void paged_append_rows(PagedView pv, PagedBatchOf<N> b, const float* __restrict__ k,
                                                          const float* __restrict__ v, const float* __restrict__ k_norm,
                                                          double eps, long unit0) {
     const int lane = threadIdx.x & 63;
@@ -84,9 +84,9 @@ __global__ __launch_bounds__(256) void paged_append_rows(PagedView pv, PagedBatc
 
 // Rows read back, one wave per (row, kv head): row `row` of the call is row first + (its
 // place) of its sequence.  Rows of pages that are not mapped are zeros.
-template <typename T>
-__global__ __launch_bounds__(256) void paged_rows(PagedView pv, PagedBatch b, PagedFirst first, float* __restrict__ k,
-                                                  float* __restrict__ v, long unit0) {
+template <typename T, int N>
+__global__ __launch_bounds__(256) void paged_rows(PagedView pv, PagedBatchOf<N> b, PagedFirstOf<N> first,
+                                                  float* __restrict__ k, float* __restrict__ v, long unit0) {
     const int lane = threadIdx.x & 63;
     const long unit = unit0 + (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = (int)(unit / pv.nkv), kvh = (int)(unit % pv.nkv);
@@ -152,40 +152,48 @@ hipError_t launch_paged_append(q35m_paged* p, int layer, const PagedBatch& b, co
     // (a grid holds fewer than 2^32 threads, 2^26 units)
     constexpr long kMost = 1L << 22;
     const long units = (long)b.off[b.n] * c->d.nkv;
-    for (long u = 0; u < units; u += kMost) {
-        ProfScope ps(c, K_PAGED_APPEND);
-        auto go = [&](auto kern) {
-            const long n = units - u < kMost ? units - u : kMost;
-            hipExtLaunchKernelGGL(kern, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, c->stream, ps.a, ps.b, 0,
-                                  p->view(layer), b, k, v, c->full[layer].k_norm, (double)c->d.eps, u);
-        };
-        if (p->type == Q35M_KV_MXFP4) go(paged_append_rows<Mx4>);
-        else if (p->type == Q35M_KV_F16) go(paged_append_rows<_Float16>);
-        else go(paged_append_rows<float>);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    return hipSuccess;
+    return with_batch(b, [&](const auto& some) {
+        constexpr int N = std::decay_t<decltype(some)>::kSeqs;
+        for (long u = 0; u < units; u += kMost) {
+            ProfScope ps(c, K_PAGED_APPEND);
+            auto go = [&](auto kern) {
+                const long n = units - u < kMost ? units - u : kMost;
+                hipExtLaunchKernelGGL(kern, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, c->stream, ps.a, ps.b, 0,
+                                      p->view(layer), some, k, v, c->full[layer].k_norm, (double)c->d.eps, u);
+            };
+            if (p->type == Q35M_KV_MXFP4) go(paged_append_rows<Mx4, N>);
+            else if (p->type == Q35M_KV_F16) go(paged_append_rows<_Float16, N>);
+            else go(paged_append_rows<float, N>);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
+    });
 }
 
 hipError_t launch_paged_rows(q35m_paged* p, int layer, const PagedBatch& b, const PagedFirst& first, float* k, float* v) {
     q35m_ctx* c = p->ctx;
     constexpr long kMost = 1L << 22;
     const long units = (long)b.off[b.n] * c->d.nkv;
-    for (long u = 0; u < units; u += kMost) {
-        ProfScope ps(c, K_PAGED_ROWS);
-        auto go = [&](auto kern) {
-            const long n = units - u < kMost ? units - u : kMost;
-            hipExtLaunchKernelGGL(kern, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, c->stream, ps.a, ps.b, 0,
-                                  p->view(layer), b, first, k, v, u);
-        };
-        if (p->type == Q35M_KV_MXFP4) go(paged_rows<Mx4>);
-        else if (p->type == Q35M_KV_F16) go(paged_rows<_Float16>);
-        else go(paged_rows<float>);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    return hipSuccess;
+    return with_batch(b, [&](const auto& some) {
+        constexpr int N = std::decay_t<decltype(some)>::kSeqs;
+        PagedFirstOf<N> from;
+        for (int i = 0; i < N; ++i) from.row[i] = i < b.n ? first.row[i] : 0;
+        for (long u = 0; u < units; u += kMost) {
+            ProfScope ps(c, K_PAGED_ROWS);
+            auto go = [&](auto kern) {
+                const long n = units - u < kMost ? units - u : kMost;
+                hipExtLaunchKernelGGL(kern, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, c->stream, ps.a, ps.b, 0,
+                                      p->view(layer), some, from, k, v, u);
+            };
+            if (p->type == Q35M_KV_MXFP4) go(paged_rows<Mx4, N>);
+            else if (p->type == Q35M_KV_F16) go(paged_rows<_Float16, N>);
+            else go(paged_rows<float, N>);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+        return hipSuccess;
+    });
 }
 
 }  // namespace q35

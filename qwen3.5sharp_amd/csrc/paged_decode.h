@@ -28,7 +28,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 struct Units {
     int rows, tiles, end, total;
 };
-__device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch& b, int groups, int unit, int lane) {
+template <int N>
+__device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatchOf<N>& b, int groups, int unit, int lane) {
     Units u;
     // (the row past max_rows of a replayed call that its caller let run over)
     u.rows = lane < b.n ? min(pv.lens[b.seq[lane]] + 1, pv.max_rows) : 0;
@@ -49,7 +50,8 @@ __host__ __device__ __forceinline__ bool left_whole(int groups, int units, int l
     return groups <= nwg && (each - 4) * n_cu < units;
 }
 // The units of such a cache, and how many rows one has.
-__device__ __forceinline__ Units units_or_whole(const PagedView& pv, const PagedBatch& b, int groups, int& unit, int n_cu,
+template <int N>
+__device__ __forceinline__ Units units_or_whole(const PagedView& pv, const PagedBatchOf<N>& b, int groups, int& unit, int n_cu,
                                                 int nwg, int lane) {
     Units u = units_of(pv, b, groups, unit, lane);
     const int longest = __builtin_amdgcn_readfirstlane((int)wave_max((float)u.tiles));
@@ -66,8 +68,8 @@ __device__ __forceinline__ Units units_or_whole(const PagedView& pv, const Paged
 // workgroups: waves take parts in turn, a lane four dims.  n_cu: 0, or the CUs of a call
 // whose sequences may turn out to be whole.
 constexpr int MW = 8;      // waves
-template <int UNIT>
-__global__ __launch_bounds__(MW * kWave) void paged_decode_merge(PagedView pv, PagedBatch b,
+template <int UNIT, int N = kMaxBatch>
+__global__ __launch_bounds__(MW * kWave) void paged_decode_merge(PagedView pv, PagedBatchOf<N> b,
                                                                  const float* __restrict__ part_o,
                                                                  const float* __restrict__ part_ml,
                                                                  const float* __restrict__ q_gate,

@@ -250,8 +250,8 @@ __device__ __forceinline__ void put_digits(uint32_t (*codes)[kDigitWords], uint8
     }
 }
 
-template <int NQ>
-__global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedView pv, PagedBatch b, const float* __restrict__ q_gate,
+template <int NQ, int N>
+__global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedView pv, PagedBatchOf<N> b, const float* __restrict__ q_gate,
                                                           const float* __restrict__ knew, const float* __restrict__ vnew,
                                                           const float* __restrict__ q_norm,
                                                           const float* __restrict__ k_norm, float* __restrict__ out,
@@ -533,22 +533,25 @@ hipError_t launch_paged_decode_mx4(q35m_paged* p, int layer, const PagedBatch& b
     }
     const bool known = p->lengths_known(), whole = left_whole(b.n * c->d.nkv * ng, units, longest, c->n_cu, nwg);
     const int unit = !known ? 0 : whole ? kUnitRows4 * longest : kUnitRows4;
-    {
-        ProfScope ps(c, K_PAGED_DECODE);
-        auto go = [&](auto kern) {
-            hipExtLaunchKernelGGL(kern, dim3(nwg), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, b, q_gate, k, v, L.q_norm,
-                                  L.k_norm, out, part_o, part_ml, hg, ng, unit, c->n_cu, c->d.eps);
-        };
-        if (hg <= 4) go(paged_decode_mx4<1>);
-        else if (hg <= 8) go(paged_decode_mx4<2>);
-        else go(paged_decode_mx4<4>);
-    }
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || (known && whole)) return e;
-    ProfScope ps(c, K_PAGED_DECODE_MERGE);
-    hipExtLaunchKernelGGL(paged_decode_merge<kUnitRows4>, dim3(c->d.nh, b.n), dim3(MW * kWave), 0, c->stream, ps.a, ps.b, 0, pv, b,
-                          part_o, part_ml, q_gate, out, hg, ng, nwg, known ? 0 : c->n_cu);
-    return hipGetLastError();
+    return with_batch(b, [&](const auto& some) {
+        constexpr int N = std::decay_t<decltype(some)>::kSeqs;
+        {
+            ProfScope ps(c, K_PAGED_DECODE);
+            auto go = [&](auto kern) {
+                hipExtLaunchKernelGGL(kern, dim3(nwg), dim3(NT), 0, c->stream, ps.a, ps.b, 0, pv, some, q_gate, k, v, L.q_norm,
+                                      L.k_norm, out, part_o, part_ml, hg, ng, unit, c->n_cu, c->d.eps);
+            };
+            if (hg <= 4) go(paged_decode_mx4<1, N>);
+            else if (hg <= 8) go(paged_decode_mx4<2, N>);
+            else go(paged_decode_mx4<4, N>);
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || (known && whole)) return e;
+        ProfScope ps(c, K_PAGED_DECODE_MERGE);
+        hipExtLaunchKernelGGL((paged_decode_merge<kUnitRows4, N>), dim3(c->d.nh, b.n), dim3(MW * kWave), 0, c->stream, ps.a,
+                              ps.b, 0, pv, some, part_o, part_ml, q_gate, out, hg, ng, nwg, known ? 0 : c->n_cu);
+        return hipGetLastError();
+    });
 }
 
 }  // namespace q35
