@@ -261,9 +261,10 @@ typedef struct q35m_paged q35m_paged;
  * 3/2, 2, 3, 4, 6 times it, with a sign.  s is the smallest with the block's largest value at most
  * 7 2^s, within -23 .. 13; values are rounded to the nearest of these, ties to the even
  * code, and beyond the last one to it: K rows as an fp32 cache holds them, V rows as they
- * come.  Beyond what an fp16 cache's attention rounds (see above), nothing is: the
- * held values take part as they are, and q in a 4-bit cache's scores is held to 2^-19 of
- * the largest value of its 32 dims.  A block with a value that is not finite is NaN, in all of its dims. */
+ * come.  The attention takes the held values as they are; the normed q is held to
+ * 2^-20 of the largest value of its 32 dims (q35m_paged_attn_decode: 2^-24), and the softmax
+ * weights as over an fp16 cache, to no less than 2^-31 of the row's largest.  A block
+ * with a value that is not finite is NaN, in all of its dims. */
 #define Q35M_KV_MXFP4 4
 /* Values that are not finite reach the outputs of the tokens that see their row and
  * no other: an infinite V value makes its dim of the output that infinity, whatever
@@ -330,8 +331,9 @@ int q35m_paged_rows(q35m_paged* p, int layer, int n, const int* seqs, const int*
  * captured into a HIP graph on the context's stream, a replay decodes at the
  * lengths and pages of its time (the checks above are made when a call is
  * enqueued or captured: keep the pages of every row that a replay writes
- * mapped, and shared by nobody).  An eager call leaves short sequences to one
- * workgroup each, a replay does not, so the two may differ in the last bits. */
+ * mapped, and shared by nobody).  Over fp32 and fp16 an eager call leaves short
+ * sequences to one workgroup each, a replay does not, so the two may differ in the
+ * last bits; in 4 bits both are divided alike. */
 int q35m_paged_attn_decode(q35m_paged* p, int layer, int n, const int* seqs, const float* q_gate, const float* k,
                            const float* v, float* out);
 /* q35m_attn_prefill over paged rows, for chunks of new tokens of n sequences
