@@ -11,6 +11,7 @@ from __future__ import annotations
 import array
 import ctypes
 import os
+import struct
 import subprocess
 
 import numpy as np
@@ -105,16 +106,16 @@ def lib() -> ctypes.CDLL:
         _lib.q35m_paged_create.argtypes = [vp, ci, ci, ci, ci, ci, ctypes.POINTER(vp)]
         _lib.q35m_paged_destroy.argtypes = [vp]
         _lib.q35m_paged_map.argtypes = [vp, ci, ci, ci, vp]
-        _lib.q35m_paged_advance.argtypes = [vp, ci, ip, ip]
+        _lib.q35m_paged_advance.argtypes = [vp, ci, vp, vp]
         _lib.q35m_paged_truncate.argtypes = [vp, ci, ci]
         _lib.q35m_paged_len.argtypes = [vp, ci, ip]
         _lib.q35m_paged_device_ptr.argtypes = [vp, ci, ci, ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_size_t)]
-        _lib.q35m_paged_append.argtypes = [vp, ci, ci, ip, ip, vp, vp]
-        _lib.q35m_paged_rows.argtypes = [vp, ci, ci, ip, ip, ip, vp, vp]
+        _lib.q35m_paged_append.argtypes = [vp, ci, ci, vp, vp, vp, vp]
+        _lib.q35m_paged_rows.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp]
         _lib.q35m_paged_plan.argtypes = [vp, ci, vp, vp, vp, ci, vp, ctypes.c_size_t, vp]
         _lib.q35m_paged_tables.argtypes = [vp, ctypes.POINTER(vp), ctypes.POINTER(vp), ip]
-        _lib.q35m_paged_attn_decode.argtypes = [vp, ci, ci, ip, vp, vp, vp, vp]
-        _lib.q35m_paged_attn_prefill.argtypes = [vp, ci, ci, ip, ip, vp, vp, vp, vp]
+        _lib.q35m_paged_attn_decode.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp]
+        _lib.q35m_paged_attn_prefill.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp, vp]
     return _lib
 
 
@@ -319,6 +320,23 @@ def _seqs(seqs):
     if len(seqs) < 8:
         return (ctypes.c_int * len(seqs))(*seqs)
     return (ctypes.c_int * len(seqs)).from_buffer(array.array("i", seqs))
+
+
+_packers = {}
+
+
+def _ints(values):
+    """C ints of a short list as a call takes them: bytes, which are made and passed in half the time of an array."""
+    n = len(values)
+    pack = _packers.get(n)
+    if pack is None:
+        if n > 64:                                          # (more than any call takes)
+            return _seqs(values)
+        pack = _packers[n] = struct.Struct(f"{n}i").pack
+    try:
+        return pack(*values)
+    except struct.error:                                    # (not ints, or too large: what an array does with them)
+        return _seqs(values)
 
 
 class Context:
@@ -560,7 +578,7 @@ class PagedCache:
 
     def advance(self, seqs, tokens) -> None:
         assert len(seqs) == len(tokens)
-        check(lib().q35m_paged_advance(self.handle, len(seqs), _seqs(seqs), _seqs(tokens)))
+        check(_lib.q35m_paged_advance(self.handle, len(seqs), _ints(seqs), _ints(tokens)))
 
     def truncate(self, seq: int, length: int) -> None:
         check(lib().q35m_paged_truncate(self.handle, seq, length))
@@ -582,19 +600,19 @@ class PagedCache:
     def append(self, layer, seqs, tokens, k, v) -> None:
         """tokens[i] new rows of sequence seqs[i] from k, v [sum(tokens)][kv_heads*256]."""
         assert len(seqs) == len(tokens)
-        check(lib().q35m_paged_append(self.handle, layer, len(seqs), _seqs(seqs), _seqs(tokens), k.ptr, v.ptr))
+        check(_lib.q35m_paged_append(self.handle, layer, len(seqs), _ints(seqs), _ints(tokens), k.ptr, v.ptr))
 
     def rows(self, layer, seqs, first, count, k, v) -> None:
         """Rows first[i], ... (count[i] of them) of sequence seqs[i] as the cache holds
         them, in fp32, to k, v [sum(count)][kv_heads*256]."""
         assert len(seqs) == len(first) == len(count)
-        check(lib().q35m_paged_rows(self.handle, layer, len(seqs), _seqs(seqs), _seqs(first), _seqs(count), k.ptr, v.ptr))
+        check(_lib.q35m_paged_rows(self.handle, layer, len(seqs), _ints(seqs), _ints(first), _ints(count), k.ptr, v.ptr))
 
     def plan(self, n, rows, tokens, free, slots, taken) -> None:
         """Tables and lengths of sequences 0 .. n - 1 from device arrays (.ptr, .nbytes): rows,
         tokens [n] int32, free pages int32; slots int64, taken [n] int32 are written."""
         assert min(rows.nbytes, tokens.nbytes, taken.nbytes) >= 4 * n
-        check(lib().q35m_paged_plan(self.handle, n, rows.ptr, tokens.ptr, free.ptr, free.nbytes // 4, slots.ptr,
+        check(_lib.q35m_paged_plan(self.handle, n, rows.ptr, tokens.ptr, free.ptr, free.nbytes // 4, slots.ptr,
                                     slots.nbytes // 8, taken.ptr))
 
     def tables(self):
@@ -604,12 +622,12 @@ class PagedCache:
         return t.value, n.value, m.value
 
     def attn_decode(self, layer, seqs, q_gate, k, v, out) -> None:
-        check(lib().q35m_paged_attn_decode(self.handle, layer, len(seqs), _seqs(seqs), q_gate.ptr, k.ptr, v.ptr,
+        check(_lib.q35m_paged_attn_decode(self.handle, layer, len(seqs), _ints(seqs), q_gate.ptr, k.ptr, v.ptr,
                                            out.ptr))
 
     def attn_prefill(self, layer, seqs, tokens, q_gate, k, v, out) -> None:
         assert len(seqs) == len(tokens)
-        check(lib().q35m_paged_attn_prefill(self.handle, layer, len(seqs), _seqs(seqs), _seqs(tokens), q_gate.ptr,
+        check(_lib.q35m_paged_attn_prefill(self.handle, layer, len(seqs), _ints(seqs), _ints(tokens), q_gate.ptr,
                                             k.ptr, v.ptr, out.ptr))
 
 
