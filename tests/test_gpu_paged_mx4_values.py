@@ -305,3 +305,28 @@ def test_replayed_chunks_are_divided_alike(lens, tokens):
             for s, n in enumerate(lens):
                 p.c.truncate(s, n // 3)
         end()
+
+
+# ------------------------------------------------------------------ queries of every size
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_queries_of_every_size(T):
+    """q rows of zeros, of values whose squares vanish in fp32, of one value among zeros, of sizes 2^-12 apart within a
+    block, and norm weights of 8.  The last make scores 8 times test_gpu_paged_mx4.py's, and so 8 times what q's rounding
+    leaves of them, 1.9e-5, with the sums' 9e-6: 6e-5 covers two deviations of both together."""
+    with Mx4(max_rows=512, page_rows=32) as p:
+        p.w["q_norm"][:] = 7
+        p.ctx.set_attn_weights(0, p.w)
+        p.seed_rows([333], salt=2)
+        x = {k: v.copy() for k, v in p.inputs(T, salt=3).items()}
+        q = x["q_gate"].reshape(T, p.nh, 2, HD)[:, :, 0]
+        q[:, 0] = 0
+        q[:, 1] *= np.float32(1e-30)
+        q[:, 2, 1:] = 0
+        q[:, 3] *= np.exp2(np.random.RandomState(4).randint(-12, 1, (T, HD))).astype(np.float32)
+        q[:, 4] *= np.float32(1e15)
+        out = p.ctx.array((T, p.nh * HD))
+        d = p.dev(x, "q_gate", "k", "v")
+        p.c.attn_decode(0, [0], *d, out) if T == 1 else p.c.attn_prefill(0, [0], [T], *d, out)
+        p.put([0], [T], x)
+        say(close_to(out.download(), p.attend([0], [T], x), tol=6e-5))
