@@ -317,9 +317,12 @@ class DeviceBytes(DeviceArray):
 
 
 def _seqs(seqs):
-    if len(seqs) < 8:
-        return (ctypes.c_int * len(seqs))(*seqs)
-    return (ctypes.c_int * len(seqs)).from_buffer(array.array("i", seqs))
+    if len(seqs) >= 8:                                      # (half the time of an array's own way)
+        try:
+            return (ctypes.c_int * len(seqs)).from_buffer(array.array("i", seqs))
+        except OverflowError:
+            pass
+    return (ctypes.c_int * len(seqs))(*seqs)
 
 
 _packers = {}

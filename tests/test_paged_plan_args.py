@@ -64,3 +64,18 @@ def test_the_rows_restatement():
     assert pool.shape == (1, 1, 136 * 32) and pool[0, 0, 128 * 32 + 128 + 16 * 3 + 5] == scales[16 + 5, 3]
     back = mx4_rows.from_pool(1, pool, 32)
     assert np.array_equal(back[0][0, 0], codes[:32]) and np.array_equal(back[1][0, 0], scales[:32])
+
+
+def test_lists_as_the_calls_take_them():
+    """The front end's short and long lists: C ints of the same values, wrapped where too large, refused where not whole."""
+    import pytest
+    for n in (0, 1, 3, 7, 8, 64, 65, 200):
+        v = [(37 * i) % 101 - 50 for i in range(n)]
+        for given in (v, tuple(v), np.array(v, np.int64), np.array(v, np.int32)):
+            assert np.array_equal(np.frombuffer(q35mix._ints(given), np.int32) if n else [], v)
+            assert list(q35mix._seqs(given)) == v
+    for n in (1, 8):
+        assert list(q35mix._ints([2 ** 31] * n)) == list(q35mix._seqs([2 ** 31] * n)) == [-2 ** 31] * n
+        for f in (q35mix._ints, q35mix._seqs):
+            with pytest.raises(TypeError):
+                f([1.5] * n)
