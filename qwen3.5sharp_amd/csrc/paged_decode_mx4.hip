@@ -526,6 +526,7 @@ hipError_t launch_paged_decode_mx4(q35m_paged* p, int layer, const PagedBatch& b
     q35m_ctx* c = p->ctx;
     const int per_kv = c->d.nh / c->d.nkv;
     const int hg = per_kv <= 16 ? per_kv : per_kv % 16 == 0 ? 16 : 8;
+    // (16 heads take 470 of a lane's 512 registers: one workgroup a CU)
     const int ng = per_kv / hg, nwg = c->n_cu * (hg <= 8 ? 2 : 1);
     float* part_o = p->work;
     float* part_ml = part_o + (size_t)2 * nwg * kPagedDecodeHeads * kHd;
