@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void paged_append_rows(PagedView pv, PagedBatc
     if (pos >= pv.max_rows) return;
     const int page = page_of(pv.table + (size_t)seq * pv.max_pages, pos >> pv.page_shift, pv.max_pages, pv.n_pages);
     if (page < 0) return;
-    const float4 y = paged_key_row(xk, pv.rope + (size_t)pos * kRopeDim, k_norm, lane, eps);
+    const float4 y = paged_key_row<std::is_same_v<T, Mx4>>(xk, pv.rope + (size_t)pos * kRopeDim, k_norm, lane, eps);
     if constexpr (std::is_same_v<T, Mx4>) {
         const int in = pos & ((1 << pv.page_shift) - 1);
         mx_put_key((uint8_t*)pv.k + mx_page(pv, page, kvh), pv, in, mx_round(y), lane);

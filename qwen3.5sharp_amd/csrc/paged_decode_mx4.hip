@@ -397,7 +397,7 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
         // The wave that holds the new row makes it (every head group needs it;
         // one writes it to the page, and none reads it from there).
         if (has_new) {
-            const MxLane yk = mx_round(paged_key_row(xk, cs, sn, reinterpret_cast<const float4*>(norms[1])[lane], lane, (double)eps)), yv = mx_round(xv);
+            const MxLane yk = mx_round(paged_key_row<true>(xk, cs, sn, reinterpret_cast<const float4*>(norms[1])[lane], lane, (double)eps)), yv = mx_round(xv);
             uint8_t* const kn = newrow[wave][0];
             uint8_t* const vn = newrow[wave][1];
             reinterpret_cast<uint16_t*>(kn)[lane] = (uint16_t)yk.codes;
