@@ -223,20 +223,38 @@ class _Foreign:
 
 
 class _Owner:
-    """A context and its paged cache, closed once neither the state nor a view of their memory is left."""
+    """A context and its paged cache, as a program makes them once and keeps them while conversations come and go: another
+    state's once neither this state nor a view of their memory is left."""
+    kept = {}                       # those of the last shape that no state has
 
     def __init__(self, case, per, pool, x=None):
         here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "qwen3.5sharp_amd")
         if here not in sys.path:
             sys.path.insert(0, here)
         import q35mix
-        self.ctx = q35mix.Context(q35mix.qwen35_config(num_layers=1, num_heads=case["nh"], num_kv_heads=case["nkv"],
-                                                       is_recurrent=[0]), n_seqs=1, kv_capacity=16)
+        self.kinds = (q35mix.STATE_KEYS, q35mix.STATE_VALUES)
+        self.key = (case["nh"], case["nkv"], case["n"], per, pool, case["page"], x is None)
+        for key in [k for k in self.kept if k != self.key]:
+            for ctx, cache in self.kept.pop(key):
+                cache.close()
+                ctx.close()
+        if self.kept.get(self.key):
+            self.ctx, self.cache = self.kept[self.key].pop()
+        else:
+            self.ctx = q35mix.Context(q35mix.qwen35_config(num_layers=1, num_heads=case["nh"], num_kv_heads=case["nkv"],
+                                                           is_recurrent=[0]), n_seqs=1, kv_capacity=16)
+            self.cache = q35mix.PagedCache(self.ctx, n_seqs=case["n"], max_rows=per * case["page"], n_pages=pool,
+                                           page_rows=case["page"], kv_type=q35mix.KV_MXFP4)
         if x is not None:
             self.ctx.set_attn_weights(0, {k: x[k].cpu().numpy() for k in ("q_norm", "k_norm")})
-        self.cache = q35mix.PagedCache(self.ctx, n_seqs=case["n"], max_rows=per * case["page"], n_pages=pool,
-                                       page_rows=case["page"], kv_type=q35mix.KV_MXFP4)
-        self.kinds = (q35mix.STATE_KEYS, q35mix.STATE_VALUES)
+
+    def hold(self, lens, table):
+        """The conversations' pages and lengths, in place of the ones before."""
+        for i, (rows, pages) in enumerate(zip(lens, table)):
+            if self.cache.length(i) > rows:
+                self.cache.truncate(i, rows)
+            self.cache.map(i, 0, pages)
+        self.cache.advance(list(range(len(lens))), [rows - self.cache.length(i) for i, rows in enumerate(lens)])
 
     def put(self, which, codes, scales):
         """One pool's contents in the library's layout: of each (page, kv head) the rows' codes, then their scales, K's by
@@ -256,9 +274,7 @@ class _Owner:
 
     def __del__(self):
         if hasattr(self, "cache"):
-            self.cache.close()
-        if hasattr(self, "ctx"):
-            self.ctx.close()
+            self.kept.setdefault(self.key, []).append((self.ctx, self.cache))
 
 
 class _Buf:
@@ -276,8 +292,8 @@ def _prepare_plan(case, seed):
     s = {"case": case, "x": x, "pool": pool, "slots": torch.empty(int(counts.sum()), device="cuda", dtype=torch.int64),
          "taken": torch.empty(case["n"], device="cuda", dtype=torch.int32)}
     if own:
-        # the library's cache: its table holds the pages of the cached rows
-        s["owner"] = _Owner(case, per, pool)
+        # the library's cache: its table holds the pages of the cached rows, which a plan does not touch (one head)
+        s["owner"] = _Owner({**case, "nh": 1, "nkv": 1}, per, pool)
         s["cache"] = s["owner"].cache
         s["table"], s["lens"] = s["owner"].tables()
         s["args"] = [_Buf(t) for t in (x["rows"], x["tokens"], x["free"], s["slots"], s["taken"])]
@@ -302,12 +318,10 @@ def prepare(case, seed):
         s["out"] = torch.zeros(rows, case["nh"] * HD, device="cuda", dtype=torch.float32)
     pools = [_pool(case, seed, which, pool) for which in range(2)]
     if own:
-        # the library's cache: its pages are its own memory, the tables are set and checked once
+        # the library's cache: its pages are its own memory, its tables are set and checked as conversations come
         s["owner"] = _Owner(case, per, pool, x)
         s["cache"], s["seqs"], s["lens"], s["counts"] = s["owner"].cache, list(range(n)), lens, counts
-        for i in range(n):
-            s["cache"].map(i, 0, table[i])
-        s["cache"].advance(s["seqs"], lens)
+        s["owner"].hold(lens, table)
         for which in range(2):
             s["owner"].put(which, *pools[which])
         s["args"] = [_Buf(x[k]) for k in (("k", "v") if case["kind"] == "append" else ("q_gate", "k", "v"))]
