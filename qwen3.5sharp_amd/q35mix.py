@@ -30,6 +30,11 @@ _lib = None
 _hip = None
 
 
+class _Paged:
+    """Entry points of the paged cache as PagedCache calls them: with lists as bytes (_ints), which the library's own
+    prototypes, pointers to C ints, do not take."""
+
+
 class Q35Error(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"q35mix error {code}: {msg}")
@@ -106,16 +111,20 @@ def lib() -> ctypes.CDLL:
         _lib.q35m_paged_create.argtypes = [vp, ci, ci, ci, ci, ci, ctypes.POINTER(vp)]
         _lib.q35m_paged_destroy.argtypes = [vp]
         _lib.q35m_paged_map.argtypes = [vp, ci, ci, ci, vp]
-        _lib.q35m_paged_advance.argtypes = [vp, ci, vp, vp]
+        _lib.q35m_paged_advance.argtypes = [vp, ci, ip, ip]
         _lib.q35m_paged_truncate.argtypes = [vp, ci, ci]
         _lib.q35m_paged_len.argtypes = [vp, ci, ip]
         _lib.q35m_paged_device_ptr.argtypes = [vp, ci, ci, ctypes.POINTER(vp), ctypes.POINTER(ctypes.c_size_t)]
-        _lib.q35m_paged_append.argtypes = [vp, ci, ci, vp, vp, vp, vp]
-        _lib.q35m_paged_rows.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp]
+        _lib.q35m_paged_append.argtypes = [vp, ci, ci, ip, ip, vp, vp]
+        _lib.q35m_paged_rows.argtypes = [vp, ci, ci, ip, ip, ip, vp, vp]
         _lib.q35m_paged_plan.argtypes = [vp, ci, vp, vp, vp, ci, vp, ctypes.c_size_t, vp]
         _lib.q35m_paged_tables.argtypes = [vp, ctypes.POINTER(vp), ctypes.POINTER(vp), ip]
-        _lib.q35m_paged_attn_decode.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp]
-        _lib.q35m_paged_attn_prefill.argtypes = [vp, ci, ci, vp, vp, vp, vp, vp, vp]
+        _lib.q35m_paged_attn_decode.argtypes = [vp, ci, ci, ip, vp, vp, vp, vp]
+        _lib.q35m_paged_attn_prefill.argtypes = [vp, ci, ci, ip, ip, vp, vp, vp, vp]
+        for name in ("advance", "append", "rows", "attn_decode", "attn_prefill"):
+            call = _lib["q35m_paged_" + name]                # (a function object of its own)
+            call.argtypes = [vp if a is ip else a for a in getattr(_lib, "q35m_paged_" + name).argtypes]
+            setattr(_Paged, name, call)
     return _lib
 
 
@@ -581,7 +590,7 @@ class PagedCache:
 
     def advance(self, seqs, tokens) -> None:
         assert len(seqs) == len(tokens)
-        check(_lib.q35m_paged_advance(self.handle, len(seqs), _ints(seqs), _ints(tokens)))
+        check(_Paged.advance(self.handle, len(seqs), _ints(seqs), _ints(tokens)))
 
     def truncate(self, seq: int, length: int) -> None:
         check(lib().q35m_paged_truncate(self.handle, seq, length))
@@ -603,13 +612,13 @@ class PagedCache:
     def append(self, layer, seqs, tokens, k, v) -> None:
         """tokens[i] new rows of sequence seqs[i] from k, v [sum(tokens)][kv_heads*256]."""
         assert len(seqs) == len(tokens)
-        check(_lib.q35m_paged_append(self.handle, layer, len(seqs), _ints(seqs), _ints(tokens), k.ptr, v.ptr))
+        check(_Paged.append(self.handle, layer, len(seqs), _ints(seqs), _ints(tokens), k.ptr, v.ptr))
 
     def rows(self, layer, seqs, first, count, k, v) -> None:
         """Rows first[i], ... (count[i] of them) of sequence seqs[i] as the cache holds
         them, in fp32, to k, v [sum(count)][kv_heads*256]."""
         assert len(seqs) == len(first) == len(count)
-        check(_lib.q35m_paged_rows(self.handle, layer, len(seqs), _ints(seqs), _ints(first), _ints(count), k.ptr, v.ptr))
+        check(_Paged.rows(self.handle, layer, len(seqs), _ints(seqs), _ints(first), _ints(count), k.ptr, v.ptr))
 
     def plan(self, n, rows, tokens, free, slots, taken) -> None:
         """Tables and lengths of sequences 0 .. n - 1 from device arrays (.ptr, .nbytes): rows,
@@ -625,13 +634,12 @@ class PagedCache:
         return t.value, n.value, m.value
 
     def attn_decode(self, layer, seqs, q_gate, k, v, out) -> None:
-        check(_lib.q35m_paged_attn_decode(self.handle, layer, len(seqs), _ints(seqs), q_gate.ptr, k.ptr, v.ptr,
-                                           out.ptr))
+        check(_Paged.attn_decode(self.handle, layer, len(seqs), _ints(seqs), q_gate.ptr, k.ptr, v.ptr, out.ptr))
 
     def attn_prefill(self, layer, seqs, tokens, q_gate, k, v, out) -> None:
         assert len(seqs) == len(tokens)
-        check(_lib.q35m_paged_attn_prefill(self.handle, layer, len(seqs), _ints(seqs), _ints(tokens), q_gate.ptr,
-                                            k.ptr, v.ptr, out.ptr))
+        check(_Paged.attn_prefill(self.handle, layer, len(seqs), _ints(seqs), _ints(tokens), q_gate.ptr, k.ptr, v.ptr,
+                                  out.ptr))
 
 
 # ---- HIP event timing on the context stream ------------------------------
