@@ -31,7 +31,7 @@ _hip = None
 
 
 class _Paged:
-    """Entry points of the paged cache as PagedCache calls them: with lists as bytes (_ints), which the library's own
+    """Entry points of the paged cache as PagedCache calls them: with lists as bytes (_list), which the library's own
     prototypes, pointers to C ints, do not take."""
 
 
@@ -351,6 +351,14 @@ def _ints(values):
         return _seqs(values)
 
 
+def _list(values):
+    """A paged call's list, refused where a value is no C int: cut to 32 bits it would name another sequence or count."""
+    got = _ints(values)
+    if type(got) is not bytes and any(a != b for a, b in zip(got, values)):
+        raise ValueError(f"a list of {len(values)} values, not all of them 32-bit integers")
+    return got
+
+
 class Context:
     """One q35m_ctx: the mixer state of every layer for n_seqs sequences."""
 
@@ -590,7 +598,7 @@ class PagedCache:
 
     def advance(self, seqs, tokens) -> None:
         assert len(seqs) == len(tokens)
-        check(_Paged.advance(self.handle, len(seqs), _ints(seqs), _ints(tokens)))
+        check(_Paged.advance(self.handle, len(seqs), _list(seqs), _list(tokens)))
 
     def truncate(self, seq: int, length: int) -> None:
         check(lib().q35m_paged_truncate(self.handle, seq, length))
@@ -612,13 +620,13 @@ class PagedCache:
     def append(self, layer, seqs, tokens, k, v) -> None:
         """tokens[i] new rows of sequence seqs[i] from k, v [sum(tokens)][kv_heads*256]."""
         assert len(seqs) == len(tokens)
-        check(_Paged.append(self.handle, layer, len(seqs), _ints(seqs), _ints(tokens), k.ptr, v.ptr))
+        check(_Paged.append(self.handle, layer, len(seqs), _list(seqs), _list(tokens), k.ptr, v.ptr))
 
     def rows(self, layer, seqs, first, count, k, v) -> None:
         """Rows first[i], ... (count[i] of them) of sequence seqs[i] as the cache holds
         them, in fp32, to k, v [sum(count)][kv_heads*256]."""
         assert len(seqs) == len(first) == len(count)
-        check(_Paged.rows(self.handle, layer, len(seqs), _ints(seqs), _ints(first), _ints(count), k.ptr, v.ptr))
+        check(_Paged.rows(self.handle, layer, len(seqs), _list(seqs), _list(first), _list(count), k.ptr, v.ptr))
 
     def plan(self, n, rows, tokens, free, slots, taken) -> None:
         """Tables and lengths of sequences 0 .. n - 1 from device arrays (.ptr, .nbytes): rows,
@@ -634,11 +642,11 @@ class PagedCache:
         return t.value, n.value, m.value
 
     def attn_decode(self, layer, seqs, q_gate, k, v, out) -> None:
-        check(_Paged.attn_decode(self.handle, layer, len(seqs), _ints(seqs), q_gate.ptr, k.ptr, v.ptr, out.ptr))
+        check(_Paged.attn_decode(self.handle, layer, len(seqs), _list(seqs), q_gate.ptr, k.ptr, v.ptr, out.ptr))
 
     def attn_prefill(self, layer, seqs, tokens, q_gate, k, v, out) -> None:
         assert len(seqs) == len(tokens)
-        check(_Paged.attn_prefill(self.handle, layer, len(seqs), _ints(seqs), _ints(tokens), q_gate.ptr, k.ptr, v.ptr,
+        check(_Paged.attn_prefill(self.handle, layer, len(seqs), _list(seqs), _list(tokens), q_gate.ptr, k.ptr, v.ptr,
                                   out.ptr))
 
 

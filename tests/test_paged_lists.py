@@ -25,3 +25,39 @@ def test_prototypes_take_pointers_to_c_ints_alone(name):
             args[at] = wrong
             with pytest.raises(ctypes.ArgumentError):
                 call(*args)
+
+
+BIG = (2 ** 32, 2 ** 32 + 1, 2 ** 31, -2 ** 31 - 1, 2 ** 70)
+
+
+@pytest.mark.parametrize("n", [1, 3, 8, 64, 65])
+def test_calls_refuse_values_that_are_no_c_ints(n):
+    """Cut to 32 bits they would be another conversation's number, or another count of rows."""
+    c = object.__new__(q35mix.PagedCache)
+    c.handle = None                                             # (what is not refused before ends at the null handle)
+    x = type("Null", (), {"ptr": None})()
+    good = list(range(n))
+
+    def calls(lists):
+        yield lambda: c.advance(lists(0), lists(1))
+        yield lambda: c.append(0, lists(0), lists(1), x, x)
+        yield lambda: c.rows(0, lists(0), lists(1), lists(2), x, x)
+        yield lambda: c.attn_decode(0, lists(0), x, x, x, x)
+        yield lambda: c.attn_prefill(0, lists(0), lists(1), x, x, x, x)
+
+    for call in calls(lambda k: good):
+        with pytest.raises(q35mix.Q35Error):
+            call()
+    for big in BIG:
+        for where in (0, 1, 2):
+            for kind in (list, tuple, np.array):
+                if kind is np.array and abs(big) > 2 ** 40:
+                    continue
+                bad = kind(good[:-1] + [big])
+                for k, call in enumerate(calls(lambda k: bad if k == where else good)):
+                    if where < (2, 2, 3, 1, 2)[k]:
+                        with pytest.raises(ValueError):
+                            call()
+    for wrong in ([1.5] * n, ["a"] * n, [None] * n):
+        with pytest.raises(TypeError):
+            c.advance(wrong, good)
