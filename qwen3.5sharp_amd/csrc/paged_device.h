@@ -19,13 +19,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // makes of pointers whose origin it has lost, are waited for at every LDS barrier.
 template <typename T>
 __device__ __forceinline__ T from_global(const void* p) {
-    typedef const __attribute__((address_space(1))) u32x4 vec;
-    if constexpr (std::is_same_v<T, float4>) {             // (a struct, which has no such copy)
-        const u32x4 x = *(vec*)(uintptr_t)p;
-        return make_float4(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3]));
-    } else {
-        return *(const __attribute__((address_space(1))) T*)(uintptr_t)p;
-    }
+    return *(const __attribute__((address_space(1))) T*)(uintptr_t)p;
 }
 __device__ __forceinline__ void to_global(void* p, float4 x) {
     typedef __attribute__((address_space(1))) f32x4 vec;
