@@ -1,0 +1,73 @@
+"""States of the performance cases of the 4-bit cache: a program makes its context and cache once and keeps them, so a new
+state takes those that an earlier one has left, and gives what one of its own handles gives.
+"""
+import importlib.util
+import os
+
+import pytest
+
+import q35mix
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+A = {"nh": 16, "nkv": 4, "page": 16, "ragged": True, "n": 3}
+CASES = [{"kind": "append", "rows": 40, "tokens": 20, **A}, {"kind": "decode", "rows": 300, "tokens": 1, **A},
+         {"kind": "prefill", "rows": 90, "tokens": 33, **A}, {"kind": "plan", "rows": 200, "tokens": 30, "short": 1, **A}]
+
+
+@pytest.fixture
+def cases(monkeypatch):
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "perf", "more_operators.py")
+    spec = importlib.util.spec_from_file_location("more_operators", at)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    m.own, m.made = True, []
+
+    class Counted(q35mix.PagedCache):
+        def __init__(self, *a, **k):
+            m.made.append(k)
+            super().__init__(*a, **k)
+    monkeypatch.setattr(q35mix, "PagedCache", Counted)
+    yield m
+    for handles in m._Owner.kept.values():
+        for ctx, cache in handles:
+            cache.close()
+            ctx.close()
+
+
+def answer(m, state):
+    got = m.run(state)
+    torch.cuda.synchronize()
+    return {k: t.clone() for k, t in got.items()}
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: c["kind"])
+def test_a_new_state_takes_the_handles_that_are_free(cases, case):
+    first = {seed: answer(cases, cases.prepare(case, seed)) for seed in (1, 2, 3)}
+    assert len(cases.made) == 1
+    a, b = cases.prepare(case, 1), cases.prepare(case, 2)           # two at once: handles of their own
+    assert len(cases.made) == 2 and a["cache"] is not b["cache"]
+    for _ in range(2):
+        for seed, s in ((1, a), (2, b)):
+            got = answer(cases, s)
+            assert all(torch.equal(got[k], first[seed][k]) for k in got)
+    del a, s
+    c = cases.prepare(case, 3)
+    assert len(cases.made) == 2
+    got = answer(cases, c)
+    assert all(torch.equal(got[k], first[3][k]) for k in got)
+    assert any(not torch.equal(first[1][k], first[3][k]) for k in got)
+
+
+def test_other_lengths_and_shapes(cases):
+    """Fewer and more rows in the same handles; another shape closes those that nobody has."""
+    short, long = {**CASES[2], "rows": 85}, {**CASES[2], "rows": 88}          # (8 pages a sequence at most, both)
+    want = {}
+    for c in (long, short, long):
+        got = answer(cases, cases.prepare(c, 5))
+        for k in got:
+            assert torch.equal(want.setdefault((c["rows"], k), got[k]), got[k])
+    assert len(cases.made) == 1
+    answer(cases, cases.prepare({**CASES[2], "nh": 8}, 5))
+    assert len(cases.made) == 2 and len(cases._Owner.kept) == 1
