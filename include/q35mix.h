@@ -361,7 +361,8 @@ int q35m_paged_attn_prefill(q35m_paged* p, int layer, int n, const int* seqs, co
  * 65535 requests.
  * rows and tokens are taken within 0 and max_rows, in that order; page ids of the list
  * outside [0, n_pages) count as no page.  Arrays that are written overlap no other one and
- * not the cache's own (Q35M_ERR_INVALID); rows may be the cache's lengths (below).
+ * none of the cache's memory, its pages and workspace among it (Q35M_ERR_INVALID); rows may be the
+ * cache's lengths (below).
  * A first call gives the lengths and tables over to the device: q35m_paged_map, _advance,
  * _truncate and _len are refused from then on (Q35M_ERR_INVALID), the operators above
  * no longer check lengths or pages but bring up to max_rows rows a sequence, leave out rows

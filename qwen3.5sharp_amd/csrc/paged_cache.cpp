@@ -151,28 +151,26 @@ int not_capturing(const q35m_paged* p, const char* what) {
     return Q35M_OK;
 }
 
-// Whether what a plan writes is also what it reads, or writes elsewhere: requests are planned
-// side by side.  (rows may be the lengths themselves, which it leaves as it reads them.)
-struct Span {
-    const void* at;
-    size_t bytes;
-    bool meets(const Span& o) const {
-        const uintptr_t a = (uintptr_t)at, b = (uintptr_t)o.at;
-        return bytes && o.bytes && (a < b ? b - a < bytes : a - b < o.bytes);
-    }
-};
+// Whether what a plan writes is also what it reads, or writes elsewhere (requests are planned
+// side by side), or other memory of the cache.  (rows may be the lengths themselves, which it leaves
+// as it reads them.)
 bool plan_overlaps(const q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
                    const int64_t* slots, size_t n_slots, const int* taken) {
+    using q35::Span;
     const size_t seqs = (size_t)p->map.n_seqs(), most = (size_t)n * p->map.max_rows();
     const Span in[] = {{rows, n * sizeof(int)}, {tokens, n * sizeof(int)}, {free_pages, n_free * sizeof(int)}};
-    const Span out[] = {{slots, std::min(n_slots, most) * sizeof(int64_t)}, {taken, n * sizeof(int)},
-                        {p->dev_table, seqs * p->map.max_pages() * sizeof(int)}, {p->dev_len, seqs * sizeof(int)}};
+    const Span out[] = {{slots, std::min(n_slots, most) * sizeof(int64_t)}, {taken, n * sizeof(int)}};
+    const Span own[] = {{p->dev_table, seqs * p->map.max_pages() * sizeof(int)}, {p->dev_len, seqs * sizeof(int)}};
+    if (out[0].meets(out[1])) return true;
     for (const Span& o : out) {
         for (const Span& i : in)
-            if (o.meets(i) && !(&i == &in[0] && &o == &out[3] && i.at == o.at)) return true;
-        for (const Span& x : out)
-            if (&o != &x && o.meets(x)) return true;
+            if (o.meets(i)) return true;
+        for (const Span& x : p->allocations)
+            if (o.meets(x)) return true;
     }
+    for (const Span& o : own)
+        for (const Span& i : in)
+            if (o.meets(i) && !(&i == &in[0] && &o == &own[1] && i.at == o.at)) return true;
     return false;
 }
 
@@ -183,14 +181,14 @@ int not_planned(const q35m_paged* p, const char* what) {
 
 void release(q35m_paged* p) {
     if (p->ctx->stream) (void)hipStreamSynchronize(p->ctx->stream);
-    for (void* x : p->allocations) (void)hipFree(x);
+    for (const q35::Span& x : p->allocations) (void)hipFree(const_cast<void*>(x.at));
     p->allocations.clear();
 }
 
 int alloc(q35m_paged* p, void** x, size_t bytes, bool zero) {
     *x = nullptr;
     PHIP_TRY(hipMalloc(x, bytes), "hipMalloc");
-    p->allocations.push_back(*x);
+    p->allocations.push_back({*x, bytes});
     if (zero) PHIP_TRY(hipMemsetAsync(*x, 0, bytes, p->ctx->stream), "hipMemsetAsync");
     return Q35M_OK;
 }

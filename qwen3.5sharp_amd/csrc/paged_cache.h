@@ -2,6 +2,7 @@
 // call and the launchers (paged_cache.cpp holds the C entry points).
 #pragma once
 
+#include <cstdint>
 #include <vector>
 
 #include "page_map.h"
@@ -59,6 +60,16 @@ constexpr int kPagedTileRows = 64;       // query rows of a prefill workgroup
 // i, and 8 block scales, one of 32 dims each.
 constexpr int kMxCodes = kHd / 2, kMxBlock = 32, kMxBlocks = kHd / kMxBlock, kMxRow = kMxCodes + kMxBlocks;
 
+// Memory of the device.
+struct Span {
+    const void* at;
+    size_t bytes;
+    bool meets(const Span& o) const {
+        const uintptr_t a = (uintptr_t)at, b = (uintptr_t)o.at;
+        return bytes && o.bytes && (a < b ? b - a < bytes : a - b < o.bytes);
+    }
+};
+
 }  // namespace q35
 
 struct q35m_paged {
@@ -73,7 +84,7 @@ struct q35m_paged {
     double* rope = nullptr;
     float* work = nullptr;               // partial results of one attention call
     size_t work_bytes = 0;
-    std::vector<void*> allocations;
+    std::vector<q35::Span> allocations;
     bool planned = false;                // q35m_paged_plan has run: lengths and tables are the device's alone
 
     q35m_paged(int n_seqs, int max_rows, int n_pages_, int page_rows)
