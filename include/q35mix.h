@@ -359,8 +359,9 @@ int q35m_paged_attn_prefill(q35m_paged* p, int layer, int n, const int* seqs, co
  * by the row in it: page * page_rows + row; -1 where the token has no page) come for the
  * tokens of all requests in order, up to n_slots of them; what is behind stays.  Up to
  * 65535 requests.
- * rows and tokens are taken within 0 and max_rows, in that order; page ids of the list
- * outside [0, n_pages) count as no page.  Arrays that are written overlap no other one and
+ * rows and tokens are taken within 0 and max_rows, in that order; an entry of the list
+ * outside [0, n_pages) is dealt out as the others are and gives no page (taken counts it): a list that
+ * gets shorter is not padded with such, but counted (q35m_paged_plan_listed).  Arrays that are written overlap no other one and
  * none of the cache's memory, its pages and workspace among it (Q35M_ERR_INVALID); rows may be the
  * cache's lengths (below).
  * A first call gives the lengths and tables over to the device: q35m_paged_map, _advance,
@@ -372,6 +373,12 @@ int q35m_paged_attn_prefill(q35m_paged* p, int layer, int n, const int* seqs, co
  * lengths of their time. */
 int q35m_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
                     int64_t* slots, size_t n_slots, int* taken);
+/* The same from a list whose length is the device's too, as in a captured step whose list gets
+ * shorter and longer between replays: of the n_free entries that free_pages has room for the first
+ * *n_listed (DEVICE memory, taken within 0 and n_free) are the list; a request past them is one
+ * that the list is too short for.  NULL: all of them. */
+int q35m_paged_plan_listed(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
+                           const int* n_listed, int64_t* slots, size_t n_slots, int* taken);
 /* Device addresses of the tables [n_seqs][*max_pages] (page ids, -1: not mapped) and
  * the lengths [n_seqs], which the calls on the context's stream read and a plan writes.
  * A caller may set entries of the tables before a plan (a shared prefix's pages); the lengths are

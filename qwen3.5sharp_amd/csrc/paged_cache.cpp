@@ -155,10 +155,11 @@ int not_capturing(const q35m_paged* p, const char* what) {
 // side by side), or other memory of the cache.  (rows may be the lengths themselves, which it leaves
 // as it reads them.)
 bool plan_overlaps(const q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
-                   const int64_t* slots, size_t n_slots, const int* taken) {
+                   const int* n_listed, const int64_t* slots, size_t n_slots, const int* taken) {
     using q35::Span;
     const size_t seqs = (size_t)p->map.n_seqs(), most = (size_t)n * p->map.max_rows();
-    const Span in[] = {{rows, n * sizeof(int)}, {tokens, n * sizeof(int)}, {free_pages, n_free * sizeof(int)}};
+    const Span in[] = {{rows, n * sizeof(int)}, {tokens, n * sizeof(int)}, {free_pages, n_free * sizeof(int)},
+                       {n_listed, n_listed ? sizeof(int) : 0}};
     const Span out[] = {{slots, std::min(n_slots, most) * sizeof(int64_t)}, {taken, n * sizeof(int)}};
     const Span own[] = {{p->dev_table, seqs * p->map.max_pages() * sizeof(int)}, {p->dev_len, seqs * sizeof(int)}};
     if (out[0].meets(out[1])) return true;
@@ -409,8 +410,8 @@ int q35m_paged_rows(q35m_paged* p, int layer, int n, const int* seqs, const int*
     return Q35M_OK;
 }
 
-int q35m_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
-                    int64_t* slots, size_t n_slots, int* taken) {
+int q35m_paged_plan_listed(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
+                           const int* n_listed, int64_t* slots, size_t n_slots, int* taken) {
     if (!p) return pfail(Q35M_ERR_INVALID, "null paged cache");
     if (n < 1 || n > p->map.n_seqs())
         return pfail(Q35M_ERR_CAPACITY, "%d requests (1..%d, the cache's sequences)", n, p->map.n_seqs());
@@ -418,14 +419,20 @@ int q35m_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, co
     if (n_free < 0) return pfail(Q35M_ERR_INVALID, "%d free pages", n_free);
     if (!rows || !tokens || !taken || (!free_pages && n_free) || (!slots && n_slots))
         return pfail(Q35M_ERR_INVALID, "null array of a plan");
-    if (((uintptr_t)rows | (uintptr_t)tokens | (uintptr_t)taken | (uintptr_t)free_pages) & 3 || (uintptr_t)slots & 7)
+    if (((uintptr_t)rows | (uintptr_t)tokens | (uintptr_t)taken | (uintptr_t)free_pages | (uintptr_t)n_listed) & 3 ||
+        (uintptr_t)slots & 7)
         return pfail(Q35M_ERR_INVALID, "arrays of a plan must be aligned to their values");
-    if (plan_overlaps(p, n, rows, tokens, free_pages, n_free, slots, n_slots, taken))
+    if (plan_overlaps(p, n, rows, tokens, free_pages, n_free, n_listed, slots, n_slots, taken))
         return pfail(Q35M_ERR_INVALID, "an array that a plan writes overlaps another one");
     DeviceScope dev(p->ctx->device);
-    PHIP_TRY(q35::launch_paged_plan(p, n, rows, tokens, free_pages, n_free, slots, n_slots, taken), "paged_plan");
+    PHIP_TRY(q35::launch_paged_plan(p, n, rows, tokens, free_pages, n_free, n_listed, slots, n_slots, taken), "paged_plan");
     p->planned = true;
     return Q35M_OK;
+}
+
+int q35m_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
+                    int64_t* slots, size_t n_slots, int* taken) {
+    return q35m_paged_plan_listed(p, n, rows, tokens, free_pages, n_free, nullptr, slots, n_slots, taken);
 }
 
 int q35m_paged_tables(q35m_paged* p, int** table, int** lens, int* max_pages) {

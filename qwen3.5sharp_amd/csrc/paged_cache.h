@@ -122,8 +122,9 @@ struct PagedFirstOf {
 };
 using PagedFirst = PagedFirstOf<kMaxBatch>;
 hipError_t launch_paged_rows(q35m_paged* p, int layer, const PagedBatch& b, const PagedFirst& first, float* k, float* v);
+// n_listed: null, or how many of the n_free pages there are, read on the device.
 hipError_t launch_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
-                             int64_t* slots, size_t n_slots, int* taken);
+                             const int* n_listed, int64_t* slots, size_t n_slots, int* taken);
 size_t paged_decode_work_bytes(const q35m_ctx* c);
 hipError_t launch_paged_decode(q35m_paged* p, int layer, const PagedBatch& b, const float* q_gate, const float* k,
                                const float* v, float* out);

@@ -2,7 +2,8 @@
 //
 // Request i holds R_i rows, in the first have_i = ceil(R_i / P) entries of its table, and
 // brings T_i tokens, for which it needs need_i = ceil((R_i + T_i) / P) - have_i pages more.
-// With c_i the sum of need_j over j < i and o_i that of T_j:
+// With c_i the sum of need_j over j < i, o_i that of T_j, and n_free the list's length as the host
+// or, in n_listed, the device has it:
 //   table[i][have_i + e] = free[c_i + e], e < need_i, if need_i = 0 or c_i + need_i <= n_free, else -1
 //   table[i][e] = -1 behind these
 //   slots[o_i + t] = P table[i][(R_i + t) / P] + (R_i + t) % P
@@ -28,10 +29,12 @@ __device__ __forceinline__ long plan_sum(long v) {
 }
 
 __global__ __launch_bounds__(PT) void paged_plan(int* __restrict__ table, int* lens, const int* rows, const int* tokens,
-                                                 const int* __restrict__ free_pages, long n_free,
-                                                 int64_t* __restrict__ slots, size_t n_slots, int* __restrict__ taken,
-                                                 int max_rows, int max_pages, int n_pages, int shift) {
+                                                 const int* __restrict__ free_pages, int n_free,
+                                                 const int* __restrict__ n_listed, int64_t* __restrict__ slots,
+                                                 size_t n_slots, int* __restrict__ taken, int max_rows, int max_pages,
+                                                 int n_pages, int shift) {
     const int tid = threadIdx.x, i = blockIdx.y;
+    if (n_listed) n_free = min(max(*n_listed, 0), n_free);
     struct Need {
         int rows, tokens, have, more;
     };
@@ -87,7 +90,7 @@ __global__ __launch_bounds__(PT) void paged_plan(int* __restrict__ table, int* l
 }  // namespace
 
 hipError_t launch_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
-                             int64_t* slots, size_t n_slots, int* taken) {
+                             const int* n_listed, int64_t* slots, size_t n_slots, int* taken) {
     q35m_ctx* c = p->ctx;
     // Workgroups a request: four a CU over all requests, and none without an entry or a
     // token of its own.
@@ -96,7 +99,7 @@ hipError_t launch_paged_plan(q35m_paged* p, int n, const int* rows, const int* t
     x = x < 1 ? 1 : x > most ? most : x;
     ProfScope ps(c, K_PAGED_PLAN);
     hipExtLaunchKernelGGL(paged_plan, dim3(x, n), dim3(PT), 0, c->stream, ps.a, ps.b, 0, p->dev_table, p->dev_len, rows, tokens,
-                          free_pages, (long)n_free, slots, n_slots, taken, p->map.max_rows(), p->map.max_pages(),
+                          free_pages, n_free, n_listed, slots, n_slots, taken, p->map.max_rows(), p->map.max_pages(),
                           p->n_pages, p->page_shift);
     return hipGetLastError();
 }

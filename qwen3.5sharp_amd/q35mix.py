@@ -118,6 +118,7 @@ def lib() -> ctypes.CDLL:
         _lib.q35m_paged_append.argtypes = [vp, ci, ci, ip, ip, vp, vp]
         _lib.q35m_paged_rows.argtypes = [vp, ci, ci, ip, ip, ip, vp, vp]
         _lib.q35m_paged_plan.argtypes = [vp, ci, vp, vp, vp, ci, vp, ctypes.c_size_t, vp]
+        _lib.q35m_paged_plan_listed.argtypes = [vp, ci, vp, vp, vp, ci, vp, vp, ctypes.c_size_t, vp]
         _lib.q35m_paged_tables.argtypes = [vp, ctypes.POINTER(vp), ctypes.POINTER(vp), ip]
         _lib.q35m_paged_attn_decode.argtypes = [vp, ci, ci, ip, vp, vp, vp, vp]
         _lib.q35m_paged_attn_prefill.argtypes = [vp, ci, ci, ip, ip, vp, vp, vp, vp]
@@ -628,12 +629,14 @@ class PagedCache:
         assert len(seqs) == len(first) == len(count)
         check(_Paged.rows(self.handle, layer, len(seqs), _list(seqs), _list(first), _list(count), k.ptr, v.ptr))
 
-    def plan(self, n, rows, tokens, free, slots, taken) -> None:
+    def plan(self, n, rows, tokens, free, slots, taken, listed=None) -> None:
         """Tables and lengths of sequences 0 .. n - 1 from device arrays (.ptr, .nbytes): rows,
-        tokens [n] int32, free pages int32; slots int64, taken [n] int32 are written."""
+        tokens [n] int32, free pages int32; slots int64, taken [n] int32 are written.  listed: how many of the
+        free pages there are, one int32 on the device (all of them)."""
         assert min(rows.nbytes, tokens.nbytes, taken.nbytes) >= 4 * n
-        check(_lib.q35m_paged_plan(self.handle, n, rows.ptr, tokens.ptr, free.ptr, free.nbytes // 4, slots.ptr,
-                                    slots.nbytes // 8, taken.ptr))
+        assert listed is None or listed.nbytes >= 4
+        check(_lib.q35m_paged_plan_listed(self.handle, n, rows.ptr, tokens.ptr, free.ptr, free.nbytes // 4,
+                                          None if listed is None else listed.ptr, slots.ptr, slots.nbytes // 8, taken.ptr))
 
     def tables(self):
         """(device address of the tables [n_seqs][max_pages], of the lengths [n_seqs], max_pages)."""
