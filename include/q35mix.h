@@ -364,12 +364,19 @@ int q35m_paged_attn_prefill(q35m_paged* p, int layer, int n, const int* seqs, co
  * gets shorter is not padded with such, but counted (q35m_paged_plan_listed).  Arrays that are written overlap no other one and
  * none of the cache's memory, its pages and workspace among it (Q35M_ERR_INVALID); rows may be the
  * cache's lengths (below).
- * A first call gives the lengths and tables over to the device: q35m_paged_map, _advance,
+ * A first call, also one that is only captured, gives the lengths and tables over to the
+ * device for good: q35m_paged_map, _advance,
  * _truncate and _len are refused from then on (Q35M_ERR_INVALID), the operators above
  * no longer check lengths or pages but bring up to max_rows rows a sequence, leave out rows
  * that have no page, and what they give for a token whose rows are not all mapped is
  * undefined (no other token's is).  Which pages requests share is the caller's
- * to keep: no page that is taken may be in another's rows.  Capturable; replays plan the
+ * to keep, and no call refuses a shared page any more: a page that is taken may not be in
+ * another's rows, and nor may the last page of a request's rows where these end inside it, since its
+ * tokens go on there (they would be written over the other request's).  Requests behind a prefix
+ * share its whole pages, and each has its own copy of the one that it ends in.
+ * The operators above find rows by tables and lengths; slots are for kernels of the caller's.
+ * Every plan writes all of the tables' entries behind the requests' rows, n times max_rows / page_rows
+ * at most.  Capturable; replays plan the
  * lengths of their time. */
 int q35m_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
                     int64_t* slots, size_t n_slots, int* taken);
@@ -381,8 +388,8 @@ int q35m_paged_plan_listed(q35m_paged* p, int n, const int* rows, const int* tok
                            const int* n_listed, int64_t* slots, size_t n_slots, int* taken);
 /* Device addresses of the tables [n_seqs][*max_pages] (page ids, -1: not mapped) and
  * the lengths [n_seqs], which the calls on the context's stream read and a plan writes.
- * A caller may set entries of the tables before a plan (a shared prefix's pages); the lengths are
- * to be read only. */
+ * A caller may set entries of the tables before a plan (the whole pages of a shared prefix, and a
+ * page of the request's own with a copy of the one that it ends in); the lengths are to be read only. */
 int q35m_paged_tables(q35m_paged* p, int** table, int** lens, int* max_pages);
 
 /* ---- one decode step of every layer, captured once, replayed per token ---- */
