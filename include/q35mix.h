@@ -262,7 +262,7 @@ typedef struct q35m_paged q35m_paged;
  * 7 2^s, within -23 .. 13; values are rounded to the nearest of these, ties to the even
  * code, and beyond the last one to it: K rows as an fp32 cache holds them, V rows as they
  * come.  The attention takes the held values as they are; the normed q is held to
- * 2^-20 of the largest value of its 32 dims (q35m_paged_attn_decode: 2^-24), and the softmax
+ * 2^-20 of the largest value of its 32 dims (q35m_paged_attn_decode: 2^-23), and the softmax
  * weights as over an fp16 cache, to no less than 2^-31 of the row's largest
  * (q35m_paged_attn_decode: 2^-38).  A block
  * with a value that is not finite is NaN, in all of its dims. */

@@ -6,7 +6,7 @@
 // 8-bit floats multiplies blocks of 32 values that share a power of two, which is how a
 // row is held.  q takes part in the 6-bit type (3 bits of mantissa, up to 7.5): each
 // block of 32 dims is cut into six digits of base 16, x = sum d_k 2^{e - 4 k}, |d_k| <= 8, which
-// reach 2^-24 of the block's largest value, one power of two each.  The digits are columns
+// leave 2^-23 of the block's largest value at most, one power of two each.  The digits are columns
 // of the operand: 16 of them are four heads by four digits, so a second product brings
 // the last two, and the columns of a head are added at the end: a score to fp32 precision
 // at two products of 16 x 16 x 128 a head quad, and no K value is converted.
