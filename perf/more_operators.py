@@ -223,9 +223,10 @@ class _Foreign:
 
 
 class _Owner:
-    """A context and its paged cache, as a program makes them once and keeps them while conversations come and go: another
-    state's once neither this state nor a view of their memory is left."""
-    kept = {}                       # those of the last shape that no state has
+    """A paged cache, and the layer of its context that has the state's weights.  A program has one context, of several layers,
+    whose calls follow each other on one stream, and makes a cache once for conversations that come and go: a state takes
+    one that neither an earlier state nor a view of its memory has any more."""
+    program = None
 
     def __init__(self, case, per, pool, x=None):
         here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "qwen3.5sharp_amd")
@@ -233,20 +234,18 @@ class _Owner:
             sys.path.insert(0, here)
         import q35mix
         self.kinds = (q35mix.STATE_KEYS, q35mix.STATE_VALUES)
-        self.key = (case["nh"], case["nkv"], case["n"], per, pool, case["page"], x is None)
-        for key in [k for k in self.kept if k != self.key]:
-            for ctx, cache in self.kept.pop(key):
-                cache.close()
-                ctx.close()
-        if self.kept.get(self.key):
-            self.ctx, self.cache = self.kept[self.key].pop()
-        else:
-            self.ctx = q35mix.Context(q35mix.qwen35_config(num_layers=1, num_heads=case["nh"], num_kv_heads=case["nkv"],
-                                                           is_recurrent=[0]), n_seqs=1, kv_capacity=16)
-            self.cache = q35mix.PagedCache(self.ctx, n_seqs=case["n"], max_rows=per * case["page"], n_pages=pool,
-                                           page_rows=case["page"], kv_type=q35mix.KV_MXFP4)
+        key = (case["nh"], case["nkv"], case["n"], per, pool, case["page"], x is None)
+        if _Owner.program is None or _Owner.program.key != key or not _Owner.program.places:
+            _Owner.program = _Program(q35mix, key, 1 if x is None else 5)
+        self.of = _Owner.program
+        self.ctx, self.place = self.of.ctx, self.of.places.pop(0)
+        self.layer = 0 if x is None else self.place
+        if self.place not in self.of.caches:
+            self.of.caches[self.place] = q35mix.PagedCache(self.ctx, n_seqs=case["n"], max_rows=per * case["page"], n_pages=pool,
+                                                           page_rows=case["page"], kv_type=q35mix.KV_MXFP4)
+        self.cache = self.of.caches[self.place]
         if x is not None:
-            self.ctx.set_attn_weights(0, {k: x[k].cpu().numpy() for k in ("q_norm", "k_norm")})
+            self.ctx.set_attn_weights(self.layer, {k: x[k].cpu().numpy() for k in ("q_norm", "k_norm")})
 
     def hold(self, lens, table):
         """The conversations' pages and lengths, in place of the ones before."""
@@ -260,7 +259,7 @@ class _Owner:
         """One pool's contents in the library's layout: of each (page, kv head) the rows' codes, then their scales, K's by
         row and V's by 16 rows, block by block."""
         pool, nkv, page = codes.shape[:3]
-        to = torch.as_tensor(_Foreign(self, self.cache.device_ptr(0, self.kinds[which])[0], (pool, nkv, page * 136), "|u1"),
+        to = torch.as_tensor(_Foreign(self, self.cache.device_ptr(self.layer, self.kinds[which])[0], (pool, nkv, page * 136), "|u1"),
                              device="cuda")
         to[..., :page * 128] = codes.view(pool, nkv, -1)
         if which:
@@ -274,7 +273,22 @@ class _Owner:
 
     def __del__(self):
         if hasattr(self, "cache"):
-            self.kept.setdefault(self.key, []).append((self.ctx, self.cache))
+            self.of.places.insert(0, self.place)
+
+
+class _Program:
+    """A context and its caches, for five states at once, closed when none has them and another shape is asked for."""
+
+    def __init__(self, q35mix, key, layers):
+        self.key, self.places, self.caches = key, list(range(5)), {}
+        self.ctx = q35mix.Context(q35mix.qwen35_config(num_layers=layers, num_heads=key[0], num_kv_heads=key[1],
+                                                       is_recurrent=[0] * layers), n_seqs=1, kv_capacity=16)
+
+    def __del__(self):
+        if hasattr(self, "ctx") and not sys.is_finalizing():
+            for cache in self.caches.values():
+                cache.close()
+            self.ctx.close()
 
 
 class _Buf:
@@ -320,7 +334,7 @@ def prepare(case, seed):
     if own:
         # the library's cache: its pages are its own memory, its tables are set and checked as conversations come
         s["owner"] = _Owner(case, per, pool, x)
-        s["cache"], s["seqs"], s["lens"], s["counts"] = s["owner"].cache, list(range(n)), lens, counts
+        s["cache"], s["layer"], s["seqs"], s["lens"], s["counts"] = s["owner"].cache, s["owner"].layer, list(range(n)), lens, counts
         s["owner"].hold(lens, table)
         for which in range(2):
             s["owner"].put(which, *pools[which])
@@ -421,12 +435,12 @@ def run(s):
         return {k: s[k] for k in ("table", "lens", "slots", "taken")}
     if own:
         if kind == "append":
-            s["cache"].append(0, s["seqs"], s["counts"], *s["args"])
+            s["cache"].append(s["layer"], s["seqs"], s["counts"], *s["args"])
         elif kind == "decode":
-            s["cache"].attn_decode(0, s["seqs"], *s["args"])
+            s["cache"].attn_decode(s["layer"], s["seqs"], *s["args"])
         else:
-            s["cache"].attn_prefill(0, s["seqs"], s["counts"], *s["args"])
-        s["cache"].rows(0, s["seqs"], s["lens"], s["counts"], *s["held"])
+            s["cache"].attn_prefill(s["layer"], s["seqs"], s["counts"], *s["args"])
+        s["cache"].rows(s["layer"], s["seqs"], s["lens"], s["counts"], *s["held"])
     else:
         _plain_append(s)
         if kind != "append":
