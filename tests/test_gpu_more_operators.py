@@ -1,5 +1,6 @@
-"""States of the performance cases of the 4-bit cache: a program makes its context and cache once and keeps them, so a new
-state takes those that an earlier one has left, and gives what one of its own handles gives.
+"""States of the performance cases of the 4-bit cache: a program makes its context and caches once and keeps them, so a new
+state takes those that an earlier one has left, and gives what one of its own handles gives; two states' calls follow each
+other on one stream.
 """
 import importlib.util
 import os
@@ -30,10 +31,7 @@ def cases(monkeypatch):
             super().__init__(*a, **k)
     monkeypatch.setattr(q35mix, "PagedCache", Counted)
     yield m
-    for handles in m._Owner.kept.values():
-        for ctx, cache in handles:
-            cache.close()
-            ctx.close()
+    m._Owner.program = None
 
 
 def answer(m, state):
@@ -47,7 +45,7 @@ def test_a_new_state_takes_the_handles_that_are_free(cases, case):
     first = {seed: answer(cases, cases.prepare(case, seed)) for seed in (1, 2, 3)}
     assert len(cases.made) == 1
     a, b = cases.prepare(case, 1), cases.prepare(case, 2)           # two at once: handles of their own
-    assert len(cases.made) == 2 and a["cache"] is not b["cache"]
+    assert len(cases.made) == 2 and a["cache"] is not b["cache"] and a["owner"].ctx is b["owner"].ctx
     for _ in range(2):
         for seed, s in ((1, a), (2, b)):
             got = answer(cases, s)
@@ -70,4 +68,13 @@ def test_other_lengths_and_shapes(cases):
             assert torch.equal(want.setdefault((c["rows"], k), got[k]), got[k])
     assert len(cases.made) == 1
     answer(cases, cases.prepare({**CASES[2], "nh": 8}, 5))
-    assert len(cases.made) == 2 and len(cases._Owner.kept) == 1
+    assert len(cases.made) == 2 and len(cases._Owner.program.caches) == 1
+
+
+def test_more_states_than_a_program_has_places_for(cases):
+    want = [answer(cases, cases.prepare(CASES[1], seed)) for seed in range(7)]
+    states = [cases.prepare(CASES[1], seed) for seed in range(7)]
+    assert len({id(s["owner"].ctx) for s in states}) == 2 and len({id(s["cache"]) for s in states}) == 7
+    for s, w in zip(states, want):
+        got = answer(cases, s)
+        assert all(torch.equal(got[k], w[k]) for k in got)
