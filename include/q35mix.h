@@ -263,8 +263,7 @@ typedef struct q35m_paged q35m_paged;
  * code, and beyond the last one to it: K rows as an fp32 cache holds them, V rows as they
  * come.  The attention takes the held values as they are; the normed q is held to
  * 2^-20 of the largest value of its 32 dims (q35m_paged_attn_decode: 2^-23), and the softmax
- * weights as over an fp16 cache, to no less than 2^-31 of the row's largest
- * (q35m_paged_attn_decode: 2^-38).  A block
+ * weights as over an fp16 cache.  A block
  * with a value that is not finite is NaN, in all of its dims. */
 #define Q35M_KV_MXFP4 4
 /* Values that are not finite reach the outputs of the tokens that see their row and

@@ -37,11 +37,11 @@ constexpr int kDigits = 6;
 constexpr int kDigitWords = 50;                  // 48 words of 6-bit codes, and 2 for the banks
 // P is e^{s - m} 2^kShift4, and m is behind the largest score by up to kMove4 (in log2): the
 // output is scaled (128 instructions of the tile's 370) only when a score passes m by that.
-// Weights are below 2^15.9, in fp16's range, and their low halves in steps of 2^-37 of the
-// largest weight or finer.  The two are one bound, which a finer step takes from the distance: 2^-30
-// (6 and 9.9) 36.0 us for 64 sequences of up to 4000 rows and 19.1 for 32 of up to 6000 under 16 heads on
-// one kv head; 2^-37 36.3 and 19.6; 2^-39 (15 and 0.9), an fp16 cache's, 36.7 and 20.3.
-constexpr float kShift4 = 13.0f, kMove4 = 2.9f;
+// Weights are below 2^15.9, in fp16's range, and their low halves in steps of 2^-39 of the
+// largest weight or finer, as over an fp16 cache.  The two share that range: steps of 2^-30 (6 and
+// 9.9) 51.5 us for 64 sequences of up to 4000 rows and 38.8 for 32 of up to 6000 under 16 heads on one
+// kv head, 2^-37 (13 and 2.9) 51.7 and 39.4, 2^-39 51.9 and 40.2.
+constexpr float kShift4 = 15.0f, kMove4 = 0.9f;
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 

@@ -10,8 +10,8 @@
 // the block's largest value at most (2^-22 unless that is within 1 / 32 below a power of two), at
 // 5 / 4 of one fp16 product's time where two would be taken.  Five and not six, which would leave
 // a sixteenth of that: of the outputs' 6e-7 over normal rows (fp32's sums) q's parts are the less, and
-// a unit's products are 52 instead of 56, 248 us against 263 for 512 rows behind 16000, 93
-// against 98.5 for 2048 (where q alone decides, small values of a block beside a large one and scores
+// a unit's products are 52 instead of 56, 240 us against 250 for 512 rows behind 16000, 100.5
+// against 103 for 2048 (where q alone decides, small values of a block beside a large one and scores
 // of 6, the outputs are off by up to 2.5e-5, six parts' bound being 1.5e-6).
 // The output's products are fp16's, with P as hi + lo: a block's power of two is a row's,
 // along that product's sum.  V is converted into LDS, once a workgroup, beside products.
