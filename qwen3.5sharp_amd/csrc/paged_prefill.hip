@@ -79,13 +79,15 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
                                                            const float* __restrict__ q_norm, float* __restrict__ out,
                                                            float* __restrict__ part_o, float* __restrict__ part_ml,
                                                            int hg_shift, int ng, int more, float eps) {
-    // Weights are e^{s - m} 2^kShift, and m is behind the largest score by up to kMove
-    // (in log2): below 2^15.9, in fp16's range, and in steps of 2^-24, 2^-30 of the largest
-    // weight or finer.  Half a step, 2^-31, is less than what adding 16 rows to an fp32
-    // sum rounds off a row (2^-25 / 16).  A smaller kMove scales the output more often:
-    // 2048 rows 92.7 us at (7, 8), 90.4 here, 88.5 at (1, 14), whose steps lose rows 18
-    // nats below the largest.
-    constexpr float kShift = 6.0f, kMove = 9.9f;
+    // Weights are 2^{s - m} (s in log2), and m, which begins kShift below the largest score, moves
+    // when one is more than kTop above it: below 2^15.9, in fp16's range, and in steps of 2^-24, 2^-30 of
+    // the largest weight or finer.  Half a step, 2^-31, is less than what adding 16 rows to an fp32
+    // sum rounds off a row (2^-25 / 16).  A larger kShift scales the output more often:
+    // 2048 rows 92.7 us at 7 (and kTop 15), 90.4 here, 88.5 at 1, whose steps lose rows 18
+    // nats below the largest.  What is compared is the difference, which is the weight's exponent as it
+    // is formed: beside scores of millions a sum rounds to the next quarter or whole number, and a
+    // weight to 2^16.
+    constexpr float kShift = 6.0f, kTop = 15.9f;
     __shared__ __align__(16) F16Tile st;
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -271,11 +273,12 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
         float sub;                                         // what the weights' exponents have added
         auto meet = [&](float other) {
             mx = fmaxf(mx, other);
-            moves = __any(mx > m_run + kMove);             // (m_run is -inf at first)
+            moves = __any(mx - m_run > kTop);              // (m_run is -inf at first)
         };
         auto move = [&]() {
             if (__builtin_expect_with_probability(moves, 0, 0.99)) {
-                const float m_new = fmaxf(m_run, mx);
+                float m_new = fmaxf(m_run, mx - kShift);
+                if (mx - m_new > kTop) m_new = mx;         // (mx so large that it is rounded)
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
                 m_run = m_new;
                 l_run *= alpha;
@@ -284,7 +287,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_f16(PagedView pv, PagedBa
                 for (int d = 0; d < 4; ++d) o[d] *= alpha;
                 pin();
             }
-            sub = kShift - (m_run == -INFINITY ? 0.0f : m_run);
+            sub = m_run == -INFINITY ? 0.0f : -m_run;
         };
         f16x8 ph[2], pl[2];
         float p_even = 0.0f, p_sum = 0.0f;                 // (of the unit: one small weight at a time would be lost
