@@ -35,13 +35,13 @@ constexpr int kTileRows = 32;                    // of a wave
 constexpr int kUnitRows4 = 4 * kTileRows;
 constexpr int kDigits = 6;
 constexpr int kDigitWords = 50;                  // 48 words of 6-bit codes, and 2 for the banks
-// P is e^{s - m} 2^kShift4, and m is behind the largest score by up to kMove4 (in log2): the
-// output is scaled (128 instructions of the tile's 370) only when a score passes m by that.
-// Weights are below 2^15.9, in fp16's range, and their low halves in steps of 2^-39 of the
-// largest weight or finer, as over an fp16 cache.  The two share that range: steps of 2^-30 (6 and
-// 9.9) 51.5 us for 64 sequences of up to 4000 rows and 38.8 for 32 of up to 6000 under 16 heads on one
-// kv head, 2^-37 (13 and 2.9) 51.7 and 39.4, 2^-39 51.9 and 40.2.
-constexpr float kShift4 = 15.0f, kMove4 = 0.9f;
+// P is 2^{s - m} (s in log2), and m begins kShift4 below the largest score: the output is scaled
+// (128 instructions of the tile's 370) only when a score is more than kTop4 above m (the difference is
+// compared, as in the fp16 prefill).  Weights are below 2^15.9, in fp16's range, and their low
+// halves in steps of 2^-39 of the largest weight or finer, as over an fp16 cache.  Steps of 2^-30
+// (kShift4 6) 51.5 us for 64 sequences of up to 4000 rows and 38.8 for 32 of up to 6000 under 16 heads on
+// one kv head, 2^-37 (13) 51.7 and 39.4, 2^-39 51.9 and 40.2.
+constexpr float kShift4 = 15.0f, kTop4 = 15.9f;
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -434,14 +434,15 @@ __global__ __launch_bounds__(NT, NQ == 4 ? 1 : 2) void paged_decode_mx4(PagedVie
                 mx = fmaxf(mx, s[j]);
             }
             mx = xor16_max(xor32_max(mx));
-            if (__builtin_expect(__any(mx > m_run + kMove4), 0)) {         // (m_run is -inf at first)
-                const float m_new = fmaxf(m_run, mx);
+            if (__builtin_expect(__any(mx - m_run > kTop4), 0)) {          // (m_run is -inf at first)
+                float m_new = fmaxf(m_run, mx - kShift4);
+                if (mx - m_new > kTop4) m_new = mx;        // (mx so large that it is rounded)
                 const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
                 m_run = m_new;
                 l_run *= alpha;
                 tl.scale(alpha);
             }
-            const float sub = kShift4 - (m_run == -INFINITY ? 0.0f : m_run);
+            const float sub = m_run == -INFINITY ? 0.0f : -m_run;
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {

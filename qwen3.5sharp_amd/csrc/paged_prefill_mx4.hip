@@ -92,7 +92,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
                                                            float* __restrict__ part_o, float* __restrict__ part_ml,
                                                            int hg_shift, int ng, int more, float eps) {
     // (as in the fp16 kernel)
-    constexpr float kShift = 6.0f, kMove = 9.9f;
+    constexpr float kShift = 6.0f, kTop = 15.9f;
     __shared__ __align__(16) Mx4Tile st;
     const int tid = threadIdx.x;
     const int tm = kPagedTileRows >> hg_shift;
@@ -353,18 +353,19 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
         float sub;                                         // what the weights' exponents have added
         auto meet = [&](float other) {
             mx = fmaxf(mx, other);
-            moves = __any(mx > m_run + kMove);             // (m_run is -inf at first)
+            moves = __any(mx - m_run > kTop);              // (m_run is -inf at first)
         };
         float alpha;
         auto move = [&]() {
             alpha = 1.0f;
             if (__builtin_expect_with_probability(moves, 0, 0.99)) {
-                const float m_new = fmaxf(m_run, mx);
+                float m_new = fmaxf(m_run, mx - kShift);
+                if (mx - m_new > kTop) m_new = mx;
                 alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
                 m_run = m_new;
                 l_run *= alpha;
             }
-            sub = kShift - (m_run == -INFINITY ? 0.0f : m_run);
+            sub = m_run == -INFINITY ? 0.0f : -m_run;
         };
         auto scale = [&]() {                               // (once what refers to the maximum before is added)
             if (__builtin_expect_with_probability(moves, 0, 0.99)) {

@@ -13,7 +13,7 @@ from test_gpu_paged_mx4 import Mx4
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16])
+@pytest.mark.parametrize("kv_type", [KV_F32, KV_F16, KV_MXFP4])
 @pytest.mark.parametrize("base", [16384.0, -16384.0, 40960.0])
 @pytest.mark.parametrize("T", [1, 48])
 def test_scores_of_millions(kv_type, base, T):
