@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void paged_append_rows(PagedView pv, PagedBatc
 
 // Rows read back, one wave per (row, kv head): row `row` of the call is row first + (its
 // place) of its sequence.  Rows of pages that are not mapped are zeros.
-// Bound by what it writes: 2048 rows of 4 kv heads in 4 bits, 2.2 MB read and 16.8 written, 6.6 us.
+// Bound by what it writes: 2048 rows of 4 kv heads in 4 bits, 2.2 MB read and 16.8 written, 6.7 us.
 template <typename T, int N>
 __global__ __launch_bounds__(256) void paged_rows(PagedView pv, PagedBatchOf<N> b, PagedFirstOf<N> first,
                                                   float* __restrict__ k, float* __restrict__ v, long unit0) {

@@ -43,8 +43,8 @@ __device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatchO
 // Whether a 4-bit cache's sequences are left whole, each (sequence, head group) to a
 // workgroup, so that nothing is to be joined: where the busiest CU gets up to 3 units
 // more than if they are dealt out (a launch against 1.1 us a unit).  450 rows, 4
-// units for 1: 10.3 us against 11.3; 16 sequences of 600, 5 for 2: 12.9 against 14.3, of
-// 1000, 8 for 2: 16.1 against 14.5; 64 of 3000, as many: 37 against 41.
+// units for 1: 10.9 us against 11.1; 16 sequences of 600, 5 for 2: 13.2 against 14.5, of
+// 1000, 8 for 2: 16.5 against 15.7; 64 of 3000, as many: 38.9 against 43.7.
 __host__ __device__ __forceinline__ bool left_whole(int groups, int units, int longest, int n_cu, int nwg) {
     const int each = (groups <= n_cu ? 1 : 2) * longest;   // (nwg: one or two a CU)
     return groups <= nwg && (each - 4) * n_cu < units;

@@ -16,13 +16,16 @@
 // matrix instruction's own cannot serve here.  P is two fp16 values (hi + lo, to 2^-23 of
 // it), which are columns too up to 8 heads.
 //
-// What bounds it is the cache's bytes: 64 sequences of up to 4000 rows are 191 MB, 29 us at
-// the 6.5 TB/s that a large read reaches, and take 36 in calls one after the other (the
-// kernel by itself 38, the joining 5); 8 of up to 32768 rows, 202 MB, 33.5.  Two workgroups
-// a CU with a tile ahead each against one with two tiles ahead: 38.1 and 35.6 us against 39.8
-// and 34.7; a workgroup's start (lengths, pages, q and the first rows, one after the
-// other, 4500 cycles) hides behind the other's rows.  Parts joined by the last workgroup
-// to finish instead of by a second launch: 47 us for 43.
+// What bounds it: the cache's bytes and, near to them, the vector work on them.  Calls over caches
+// in turn, too many for the last-level cache: 64 sequences of up to 4000 rows are 191 MB, 29 us at the
+// 6.5 TB/s that a large read reaches, and take 42 (4.6 TB/s) and the joining 5; 8 of up to 32768 rows, 202
+// MB, 39 and 5.  A wave issues vector instructions in 29 % of its cycles, with another one on
+// its SIMD, and waits in 30 %.  Two workgroups a CU with a tile ahead each against one with two
+// tiles ahead, calls with their rows read back: 51.9 and 48.2 us against 55.9 and 48.1, three short
+// sequences 11.6 against 12.2, 32 sequences of up to 6000 rows under 8 heads a kv head (whose loop
+// spills 7 registers at two a CU) 39.9 against 37.5; a workgroup's start (lengths, pages, q and the first
+// rows, one after the other, 4500 cycles) hides behind the other's rows.  Parts joined by the last
+// workgroup to finish instead of by a second launch: 47 us for 43.
 #include <algorithm>
 
 #include "paged_decode.h"
@@ -85,8 +88,8 @@ struct Tile4 {
                     for (int w = 0; w < 6; ++w) q[a][s][t][w] = digit < kDigits ? codes[head][d][12 * g + 6 * t + w] : 0u;
             }
     }
-    // (K without the hint that it is read once: an instruction takes half of each line, 44.2 us
-    // against 47.9 for 64 sequences of up to 4000 rows.)
+    // (K without the hint that it is read once: an instruction takes half of each line, 48.2 us
+    // against 50.4 for 8 sequences of up to 32639 rows.)
     // 16 rows, whose codes begin at `codes` and scales at `scales` (the same for all lanes).
     static __device__ __forceinline__ void load_k(Rows& r, const uint8_t* codes, const uint8_t* scales, int kb, int lane) {
         const int n = lane & 15, g = lane >> 4;

@@ -116,7 +116,7 @@ __device__ __forceinline__ double wave_sum(double v) {
 // 2^13 values, and such a value is 2^-11 off.  A row is 256 values once per
 // token, so the cost is not seen.  c, s: the rotation of dims 4 (lane % 8) ..,
 // ww: the norm's weights.  RSQRT: the norm by the function of that name, 1 ulp instead of two
-// roundings and a third of the instructions (six sequences' 1300 rows in 4 bits 12.7 -> 12.4 us).
+// roundings and a third of the instructions (six sequences' 1300 rows in 4 bits 18.9 -> 17.9 us).
 template <bool RSQRT = false>
 __device__ __forceinline__ float4 paged_key_row(float4 x, const double (&c)[4], const double (&s)[4], float4 ww, int lane,
                                                 double eps) {

@@ -96,9 +96,9 @@ __device__ __forceinline__ Units units_of(const PagedView& pv, const PagedBatch&
 
 // In 4 bits tiles are left whole, dealt out in pairs of first and last, which are alike,
 // where that leaves the busiest workgroup up to 12 units more than cutting: a cut tile
-// is begun and ended once more, 14 us at 1.55 a unit, and joined.  1000 tokens, 16 units
-// for 9: 47 us against 66; 2000, 34 for 32: 88 against 106; 800 behind 1000, 29 for 18: 67
-// against 70; 512 behind 1000, 24 for 11: 59 against 55.
+// is begun and ended once more, 14 us at 1.5 a unit, and joined.  1000 tokens, 16 units
+// for 9: 46 us against 66; 2000, 34 for 32: 91 against 111; 800 behind 1000, 29 for 18: 66.5
+// against 69.5; 512 behind 1000, 24 for 11: 58.5 against 54.
 // Returned is log2 of what a unit is over 64 rows then, of which a tile has one (0: cut).
 // longest: rows that a tile may see; pair: units of a sequence's first and last tile.
 __host__ __device__ __forceinline__ int whole_tiles(long tiles, long units, int longest, int pair, int nwg) {

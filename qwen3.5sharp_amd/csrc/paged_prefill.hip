@@ -999,7 +999,7 @@ hipError_t launch_paged_prefill(q35m_paged* p, int layer, const PagedBatch& b, c
         more = known ? whole_tiles(tiles, units, (int)longest, most, nwg) : -1;      // (-1: the kernels find it)
     }
     // Nor is a tile where each workgroup's share is a number of whole pairs (2048 tokens of
-    // a new sequence in 4 bits: 102 us instead of 105).
+    // a new sequence, fp16: 95.5 us instead of 101; fp32 234 instead of 238).
     const bool cut = more <= 0 && !(known && pair > 0 && (units + nwg - 1) / nwg % pair == 0);
     {
         ProfScope ps(c, K_PAGED_PREFILL);

@@ -16,12 +16,13 @@
 // The output's products are fp16's, with P as hi + lo: a block's power of two is a row's,
 // along that product's sum.  V is converted into LDS, once a workgroup, beside products.
 //
-// What bounds it: the power that the matrix pipe takes.  A unit of 64 x 64 is 52 products a
-// SIMD, which on random values take 23.5 ns each in every CU at once (14 to 16 on zeros): 1.22 us,
-// of the 1.49 that it takes; the pipe is busy 43 % of the cycles, at 2.3 GHz.  512 rows
-// behind 16000: 219 to 232 us, 591 TFLOP/s of the scores and outputs in all.  A tile's beginning
-// and end are 33000 cycles, 14 us, one step after the other (a fifth of it waits): 2048 rows, two
-// tiles a workgroup and 33 units, 83 us.
+// What bounds it: the matrix pipe, by the power that it takes, and what one wave a SIMD issues beside
+// it.  A unit of 64 x 64 is 52 products a SIMD; on random values in every CU at once the scores'
+// take 22.7 ns each, the output's 18.3, and the two in turn 20.9 (14 to 16 on zeros): 1.09 us of the
+// 1.48 that it takes.  The pipe is busy 43 % of the cycles, the wave issues vector instructions
+// in 34 % and waits in 15 %.  512 rows behind 16000: 226 us, 591 TFLOP/s of the scores and outputs
+// in all.  A tile's beginning and end are 33000 cycles, 14 us, one step after the other (a fifth of it
+// waits), and a launch's first ones more: 2048 rows, two tiles a workgroup and 33 units, 86 us.
 #include <type_traits>
 
 #include "paged_prefill.h"
@@ -301,8 +302,7 @@ __global__ __launch_bounds__(NT, 1) void paged_prefill_mx4(PagedView pv, PagedBa
             *(lds_u32x4*)(uintptr_t)(vto[c & 3] + buf * kBuf + (c >> 2) * (8 * kHd * 2)) = y;
         };
         // The products between two barriers, with beside(i) behind the i-th slot of 40: 20 of
-        // scores, of which each waits for the one before (23 ns, where independent ones take
-        // 18), and between them, if `left`, the 16 that the unit before has left.  A block's
+        // scores, of which each waits for the one before, and between them, if `left`, the 16 that the unit before has left.  A block's
         // codes are replaced by the next unit's once it is done.
         f16x8 v0[4], v1[4], w0[4], w1[4], h0, l0, h1, l1;
         auto left_over = [&](int i) {
