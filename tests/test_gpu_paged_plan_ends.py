@@ -113,3 +113,25 @@ def test_a_captured_plan_whose_list_runs_short():
             now = [a + t if g >= 0 else a for a, t, g in zip(now, tokens, got)]
         assert all_taken == [[1, 3, 1, 2], [0, -1, 0, -1], [0, 2, 0, 1]]
         end()
+
+
+# ------------------------------------------------------------------ many requests
+
+def test_tens_of_thousands_of_requests():
+    """Each request's pages and slots come behind the sums of all before it; as many requests as one plan takes."""
+    n, max_rows, page = 65535, 32, 16
+    rng = np.random.RandomState(6)
+    rows, tokens = rng.randint(0, 25, n), rng.randint(0, 8, n)
+    need = -(-(rows + tokens) // page) - -(-rows // page)
+    with Planner(n + 1, max_rows, page, 3 * n) as p:
+        ids = rng.permutation(3 * n)
+        table = np.full((n + 1, 2), -1, np.int32)
+        kept = -(-rows // page)
+        for e in range(2):
+            some = np.nonzero(kept > e)[0]
+            table[some, e], ids = ids[:some.size], ids[some.size:]
+        p.set_table(table)
+        want = p.check(list(rows), list(tokens), list(ids[:need.sum() - 5]), n=n)
+        assert (want[3][:-200] >= 0).all() and (want[3] == -1).any()
+        a = Ints(p.ctx, np.zeros(n + 1, np.int32))
+        refused(q35mix.ERR_UNSUPPORTED, lambda: p.c.plan(n + 1, a, a, a, Ints(p.ctx, [0], np.int64), Ints(p.ctx, np.zeros(n + 1))), "65535")
