@@ -279,7 +279,7 @@ class DecodeGraph:
         for l, bufs in enumerate(io):
             arr[l] = DecodeIO(*[None if b is None else b.ptr for b in bufs])
         h = ctypes.c_void_p()
-        check(lib().q35m_decode_graph_create(ctypes.c_void_p(ctx.handle), len(seqs), _seqs(seqs), arr, max_len,
+        check(lib().q35m_decode_graph_create(ctypes.c_void_p(ctx.handle), len(seqs), _list(seqs), arr, max_len,
                                              ctypes.byref(h)))
         self.handle = h.value
         self._io = io
@@ -353,7 +353,7 @@ def _ints(values):
 
 
 def _list(values):
-    """A paged call's list, refused where a value is no C int: cut to 32 bits it would name another sequence or count."""
+    """A call's list, refused where a value is no C int: cut to 32 bits it would name another sequence or count."""
     got = _ints(values)
     if type(got) is not bytes and any(a != b for a, b in zip(got, values)):
         raise ValueError(f"a list of {len(values)} values, not all of them 32-bit integers")
@@ -427,7 +427,7 @@ class Context:
     # ---- mixers (device arrays) -----------------------------------------
     def deltanet_decode(self, layer, seqs, qkv, z, b, a, out) -> None:
         check(lib().q35m_deltanet_decode(ctypes.c_void_p(self.handle), layer, len(seqs),
-                                         _seqs(seqs), *[ctypes.c_void_p(x.ptr) for x in
+                                         _list(seqs), *[ctypes.c_void_p(x.ptr) for x in
                                                         (qkv, z, b, a, out)]))
 
     def deltanet_prefill(self, layer, seq, T, qkv, z, b, a, out) -> None:
@@ -436,14 +436,14 @@ class Context:
 
     def attn_decode(self, layer, seqs, q_gate, k, v, out) -> None:
         check(lib().q35m_attn_decode(ctypes.c_void_p(self.handle), layer, len(seqs),
-                                     _seqs(seqs), *[ctypes.c_void_p(x.ptr) for x in
+                                     _list(seqs), *[ctypes.c_void_p(x.ptr) for x in
                                                     (q_gate, k, v, out)]))
 
     def attn_decode_noalloc(self, layer, seqs, q_gate, k, v, out) -> None:
         """q35m_attn_decode with the split-K partials in the library's fixed
         device scratch (no allocation)."""
         check(lib().q35m_attn_decode_noalloc(ctypes.c_void_p(self.handle), layer, len(seqs),
-                                             _seqs(seqs), *[ctypes.c_void_p(x.ptr) for x in
+                                             _list(seqs), *[ctypes.c_void_p(x.ptr) for x in
                                                             (q_gate, k, v, out)]))
 
     def attn_prefill(self, layer, seq, T, q_gate, k, v, out) -> None:

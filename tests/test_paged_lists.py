@@ -1,5 +1,5 @@
-"""Lists of sequences, tokens and rows at the paged cache's entry points, without a device: what a list may be made of, from
-the C functions' prototypes and from the front end's calls.
+"""Lists of sequences, tokens and rows at the entry points, without a device: what a list may be made of, from the paged C
+functions' prototypes and from the front end's calls.
 """
 import ctypes
 
@@ -61,3 +61,18 @@ def test_calls_refuse_values_that_are_no_c_ints(n):
     for wrong in ([1.5] * n, ["a"] * n, [None] * n):
         with pytest.raises(TypeError):
             c.advance(wrong, good)
+
+
+@pytest.mark.parametrize("n", [1, 8])
+def test_calls_over_the_context_s_own_caches_refuse_them_too(n):
+    c = object.__new__(q35mix.Context)
+    c.handle = None
+    x = type("Null", (), {"ptr": None})()
+    calls = (lambda v: c.deltanet_decode(0, v, x, x, x, x, x), lambda v: c.attn_decode(0, v, x, x, x, x),
+             lambda v: c.attn_decode_noalloc(0, v, x, x, x, x), lambda v: q35mix.DecodeGraph(c, v, [], 16))
+    for call in calls:
+        with pytest.raises(q35mix.Q35Error):
+            call(list(range(n)))
+        for big in BIG:
+            with pytest.raises(ValueError):
+                call(list(range(n - 1)) + [big])
