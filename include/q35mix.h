@@ -263,8 +263,8 @@ typedef struct q35m_paged q35m_paged;
  * code, and beyond the last one to it: K rows as an fp32 cache holds them, V rows as they
  * come.  The attention takes the held values as they are; the normed q is held to
  * 2^-20 of the largest value of its 32 dims (q35m_paged_attn_decode: 2^-23), and the softmax
- * weights as over an fp16 cache.  A block
- * with a value that is not finite is NaN, in all of its dims. */
+ * weights as over an fp16 cache.  A block with a value that is not finite is NaN, in all of
+ * its dims. */
 #define Q35M_KV_MXFP4 4
 /* Values that are not finite reach the outputs of the tokens that see their row and
  * no other: an infinite V value makes its dim of the output that infinity, whatever
@@ -360,24 +360,22 @@ int q35m_paged_attn_prefill(q35m_paged* p, int layer, int n, const int* seqs, co
  * tokens of all requests in order, up to n_slots of them; what is behind stays.  Up to
  * 65535 requests.
  * rows and tokens are taken within 0 and max_rows, in that order; an entry of the list
- * outside [0, n_pages) is dealt out as the others are and gives no page (taken counts it): a list that
- * gets shorter is not padded with such, but counted (q35m_paged_plan_listed).  Arrays that are written overlap no other one and
- * none of the cache's memory, its pages and workspace among it (Q35M_ERR_INVALID); rows may be the
- * cache's lengths (below).
+ * outside [0, n_pages) is dealt out as the others are and gives no page (taken counts it): a
+ * list that gets shorter is not padded with such, but counted (q35m_paged_plan_listed).  Arrays
+ * that are written overlap no other one and none of the cache's memory, its pages and workspace
+ * among it (Q35M_ERR_INVALID); rows may be the cache's lengths (below).
  * A first call, also one that is only captured, gives the lengths and tables over to the
- * device for good: q35m_paged_map, _advance,
- * _truncate and _len are refused from then on (Q35M_ERR_INVALID), the operators above
- * no longer check lengths or pages but bring up to max_rows rows a sequence, leave out rows
- * that have no page, and what they give for a token whose rows are not all mapped is
- * undefined (no other token's is).  Which pages requests share is the caller's
+ * device for good: q35m_paged_map, _advance, _truncate and _len are refused from then on
+ * (Q35M_ERR_INVALID), the operators above no longer check lengths or pages but bring up to
+ * max_rows rows a sequence, leave out rows that have no page, and what they give for a token
+ * whose rows are not all mapped is undefined (no other token's is).  Which pages requests share is the caller's
  * to keep, and no call refuses a shared page any more: a page that is taken may not be in
  * another's rows, and nor may the last page of a request's rows where these end inside it, since its
  * tokens go on there (they would be written over the other request's).  Requests behind a prefix
  * share its whole pages, and each has its own copy of the one that it ends in.
  * The operators above find rows by tables and lengths; slots are for kernels of the caller's.
- * Every plan writes all of the tables' entries behind the requests' rows, n times max_rows / page_rows
- * at most.  Capturable; replays plan the
- * lengths of their time. */
+ * Every plan writes all of the tables' entries behind the requests' rows, n times
+ * max_rows / page_rows at most.  Capturable; replays plan the lengths of their time. */
 int q35m_paged_plan(q35m_paged* p, int n, const int* rows, const int* tokens, const int* free_pages, int n_free,
                     int64_t* slots, size_t n_slots, int* taken);
 /* The same from a list whose length is the device's too, as in a captured step whose list gets
